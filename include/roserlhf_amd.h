@@ -482,6 +482,27 @@ RRL_API int rrl_sample_logprobs(const void* logits, int32_t logits_dtype, int64_
                         int32_t do_sample, uint64_t seed, uint64_t offset, int64_t* token_out,
                         float* logp_out, float* logq_out, int32_t* status, void* stream);
 
+/* ---- the token embedding ------------------------------------------------------
+ * Lookup: out[i] = scale * weight[id_i], rounded once to `dtype` (F32, BF16 or
+ * F16; out is contiguous [N, H], the weight's rows w_ld elements apart).  An id
+ * equal to padding_idx (has_padding != 0; it may be negative) takes a row of
+ * zeros; any other id outside [0, V) takes a row of NaN.  ids: I32 or I64,
+ * contiguous.
+ * Gradient: dweight[v] = scale * sum of grad[i] over id_i = v, every row of
+ * dweight written (zeros where v does not occur, padding and out-of-range ids
+ * left out), sums in float32 in an order that depends on the ids alone, rounded
+ * once.  workspace: rrl_embedding_bwd_workspace_bytes(N, V, H) bytes of caller
+ * device memory (16-byte aligned; contents in and out are of no meaning).
+ * (rosetrainer/model.py and qwen3.py look their tokens up with nn.Embedding.) */
+RRL_API int rrl_embedding_fwd(const void* ids, int32_t ids_dtype, int64_t N, const void* weight,
+                    int32_t dtype, int64_t V, int64_t H, int64_t w_ld, double scale,
+                    int64_t padding_idx, int32_t has_padding, void* out, void* stream);
+RRL_API size_t rrl_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t H);
+RRL_API int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, const void* grad,
+                    int32_t dtype, int64_t V, int64_t H, int64_t g_ld, double scale,
+                    int64_t padding_idx, int32_t has_padding, void* dweight, int64_t dw_ld,
+                    void* workspace, void* stream);
+
 /* Philox4x32-10 on the host (the generator rrl_sample_logprobs draws from):
  * ctr[4] is replaced by the 4 output words. */
 RRL_API void rrl_philox4x32_10(uint32_t ctr[4], const uint32_t key[2]);

@@ -133,6 +133,9 @@ SIGNATURES = {
     "rrl_lm_head_dweight_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
     "rrl_lm_head_dweight": (ctypes.c_int, [_P, _P, _I32, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _I32, _I64, _P]),
     "rrl_transpose16": (ctypes.c_int, [_P, _I64, _I64, _I64, _P, _I64, _P]),
+    "rrl_embedding_fwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _D, _I64, _I32, _P, _P]),
+    "rrl_embedding_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
+    "rrl_embedding_bwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _D, _I64, _I32, _P, _I64, _P, _P]),
     "rrl_philox4x32_10": (None, [ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(ctypes.c_uint32)]),
 }
 
@@ -233,6 +236,17 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = lib().rrl_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed ({rc}): {msg}")
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with ``device`` current: a launch goes to the current device,
+    whatever device its stream belongs to."""
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
 
 
 # ---------------------------------------------------------------------------

@@ -32,6 +32,7 @@ SOURCES = [
     "sampler.hip",
     "lm_head.hip",
     "layout.hip",
+    "embedding.hip",
 ]
 
 ARCH = os.environ.get("ROSELLM_AMD_ARCH", "gfx950")
