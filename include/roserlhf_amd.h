@@ -503,6 +503,36 @@ RRL_API int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, con
                     int64_t padding_idx, int32_t has_padding, void* dweight, int64_t dw_ld,
                     void* workspace, void* stream);
 
+/* ---- rollout side: verification of drafted tokens ------------------------------
+ * Speculative sampling from given uniforms (the reference decodes one token per
+ * step, roseinfer/engine.py:1103-1171).  target: logits [B, K + 1, V], draft:
+ * logits [B, K, V] or NULL, both `dtype` (F32, BF16 or F16), row (b, k) at
+ * b*sb + k*sk elements.  drafts: [B, K] I32 or I64; a negative one ends the
+ * sequence's draft at L, and rows behind it are not read.  uniforms: contiguous
+ * float32 [B, K + 1] in [0, 1).  With p = softmax(target / T), q =
+ * softmax(draft / T) (one-hot at the draft when draft is NULL), draft j is
+ * accepted while u[j] q(d_j) < p(d_j); n = the first that is not, or L.  The next
+ * token is the first v whose running sum of rest exceeds u[K] sum(rest), rest =
+ * max(p_n - q_n, 0) after a rejection (p_n where that has no mass), p_L else.
+ * Greedy (do_sample == 0 or temperature <= 0): accepted while d_j is the target's
+ * first maximum, the next token is row n's; draft and uniforms are not read and
+ * T = 1.  Sums and exponentials are float64 (1.1e-12 relative).
+ * token_out (int64 [B, K + 1]): the accepted drafts, the next token, then -1;
+ * count_out (int64 [B]): n; logp_out (float32 [B, K + 1]): the tokens'
+ * log_softmax(target / T), 0 behind the last.  A needed row with NaN or +inf, or
+ * with nothing above -inf, and a draft of V or more end the sequence there with
+ * token -1 and log-prob NaN.  workspace:
+ * rrl_verify_drafts_workspace_bytes(B, K, V, draft != NULL) bytes of caller
+ * device memory (16-byte aligned; contents of no meaning; 0 for sizes that
+ * rrl_verify_drafts refuses). */
+RRL_API size_t rrl_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V,
+                    int32_t with_draft_logits);
+RRL_API int rrl_verify_drafts(const void* target, const void* draft, int32_t dtype, int64_t B,
+                    int64_t K, int64_t V, int64_t t_sb, int64_t t_sk, int64_t d_sb, int64_t d_sk,
+                    rrl_view drafts, const float* uniforms, double temperature,
+                    int32_t do_sample, int64_t* token_out, int64_t* count_out, float* logp_out,
+                    void* workspace, void* stream);
+
 /* Philox4x32-10 on the host (the generator rrl_sample_logprobs draws from):
  * ctr[4] is replaced by the 4 output words. */
 RRL_API void rrl_philox4x32_10(uint32_t ctr[4], const uint32_t key[2]);

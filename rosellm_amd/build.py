@@ -33,6 +33,7 @@ SOURCES = [
     "lm_head.hip",
     "layout.hip",
     "embedding.hip",
+    "verify.hip",
 ]
 
 ARCH = os.environ.get("ROSELLM_AMD_ARCH", "gfx950")
