@@ -533,6 +533,30 @@ RRL_API int rrl_verify_drafts(const void* target, const void* draft, int32_t dty
                     int32_t do_sample, int64_t* token_out, int64_t* count_out, float* logp_out,
                     void* workspace, void* stream);
 
+/* ---- rollout side: a draft head in microscaled 4-bit floating point --------------
+ * OCP MX blocks of 32 entries along a row: e2m1 elements and an e8m0 scale.  With
+ * amax the block's largest magnitude and e = max(floor(log2 amax) - 2, -127), the
+ * scale byte is e + 127 (255, NaN, where the block holds NaN or infinity; 0 for a
+ * block of zeros) and an element x / 2^e rounded to nearest, ties to even,
+ * saturating at 6.  Rows are padded with zeros to P = H rounded up to a multiple
+ * of 128: codes [R, P / 2] (two entries a byte, the first in the low half),
+ * scales [R, P / 32], both contiguous, codes 16-byte aligned.
+ * rrl_mxfp4_quantize: x [R, H] F32, BF16 or F16, rows ld elements apart.
+ * rrl_mxfp4_dequantize: the numbers they stand for, contiguous [R, H].
+ * rrl_mxfp4_linear: out[m, n] = sum_k xq[m, k] wq[n, k], contiguous [M, N]; x is
+ * quantised as above within the call, products are summed in float32 and rounded
+ * once to out_dtype.  workspace: rrl_mxfp4_linear_workspace_bytes(M, H) bytes of
+ * caller device memory (16-byte aligned; contents of no meaning).
+ * (The reference's heads are F.linear, rosetrainer/model.py:641.) */
+RRL_API int rrl_mxfp4_quantize(const void* x, int32_t dtype, int64_t R, int64_t H, int64_t ld,
+                    uint8_t* codes, uint8_t* scales, void* stream);
+RRL_API int rrl_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t R, int64_t H,
+                    void* out, int32_t dtype, void* stream);
+RRL_API size_t rrl_mxfp4_linear_workspace_bytes(int64_t M, int64_t H);
+RRL_API int rrl_mxfp4_linear(const void* x, int32_t dtype, int64_t M, int64_t H, int64_t x_ld,
+                    const uint8_t* codes, const uint8_t* scales, int64_t N, void* out,
+                    int32_t out_dtype, void* workspace, void* stream);
+
 /* Philox4x32-10 on the host (the generator rrl_sample_logprobs draws from):
  * ctr[4] is replaced by the 4 output words. */
 RRL_API void rrl_philox4x32_10(uint32_t ctr[4], const uint32_t key[2]);

@@ -136,6 +136,10 @@ SIGNATURES = {
     "rrl_verify_drafts_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I32]),
     "rrl_verify_drafts": (ctypes.c_int, [_P, _P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _V, _P, _D,
                                          _I32, _P, _P, _P, _P, _P]),
+    "rrl_mxfp4_quantize": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),
+    "rrl_mxfp4_dequantize": (ctypes.c_int, [_P, _P, _I64, _I64, _P, _I32, _P]),
+    "rrl_mxfp4_linear_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "rrl_mxfp4_linear": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _P]),
     "rrl_embedding_fwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _D, _I64, _I32, _P, _P]),
     "rrl_embedding_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
     "rrl_embedding_bwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _D, _I64, _I32, _P, _I64, _P, _P]),

@@ -34,6 +34,7 @@ SOURCES = [
     "layout.hip",
     "embedding.hip",
     "verify.hip",
+    "mxfp4.hip",
 ]
 
 ARCH = os.environ.get("ROSELLM_AMD_ARCH", "gfx950")
