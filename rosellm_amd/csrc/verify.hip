@@ -15,18 +15,18 @@
 // pass a wrong one every some ten rows of 150,000 entries.  Exponentials and sums
 // are therefore float64, the exponential a polynomial good to 1.1e-12.
 //
-// Rows are cut into chunks, so that a single sequence fills the chip:
-//   1. verify_stats: every needed row's chunks: maximum, sum of exponentials
-//   2. verify_decide: a workgroup per sequence joins them and finds n
-//   3. verify_rest: after a rejection, the mass of rest in every chunk of row n
-//   4. verify_draw: a workgroup per sequence finds the chunk, then the entry
+// Rows are cut into chunks, a wave each, so that a single sequence fills the chip:
+//   1. verify_stats: the chunks of every row that may be needed: maximum, sum
+//   2. verify_rest: joins the rows' chunks and finds n (every workgroup for itself,
+//      which is shorter than another launch), then, after a rejection, the mass of
+//      rest in each chunk of row n
+//   3. verify_draw: a workgroup per sequence finds the chunk, then the entry
 #include "slab_common.hpp"
 
 namespace rrl {
 namespace {
 
 constexpr int kVT = 256;        // threads of a workgroup
-constexpr int kChunk = 4096;    // entries of a chunk
 
 // 2^r for |r| <= 1/2: the polynomial through 2^r at the nine Chebyshev nodes of
 // that interval, within 1.1e-12 of it, relative.
@@ -42,13 +42,19 @@ __device__ __forceinline__ double exp2_poly(double r) {
   return fma(p, r, 1.0);
 }
 
-// 2^t for t <= 0 (0 for -inf).  Below -1000 the result, under 1e-301 beside a
-// maximum of 1, is taken as 2^-1000.. of the clamped t: it is left at 0.
-__device__ __forceinline__ double exp2_neg(double t) {
-  if (!(t > -1000.0)) return 0.0;
-  const double n = rint(t);
-  return ldexp(exp2_poly(t - n), (int)n);
+// 2^max(t, -1000) for t <= 0: beside a maximum of 1 what is below counts for
+// nothing.  Adding 1.5 2^52 rounds t to a whole number, which the sum's low word
+// then holds, and the exponent field takes it as it is.
+__device__ __forceinline__ double exp2_clamped(double t) {
+  t = fmax(t, -1000.0);
+  const double whole = t + 0x1.8p52;
+  const double p = exp2_poly(t - (whole - 0x1.8p52));
+  return __hiloint2double(__double2hiint(p) + (int)((uint32_t)__double2loint(whole) << 20),
+                          __double2loint(p));
 }
+
+// The same with 0 below -1000, so that what is impossible weighs nothing.
+__device__ __forceinline__ double exp2_neg(double t) { return t > -1000.0 ? exp2_clamped(t) : 0.0; }
 
 struct VerifyArgs {
   const char *x, *y;            // target, draft logits (y may be null)
@@ -61,7 +67,7 @@ struct VerifyArgs {
   double c;                     // log2(e) / T
   int greedy;
   int rows;                     // rows per sequence: K + 1 target rows, then the draft's
-  int chunks;
+  int chunks, chunk;            // chunks of a row, and a chunk's entries (1024 or 4096)
   int64_t* token_out;           // [B, K + 1]
   int64_t* count_out;           // [B]
   float* logp_out;              // [B, K + 1]
@@ -134,154 +140,138 @@ __device__ __forceinline__ float load_entry(const char* row, int64_t i) {
   else return Pack16<Tag>::one(reinterpret_cast<const uint16_t*>(row)[i]);
 }
 
+// Butterfly over a row of 16 lanes, and over the wave.
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+  return __hiloint2double(dpp_i<CTRL>(__double2hiint(v)), dpp_i<CTRL>(__double2loint(v)));
+}
+__device__ __forceinline__ double row16_sum(double v) {
+  v += dpp_d<kDppXor1>(v);
+  v += dpp_d<kDppXor2>(v);
+  v += dpp_d<kDppHalfMirror>(v);
+  return v + dpp_d<kDppMirror>(v);
+}
+__device__ __forceinline__ float row16_max(float v) {
+  v = fmaxf(v, dpp_f<kDppXor1>(v));
+  v = fmaxf(v, dpp_f<kDppXor2>(v));
+  v = fmaxf(v, dpp_f<kDppHalfMirror>(v));
+  return fmaxf(v, dpp_f<kDppMirror>(v));
+}
+__device__ __forceinline__ int row16_min(int v) {
+  v = min(v, dpp_i<kDppXor1>(v));
+  v = min(v, dpp_i<kDppXor2>(v));
+  v = min(v, dpp_i<kDppHalfMirror>(v));
+  return min(v, dpp_i<kDppMirror>(v));
+}
+__device__ __forceinline__ double lane_read_d(double v, int l) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l),
+                          __builtin_amdgcn_readlane(__double2loint(v), l));
+}
+__device__ __forceinline__ double wave_sum_d(double v) {
+  v = row16_sum(v);
+  return (lane_read_d(v, 0) + lane_read_d(v, 16)) + (lane_read_d(v, 32) + lane_read_d(v, 48));
+}
+
+// Whether one of the sequence's first `n` drafts is missing; the whole wave takes part.
+__device__ __forceinline__ bool draft_ends_before(const VerifyArgs& a, int64_t b, int n) {
+  const int lane = threadIdx.x & 63;
+  for (int k = 0; k < n; k += 64)
+    if (__any(k + lane < n && draft_at(a, b, k + lane) < 0)) return true;
+  return false;
+}
+
 // ---- 1: chunks -----------------------------------------------------------------------
 
-template <class Tag>
+template <class Tag, int NS>
 __global__ __launch_bounds__(kVT) void verify_stats_kernel(VerifyArgs a, Ws ws) {
-  constexpr int EPV = Pack16<Tag>::EPV, NS = kChunk / (kVT * EPV);
-  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
-  const int64_t id = blockIdx.x;
-  const int chunk = (int)(id % a.chunks);
-  const int64_t rid = id / a.chunks, b = rid / a.rows;
+  constexpr int EPV = Pack16<Tag>::EPV;
+  const int lane = threadIdx.x & 63;
+  const uint32_t id = __builtin_amdgcn_readfirstlane(blockIdx.x * (kVT / 64) + (threadIdx.x >> 6));
+  const uint32_t rid = id / a.chunks, chunk = id % a.chunks;
+  const int64_t b = rid / a.rows;
   const int r = (int)(rid % a.rows);
+  if (b >= a.B) return;
   // target row j serves only if the j drafts before it exist, draft row j also its own
   const bool is_draft = r > a.K;
   const int j = is_draft ? r - (int)a.K - 1 : r;
-  for (int k = 0; k < j + (is_draft ? 1 : 0); ++k)
-    if (draft_at(a, b, k) < 0) return;
   const char* row = is_draft ? draft_row<Tag>(a, b, j) : target_row<Tag>(a, b, j);
-
-  float x[NS][EPV];
-  const int64_t lo = (int64_t)chunk * kChunk + t * EPV;
+  const int64_t lo = (int64_t)chunk * (NS * 64 * EPV) + lane * EPV;
+  u32x4 raw[NS];
+  const bool whole = (int64_t)(chunk + 1) * (NS * 64 * EPV) <= a.V;
+  if (whole) {
 #pragma unroll
-  for (int s = 0; s < NS; ++s) load_entries<Tag>(row, lo + s * kVT * EPV, a.V, x[s]);
-  float m = -M<float>::inf();
-  bool bad = false;
+    for (int s = 0; s < NS; ++s)
+      raw[s] = reinterpret_cast<const Any16*>(row + (lo + s * 64 * EPV) * (16 / EPV))->v;
+  }
+  if (draft_ends_before(a, b, j + (is_draft ? 1 : 0))) return;
+  if (!whole) {
 #pragma unroll
-  for (int s = 0; s < NS; ++s)
-#pragma unroll
-    for (int k = 0; k < EPV; ++k) {
-      m = fmaxf(m, x[s][k]);
-      bad |= !(x[s][k] < M<float>::inf());  // NaN or +inf
+    for (int s = 0; s < NS; ++s) {
+      float x[EPV];
+      load_entries<Tag>(row, lo + s * 64 * EPV, a.V, x);
+      raw[s] = Pack16<Tag>::pack(x);
     }
-  if (bad) m = M<float>::inf();
-  __shared__ float sm[kVT / 64];
-  __shared__ double ss[kVT / 64];
-  __shared__ int sat[kVT / 64];
+  }
+  float m = -M<float>::inf();
+  bool nan = false;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    float x[EPV];
+    Pack16<Tag>::unpack(raw[s], x);
+#pragma unroll
+    for (int k = 0; k < EPV; k += 2) {
+      m = fmaxf(m, fmaxf(x[k], x[k + 1]));
+      nan |= __builtin_isunordered(x[k], x[k + 1]);
+    }
+  }
   m = wave_max_dpp(m);
-  if (lane == 0) sm[wv] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  if (__any(nan)) m = M<float>::inf();
   int at = 0x7fffffff;
   double sum = 0.0;
   if (m > -M<float>::inf() && m < M<float>::inf()) {
+    const double md = m;
+    double part[2] = {0.0, 0.0};
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
+    for (int s = 0; s < NS; ++s) {
+      float x[EPV];
+      Pack16<Tag>::unpack(raw[s], x);
 #pragma unroll
-      for (int k = 0; k < EPV; ++k) sum += exp2_neg(((double)x[s][k] - (double)m) * a.c);
+      for (int k = 0; k < EPV; ++k) part[k & 1] += exp2_clamped(((double)x[k] - md) * a.c);
+    }
+    sum = wave_sum_d(part[0] + part[1]);
     if (a.greedy) {
 #pragma unroll
-      for (int s = NS - 1; s >= 0; --s)
+      for (int s = NS - 1; s >= 0; --s) {
+        float x[EPV];
+        Pack16<Tag>::unpack(raw[s], x);
 #pragma unroll
         for (int k = EPV - 1; k >= 0; --k)
-          if (x[s][k] == m) at = (int)(lo + s * kVT * EPV + k);
+          if (x[k] == m) at = (int)(lo + s * 64 * EPV + k);
+      }
+      at = wave_min_dpp(at);
     }
   }
-  sum = wave_sum(sum);
-  at = wave_min_dpp(at);
-  if (lane == 0) {
-    ss[wv] = sum;
-    sat[wv] = at;
-  }
-  __syncthreads();
-  if (t == 0)
-    ws.stat[id] = ChunkStat{(ss[0] + ss[1]) + (ss[2] + ss[3]), m,
-                            min(min(sat[0], sat[1]), min(sat[2], sat[3]))};
+  if (lane == 0) ws.stat[id] = ChunkStat{sum, m, at};
 }
 
-// ---- 2: rows, and how far the draft is accepted -----------------------------------------
+// ---- 2: rows, how far the draft is accepted, and the rest's chunks ------------------------
 
-// Joins the chunks of one row; the whole wave takes part.
+// Joins the chunks of one row; 16 lanes take part.
 __device__ __forceinline__ RowStat join_row(const ChunkStat* st, int chunks, double c) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 15;
   float m = -M<float>::inf();
-  for (int k = lane; k < chunks; k += 64) m = fmaxf(m, st[k].m);
-  m = wave_max_dpp(m);
+  for (int k = lane; k < chunks; k += 16) m = fmaxf(m, st[k].m);
+  m = row16_max(m);
   double s = 0.0;
   int at = 0x7fffffff;
   if (m == -M<float>::inf()) m = M<float>::inf();  // nothing is possible: no distribution
   if (m < M<float>::inf())
-    for (int k = lane; k < chunks; k += 64) {
+    for (int k = lane; k < chunks; k += 16) {
       s += st[k].s * exp2_neg(((double)st[k].m - (double)m) * c);
       if (st[k].m == m) at = min(at, st[k].at);
     }
-  return RowStat{wave_sum(s), m, wave_min_dpp(at)};
+  return RowStat{row16_sum(s), m, row16_min(at)};
 }
-
-template <class Tag>
-__global__ __launch_bounds__(kVT) void verify_decide_kernel(VerifyArgs a, Ws ws) {
-  const int64_t b = blockIdx.x;
-  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
-  __shared__ int sh_len, sh_n, sh_rest;
-  if (t == 0) {
-    int len = 0;
-    while (len < a.K && draft_at(a, b, len) >= 0) ++len;
-    sh_len = len;
-    sh_n = len;
-    sh_rest = REST_P;
-  }
-  __syncthreads();
-  const int L = sh_len;
-  const bool has_q = a.y != nullptr;
-  RowStat* row = ws.row + b * a.rows;
-  for (int r = wv; r < a.rows; r += kVT / 64) {
-    const bool is_draft = r > a.K;
-    if (is_draft ? r - (int)a.K - 1 >= L : r > L) continue;
-    const RowStat s = join_row(ws.stat + (b * a.rows + r) * a.chunks, a.chunks, a.c);
-    if (lane == 0) row[r] = s;
-  }
-  __syncthreads();
-  // positions in turn, kVT at a time: the first that does not accept its draft
-  for (int j0 = 0; j0 < L && sh_n == L; j0 += kVT) {
-    const int j = j0 + t;
-    int rest = -1;
-    if (j < L) {
-      const RowStat p = row[j];
-      const int64_t d = draft_at(a, b, j);
-      if (!(p.m < M<float>::inf()) || d >= a.V) {
-        rest = REST_BAD;
-      } else if (a.greedy) {
-        if (d != p.at) rest = REST_P;
-      } else {
-        const double px =
-            exp2_neg(((double)load_entry<Tag>(target_row<Tag>(a, b, j), d) - (double)p.m) * a.c) / p.s;
-        double qx = 1.0;
-        bool bad = false;
-        if (has_q) {
-          const RowStat q = row[a.K + 1 + j];
-          bad = !(q.m < M<float>::inf());
-          if (!bad)
-            qx = exp2_neg(((double)load_entry<Tag>(draft_row<Tag>(a, b, j), d) - (double)q.m) * a.c) /
-                 q.s;
-        }
-        if (bad) rest = REST_BAD;
-        else if (!((double)a.u[b * (a.K + 1) + j] * qx < px))
-          rest = has_q ? REST_PQ : REST_P_WITHOUT_DRAFT;
-      }
-    }
-    __syncthreads();
-    if (rest >= 0) atomicMin(&sh_n, j);
-    __syncthreads();
-    if (rest >= 0 && sh_n == j) sh_rest = rest;
-    __syncthreads();
-  }
-  if (t == 0) {
-    if (sh_n == L && !(row[L].m < M<float>::inf())) sh_rest = REST_BAD;
-    ws.plan[b] = Plan{sh_n, sh_rest};
-  }
-}
-
-// ---- 3 and 4: the last token -------------------------------------------------------------
 
 // What an entry of the deciding row weighs.
 template <class Tag>
@@ -291,15 +281,15 @@ struct Rest {
   int64_t skip;              // an entry without mass (the rejected draft), or -1
   __device__ __forceinline__ void weights(int64_t i, int64_t V, double (&w)[Pack16<Tag>::EPV]) const {
     constexpr int EPV = Pack16<Tag>::EPV;
-    float v[EPV];
+    float v[EPV], d[EPV];
     load_entries<Tag>(x, i, V, v);
+    if (y) load_entries<Tag>(y, i, V, d);
 #pragma unroll
     for (int k = 0; k < EPV; ++k) w[k] = exp2_neg(((double)v[k] - mp) * c) * ip;
     if (y) {
-      load_entries<Tag>(y, i, V, v);
 #pragma unroll
       for (int k = 0; k < EPV; ++k)
-        w[k] = fmax(w[k] - exp2_neg(((double)v[k] - mq) * c) * iq, 0.0);
+        w[k] = fmax(w[k] - exp2_neg(((double)d[k] - mq) * c) * iq, 0.0);
     }
 #pragma unroll
     for (int k = 0; k < EPV; ++k)
@@ -308,12 +298,12 @@ struct Rest {
 };
 
 template <class Tag>
-__device__ __forceinline__ Rest<Tag> rest_of(const VerifyArgs& a, const Ws& ws, int64_t b, int n,
-                                             int kind) {
-  const RowStat p = ws.row[b * a.rows + n];
+__device__ __forceinline__ Rest<Tag> rest_of(const VerifyArgs& a, const RowStat* row, int64_t b,
+                                             int n, int kind) {
+  const RowStat p = row[n];
   Rest<Tag> r{target_row<Tag>(a, b, n), nullptr, p.m, 0.0, 1.0 / p.s, 0.0, a.c, -1};
   if (kind == REST_PQ) {
-    const RowStat q = ws.row[b * a.rows + a.K + 1 + n];
+    const RowStat q = row[a.K + 1 + n];
     r.y = draft_row<Tag>(a, b, n);
     r.mq = q.m;
     r.iq = 1.0 / q.s;
@@ -323,28 +313,94 @@ __device__ __forceinline__ Rest<Tag> rest_of(const VerifyArgs& a, const Ws& ws, 
   return r;
 }
 
+// Position j's verdict: -1 (accepted), or what the next token is drawn from.
 template <class Tag>
-__global__ __launch_bounds__(kVT) void verify_rest_kernel(VerifyArgs a, Ws ws) {
-  constexpr int EPV = Pack16<Tag>::EPV, NS = kChunk / (kVT * EPV);
-  const int64_t b = blockIdx.x / a.chunks;
-  const int chunk = (int)(blockIdx.x % a.chunks), t = threadIdx.x;
-  const Plan pl = ws.plan[b];
-  if (pl.rest != REST_PQ && pl.rest != REST_P_WITHOUT_DRAFT) return;
-  const Rest<Tag> r = rest_of<Tag>(a, ws, b, pl.n, pl.rest);
+__device__ __forceinline__ int judge(const VerifyArgs& a, const RowStat* row, int64_t b, int j) {
+  const RowStat p = row[j];
+  const int64_t d = draft_at(a, b, j);
+  if (!(p.m < M<float>::inf()) || d >= a.V) return REST_BAD;
+  if (a.greedy) return d == p.at ? -1 : REST_P;
+  double qx = 1.0;
+  if (a.y) {
+    const RowStat q = row[a.K + 1 + j];
+    if (!(q.m < M<float>::inf())) return REST_BAD;
+    qx = exp2_neg(((double)load_entry<Tag>(draft_row<Tag>(a, b, j), d) - (double)q.m) * a.c) / q.s;
+  }
+  const double px =
+      exp2_neg(((double)load_entry<Tag>(target_row<Tag>(a, b, j), d) - (double)p.m) * a.c) / p.s;
+  if ((double)a.u[b * (a.K + 1) + j] * qx < px) return -1;
+  return a.y ? REST_PQ : REST_P_WITHOUT_DRAFT;
+}
+
+constexpr int kRowsHeld = 64;  // rows whose statistics a workgroup keeps in LDS
+
+template <class Tag, int NS>
+__global__ __launch_bounds__(kVT) void verify_rest_kernel(VerifyArgs a, Ws ws, int groups) {
+  constexpr int EPV = Pack16<Tag>::EPV;
+  const int64_t b = blockIdx.x / groups;
+  const int group = (int)(blockIdx.x % groups), t = threadIdx.x, lane = t & 63;
+  __shared__ int sh_len, sh_n, sh_rest;
+  __shared__ RowStat held[kRowsHeld];
+  if (t < 64) {
+    int len = (int)a.K;
+    for (int k = 0; k < a.K; k += 64) {
+      const uint64_t gone = __ballot(k + lane < a.K && draft_at(a, b, k + lane) < 0);
+      if (gone) {
+        len = k + __ffsll((unsigned long long)gone) - 1;
+        break;
+      }
+    }
+    if (t == 0) {
+      sh_len = sh_n = len;
+      sh_rest = REST_P;
+    }
+  }
+  __syncthreads();
+  const int L = sh_len;
+  // a workgroup's own copy, in LDS or, for long drafts, in the workspace: groups
+  // then write equal values
+  RowStat* row = a.rows <= kRowsHeld ? held : ws.row + b * a.rows;
+  for (int r = t / 16; r < a.rows; r += kVT / 16) {
+    const bool is_draft = r > a.K;
+    if (is_draft ? r - (int)a.K - 1 >= L : r > L) continue;
+    const RowStat s = join_row(ws.stat + (b * a.rows + r) * a.chunks, a.chunks, a.c);
+    if ((t & 15) == 0) {
+      row[r] = s;
+      if (group == 0) ws.row[b * a.rows + r] = s;
+    }
+  }
+  __syncthreads();
+  // positions in turn, kVT at a time: the first that does not accept its draft
+  for (int j0 = 0; j0 < L && sh_n == L; j0 += kVT) {
+    const int j = j0 + t;
+    const int rest = j < L ? judge<Tag>(a, row, b, j) : -1;
+    __syncthreads();
+    if (rest >= 0) atomicMin(&sh_n, j);
+    __syncthreads();
+    if (rest >= 0 && sh_n == j) sh_rest = rest;
+    __syncthreads();
+  }
+  const int n = sh_n;
+  int kind = sh_rest;
+  if (n == L && !(row[L].m < M<float>::inf())) kind = REST_BAD;
+  if (group == 0 && t == 0) ws.plan[b] = Plan{n, kind};
+  if (kind != REST_PQ && kind != REST_P_WITHOUT_DRAFT) return;
+  const int chunk = group * (kVT / 64) + (t >> 6);
+  if (chunk >= a.chunks) return;
+  const Rest<Tag> r = rest_of<Tag>(a, row, b, n, kind);
   double sum = 0.0;
-#pragma unroll
+#pragma unroll 2
   for (int s = 0; s < NS; ++s) {
     double w[EPV];
-    r.weights((int64_t)chunk * kChunk + (s * kVT + t) * EPV, a.V, w);
+    r.weights((int64_t)chunk * (NS * 64 * EPV) + (s * 64 + lane) * EPV, a.V, w);
 #pragma unroll
     for (int k = 0; k < EPV; ++k) sum += w[k];
   }
-  __shared__ double ss[kVT / 64];
-  sum = wave_sum(sum);
-  if ((t & 63) == 0) ss[t >> 6] = sum;
-  __syncthreads();
-  if (t == 0) ws.mass[blockIdx.x] = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+  sum = wave_sum_d(sum);
+  if (lane == 0) ws.mass[b * a.chunks + chunk] = sum;
 }
+
+// ---- 3: the last token -------------------------------------------------------------------
 
 // Inclusive running sum over the workgroup; total to every thread.
 __device__ __forceinline__ double block_scan(double v, double& total, double* sh) {
@@ -366,80 +422,76 @@ __device__ __forceinline__ double block_scan(double v, double& total, double* sh
   }
   return before + v;
 }
+// Least value over the workgroup.
+__device__ __forceinline__ int block_min(int v, int* sh) {
+  v = wave_min_dpp(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return min(min(sh[0], sh[1]), min(sh[2], sh[3]));
+}
 
 template <class Tag>
 __global__ __launch_bounds__(kVT) void verify_draw_kernel(VerifyArgs a, Ws ws) {
-  constexpr int EPV = Pack16<Tag>::EPV, NS = kChunk / (kVT * EPV);
+  constexpr int EPV = Pack16<Tag>::EPV;
+  constexpr int kNone = 0x7fffffff;
   const int64_t b = blockIdx.x;
   const int t = threadIdx.x;
   const Plan pl = ws.plan[b];
   const int n = pl.n;
   const RowStat* rows = ws.row + b * a.rows;
   __shared__ double sh[kVT / 64];
-  __shared__ int first, last;  // chunk, then entry within the chunk
+  __shared__ int shi[kVT / 64];
   __shared__ double sh_rem;
   int64_t token = -1;
   if (pl.rest != REST_BAD && a.greedy) {
     token = rows[n].at;
   } else if (pl.rest != REST_BAD) {
     const double u = a.u[b * (a.K + 1) + a.K];
-    int kind = pl.rest;
-    double total = 0.0;
-    if (kind != REST_P) {
-      double v = 0.0;
-      for (int k = t; k < a.chunks; k += kVT) v += ws.mass[b * a.chunks + k];
-      block_scan(v, total, sh);
-      if (!(total > 0.0)) kind = REST_P;  // the two rows are equal to within rounding
-    }
-    const Rest<Tag> r = rest_of<Tag>(a, ws, b, n, kind);
     const ChunkStat* st = ws.stat + (b * a.rows + n) * a.chunks;
+    const RowStat p = rows[n];
+    int kind = pl.rest;
     auto chunk_mass = [&](int k) {
       if (k >= a.chunks) return 0.0;
       if (kind != REST_P) return ws.mass[b * a.chunks + k];
-      return st[k].s * exp2_neg(((double)st[k].m - r.mp) * a.c) * r.ip;
+      return st[k].s * exp2_neg(((double)st[k].m - (double)p.m) * a.c) / p.s;
     };
-    if (kind == REST_P) {
-      double v = 0.0;
+    auto whole_mass = [&]() {
+      double v = 0.0, total;
       for (int k = t; k < a.chunks; k += kVT) v += chunk_mass(k);
       block_scan(v, total, sh);
+      return total;
+    };
+    double total = whole_mass();
+    if (!(total > 0.0)) {  // the two rows are equal to within rounding
+      kind = REST_P;
+      total = whole_mass();
     }
-    const double border = u * total;
     // the first chunk whose running sum passes the border, else the last with any mass
-    if (t == 0) {
-      first = 0x7fffffff;
-      last = -1;
-    }
+    const double border = u * total;
     double before = 0.0;
-    __syncthreads();
-    for (int k0 = 0; k0 < a.chunks; k0 += kVT) {
+    int chunk = kNone, last = kNone;  // last: negated
+    for (int k0 = 0; k0 < a.chunks && chunk == kNone; k0 += kVT) {
       const double w = chunk_mass(k0 + t);
       double sum;
       const double incl = block_scan(w, sum, sh) + before;
-      if (w > 0.0) {
-        atomicMax(&last, k0 + t);
-        if (incl > border) atomicMin(&first, k0 + t);
-      }
-      __syncthreads();
-      if (first == k0 + t) sh_rem = border - (incl - w);
+      chunk = block_min(w > 0.0 && incl > border ? k0 + t : kNone, shi);
+      last = min(last, block_min(w > 0.0 ? -(k0 + t) : kNone, shi));
+      if (chunk == k0 + t) sh_rem = border - (incl - w);
       before += sum;
-      __syncthreads();
-      if (first != 0x7fffffff) break;
     }
-    const bool over = first == 0x7fffffff;
-    const int chunk = over ? last : first;
+    __syncthreads();
+    const bool over = chunk == kNone;
+    if (over) chunk = -last;
     const double rem = over ? M<double>::inf() : sh_rem;
-    __syncthreads();
-    if (t == 0) {
-      first = 0x7fffffff;
-      last = -1;
-    }
+    const Rest<Tag> r = rest_of<Tag>(a, rows, b, n, kind);
+    int first = kNone;
+    last = kNone;
     before = 0.0;
-    __syncthreads();
-#pragma unroll 1
-    for (int s = 0; s < NS; ++s) {
-      double w[EPV], mine = 0.0, sum;
-      const int e0 = (s * kVT + t) * EPV;
-      r.weights((int64_t)chunk * kChunk + e0, a.V, w);
+    for (int e = 0; e < a.chunk; e += kVT * EPV) {
+      const int e0 = e + t * EPV;
+      double w[EPV] = {}, mine = 0.0, sum;
+      if (e0 < a.chunk) r.weights((int64_t)chunk * a.chunk + e0, a.V, w);
 #pragma unroll
       for (int k = 0; k < EPV; ++k) mine += w[k];
       double at = block_scan(mine, sum, sh) - mine + before;
@@ -447,14 +499,15 @@ __global__ __launch_bounds__(kVT) void verify_draw_kernel(VerifyArgs a, Ws ws) {
       for (int k = 0; k < EPV; ++k) {
         at += w[k];
         if (w[k] > 0.0) {
-          atomicMax(&last, e0 + k);
-          if (at > rem) atomicMin(&first, e0 + k);
+          last = min(last, -(e0 + k));
+          if (at > rem) first = min(first, e0 + k);
         }
       }
       before += sum;
     }
-    __syncthreads();
-    token = (int64_t)chunk * kChunk + (first != 0x7fffffff ? first : last);
+    first = block_min(first, shi);
+    last = block_min(last, shi);
+    token = (int64_t)chunk * a.chunk + (first != kNone ? first : -last);
   }
   // the accepted drafts, the last token, and nothing behind it
   for (int64_t j = t; j <= a.K; j += kVT) {
@@ -476,15 +529,22 @@ __global__ __launch_bounds__(kVT) void verify_draw_kernel(VerifyArgs a, Ws ws) {
 
 // ---- host ---------------------------------------------------------------------------------
 
+// Entries of a chunk: 1024 while that leaves every SIMD a few waves to hide loads
+// behind, 4096 beyond, where its longer sums cost less.
+inline int chunk_entries(int64_t rows, int64_t V) {
+  return rows * ((V + 1023) / 1024) <= 4096 ? 1024 : 4096;
+}
+
 struct VerifyLayout {
-  int rows;
+  int rows, chunk;
   int64_t chunks;
   size_t stat, row, mass, plan, total;
 };
 inline VerifyLayout verify_layout(int64_t B, int64_t K, int64_t V, bool with_draft) {
   VerifyLayout l;
   l.rows = (int)(K + 1 + (with_draft ? K : 0));
-  l.chunks = (V + kChunk - 1) / kChunk;
+  l.chunk = chunk_entries(B * l.rows, V);
+  l.chunks = (V + l.chunk - 1) / l.chunk;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -499,27 +559,30 @@ inline VerifyLayout verify_layout(int64_t B, int64_t K, int64_t V, bool with_dra
   return l;
 }
 
-template <class Tag>
+template <class Tag, int CHUNK>
 int launch_verify(const VerifyArgs& a, const Ws& ws, hipStream_t st) {
-  const uint32_t B = (uint32_t)a.B;
-  hipLaunchKernelGGL(verify_stats_kernel<Tag>, dim3(B * a.rows * a.chunks), dim3(kVT), 0, st, a, ws);
+  constexpr int kWaves = kVT / 64, NS = CHUNK / (64 * Pack16<Tag>::EPV);
+  const uint32_t B = (uint32_t)a.B, waves = B * a.rows * a.chunks;
+  const uint32_t groups = a.greedy ? 1 : (uint32_t)(a.chunks + kWaves - 1) / kWaves;
+  hipLaunchKernelGGL((verify_stats_kernel<Tag, NS>), dim3((waves + kWaves - 1) / kWaves), dim3(kVT), 0,
+                     st, a, ws);
   if (int rc = check_launch("verify_stats_kernel")) return rc;
-  hipLaunchKernelGGL(verify_decide_kernel<Tag>, dim3(B), dim3(kVT), 0, st, a, ws);
-  if (int rc = check_launch("verify_decide_kernel")) return rc;
-  if (!a.greedy) {
-    hipLaunchKernelGGL(verify_rest_kernel<Tag>, dim3(B * a.chunks), dim3(kVT), 0, st, a, ws);
-    if (int rc = check_launch("verify_rest_kernel")) return rc;
-  }
+  hipLaunchKernelGGL((verify_rest_kernel<Tag, NS>), dim3(B * groups), dim3(kVT), 0, st, a, ws,
+                     (int)groups);
+  if (int rc = check_launch("verify_rest_kernel")) return rc;
   hipLaunchKernelGGL(verify_draw_kernel<Tag>, dim3(B), dim3(kVT), 0, st, a, ws);
   return check_launch("verify_draw_kernel");
+}
+template <class Tag>
+int launch_verify(const VerifyArgs& a, const Ws& ws, hipStream_t st) {
+  return a.chunk == 1024 ? launch_verify<Tag, 1024>(a, ws, st) : launch_verify<Tag, 4096>(a, ws, st);
 }
 
 // Sizes whose index arithmetic and grids fit (a grid's threads are counted in 32 bits).
 inline bool verify_fits(int64_t B, int64_t K, int64_t V) {
-  if (B < 0 || K < 0 || V < 1 || B > (1 << 20) || K > (1 << 16) || V > ((int64_t)1 << 31) - kChunk)
+  if (B < 0 || K < 0 || V < 1 || B > (1 << 20) || K > (1 << 16) || V > ((int64_t)1 << 31) - 4096)
     return false;
-  const int64_t chunks = (V + kChunk - 1) / kChunk;
-  return B * (2 * K + 1) <= (((int64_t)1 << 32) / kVT - 1) / chunks;
+  return B * (2 * K + 1) <= ((int64_t)1 << 25) / ((V + 4095) / 4096);
 }
 
 }  // namespace
@@ -546,7 +609,7 @@ extern "C" int rrl_verify_drafts(const void* target, const void* draft, int32_t 
   if (B == 0) return RRL_OK;
   RRL_REQUIRE(V >= 1, RRL_EINVAL, "rrl_verify_drafts: logits need at least one vocabulary entry");
   RRL_REQUIRE(verify_fits(B, K, V), RRL_EINVAL,
-              "rrl_verify_drafts: too large (rows * chunks of 4096 entries below 2^24)");
+              "rrl_verify_drafts: too large (2^25 chunks of 4096 entries)");
   RRL_REQUIRE(temperature == temperature && temperature < HUGE_VAL, RRL_EINVAL,
               "rrl_verify_drafts: the temperature must be a finite number");
   const bool greedy = !do_sample || temperature <= 0.0;
@@ -584,6 +647,7 @@ extern "C" int rrl_verify_drafts(const void* target, const void* draft, int32_t 
   a.greedy = greedy;
   a.rows = l.rows;
   a.chunks = (int)l.chunks;
+  a.chunk = l.chunk;
   a.token_out = token_out;
   a.count_out = count_out;
   a.logp_out = logp_out;
