@@ -17,9 +17,9 @@
 //
 // Rows are cut into chunks, a wave each, so that a single sequence fills the chip:
 //   1. verify_stats: the chunks of every row that may be needed: maximum, sum
-//   2. verify_rest: joins the rows' chunks and finds n (every workgroup for itself,
-//      which is shorter than another launch), then, after a rejection, the mass of
-//      rest in each chunk of row n
+//   2. verify_rest: joins the rows' chunks and finds n (few sequences: every workgroup
+//      for itself, which is shorter than the launch of verify_decide ahead of it),
+//      then, after a rejection, the mass of rest in each part of row n
 //   3. verify_draw: a workgroup per sequence finds the chunk, then the entry
 #include "slab_common.hpp"
 
@@ -27,6 +27,7 @@ namespace rrl {
 namespace {
 
 constexpr int kVT = 256;        // threads of a workgroup
+constexpr int kMass = 1024;     // entries whose rest is summed by a wave
 
 // 2^r for |r| <= 1/2: the polynomial through 2^r at the nine Chebyshev nodes of
 // that interval, within 1.1e-12 of it, relative.
@@ -42,19 +43,67 @@ __device__ __forceinline__ double exp2_poly(double r) {
   return fma(p, r, 1.0);
 }
 
-// 2^max(t, -1000) for t <= 0: beside a maximum of 1 what is below counts for
-// nothing.  Adding 1.5 2^52 rounds t to a whole number, which the sum's low word
-// then holds, and the exponent field takes it as it is.
-__device__ __forceinline__ double exp2_clamped(double t) {
-  t = fmax(t, -1000.0);
-  const double whole = t + 0x1.8p52;
-  const double p = exp2_poly(t - (whole - 0x1.8p52));
+// Weights below this count as none.
+constexpr double kNothing = 0x1p-960;
+
+// Takes a whole number n, held in the low word of 1.5 2^52 + n, as an exponent.
+__device__ __forceinline__ double with_exponent(double p, double whole) {
   return __hiloint2double(__double2hiint(p) + (int)((uint32_t)__double2loint(whole) << 20),
                           __double2loint(p));
 }
 
-// The same with 0 below -1000, so that what is impossible weighs nothing.
-__device__ __forceinline__ double exp2_neg(double t) { return t > -1000.0 ? exp2_clamped(t) : 0.0; }
+// 2^max(t, -1000) for t <= 0.
+__device__ __forceinline__ double exp2_neg(double t) {
+  t = fmax(t, -1000.0);
+  const double whole = t + 0x1.8p52;
+  return with_exponent(exp2_poly(t - (whole - 0x1.8p52)), whole);
+}
+
+// max(a, b) of numbers that are not NaN: one instruction, where fmaxf spends a
+// second on quieting its operand.
+__device__ __forceinline__ float max2(float a, float b) {
+  return __builtin_amdgcn_fmed3f(a, b, M<float>::inf());
+}
+
+// k 2^(c (x - m)) for the entries x <= m of a row.  With i = rint(c m), and x
+// lifted to where its weight is 2^-1000 (so are impossible entries, -inf),
+//   w = 1.5 2^52 - i + c x    holds rint(c x) - i in its low word
+//   r = c x - rint(c x)       one fma, exact but for its rounding
+// so an entry takes no reduction by its own maximum: 2^(i - c m) goes into k.
+// Outside the range of that (c m past 2^20, or c so small that no float weighs
+// 2^-1000) c (x - m) is formed first.
+struct Weight {
+  double c, scale, k, m, magic;  // k: scale 2^(i - c m)
+  float least;
+  bool direct;
+  __device__ __forceinline__ Weight() {}
+  __device__ __forceinline__ Weight(float max, double c_, double scale_)
+      : c(c_), scale(scale_), k(scale_), m(max), magic(0x1.8p52) {
+    const double mc = m * c, low = m - 1000.0 / c;
+    direct = fabs(mc) < 0x1p20 && low > -3e38;
+    least = (float)low;
+    if (direct) {
+      const double i = rint(mc);
+      magic -= i;
+      k *= exp2_poly(fma(-m, c, i));
+    }
+  }
+  template <bool DIRECT>
+  __device__ __forceinline__ double factor() const { return DIRECT ? k : scale; }
+  template <bool DIRECT>
+  __device__ __forceinline__ double unscaled(float x) const {
+    if constexpr (DIRECT) {
+      const double v = max2(x, least);
+      const double whole = fma(v, c, magic);
+      return with_exponent(exp2_poly(fma(v, c, magic - whole)), whole);
+    } else {
+      return exp2_neg(((double)x - m) * c);
+    }
+  }
+  __device__ __forceinline__ double one(float x) const {
+    return direct ? unscaled<true>(x) * k : unscaled<false>(x) * scale;
+  }
+};
 
 struct VerifyArgs {
   const char *x, *y;            // target, draft logits (y may be null)
@@ -67,7 +116,8 @@ struct VerifyArgs {
   double c;                     // log2(e) / T
   int greedy;
   int rows;                     // rows per sequence: K + 1 target rows, then the draft's
-  int chunks, chunk;            // chunks of a row, and a chunk's entries (1024 or 4096)
+  int chunks, chunk;            // chunks of a row, and a chunk's entries (1024, 2048 or 4096)
+  int masses;                   // parts of kMass entries
   int64_t* token_out;           // [B, K + 1]
   int64_t* count_out;           // [B]
   float* logp_out;              // [B, K + 1]
@@ -91,7 +141,7 @@ struct Plan {
 struct Ws {
   ChunkStat* stat;  // [B, rows, chunks]
   RowStat* row;     // [B, rows]
-  double* mass;     // [B, chunks]
+  double* mass;     // [B, masses]
   Plan* plan;       // [B]
 };
 
@@ -182,6 +232,24 @@ __device__ __forceinline__ bool draft_ends_before(const VerifyArgs& a, int64_t b
 
 // ---- 1: chunks -----------------------------------------------------------------------
 
+template <class Tag, int NS, bool DIRECT>
+__device__ __forceinline__ double weigh(u32x4 (&raw)[NS], const Weight& weight) {
+  constexpr int EPV = Pack16<Tag>::EPV;
+  double part[2] = {0.0, 0.0};
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    // unpacked again here, a slab at a time: values kept since the maximum, or more
+    // slabs in flight, would take registers that more waves make better use of
+    asm volatile("" : "+v"(raw[s]));
+    float x[EPV];
+    Pack16<Tag>::unpack(raw[s], x);
+#pragma unroll
+    for (int k = 0; k < EPV; ++k) part[k & 1] += weight.unscaled<DIRECT>(x[k]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  return (part[0] + part[1]) * weight.factor<DIRECT>();
+}
+
 template <class Tag, int NS>
 __global__ __launch_bounds__(kVT) void verify_stats_kernel(VerifyArgs a, Ws ws) {
   constexpr int EPV = Pack16<Tag>::EPV;
@@ -220,7 +288,8 @@ __global__ __launch_bounds__(kVT) void verify_stats_kernel(VerifyArgs a, Ws ws) 
     Pack16<Tag>::unpack(raw[s], x);
 #pragma unroll
     for (int k = 0; k < EPV; k += 2) {
-      m = fmaxf(m, fmaxf(x[k], x[k + 1]));
+      // with NaN among them the result is not used
+      asm("v_max3_f32 %0, %1, %2, %0" : "+v"(m) : "v"(x[k]), "v"(x[k + 1]));
       nan |= __builtin_isunordered(x[k], x[k + 1]);
     }
   }
@@ -229,21 +298,13 @@ __global__ __launch_bounds__(kVT) void verify_stats_kernel(VerifyArgs a, Ws ws) 
   int at = 0x7fffffff;
   double sum = 0.0;
   if (m > -M<float>::inf() && m < M<float>::inf()) {
-    const double md = m;
-    double part[2] = {0.0, 0.0};
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      float x[EPV];
-      Pack16<Tag>::unpack(raw[s], x);
-#pragma unroll
-      for (int k = 0; k < EPV; ++k) part[k & 1] += exp2_clamped(((double)x[k] - md) * a.c);
-    }
-    sum = wave_sum_d(part[0] + part[1]);
-    if (a.greedy) {
-#pragma unroll
+    const Weight weight(m, a.c, 1.0);
+    sum = weight.direct ? weigh<Tag, NS, true>(raw, weight) : weigh<Tag, NS, false>(raw, weight);
+    sum = wave_sum_d(sum);
+    if (a.greedy) {  // read again: kept, the entries would take registers from sampling
       for (int s = NS - 1; s >= 0; --s) {
         float x[EPV];
-        Pack16<Tag>::unpack(raw[s], x);
+        load_entries<Tag>(row, lo + s * 64 * EPV, a.V, x);
 #pragma unroll
         for (int k = EPV - 1; k >= 0; --k)
           if (x[k] == m) at = (int)(lo + s * 64 * EPV + k);
@@ -256,20 +317,34 @@ __global__ __launch_bounds__(kVT) void verify_stats_kernel(VerifyArgs a, Ws ws) 
 
 // ---- 2: rows, how far the draft is accepted, and the rest's chunks ------------------------
 
-// Joins the chunks of one row; 16 lanes take part.
+// Joins the chunks of one row; 16 lanes take part.  The first kAhead of a lane's
+// chunks are loaded together.
 __device__ __forceinline__ RowStat join_row(const ChunkStat* st, int chunks, double c) {
+  constexpr int kAhead = 10;
   const int lane = threadIdx.x & 15;
+  ChunkStat mine[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const int i = lane + 16 * k;
+    mine[k] = i < chunks ? st[i] : ChunkStat{0.0, -M<float>::inf(), 0x7fffffff};
+  }
   float m = -M<float>::inf();
-  for (int k = lane; k < chunks; k += 16) m = fmaxf(m, st[k].m);
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) m = fmaxf(m, mine[k].m);
+  for (int i = lane + 16 * kAhead; i < chunks; i += 16) m = fmaxf(m, st[i].m);
   m = row16_max(m);
+  if (m == -M<float>::inf()) m = M<float>::inf();  // nothing is possible: no distribution
   double s = 0.0;
   int at = 0x7fffffff;
-  if (m == -M<float>::inf()) m = M<float>::inf();  // nothing is possible: no distribution
-  if (m < M<float>::inf())
-    for (int k = lane; k < chunks; k += 16) {
-      s += st[k].s * exp2_neg(((double)st[k].m - (double)m) * c);
-      if (st[k].m == m) at = min(at, st[k].at);
-    }
+  auto add = [&](const ChunkStat& v) {
+    s += v.s * exp2_neg(((double)v.m - (double)m) * c);
+    if (v.m == m) at = min(at, v.at);
+  };
+  if (m < M<float>::inf()) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) add(mine[k]);
+    for (int i = lane + 16 * kAhead; i < chunks; i += 16) add(st[i]);
+  }
   return RowStat{row16_sum(s), m, row16_min(at)};
 }
 
@@ -277,70 +352,114 @@ __device__ __forceinline__ RowStat join_row(const ChunkStat* st, int chunks, dou
 template <class Tag>
 struct Rest {
   const char *x, *y;
-  double mp, mq, ip, iq, c;  // maxima and 1 / sums
-  int64_t skip;              // an entry without mass (the rejected draft), or -1
+  Weight p, q;
+  int64_t skip;  // an entry without mass (the rejected draft), or -1
+  bool direct;
+  template <bool DIRECT>
   __device__ __forceinline__ void weights(int64_t i, int64_t V, double (&w)[Pack16<Tag>::EPV]) const {
     constexpr int EPV = Pack16<Tag>::EPV;
     float v[EPV], d[EPV];
     load_entries<Tag>(x, i, V, v);
     if (y) load_entries<Tag>(y, i, V, d);
 #pragma unroll
-    for (int k = 0; k < EPV; ++k) w[k] = exp2_neg(((double)v[k] - mp) * c) * ip;
+    for (int k = 0; k < EPV; ++k) w[k] = p.template unscaled<DIRECT>(v[k]) * p.template factor<DIRECT>();
     if (y) {
+      const double f = -q.template factor<DIRECT>();
 #pragma unroll
-      for (int k = 0; k < EPV; ++k)
-        w[k] = fmax(w[k] - exp2_neg(((double)d[k] - mq) * c) * iq, 0.0);
+      for (int k = 0; k < EPV; ++k) w[k] = fmax(fma(f, q.template unscaled<DIRECT>(d[k]), w[k]), 0.0);
     }
 #pragma unroll
     for (int k = 0; k < EPV; ++k)
       if (i + k == skip) w[k] = 0.0;
+  }
+  __device__ __forceinline__ void weights(int64_t i, int64_t V, double (&w)[Pack16<Tag>::EPV]) const {
+    if (direct) weights<true>(i, V, w);
+    else weights<false>(i, V, w);
   }
 };
 
 template <class Tag>
 __device__ __forceinline__ Rest<Tag> rest_of(const VerifyArgs& a, const RowStat* row, int64_t b,
                                              int n, int kind) {
-  const RowStat p = row[n];
-  Rest<Tag> r{target_row<Tag>(a, b, n), nullptr, p.m, 0.0, 1.0 / p.s, 0.0, a.c, -1};
+  Rest<Tag> r;
+  r.x = target_row<Tag>(a, b, n);
+  r.y = nullptr;
+  r.p = Weight(row[n].m, a.c, 1.0 / row[n].s);
+  r.skip = -1;
+  r.direct = r.p.direct;
   if (kind == REST_PQ) {
     const RowStat q = row[a.K + 1 + n];
     r.y = draft_row<Tag>(a, b, n);
-    r.mq = q.m;
-    r.iq = 1.0 / q.s;
+    r.q = Weight(q.m, a.c, 1.0 / q.s);
+    r.direct &= r.q.direct;
   } else if (kind == REST_P_WITHOUT_DRAFT) {
     r.skip = draft_at(a, b, n);
   }
   return r;
 }
 
-// Position j's verdict: -1 (accepted), or what the next token is drawn from.
+// What deciding position j takes from its rows; beyond the draft's end, and
+// where the draft names no entry, only d.
+struct Position {
+  int64_t d;
+  float x, y, u;
+};
 template <class Tag>
-__device__ __forceinline__ int judge(const VerifyArgs& a, const RowStat* row, int64_t b, int j) {
+__device__ __forceinline__ Position position(const VerifyArgs& a, int64_t b, int64_t j) {
+  Position p{-1, 0.0f, 0.0f, 0.0f};
+  if (j >= a.K) return p;
+  p.d = draft_at(a, b, j);
+  if (p.d < 0 || p.d >= a.V || a.greedy) return p;
+  p.x = load_entry<Tag>(target_row<Tag>(a, b, j), p.d);
+  if (a.y) p.y = load_entry<Tag>(draft_row<Tag>(a, b, j), p.d);
+  p.u = a.u[b * (a.K + 1) + j];
+  return p;
+}
+
+// Its verdict: -1 (accepted), or what the next token is drawn from.
+__device__ __forceinline__ int judge(const VerifyArgs& a, const RowStat* row, int64_t j,
+                                     const Position& at) {
   const RowStat p = row[j];
-  const int64_t d = draft_at(a, b, j);
-  if (!(p.m < M<float>::inf()) || d >= a.V) return REST_BAD;
-  if (a.greedy) return d == p.at ? -1 : REST_P;
+  if (!(p.m < M<float>::inf()) || at.d >= a.V) return REST_BAD;
+  if (a.greedy) return at.d == p.at ? -1 : REST_P;
   double qx = 1.0;
   if (a.y) {
     const RowStat q = row[a.K + 1 + j];
     if (!(q.m < M<float>::inf())) return REST_BAD;
-    qx = exp2_neg(((double)load_entry<Tag>(draft_row<Tag>(a, b, j), d) - (double)q.m) * a.c) / q.s;
+    qx = Weight(q.m, a.c, 1.0 / q.s).one(at.y);
+    if (!(qx > kNothing)) qx = 0.0;
   }
-  const double px =
-      exp2_neg(((double)load_entry<Tag>(target_row<Tag>(a, b, j), d) - (double)p.m) * a.c) / p.s;
-  if ((double)a.u[b * (a.K + 1) + j] * qx < px) return -1;
+  double px = Weight(p.m, a.c, 1.0 / p.s).one(at.x);
+  if (!(px > kNothing)) px = 0.0;
+  if ((double)at.u * qx < px) return -1;
   return a.y ? REST_PQ : REST_P_WITHOUT_DRAFT;
+}
+
+template <class Tag, int NS, bool DIRECT>
+__device__ __forceinline__ double rest_sum(const Rest<Tag>& r, int64_t lo, int64_t V) {
+  constexpr int EPV = Pack16<Tag>::EPV;
+  double sum = 0.0;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    double w[EPV];
+    r.template weights<DIRECT>(lo + s * 64 * EPV, V, w);
+#pragma unroll
+    for (int k = 0; k < EPV; ++k) sum += w[k];
+  }
+  return sum;
 }
 
 constexpr int kRowsHeld = 64;  // rows whose statistics a workgroup keeps in LDS
 
-template <class Tag, int NS>
-__global__ __launch_bounds__(kVT) void verify_rest_kernel(VerifyArgs a, Ws ws, int groups) {
-  constexpr int EPV = Pack16<Tag>::EPV;
-  const int64_t b = blockIdx.x / groups;
-  const int group = (int)(blockIdx.x % groups), t = threadIdx.x, lane = t & 63;
+// Joins the sequence's rows and finds its plan; the whole workgroup takes part.
+// The rows' statistics are left in `held`, or, for long drafts, in the workspace,
+// where they go also if `write`.
+template <class Tag>
+__device__ __forceinline__ Plan decide(const VerifyArgs& a, const Ws& ws, int64_t b, bool write,
+                                       RowStat* held, const RowStat*& rows) {
+  const int t = threadIdx.x, lane = t & 63;
   __shared__ int sh_len, sh_n, sh_rest;
-  __shared__ RowStat held[kRowsHeld];
+  Position at = position<Tag>(a, b, t);
   if (t < 64) {
     int len = (int)a.K;
     for (int k = 0; k < a.K; k += 64) {
@@ -357,47 +476,61 @@ __global__ __launch_bounds__(kVT) void verify_rest_kernel(VerifyArgs a, Ws ws, i
   }
   __syncthreads();
   const int L = sh_len;
-  // a workgroup's own copy, in LDS or, for long drafts, in the workspace: groups
-  // then write equal values
+  // in the workspace, the groups of a sequence write equal values
   RowStat* row = a.rows <= kRowsHeld ? held : ws.row + b * a.rows;
+  rows = row;
   for (int r = t / 16; r < a.rows; r += kVT / 16) {
     const bool is_draft = r > a.K;
     if (is_draft ? r - (int)a.K - 1 >= L : r > L) continue;
     const RowStat s = join_row(ws.stat + (b * a.rows + r) * a.chunks, a.chunks, a.c);
     if ((t & 15) == 0) {
       row[r] = s;
-      if (group == 0) ws.row[b * a.rows + r] = s;
+      if (write) ws.row[b * a.rows + r] = s;
     }
   }
   __syncthreads();
   // positions in turn, kVT at a time: the first that does not accept its draft
   for (int j0 = 0; j0 < L && sh_n == L; j0 += kVT) {
     const int j = j0 + t;
-    const int rest = j < L ? judge<Tag>(a, row, b, j) : -1;
+    if (j0 > 0) at = position<Tag>(a, b, j);
+    const int rest = j < L ? judge(a, row, j, at) : -1;
     __syncthreads();
     if (rest >= 0) atomicMin(&sh_n, j);
     __syncthreads();
     if (rest >= 0 && sh_n == j) sh_rest = rest;
     __syncthreads();
   }
-  const int n = sh_n;
-  int kind = sh_rest;
-  if (n == L && !(row[L].m < M<float>::inf())) kind = REST_BAD;
-  if (group == 0 && t == 0) ws.plan[b] = Plan{n, kind};
-  if (kind != REST_PQ && kind != REST_P_WITHOUT_DRAFT) return;
-  const int chunk = group * (kVT / 64) + (t >> 6);
-  if (chunk >= a.chunks) return;
-  const Rest<Tag> r = rest_of<Tag>(a, row, b, n, kind);
-  double sum = 0.0;
-#pragma unroll 2
-  for (int s = 0; s < NS; ++s) {
-    double w[EPV];
-    r.weights((int64_t)chunk * (NS * 64 * EPV) + (s * 64 + lane) * EPV, a.V, w);
-#pragma unroll
-    for (int k = 0; k < EPV; ++k) sum += w[k];
+  Plan pl{sh_n, sh_rest};
+  if (pl.n == L && !(row[L].m < M<float>::inf())) pl.rest = REST_BAD;
+  if (write && t == 0) ws.plan[b] = pl;
+  return pl;
+}
+
+template <class Tag>
+__global__ __launch_bounds__(kVT) void verify_decide_kernel(VerifyArgs a, Ws ws) {
+  __shared__ RowStat held[kRowsHeld];
+  const RowStat* row;
+  decide<Tag>(a, ws, blockIdx.x, true, held, row);
+}
+
+template <class Tag, bool DECIDED>
+__global__ __launch_bounds__(kVT) void verify_rest_kernel(VerifyArgs a, Ws ws, int groups) {
+  constexpr int EPV = Pack16<Tag>::EPV, NS = kMass / (64 * EPV);
+  const int64_t b = blockIdx.x / groups;
+  const int group = (int)(blockIdx.x % groups), t = threadIdx.x, lane = t & 63;
+  __shared__ RowStat held[DECIDED ? 1 : kRowsHeld];
+  const RowStat* row = ws.row + b * a.rows;
+  Plan pl;
+  if constexpr (DECIDED) pl = ws.plan[b];
+  else pl = decide<Tag>(a, ws, b, group == 0, held, row);
+  if (pl.rest != REST_PQ && pl.rest != REST_P_WITHOUT_DRAFT) return;
+  const Rest<Tag> r = rest_of<Tag>(a, row, b, pl.n, pl.rest);
+  for (int part = group * (kVT / 64) + (t >> 6); part < a.masses; part += groups * (kVT / 64)) {
+    const int64_t lo = (int64_t)part * kMass + lane * EPV;
+    double sum = r.direct ? rest_sum<Tag, NS, true>(r, lo, a.V) : rest_sum<Tag, NS, false>(r, lo, a.V);
+    sum = wave_sum_d(sum);
+    if (lane == 0) ws.mass[b * a.masses + part] = sum;
   }
-  sum = wave_sum_d(sum);
-  if (lane == 0) ws.mass[b * a.chunks + chunk] = sum;
 }
 
 // ---- 3: the last token -------------------------------------------------------------------
@@ -450,33 +583,35 @@ __global__ __launch_bounds__(kVT) void verify_draw_kernel(VerifyArgs a, Ws ws) {
     const double u = a.u[b * (a.K + 1) + a.K];
     const ChunkStat* st = ws.stat + (b * a.rows + n) * a.chunks;
     const RowStat p = rows[n];
-    int kind = pl.rest;
-    auto chunk_mass = [&](int k) {
-      if (k >= a.chunks) return 0.0;
-      if (kind != REST_P) return ws.mass[b * a.chunks + k];
+    int kind = pl.rest, parts, size;
+    auto part_mass = [&](int k) {
+      if (k >= parts) return 0.0;
+      if (kind != REST_P) return ws.mass[b * a.masses + k];
       return st[k].s * exp2_neg(((double)st[k].m - (double)p.m) * a.c) / p.s;
     };
     auto whole_mass = [&]() {
+      parts = kind != REST_P ? a.masses : a.chunks;
+      size = kind != REST_P ? kMass : a.chunk;
       double v = 0.0, total;
-      for (int k = t; k < a.chunks; k += kVT) v += chunk_mass(k);
+      for (int k = t; k < parts; k += kVT) v += part_mass(k);
       block_scan(v, total, sh);
       return total;
     };
     double total = whole_mass();
-    if (!(total > 0.0)) {  // the two rows are equal to within rounding
+    if (!(total > kNothing)) {  // the two rows are equal to within rounding
       kind = REST_P;
       total = whole_mass();
     }
-    // the first chunk whose running sum passes the border, else the last with any mass
+    // the first part whose running sum passes the border, else the last with any mass
     const double border = u * total;
     double before = 0.0;
     int chunk = kNone, last = kNone;  // last: negated
-    for (int k0 = 0; k0 < a.chunks && chunk == kNone; k0 += kVT) {
-      const double w = chunk_mass(k0 + t);
+    for (int k0 = 0; k0 < parts && chunk == kNone; k0 += kVT) {
+      const double w = part_mass(k0 + t);
       double sum;
       const double incl = block_scan(w, sum, sh) + before;
-      chunk = block_min(w > 0.0 && incl > border ? k0 + t : kNone, shi);
-      last = min(last, block_min(w > 0.0 ? -(k0 + t) : kNone, shi));
+      chunk = block_min(w > kNothing && incl > border ? k0 + t : kNone, shi);
+      last = min(last, block_min(w > kNothing ? -(k0 + t) : kNone, shi));
       if (chunk == k0 + t) sh_rem = border - (incl - w);
       before += sum;
     }
@@ -488,17 +623,17 @@ __global__ __launch_bounds__(kVT) void verify_draw_kernel(VerifyArgs a, Ws ws) {
     int first = kNone;
     last = kNone;
     before = 0.0;
-    for (int e = 0; e < a.chunk; e += kVT * EPV) {
+    for (int e = 0; e < size; e += kVT * EPV) {
       const int e0 = e + t * EPV;
       double w[EPV] = {}, mine = 0.0, sum;
-      if (e0 < a.chunk) r.weights((int64_t)chunk * a.chunk + e0, a.V, w);
+      if (e0 < size) r.weights((int64_t)chunk * size + e0, a.V, w);
 #pragma unroll
       for (int k = 0; k < EPV; ++k) mine += w[k];
       double at = block_scan(mine, sum, sh) - mine + before;
 #pragma unroll
       for (int k = 0; k < EPV; ++k) {
         at += w[k];
-        if (w[k] > 0.0) {
+        if (w[k] > kNothing) {
           last = min(last, -(e0 + k));
           if (at > rem) first = min(first, e0 + k);
         }
@@ -507,7 +642,7 @@ __global__ __launch_bounds__(kVT) void verify_draw_kernel(VerifyArgs a, Ws ws) {
     }
     first = block_min(first, shi);
     last = block_min(last, shi);
-    token = (int64_t)chunk * a.chunk + (first != kNone ? first : -last);
+    token = (int64_t)chunk * size + (first != kNone ? first : -last);
   }
   // the accepted drafts, the last token, and nothing behind it
   for (int64_t j = t; j <= a.K; j += kVT) {
@@ -529,15 +664,19 @@ __global__ __launch_bounds__(kVT) void verify_draw_kernel(VerifyArgs a, Ws ws) {
 
 // ---- host ---------------------------------------------------------------------------------
 
-// Entries of a chunk: 1024 while that leaves every SIMD a few waves to hide loads
-// behind, 4096 beyond, where its longer sums cost less.
+// Entries of a chunk: as many as leave the 1024 SIMDs enough waves to hide loads
+// behind, for a longer chunk spends less on its sum.  verify_stats took, with 1024 /
+// 2048 / 4096 entries: 13.8 / 14.6 / 17.0 us at 12,950 chunks of 1024 (half of them
+// behind a draft's end), 18.5 / 17.4 / 19.2 us at 19,072, 2048 / 4096: 85 / 81 us at
+// 104,896.
 inline int chunk_entries(int64_t rows, int64_t V) {
-  return rows * ((V + 1023) / 1024) <= 4096 ? 1024 : 4096;
+  const int64_t least = rows * ((V + 1023) / 1024);
+  return least <= 16384 ? 1024 : (least <= 40960 ? 2048 : 4096);
 }
 
 struct VerifyLayout {
   int rows, chunk;
-  int64_t chunks;
+  int64_t chunks, masses;
   size_t stat, row, mass, plan, total;
 };
 inline VerifyLayout verify_layout(int64_t B, int64_t K, int64_t V, bool with_draft) {
@@ -553,7 +692,8 @@ inline VerifyLayout verify_layout(int64_t B, int64_t K, int64_t V, bool with_dra
   };
   l.stat = take(sizeof(ChunkStat) * (size_t)(B * l.rows * l.chunks));
   l.row = take(sizeof(RowStat) * (size_t)(B * l.rows));
-  l.mass = take(sizeof(double) * (size_t)(B * l.chunks));
+  l.masses = (V + kMass - 1) / kMass;
+  l.mass = take(sizeof(double) * (size_t)(B * l.masses));
   l.plan = take(sizeof(Plan) * (size_t)B);
   l.total = at;
   return l;
@@ -563,26 +703,36 @@ template <class Tag, int CHUNK>
 int launch_verify(const VerifyArgs& a, const Ws& ws, hipStream_t st) {
   constexpr int kWaves = kVT / 64, NS = CHUNK / (64 * Pack16<Tag>::EPV);
   const uint32_t B = (uint32_t)a.B, waves = B * a.rows * a.chunks;
-  const uint32_t groups = a.greedy ? 1 : (uint32_t)(a.chunks + kWaves - 1) / kWaves;
+  const uint32_t groups = (uint32_t)(a.masses + kWaves - 1) / kWaves;
   hipLaunchKernelGGL((verify_stats_kernel<Tag, NS>), dim3((waves + kWaves - 1) / kWaves), dim3(kVT), 0,
                      st, a, ws);
   if (int rc = check_launch("verify_stats_kernel")) return rc;
-  hipLaunchKernelGGL((verify_rest_kernel<Tag, NS>), dim3(B * groups), dim3(kVT), 0, st, a, ws,
-                     (int)groups);
+  if (a.greedy || B * groups > 1024) {  // more workgroups than run at once
+    hipLaunchKernelGGL(verify_decide_kernel<Tag>, dim3(B), dim3(kVT), 0, st, a, ws);
+    if (int rc = check_launch("verify_decide_kernel")) return rc;
+    if (!a.greedy)
+      hipLaunchKernelGGL((verify_rest_kernel<Tag, true>), dim3(B * groups), dim3(kVT), 0, st, a, ws,
+                         (int)groups);
+  } else {
+    hipLaunchKernelGGL((verify_rest_kernel<Tag, false>), dim3(B * groups), dim3(kVT), 0, st, a, ws,
+                       (int)groups);
+  }
   if (int rc = check_launch("verify_rest_kernel")) return rc;
   hipLaunchKernelGGL(verify_draw_kernel<Tag>, dim3(B), dim3(kVT), 0, st, a, ws);
   return check_launch("verify_draw_kernel");
 }
 template <class Tag>
 int launch_verify(const VerifyArgs& a, const Ws& ws, hipStream_t st) {
-  return a.chunk == 1024 ? launch_verify<Tag, 1024>(a, ws, st) : launch_verify<Tag, 4096>(a, ws, st);
+  if (a.chunk == 1024) return launch_verify<Tag, 1024>(a, ws, st);
+  if (a.chunk == 2048) return launch_verify<Tag, 2048>(a, ws, st);
+  return launch_verify<Tag, 4096>(a, ws, st);
 }
 
 // Sizes whose index arithmetic and grids fit (a grid's threads are counted in 32 bits).
 inline bool verify_fits(int64_t B, int64_t K, int64_t V) {
   if (B < 0 || K < 0 || V < 1 || B > (1 << 20) || K > (1 << 16) || V > ((int64_t)1 << 31) - 4096)
     return false;
-  return B * (2 * K + 1) <= ((int64_t)1 << 25) / ((V + 4095) / 4096);
+  return B * (2 * K + 1) <= ((int64_t)1 << 23) / ((V + 4095) / 4096);
 }
 
 }  // namespace
@@ -609,7 +759,7 @@ extern "C" int rrl_verify_drafts(const void* target, const void* draft, int32_t 
   if (B == 0) return RRL_OK;
   RRL_REQUIRE(V >= 1, RRL_EINVAL, "rrl_verify_drafts: logits need at least one vocabulary entry");
   RRL_REQUIRE(verify_fits(B, K, V), RRL_EINVAL,
-              "rrl_verify_drafts: too large (2^25 chunks of 4096 entries)");
+              "rrl_verify_drafts: too large (over 2^23 chunks of 4096 entries)");
   RRL_REQUIRE(temperature == temperature && temperature < HUGE_VAL, RRL_EINVAL,
               "rrl_verify_drafts: the temperature must be a finite number");
   const bool greedy = !do_sample || temperature <= 0.0;
@@ -648,6 +798,7 @@ extern "C" int rrl_verify_drafts(const void* target, const void* draft, int32_t 
   a.rows = l.rows;
   a.chunks = (int)l.chunks;
   a.chunk = l.chunk;
+  a.masses = (int)l.masses;
   a.token_out = token_out;
   a.count_out = count_out;
   a.logp_out = logp_out;
