@@ -13,6 +13,8 @@
 #include "rrl_common.hpp"
 #include "slab_common.hpp"
 
+#include <type_traits>
+
 namespace rrl {
 namespace {
 
@@ -72,27 +74,49 @@ __device__ __forceinline__ uint32_t codes8(const float (&x)[8], uint32_t byte) {
   return c;
 }
 
+// Where block `b` of row `r` goes, in units of 16 bytes of codes and bytes of scales.
+// Rows: as MxFp4 keeps them.
+struct RowOrder {
+  uint32_t blocks;
+  __device__ __forceinline__ int64_t codes(int64_t r, uint32_t b) const { return r * blocks + b; }
+  __device__ __forceinline__ int64_t scale(int64_t r, uint32_t b) const { return r * blocks + b; }
+};
+// Fragments: as the product's waves read their activations.  16 rows of 128 entries
+// (a step) are 1 KB, lane 16 (b % 4) + r % 16 after lane; four steps (a stage) of a
+// lane's scales are one dword, which the matrix instruction picks its byte from.
+struct FragmentOrder {
+  uint32_t steps, stages;
+  __device__ __forceinline__ int64_t codes(int64_t r, uint32_t b) const {
+    return ((r >> 4) * steps + (b >> 2)) * 64 + (b & 3) * 16 + (r & 15);
+  }
+  __device__ __forceinline__ int64_t scale(int64_t r, uint32_t b) const {
+    return (((r >> 4) * stages + (b >> 4)) * 64 + (b & 3) * 16 + (r & 15)) * 4 + ((b >> 2) & 3);
+  }
+};
+
 // Four lanes per block, eight entries each.
-template <class Tag>
+template <class Tag, class Order>
 __global__ __launch_bounds__(kQT) void mxfp4_quantize_kernel(const char* __restrict__ x, int64_t R,
                                                              int64_t H, int64_t ld, uint32_t blocks,
+                                                             Order order,
                                                              uint8_t* __restrict__ codes,
                                                              uint8_t* __restrict__ scales) {
   constexpr int SZ = 16 / Pack16<Tag>::EPV;
   const int64_t id = ((int64_t)blockIdx.x * kQT + threadIdx.x) / 4;
   const int part = threadIdx.x & 3;
   if (id >= R * blocks) return;
-  const int64_t r = id / blocks, b = id % blocks;
+  const int64_t r = id / blocks;
+  const uint32_t b = (uint32_t)(id % blocks);
   float v[8];
-  load8<Tag>(x + r * ld * SZ, b * kBlock + part * 8, H, v);
+  load8<Tag>(x + r * ld * SZ, (int64_t)b * kBlock + part * 8, H, v);
   uint32_t m = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
   m = max(m, (uint32_t)dpp_i<kDppXor1>((int)m));
   m = max(m, (uint32_t)dpp_i<kDppXor2>((int)m));
   const uint32_t byte = scale_byte(m);
-  reinterpret_cast<uint32_t*>(codes)[id * 4 + part] = codes8(v, byte);
-  if (part == 0) scales[id] = (uint8_t)byte;
+  reinterpret_cast<uint32_t*>(codes)[order.codes(r, b) * 4 + part] = codes8(v, byte);
+  if (part == 0) scales[order.scale(r, b)] = (uint8_t)byte;
 }
 
 // The value of a code times 2^(byte - 127).
@@ -145,67 +169,176 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // D += A B^T over 128 entries: lane l holds 32 consecutive entries (block l / 16)
-// of row l % 16 of each operand and their scale; it receives rows 4 (l / 16) + i
-// of A, row l % 16 of B.
+// of row l % 16 of each operand, and their scales in byte T of a dword; it receives
+// rows 4 (l / 16) + i of A, row l % 16 of B.
+template <int T>
 __device__ __forceinline__ f32x4 mfma_fp4(const u32x4& a, uint32_t sa, const u32x4& b, uint32_t sb,
                                           const f32x4& c) {
   const i32x8 av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
   const i32x8 bv = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, (int)sa, 0, (int)sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, T, (int)sa, T, (int)sb);
 }
 
-constexpr int kLinWaves = 4;
+constexpr int kLinWaves = 4, kStage = 4;  // steps of 128 entries in a stage
 
-// A wave: VT x 16 weight rows times NT x 16 activation rows.
-template <class Out, int VT, int NT>
-__global__ __launch_bounds__(64 * kLinWaves) void mxfp4_linear_kernel(
-    const uint8_t* __restrict__ ac, const uint8_t* __restrict__ as, int64_t M,
-    const uint8_t* __restrict__ wc, const uint8_t* __restrict__ wsc, int64_t N, int64_t P,
-    char* __restrict__ out) {
-  constexpr int SZ = 16 / Pack16<Out>::EPV;
-  const int lane = threadIdx.x & 63, r16 = lane & 15, blk = lane >> 4;
-  const int64_t n0 = ((int64_t)blockIdx.x * kLinWaves + (threadIdx.x >> 6)) * (16 * VT);
-  const int64_t m0 = (int64_t)blockIdx.y * (16 * NT);
-  if (n0 >= N) return;
-  int64_t wr[VT], ar[NT];  // rows past the end read the last one, and are not stored
+struct LinearArgs {
+  const u32x4* ac;      // activations in fragment order: [fragments, steps, 64]
+  const uint32_t* as;   // [fragments, stages, 64]
+  const uint8_t* wc;    // weight codes [N, P / 2]
+  const uint8_t* ws;    // weight scales [N, P / 32]
+  int64_t M, N;
+  int32_t steps, stages, fragments;
+  int32_t token_tiles;
+  char* out;
+  int32_t out_dtype;
+};
+
+// 8 outputs of one row: 16 bytes at any address, or one by one at the row's end.
+struct __attribute__((packed, aligned(2))) Out16 {
+  u32x4 v;
+};
+template <class Tag>
+__device__ __forceinline__ void store8(char* row, int64_t n, int64_t N, const float (&v)[8]) {
+  constexpr int EPV = Pack16<Tag>::EPV, SZ = 16 / EPV;
+  if (n + 8 <= N) {
 #pragma unroll
-  for (int i = 0; i < VT; ++i) wr[i] = min(n0 + 16 * i + r16, N - 1);
+    for (int p = 0; p < 8 / EPV; ++p) {
+      float w[EPV];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) ar[j] = min(m0 + 16 * j + r16, M - 1);
-  f32x4 acc[VT][NT] = {};
-  for (int64_t k = 0; k < P; k += kDepth) {
-    u32x4 w[VT], a[NT];
-    uint32_t sw[VT], sa[NT];
-    const int64_t kb = k / kBlock + blk;
-#pragma unroll
-    for (int i = 0; i < VT; ++i) {
-      w[i] = *reinterpret_cast<const u32x4*>(wc + wr[i] * (P / 2) + kb * 16);
-      sw[i] = wsc[wr[i] * (P / kBlock) + kb];
+      for (int k = 0; k < EPV; ++k) w[k] = v[p * EPV + k];
+      reinterpret_cast<Out16*>(row + n * SZ + 16 * p)->v = Pack16<Tag>::pack(w);
     }
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      a[j] = *reinterpret_cast<const u32x4*>(ac + ar[j] * (P / 2) + kb * 16);
-      sa[j] = as[ar[j] * (P / kBlock) + kb];
-    }
-#pragma unroll
-    for (int i = 0; i < VT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = mfma_fp4(w[i], sw[i], a[j], sa[j], acc[i][j]);
+    return;
   }
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int64_t m = m0 + 16 * j + r16;
-    if (m >= M) continue;
+  for (int k = 0; k < 8; ++k)
+    if (n + k < N) {
+      if constexpr (SZ == 4) reinterpret_cast<float*>(row)[n + k] = v[k];
+      else reinterpret_cast<uint16_t*>(row)[n + k] = (uint16_t)Pack16<Tag>::pack_one(v[k]);
+    }
+}
+
+// A workgroup: 4 x VT x 16 weight rows (a wave's own VT x 16 each, straight into
+// registers) times NT x 16 activation rows (shared, through LDS a stage ahead).
+// A wave's weight rows are dealt to its fragments so that the 4 x VT outputs a
+// lane receives are runs of 8 neighbours: fragment i, row 4 b + k is weight row
+// 32 (i / 2) + 8 b + 4 (i % 2) + k of the wave's.
+template <int VT, int NT>
+__global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearArgs a) {
+  __shared__ u32x4 lds_c[2][kStage][NT][64];
+  __shared__ uint32_t lds_s[2][NT][64];
+  const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int r16 = lane & 15, blk = lane >> 4;
+  // the tiles of one weight slab follow each other on one XCD (workgroups go to the
+  // eight in turn), so that its L2 reads the slab once
+  const uint32_t xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+  const int64_t slab = (int64_t)(slot / a.token_tiles) * 8 + xcd;
+  const int f0 = (int)(slot % a.token_tiles) * NT;
+  if (slab * (16 * VT * kLinWaves) >= a.N) return;
+  const int64_t n0 = (slab * kLinWaves + wv) * (16 * VT);
+  const int64_t P = (int64_t)a.steps * kDepth;
+
+  // rows and fragments past the end read the last ones, and are not stored
+  const uint8_t* wrow[VT];
+  int srow[VT];
+#pragma unroll
+  for (int i = 0; i < VT; ++i) {
+    const int64_t r =
+        min(n0 + 32 * (i / 2) + 8 * (r16 >> 2) + 4 * (i % 2) + (r16 & 3), a.N - 1);
+    wrow[i] = a.wc + r * (P / 2) + blk * 16;
+    srow[i] = (int)(r * (P / kBlock));
+  }
+  const __amdgpu_buffer_rsrc_t srsrc = row_rsrc(a.ws, (uint32_t)(a.N * (P / kBlock)));
+  const uint32_t sel = (uint32_t)blk | (uint32_t)(4 + blk) << 8;
+
+  u32x4 stage_c[NT];
+  uint32_t stage_s[(NT + kLinWaves - 1) / kLinWaves];
+  auto fetch = [&](int s) {
+    const int step = s * kStage + wv;  // this wave's step of the stage
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int f = min(f0 + j, a.fragments - 1);
+      if (step < a.steps) stage_c[j] = a.ac[((int64_t)f * a.steps + step) * 64 + lane];
+      if (j % kLinWaves == wv) stage_s[j / kLinWaves] = a.as[((int64_t)f * a.stages + s) * 64 + lane];
+    }
+  };
+  auto put = [&](int s) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      lds_c[s & 1][wv][j][lane] = stage_c[j];
+      if (j % kLinWaves == wv) lds_s[s & 1][j][lane] = stage_s[j / kLinWaves];
+    }
+  };
+  u32x4 w[2][VT];
+  auto weights = [&](u32x4 (&dst)[VT], int step) {
+    if (step < a.steps) {
+#pragma unroll
+      for (int i = 0; i < VT; ++i)
+        dst[i] = *reinterpret_cast<const u32x4*>(wrow[i] + (int64_t)step * (kDepth / 2));
+    }
+  };
+  u32x4 sraw[VT];
+  auto scales = [&](int s) {
 #pragma unroll
     for (int i = 0; i < VT; ++i)
+      sraw[i] = __builtin_amdgcn_raw_buffer_load_b128(srsrc, srow[i] + s * 16, 0, 0);
+  };
+
+  f32x4 acc[VT][NT] = {};
+  fetch(0);
+  scales(0);
+  weights(w[0], 0);
+  put(0);
+  for (int s = 0; s < a.stages; ++s) {
+    lds_barrier();
+    uint32_t sw[VT];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int64_t n = n0 + 16 * i + 4 * blk + k;
-        if (n >= N) continue;
-        char* dst = out + (m * N + n) * SZ;
-        if constexpr (SZ == 4) *reinterpret_cast<float*>(dst) = acc[i][j][k];
-        else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)Pack16<Out>::pack_one(acc[i][j][k]);
+    for (int i = 0; i < VT; ++i) {
+      const uint32_t lo = __builtin_amdgcn_perm(sraw[i].y, sraw[i].x, sel);
+      const uint32_t hi = __builtin_amdgcn_perm(sraw[i].w, sraw[i].z, sel);
+      sw[i] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+    }
+    if (s + 1 < a.stages) {
+      fetch(s + 1);
+      scales(s + 1);
+    }
+    uint32_t sa[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) sa[j] = lds_s[s & 1][j][lane];
+    auto step = [&](auto tc) {
+      constexpr int T = decltype(tc)::value;
+      if (s * kStage + T >= a.steps) return;
+      weights(w[(T + 1) & 1], s * kStage + T + 1);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const u32x4 x = lds_c[s & 1][T][j][lane];
+#pragma unroll
+        for (int i = 0; i < VT; ++i) acc[i][j] = mfma_fp4<T>(w[T & 1][i], sw[i], x, sa[j], acc[i][j]);
       }
+    };
+    step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+    step(std::integral_constant<int, 2>{});
+    step(std::integral_constant<int, 3>{});
+    if (s + 1 < a.stages) put(s + 1);
+  }
+
+  const size_t size = a.out_dtype == RRL_F32 ? 4 : 2;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t m = (int64_t)(f0 + j) * 16 + r16;
+    if (m >= a.M) continue;
+    char* row = a.out + m * a.N * size;
+#pragma unroll
+    for (int h = 0; h < VT / 2; ++h) {
+      const int64_t n = n0 + 32 * h + 8 * blk;
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = acc[2 * h + k / 4][j][k % 4];
+      if (a.out_dtype == RRL_F32) store8<TagF32>(row, n, a.N, v);
+      else if (a.out_dtype == RRL_BF16) store8<TagBF16>(row, n, a.N, v);
+      else store8<TagF16>(row, n, a.N, v);
+    }
   }
 }
 
@@ -219,21 +352,22 @@ inline bool blocks_fit(int64_t R, int64_t H) {
          R * (padded(H) / kBlock) < ((int64_t)1 << 30) - kQT;
 }
 
-template <class Tag>
-int launch_quantize(const void* x, int64_t R, int64_t H, int64_t ld, uint8_t* codes, uint8_t* scales,
-                    hipStream_t st) {
+template <class Tag, class Order>
+int launch_quantize(const void* x, int64_t R, int64_t H, int64_t ld, const Order& order,
+                    uint8_t* codes, uint8_t* scales, hipStream_t st) {
   const int64_t blocks = padded(H) / kBlock;
-  hipLaunchKernelGGL(mxfp4_quantize_kernel<Tag>, dim3((uint32_t)((R * blocks * 4 + kQT - 1) / kQT)),
-                     dim3(kQT), 0, st, static_cast<const char*>(x), R, H, ld, (uint32_t)blocks, codes,
-                     scales);
+  hipLaunchKernelGGL((mxfp4_quantize_kernel<Tag, Order>),
+                     dim3((uint32_t)((R * blocks * 4 + kQT - 1) / kQT)), dim3(kQT), 0, st,
+                     static_cast<const char*>(x), R, H, ld, (uint32_t)blocks, order, codes, scales);
   return check_launch("mxfp4_quantize_kernel");
 }
 
-int quantize_any(const void* x, int32_t dt, int64_t R, int64_t H, int64_t ld, uint8_t* codes,
-                 uint8_t* scales, hipStream_t st) {
-  if (dt == RRL_F32) return launch_quantize<TagF32>(x, R, H, ld, codes, scales, st);
-  if (dt == RRL_BF16) return launch_quantize<TagBF16>(x, R, H, ld, codes, scales, st);
-  return launch_quantize<TagF16>(x, R, H, ld, codes, scales, st);
+template <class Order>
+int quantize_any(const void* x, int32_t dt, int64_t R, int64_t H, int64_t ld, const Order& order,
+                 uint8_t* codes, uint8_t* scales, hipStream_t st) {
+  if (dt == RRL_F32) return launch_quantize<TagF32>(x, R, H, ld, order, codes, scales, st);
+  if (dt == RRL_BF16) return launch_quantize<TagBF16>(x, R, H, ld, order, codes, scales, st);
+  return launch_quantize<TagF16>(x, R, H, ld, order, codes, scales, st);
 }
 
 template <class Tag>
@@ -248,21 +382,41 @@ int launch_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t R, in
   return check_launch("mxfp4_dequantize_kernel");
 }
 
-template <class Out>
-int launch_linear(const uint8_t* ac, const uint8_t* as, int64_t M, const uint8_t* wc,
-                  const uint8_t* wsc, int64_t N, int64_t P, void* out, hipStream_t st) {
-  auto grid = [&](int vt, int nt) {
-    const int64_t rows = 16 * vt * kLinWaves;
-    return dim3((uint32_t)((N + rows - 1) / rows), (uint32_t)((M + 16 * nt - 1) / (16 * nt)));
-  };
-  if (M <= 16) {
-    hipLaunchKernelGGL((mxfp4_linear_kernel<Out, 2, 1>), grid(2, 1), dim3(64 * kLinWaves), 0, st, ac,
-                       as, M, wc, wsc, N, P, static_cast<char*>(out));
-  } else {
-    hipLaunchKernelGGL((mxfp4_linear_kernel<Out, 4, 4>), grid(4, 4), dim3(64 * kLinWaves), 0, st, ac,
-                       as, M, wc, wsc, N, P, static_cast<char*>(out));
-  }
+struct LinearLayout {
+  int64_t fragments, steps, stages;
+  size_t scales, total;
+};
+inline LinearLayout linear_layout(int64_t M, int64_t H) {
+  LinearLayout l;
+  l.fragments = (M + 15) / 16;
+  l.steps = padded(H) / kDepth;
+  l.stages = (l.steps + kStage - 1) / kStage;
+  l.scales = (size_t)(l.fragments * l.steps) * 1024;
+  l.total = l.scales + (size_t)(l.fragments * l.stages) * 256;
+  return l;
+}
+
+template <int VT, int NT>
+int launch_linear(LinearArgs a, hipStream_t st) {
+  a.token_tiles = (a.fragments + NT - 1) / NT;
+  const int64_t slabs = (a.N + 16 * VT * kLinWaves - 1) / (16 * VT * kLinWaves);
+  const int64_t groups = (slabs + 7) / 8 * 8 * a.token_tiles;
+  RRL_REQUIRE(groups < ((int64_t)1 << 32) / (64 * kLinWaves), RRL_EINVAL,
+              "rrl_mxfp4_linear: too many output tiles");
+  hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT>), dim3((uint32_t)groups), dim3(64 * kLinWaves), 0,
+                     st, a);
   return check_launch("mxfp4_linear_kernel");
+}
+
+// Activation fragments of a tile: all of them up to 8, else tiles as even as can be.
+template <int VT>
+int launch_linear(const LinearArgs& a, hipStream_t st) {
+  const int tiles = (a.fragments + 7) / 8, need = (a.fragments + tiles - 1) / tiles;
+  if (need <= 1) return launch_linear<VT, 1>(a, st);
+  if (need <= 2) return launch_linear<VT, 2>(a, st);
+  if (need <= 4) return launch_linear<VT, 4>(a, st);
+  if (need <= 6) return launch_linear<VT, 6>(a, st);
+  return launch_linear<VT, 8>(a, st);
 }
 
 }  // namespace
@@ -283,7 +437,8 @@ extern "C" int rrl_mxfp4_quantize(const void* x, int32_t dtype, int64_t R, int64
   RRL_REQUIRE(R <= 1 || ld >= 0, RRL_EINVAL, "rrl_mxfp4_quantize: negative row stride");
   RRL_REQUIRE((uintptr_t)x % dtype_size(dtype) == 0 && (uintptr_t)codes % 16 == 0, RRL_EALIGN,
               "rrl_mxfp4_quantize: a pointer is not aligned (codes: 16 bytes)");
-  return quantize_any(x, dtype, R, H, ld, codes, scales, as_stream(stream));
+  return quantize_any(x, dtype, R, H, ld, RowOrder{(uint32_t)(padded(H) / kBlock)}, codes, scales,
+                      as_stream(stream));
 }
 
 extern "C" int rrl_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t R,
@@ -306,8 +461,7 @@ extern "C" int rrl_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales,
 
 extern "C" size_t rrl_mxfp4_linear_workspace_bytes(int64_t M, int64_t H) {
   if (M < 0 || H < 0 || !blocks_fit(M, H)) return 0;
-  const int64_t P = padded(H);
-  return (size_t)(M * (P / 2) + (M * (P / kBlock) + 255) / 256 * 256);
+  return linear_layout(M, H).total;
 }
 
 extern "C" int rrl_mxfp4_linear(const void* x, int32_t dtype, int64_t M, int64_t H, int64_t x_ld,
@@ -318,8 +472,8 @@ extern "C" int rrl_mxfp4_linear(const void* x, int32_t dtype, int64_t M, int64_t
               "rrl_mxfp4_linear: activations and outputs must be float32, bfloat16 or float16");
   RRL_REQUIRE(M >= 0 && H >= 1 && N >= 0, RRL_EINVAL, "rrl_mxfp4_linear: bad size");
   if (M == 0 || N == 0) return RRL_OK;
-  RRL_REQUIRE(blocks_fit(M, H) && blocks_fit(N, H) && M <= 65535 * 16, RRL_EINVAL,
-              "rrl_mxfp4_linear: 2^30 blocks of 32 or more, or over 1,048,560 activation rows");
+  RRL_REQUIRE(blocks_fit(M, H) && blocks_fit(N, H), RRL_EINVAL,
+              "rrl_mxfp4_linear: 2^30 blocks of 32 or more");
   RRL_REQUIRE(x != nullptr && codes != nullptr && scales != nullptr && out != nullptr &&
                   workspace != nullptr,
               RRL_EINVAL, "rrl_mxfp4_linear: null operand");
@@ -328,11 +482,23 @@ extern "C" int rrl_mxfp4_linear(const void* x, int32_t dtype, int64_t M, int64_t
                   (uintptr_t)codes % 16 == 0 && (uintptr_t)workspace % 16 == 0,
               RRL_EALIGN, "rrl_mxfp4_linear: a pointer is not aligned (codes: 16 bytes)");
   hipStream_t st = as_stream(stream);
-  const int64_t P = padded(H);
+  const LinearLayout l = linear_layout(M, H);
   uint8_t* ac = static_cast<uint8_t*>(workspace);
-  uint8_t* as = ac + M * (P / 2);
-  if (int rc = quantize_any(x, dtype, M, H, x_ld, ac, as, st)) return rc;
-  if (out_dtype == RRL_F32) return launch_linear<TagF32>(ac, as, M, codes, scales, N, P, out, st);
-  if (out_dtype == RRL_BF16) return launch_linear<TagBF16>(ac, as, M, codes, scales, N, P, out, st);
-  return launch_linear<TagF16>(ac, as, M, codes, scales, N, P, out, st);
+  uint8_t* as = ac + l.scales;
+  const FragmentOrder order{(uint32_t)l.steps, (uint32_t)l.stages};
+  if (int rc = quantize_any(x, dtype, M, H, x_ld, order, ac, as, st)) return rc;
+  LinearArgs a;
+  a.ac = reinterpret_cast<const u32x4*>(ac);
+  a.as = reinterpret_cast<const uint32_t*>(as);
+  a.wc = codes;
+  a.ws = scales;
+  a.M = M;
+  a.N = N;
+  a.steps = (int32_t)l.steps;
+  a.stages = (int32_t)l.stages;
+  a.fragments = (int32_t)l.fragments;
+  a.out = static_cast<char*>(out);
+  a.out_dtype = out_dtype;
+  // 128 weight rows to a workgroup where 256 would not give every CU two
+  return N * ((l.fragments + 7) / 8) < 256 * 512 ? launch_linear<2>(a, st) : launch_linear<4>(a, st);
 }
