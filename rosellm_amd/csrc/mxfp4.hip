@@ -179,6 +179,9 @@ __device__ __forceinline__ f32x4 mfma_fp4(const u32x4& a, uint32_t sa, const u32
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, T, (int)sa, T, (int)sb);
 }
 
+// Lambdas that hold their captures in registers only if they are inlined.
+#define RRL_INLINE __attribute__((always_inline))
+
 constexpr int kLinWaves = 4, kStage = 4;  // steps of 128 entries in a stage
 
 struct LinearArgs {
@@ -188,7 +191,7 @@ struct LinearArgs {
   const uint8_t* ws;    // weight scales [N, P / 32]
   int64_t M, N;
   int32_t steps, stages, fragments;
-  int32_t token_tiles;
+  int32_t tiles, groups;  // tiles of NT fragments, and the workgroups that share a slab's
   char* out;
   int32_t out_dtype;
 };
@@ -218,127 +221,168 @@ __device__ __forceinline__ void store8(char* row, int64_t n, int64_t N, const fl
     }
 }
 
-// A workgroup: 4 x VT x 16 weight rows (a wave's own VT x 16 each, straight into
-// registers) times NT x 16 activation rows (shared, through LDS a stage ahead).
+// A workgroup: a slab of 4 x VT x 16 weight rows (a wave's own VT x 16 each, in
+// registers) against tile after tile of NT x 16 activation rows (shared, through LDS
+// a stage ahead).  Two stages of weights are held: with up to 1024 entries a row they
+// are loaded once and stay, beyond that each step's registers are refilled for the
+// stage after next as soon as its products are issued.  Tiles and stages are one
+// sequence of turns with a barrier each, so that loads run ahead over tile borders
+// and a tile's stores leave while the next one's products run.
 // A wave's weight rows are dealt to its fragments so that the 4 x VT outputs a
 // lane receives are runs of 8 neighbours: fragment i, row 4 b + k is weight row
 // 32 (i / 2) + 8 b + 4 (i % 2) + k of the wave's.
 template <int VT, int NT>
 __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearArgs a) {
+  constexpr int kRows = 16 * VT, kSlab = kRows * kLinWaves;
   __shared__ u32x4 lds_c[2][kStage][NT][64];
-  __shared__ uint32_t lds_s[2][NT][64];
+  __shared__ uint32_t lds_a[2][NT][64];
+  __shared__ uint32_t lds_w[2][kLinWaves][VT][64];
   const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r16 = lane & 15, blk = lane >> 4;
-  // the tiles of one weight slab follow each other on one XCD (workgroups go to the
-  // eight in turn), so that its L2 reads the slab once
+  // a slab's workgroups follow each other on one XCD (they go to the eight in turn),
+  // so that its L2 reads the slab once
   const uint32_t xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
-  const int64_t slab = (int64_t)(slot / a.token_tiles) * 8 + xcd;
-  const int f0 = (int)(slot % a.token_tiles) * NT;
-  if (slab * (16 * VT * kLinWaves) >= a.N) return;
-  const int64_t n0 = (slab * kLinWaves + wv) * (16 * VT);
+  const int64_t base = ((int64_t)(slot / a.groups) * 8 + xcd) * kSlab;
+  if (base >= a.N) return;
+  const int group = (int)(slot % a.groups);
+  const int tile0 = (int)((int64_t)a.tiles * group / a.groups);
+  const int tile1 = (int)((int64_t)a.tiles * (group + 1) / a.groups);
+  const int turns = (tile1 - tile0) * a.stages;
+  const bool resident = a.stages <= 2;
+
+  // weight rows past the end are past their buffers' end: they read as zeros
   const int64_t P = (int64_t)a.steps * kDepth;
-
-  // rows and fragments past the end read the last ones, and are not stored
-  const uint8_t* wrow[VT];
-  int srow[VT];
+  const uint32_t rows = (uint32_t)min((int64_t)kSlab, a.N - base);
+  const __amdgpu_buffer_rsrc_t crsrc = row_rsrc(a.wc + base * (P / 2), rows * (uint32_t)(P / 2));
+  const __amdgpu_buffer_rsrc_t srsrc =
+      row_rsrc(a.ws + base * (P / kBlock), rows * (uint32_t)(P / kBlock));
+  int wrow[VT];
 #pragma unroll
-  for (int i = 0; i < VT; ++i) {
-    const int64_t r =
-        min(n0 + 32 * (i / 2) + 8 * (r16 >> 2) + 4 * (i % 2) + (r16 & 3), a.N - 1);
-    wrow[i] = a.wc + r * (P / 2) + blk * 16;
-    srow[i] = (int)(r * (P / kBlock));
-  }
-  const __amdgpu_buffer_rsrc_t srsrc = row_rsrc(a.ws, (uint32_t)(a.N * (P / kBlock)));
-  const uint32_t sel = (uint32_t)blk | (uint32_t)(4 + blk) << 8;
-
-  u32x4 stage_c[NT];
-  uint32_t stage_s[(NT + kLinWaves - 1) / kLinWaves];
-  auto fetch = [&](int s) {
-    const int step = s * kStage + wv;  // this wave's step of the stage
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int f = min(f0 + j, a.fragments - 1);
-      if (step < a.steps) stage_c[j] = a.ac[((int64_t)f * a.steps + step) * 64 + lane];
-      if (j % kLinWaves == wv) stage_s[j / kLinWaves] = a.as[((int64_t)f * a.stages + s) * 64 + lane];
-    }
-  };
-  auto put = [&](int s) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      lds_c[s & 1][wv][j][lane] = stage_c[j];
-      if (j % kLinWaves == wv) lds_s[s & 1][j][lane] = stage_s[j / kLinWaves];
-    }
-  };
-  u32x4 w[2][VT];
-  auto weights = [&](u32x4 (&dst)[VT], int step) {
-    if (step < a.steps) {
-#pragma unroll
-      for (int i = 0; i < VT; ++i)
-        dst[i] = *reinterpret_cast<const u32x4*>(wrow[i] + (int64_t)step * (kDepth / 2));
-    }
-  };
-  u32x4 sraw[VT];
-  auto scales = [&](int s) {
+  for (int i = 0; i < VT; ++i)
+    wrow[i] = (wv * kRows + 32 * (i / 2) + 8 * (r16 >> 2) + 4 * (i % 2) + (r16 & 3)) * (int)(P / 2) +
+              blk * 16;
+  u32x4 w[2][kStage][VT];
+  auto weights = [&](auto bc, auto tc, int stage) RRL_INLINE {
+    constexpr int B = decltype(bc)::value, T = decltype(tc)::value;
+    const int step = stage * kStage + T;
+    if (step >= a.steps) return;
 #pragma unroll
     for (int i = 0; i < VT; ++i)
-      sraw[i] = __builtin_amdgcn_raw_buffer_load_b128(srsrc, srow[i] + s * 16, 0, 0);
+      w[B][T][i] = __builtin_amdgcn_raw_buffer_load_b128(crsrc, wrow[i], step * (kDepth / 2), 0);
+  };
+
+  // what a turn needs in LDS, through registers: activations (a wave's own step),
+  // their scales, and the weights' scales (a thread's own row)
+  u32x4 turn_c[NT], turn_w;
+  uint32_t turn_a[(NT + kLinWaves - 1) / kLinWaves];
+  auto fetch = [&](int tile, int stage) RRL_INLINE {
+    const int step = min(stage * kStage + wv, a.steps - 1);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int f = min(tile * NT + j, a.fragments - 1);
+      turn_c[j] = a.ac[((int64_t)f * a.steps + step) * 64 + lane];
+      if (j % kLinWaves == wv) turn_a[j / kLinWaves] = a.as[((int64_t)f * a.stages + stage) * 64 + lane];
+    }
+    if (t < kSlab)
+      turn_w = __builtin_amdgcn_raw_buffer_load_b128(srsrc, t * (int)(P / kBlock), stage * 16, 0);
+  };
+  auto put = [&](int B, bool scales) RRL_INLINE {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      lds_c[B][wv][j][lane] = turn_c[j];
+      if (j % kLinWaves == wv) lds_a[B][j][lane] = turn_a[j / kLinWaves];
+    }
+    if (scales && t < kSlab) {  // byte T of lane 16 b + r's dword: block b of step T
+      const int local = t % kRows;
+      const int i = 2 * (local / 32) + ((local >> 2) & 1), r = 4 * ((local >> 3) & 3) + (local & 3);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const uint32_t sel = (uint32_t)b | (uint32_t)(4 + b) << 8;
+        const uint32_t lo = __builtin_amdgcn_perm(turn_w.y, turn_w.x, sel);
+        const uint32_t hi = __builtin_amdgcn_perm(turn_w.w, turn_w.z, sel);
+        lds_w[B][t / kRows][i][16 * b + r] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+      }
+    }
   };
 
   f32x4 acc[VT][NT] = {};
-  fetch(0);
-  scales(0);
-  weights(w[0], 0);
-  put(0);
-  for (int s = 0; s < a.stages; ++s) {
-    lds_barrier();
-    uint32_t sw[VT];
-#pragma unroll
-    for (int i = 0; i < VT; ++i) {
-      const uint32_t lo = __builtin_amdgcn_perm(sraw[i].y, sraw[i].x, sel);
-      const uint32_t hi = __builtin_amdgcn_perm(sraw[i].w, sraw[i].z, sel);
-      sw[i] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+  int tile = tile0, stage = 0, next_tile = tile0, next_stage = 0;
+  auto advance = [&](int& tl, int& st) RRL_INLINE {
+    if (++st == a.stages) {
+      st = 0;
+      ++tl;
     }
-    if (s + 1 < a.stages) {
-      fetch(s + 1);
-      scales(s + 1);
-    }
-    uint32_t sa[NT];
+  };
+  auto store = [&]() RRL_INLINE {
+    const size_t size = a.out_dtype == RRL_F32 ? 4 : 2;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) sa[j] = lds_s[s & 1][j][lane];
-    auto step = [&](auto tc) {
-      constexpr int T = decltype(tc)::value;
-      if (s * kStage + T >= a.steps) return;
-      weights(w[(T + 1) & 1], s * kStage + T + 1);
+    for (int j = 0; j < NT; ++j) {
+      const int64_t m = (int64_t)(tile * NT + j) * 16 + r16;
+      if (m < a.M) {
+        char* row = a.out + m * a.N * size;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const u32x4 x = lds_c[s & 1][T][j][lane];
+        for (int h = 0; h < VT / 2; ++h) {
+          const int64_t n = base + wv * kRows + 32 * h + 8 * blk;
+          float v[8];
 #pragma unroll
-        for (int i = 0; i < VT; ++i) acc[i][j] = mfma_fp4<T>(w[T & 1][i], sw[i], x, sa[j], acc[i][j]);
+          for (int k = 0; k < 8; ++k) v[k] = acc[2 * h + k / 4][j][k % 4];
+          if (a.out_dtype == RRL_F32) store8<TagF32>(row, n, a.N, v);
+          else if (a.out_dtype == RRL_BF16) store8<TagBF16>(row, n, a.N, v);
+          else store8<TagF16>(row, n, a.N, v);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < VT; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  };
+  auto turn = [&](auto bc, int it) RRL_INLINE {
+    constexpr int B = decltype(bc)::value;
+    lds_barrier();
+    const bool more = it + 1 < turns;
+    advance(next_tile, next_stage);
+    if (more) fetch(next_tile, next_stage);
+    uint32_t sw[VT], sa[NT];
+#pragma unroll
+    for (int i = 0; i < VT; ++i) sw[i] = lds_w[B][wv][i][lane];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) sa[j] = lds_a[B][j][lane];
+    const bool refill = !resident && it + 2 < turns;
+    int after = next_stage + 1;  // the stage of turn it + 2
+    if (after == a.stages) after = 0;
+    auto step = [&](auto tc) RRL_INLINE {
+      constexpr int T = decltype(tc)::value;
+      if (stage * kStage + T < a.steps) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const u32x4 x = lds_c[B][T][j][lane];
+#pragma unroll
+          for (int i = 0; i < VT; ++i)
+            acc[i][j] = mfma_fp4<T>(w[B][T][i], sw[i], x, sa[j], acc[i][j]);
+        }
+      }
+      if (refill) weights(bc, tc, after);
     };
     step(std::integral_constant<int, 0>{});
     step(std::integral_constant<int, 1>{});
     step(std::integral_constant<int, 2>{});
     step(std::integral_constant<int, 3>{});
-    if (s + 1 < a.stages) put(s + 1);
-  }
+    if (more) put(B ^ 1, !resident || it == 0);
+    if (stage == a.stages - 1) store();
+    advance(tile, stage);
+  };
 
-  const size_t size = a.out_dtype == RRL_F32 ? 4 : 2;
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int64_t m = (int64_t)(f0 + j) * 16 + r16;
-    if (m >= a.M) continue;
-    char* row = a.out + m * a.N * size;
-#pragma unroll
-    for (int h = 0; h < VT / 2; ++h) {
-      const int64_t n = n0 + 32 * h + 8 * blk;
-      float v[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = acc[2 * h + k / 4][j][k % 4];
-      if (a.out_dtype == RRL_F32) store8<TagF32>(row, n, a.N, v);
-      else if (a.out_dtype == RRL_BF16) store8<TagBF16>(row, n, a.N, v);
-      else store8<TagF16>(row, n, a.N, v);
-    }
+  const std::integral_constant<int, 0> c0;
+  const std::integral_constant<int, 1> c1;
+  const std::integral_constant<int, 2> c2;
+  const std::integral_constant<int, 3> c3;
+  fetch(tile0, 0);
+  weights(c0, c0, 0), weights(c0, c1, 0), weights(c0, c2, 0), weights(c0, c3, 0);
+  const int second = a.stages > 1 ? 1 : 0;
+  weights(c1, c0, second), weights(c1, c1, second), weights(c1, c2, second), weights(c1, c3, second);
+  put(0, true);
+  for (int it = 0; it < turns; it += 2) {
+    turn(c0, it);
+    if (it + 1 < turns) turn(c1, it + 1);
   }
 }
 
@@ -398,25 +442,23 @@ inline LinearLayout linear_layout(int64_t M, int64_t H) {
 
 template <int VT, int NT>
 int launch_linear(LinearArgs a, hipStream_t st) {
-  a.token_tiles = (a.fragments + NT - 1) / NT;
   const int64_t slabs = (a.N + 16 * VT * kLinWaves - 1) / (16 * VT * kLinWaves);
-  const int64_t groups = (slabs + 7) / 8 * 8 * a.token_tiles;
-  RRL_REQUIRE(groups < ((int64_t)1 << 32) / (64 * kLinWaves), RRL_EINVAL,
-              "rrl_mxfp4_linear: too many output tiles");
-  hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT>), dim3((uint32_t)groups), dim3(64 * kLinWaves), 0,
-                     st, a);
+  a.tiles = (a.fragments + NT - 1) / NT;
+  // workgroups for four rounds of two on each of the 256 CUs
+  a.groups = (int32_t)max((int64_t)1, min((int64_t)a.tiles, 2048 / slabs));
+  const int64_t blocks = (slabs + 7) / 8 * 8 * a.groups;
+  RRL_REQUIRE(blocks < ((int64_t)1 << 32) / (64 * kLinWaves), RRL_EINVAL,
+              "rrl_mxfp4_linear: too many weight rows");
+  hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT>), dim3((uint32_t)blocks), dim3(64 * kLinWaves), 0, st,
+                     a);
   return check_launch("mxfp4_linear_kernel");
 }
 
-// Activation fragments of a tile: all of them up to 8, else tiles as even as can be.
 template <int VT>
 int launch_linear(const LinearArgs& a, hipStream_t st) {
-  const int tiles = (a.fragments + 7) / 8, need = (a.fragments + tiles - 1) / tiles;
-  if (need <= 1) return launch_linear<VT, 1>(a, st);
-  if (need <= 2) return launch_linear<VT, 2>(a, st);
-  if (need <= 4) return launch_linear<VT, 4>(a, st);
-  if (need <= 6) return launch_linear<VT, 6>(a, st);
-  return launch_linear<VT, 8>(a, st);
+  if (a.fragments <= 1) return launch_linear<VT, 1>(a, st);
+  if (a.fragments <= 2) return launch_linear<VT, 2>(a, st);
+  return launch_linear<VT, 4>(a, st);
 }
 
 }  // namespace
@@ -500,5 +542,5 @@ extern "C" int rrl_mxfp4_linear(const void* x, int32_t dtype, int64_t M, int64_t
   a.out = static_cast<char*>(out);
   a.out_dtype = out_dtype;
   // 128 weight rows to a workgroup where 256 would not give every CU two
-  return N * ((l.fragments + 7) / 8) < 256 * 512 ? launch_linear<2>(a, st) : launch_linear<4>(a, st);
+  return N * ((l.fragments + 3) / 4) < 256 * 512 ? launch_linear<2>(a, st) : launch_linear<4>(a, st);
 }
