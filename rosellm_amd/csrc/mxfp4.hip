@@ -223,15 +223,18 @@ __device__ __forceinline__ void store8(char* row, int64_t n, int64_t N, const fl
 
 // A workgroup: a slab of 4 x VT x 16 weight rows (a wave's own VT x 16 each, in
 // registers) against tile after tile of NT x 16 activation rows (shared, through LDS
-// a stage ahead).  Two stages of weights are held: with up to 1024 entries a row they
-// are loaded once and stay, beyond that each step's registers are refilled for the
-// stage after next as soon as its products are issued.  Tiles and stages are one
-// sequence of turns with a barrier each, so that loads run ahead over tile borders
-// and a tile's stores leave while the next one's products run.
+// a stage ahead).  Two stages of weights are held: with up to 1024 entries a row
+// (RESIDENT) they are loaded once and stay, beyond that each step's registers are
+// refilled for the stage after next as soon as its products are issued.  Tiles and
+// stages are one sequence of turns with a barrier each, so that loads run ahead over
+// tile borders and a tile's stores leave while the next one's products run; a turn
+// issues its loads before its stores, for a wait on a load waits for what was issued
+// before it.  All loads are unconditional (past an end they read the last row again,
+// or zeros past the buffer): behind a branch the compiler would wait for all of them.
 // A wave's weight rows are dealt to its fragments so that the 4 x VT outputs a
 // lane receives are runs of 8 neighbours: fragment i, row 4 b + k is weight row
 // 32 (i / 2) + 8 b + 4 (i % 2) + k of the wave's.
-template <int VT, int NT>
+template <int VT, int NT, bool RESIDENT>
 __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearArgs a) {
   constexpr int kRows = 16 * VT, kSlab = kRows * kLinWaves;
   __shared__ u32x4 lds_c[2][kStage][NT][64];
@@ -248,9 +251,7 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
   const int tile0 = (int)((int64_t)a.tiles * group / a.groups);
   const int tile1 = (int)((int64_t)a.tiles * (group + 1) / a.groups);
   const int turns = (tile1 - tile0) * a.stages;
-  const bool resident = a.stages <= 2;
 
-  // weight rows past the end are past their buffers' end: they read as zeros
   const int64_t P = (int64_t)a.steps * kDepth;
   const uint32_t rows = (uint32_t)min((int64_t)kSlab, a.N - base);
   const __amdgpu_buffer_rsrc_t crsrc = row_rsrc(a.wc + base * (P / 2), rows * (uint32_t)(P / 2));
@@ -264,62 +265,66 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
   u32x4 w[2][kStage][VT];
   auto weights = [&](auto bc, auto tc, int stage) RRL_INLINE {
     constexpr int B = decltype(bc)::value, T = decltype(tc)::value;
-    const int step = stage * kStage + T;
-    if (step >= a.steps) return;
 #pragma unroll
     for (int i = 0; i < VT; ++i)
-      w[B][T][i] = __builtin_amdgcn_raw_buffer_load_b128(crsrc, wrow[i], step * (kDepth / 2), 0);
+      w[B][T][i] = __builtin_amdgcn_raw_buffer_load_b128(crsrc, wrow[i],
+                                                         (stage * kStage + T) * (kDepth / 2), 0);
   };
 
   // what a turn needs in LDS, through registers: activations (a wave's own step),
   // their scales, and the weights' scales (a thread's own row)
   u32x4 turn_c[NT], turn_w;
-  uint32_t turn_a[(NT + kLinWaves - 1) / kLinWaves];
-  auto fetch = [&](int tile, int stage) RRL_INLINE {
-    const int step = min(stage * kStage + wv, a.steps - 1);
+  uint32_t turn_a;
+  const int af = min(wv, NT - 1);  // the fragment whose scales this wave takes along
+  auto fetch = [&](int tl, int st) RRL_INLINE {
+    // fragments and steps past the end are past their buffers' end: they read as zeros
+    const int f0 = tl * NT, count = max(0, min(NT, a.fragments - f0));
+    const __amdgpu_buffer_rsrc_t cr =
+        row_rsrc(a.ac + (int64_t)f0 * a.steps * 64, (uint32_t)(count * a.steps) * 1024);
+    const __amdgpu_buffer_rsrc_t ar =
+        row_rsrc(a.as + (int64_t)f0 * a.stages * 64, (uint32_t)(count * a.stages) * 256);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int f = min(tile * NT + j, a.fragments - 1);
-      turn_c[j] = a.ac[((int64_t)f * a.steps + step) * 64 + lane];
-      if (j % kLinWaves == wv) turn_a[j / kLinWaves] = a.as[((int64_t)f * a.stages + stage) * 64 + lane];
-    }
-    if (t < kSlab)
-      turn_w = __builtin_amdgcn_raw_buffer_load_b128(srsrc, t * (int)(P / kBlock), stage * 16, 0);
+    for (int j = 0; j < NT; ++j)
+      turn_c[j] = __builtin_amdgcn_raw_buffer_load_b128(
+          cr, lane * 16, (j * a.steps + min(st * kStage + wv, a.steps - 1)) * 1024, 0);
+    turn_a = __builtin_amdgcn_raw_buffer_load_b32(ar, lane * 4, (af * a.stages + st) * 256, 0);
   };
-  auto put = [&](int B, bool scales) RRL_INLINE {
+  auto fetch_scales = [&](int stage) RRL_INLINE {
+    turn_w = __builtin_amdgcn_raw_buffer_load_b128(srsrc, (t % kSlab) * (int)(P / kBlock), stage * 16, 0);
+  };
+  auto put = [&](int B) RRL_INLINE {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      lds_c[B][wv][j][lane] = turn_c[j];
-      if (j % kLinWaves == wv) lds_a[B][j][lane] = turn_a[j / kLinWaves];
-    }
-    if (scales && t < kSlab) {  // byte T of lane 16 b + r's dword: block b of step T
-      const int local = t % kRows;
-      const int i = 2 * (local / 32) + ((local >> 2) & 1), r = 4 * ((local >> 3) & 3) + (local & 3);
+    for (int j = 0; j < NT; ++j) lds_c[B][wv][j][lane] = turn_c[j];
+    lds_a[B][af][lane] = turn_a;
+  };
+  auto put_scales = [&](int B) RRL_INLINE {
+    // byte T of lane 16 b + r's dword: block b of step T
+    const int local = t % kRows;
+    const int i = 2 * (local / 32) + ((local >> 2) & 1), r = 4 * ((local >> 3) & 3) + (local & 3);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const uint32_t sel = (uint32_t)b | (uint32_t)(4 + b) << 8;
-        const uint32_t lo = __builtin_amdgcn_perm(turn_w.y, turn_w.x, sel);
-        const uint32_t hi = __builtin_amdgcn_perm(turn_w.w, turn_w.z, sel);
-        lds_w[B][t / kRows][i][16 * b + r] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
-      }
+    for (int b = 0; b < 4; ++b) {
+      const uint32_t sel = (uint32_t)b | (uint32_t)(4 + b) << 8;
+      const uint32_t lo = __builtin_amdgcn_perm(turn_w.y, turn_w.x, sel);
+      const uint32_t hi = __builtin_amdgcn_perm(turn_w.w, turn_w.z, sel);
+      lds_w[B][t % kSlab / kRows][i][16 * b + r] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
     }
   };
 
   f32x4 acc[VT][NT] = {};
-  int tile = tile0, stage = 0, next_tile = tile0, next_stage = 0;
+  int tile = tile0, stage = 0;              // this turn
+  int next_tile = tile0, next_stage = 0;    // the one whose loads go out next
   auto advance = [&](int& tl, int& st) RRL_INLINE {
-    if (++st == a.stages) {
-      st = 0;
-      ++tl;
-    }
+    const bool wrap = st + 1 == a.stages;
+    st = wrap ? 0 : st + 1;
+    tl += wrap;
   };
   auto store = [&]() RRL_INLINE {
-    const size_t size = a.out_dtype == RRL_F32 ? 4 : 2;
+    const int64_t size = a.out_dtype == RRL_F32 ? 4 : 2;
+    const int64_t m0 = (int64_t)tile * (NT * 16) + r16;
+    char* row = a.out + m0 * a.N * size;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int64_t m = (int64_t)(tile * NT + j) * 16 + r16;
-      if (m < a.M) {
-        char* row = a.out + m * a.N * size;
+    for (int j = 0; j < NT; ++j, row += 16 * a.N * size) {
+      if (m0 + 16 * j < a.M) {
 #pragma unroll
         for (int h = 0; h < VT / 2; ++h) {
           const int64_t n = base + wv * kRows + 32 * h + 8 * blk;
@@ -335,38 +340,45 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
       for (int i = 0; i < VT; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
   };
-  auto turn = [&](auto bc, int it) RRL_INLINE {
+  uint32_t sw[2][VT];
+  auto turn = [&](auto bc) RRL_INLINE {
     constexpr int B = decltype(bc)::value;
     lds_barrier();
-    const bool more = it + 1 < turns;
-    advance(next_tile, next_stage);
-    if (more) fetch(next_tile, next_stage);
-    uint32_t sw[VT], sa[NT];
+    if constexpr (!RESIDENT) {
 #pragma unroll
-    for (int i = 0; i < VT; ++i) sw[i] = lds_w[B][wv][i][lane];
+      for (int i = 0; i < VT; ++i) sw[B][i] = lds_w[B][wv][i][lane];
+    }
+    uint32_t sa[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) sa[j] = lds_a[B][j][lane];
-    const bool refill = !resident && it + 2 < turns;
-    int after = next_stage + 1;  // the stage of turn it + 2
-    if (after == a.stages) after = 0;
+    // a fragment is read while the products of the one before run
+    u32x4 x = lds_c[B][0][0][lane];
     auto step = [&](auto tc) RRL_INLINE {
       constexpr int T = decltype(tc)::value;
       if (stage * kStage + T < a.steps) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const u32x4 x = lds_c[B][T][j][lane];
+          const u32x4 next = lds_c[B][j + 1 < NT ? T : (T + 1) % kStage][(j + 1) % NT][lane];
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int i = 0; i < VT; ++i)
-            acc[i][j] = mfma_fp4<T>(w[B][T][i], sw[i], x, sa[j], acc[i][j]);
+            acc[i][j] = mfma_fp4<T>(w[B][T][i], sw[B][i], x, sa[j], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+          x = next;
         }
       }
-      if (refill) weights(bc, tc, after);
+      if constexpr (!RESIDENT) weights(bc, tc, next_stage);
     };
     step(std::integral_constant<int, 0>{});
     step(std::integral_constant<int, 1>{});
     step(std::integral_constant<int, 2>{});
     step(std::integral_constant<int, 3>{});
-    if (more) put(B ^ 1, !resident || it == 0);
+    // the next turn's data arrived during this one's products
+    put(B ^ 1);
+    if constexpr (!RESIDENT) put_scales(B ^ 1);
+    fetch(next_tile, next_stage);
+    if constexpr (!RESIDENT) fetch_scales(next_stage);
+    advance(next_tile, next_stage);
     if (stage == a.stages - 1) store();
     advance(tile, stage);
   };
@@ -375,14 +387,28 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
   const std::integral_constant<int, 1> c1;
   const std::integral_constant<int, 2> c2;
   const std::integral_constant<int, 3> c3;
-  fetch(tile0, 0);
-  weights(c0, c0, 0), weights(c0, c1, 0), weights(c0, c2, 0), weights(c0, c3, 0);
   const int second = a.stages > 1 ? 1 : 0;
+  fetch(tile0, 0);
+  fetch_scales(0);
+  weights(c0, c0, 0), weights(c0, c1, 0), weights(c0, c2, 0), weights(c0, c3, 0);
+  put(0);
+  put_scales(0);
+  advance(next_tile, next_stage);
+  fetch(next_tile, next_stage);
+  fetch_scales(second);
+  advance(next_tile, next_stage);
   weights(c1, c0, second), weights(c1, c1, second), weights(c1, c2, second), weights(c1, c3, second);
-  put(0, true);
+  if constexpr (RESIDENT) {
+    put_scales(1);
+    lds_barrier();
+#pragma unroll
+    for (int B = 0; B < 2; ++B)
+#pragma unroll
+      for (int i = 0; i < VT; ++i) sw[B][i] = lds_w[B][wv][i][lane];
+  }
   for (int it = 0; it < turns; it += 2) {
-    turn(c0, it);
-    if (it + 1 < turns) turn(c1, it + 1);
+    turn(c0);
+    if (it + 1 < turns) turn(c1);
   }
 }
 
@@ -449,8 +475,12 @@ int launch_linear(LinearArgs a, hipStream_t st) {
   const int64_t blocks = (slabs + 7) / 8 * 8 * a.groups;
   RRL_REQUIRE(blocks < ((int64_t)1 << 32) / (64 * kLinWaves), RRL_EINVAL,
               "rrl_mxfp4_linear: too many weight rows");
-  hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT>), dim3((uint32_t)blocks), dim3(64 * kLinWaves), 0, st,
-                     a);
+  if (a.stages <= 2)
+    hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT, true>), dim3((uint32_t)blocks),
+                       dim3(64 * kLinWaves), 0, st, a);
+  else
+    hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT, false>), dim3((uint32_t)blocks),
+                       dim3(64 * kLinWaves), 0, st, a);
   return check_launch("mxfp4_linear_kernel");
 }
 
@@ -514,8 +544,9 @@ extern "C" int rrl_mxfp4_linear(const void* x, int32_t dtype, int64_t M, int64_t
               "rrl_mxfp4_linear: activations and outputs must be float32, bfloat16 or float16");
   RRL_REQUIRE(M >= 0 && H >= 1 && N >= 0, RRL_EINVAL, "rrl_mxfp4_linear: bad size");
   if (M == 0 || N == 0) return RRL_OK;
-  RRL_REQUIRE(blocks_fit(M, H) && blocks_fit(N, H), RRL_EINVAL,
-              "rrl_mxfp4_linear: 2^30 blocks of 32 or more");
+  // a slab's offsets are 32-bit
+  RRL_REQUIRE(blocks_fit(M, H) && blocks_fit(N, H) && H <= (1 << 22), RRL_EINVAL,
+              "rrl_mxfp4_linear: 2^30 blocks of 32 or more, or rows of over 2^22 entries");
   RRL_REQUIRE(x != nullptr && codes != nullptr && scales != nullptr && out != nullptr &&
                   workspace != nullptr,
               RRL_EINVAL, "rrl_mxfp4_linear: null operand");
