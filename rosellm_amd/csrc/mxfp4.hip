@@ -194,9 +194,12 @@ struct LinearArgs {
   int32_t tiles, groups;  // tiles of NT fragments, and the workgroups that share a slab's
   char* out;
   int32_t out_dtype;
+  int32_t aligned;  // outputs are rows of whole, 16-byte aligned vectors of 8
 };
 
-// 8 outputs of one row: 16 bytes at any address, or one by one at the row's end.
+// 8 outputs of one row.  store8: 16 bytes at any address, or one by one at the row's
+// end.  store8_buffer: rows of whole, aligned vectors, dropped where `off` is past the
+// buffer's end.
 struct __attribute__((packed, aligned(2))) Out16 {
   u32x4 v;
 };
@@ -220,6 +223,22 @@ __device__ __forceinline__ void store8(char* row, int64_t n, int64_t N, const fl
       else reinterpret_cast<uint16_t*>(row)[n + k] = (uint16_t)Pack16<Tag>::pack_one(v[k]);
     }
 }
+template <class Tag>
+__device__ __forceinline__ void store8_buffer(__amdgpu_buffer_rsrc_t out, int off, int soff,
+                                              const float (&v)[8]) {
+  constexpr int EPV = Pack16<Tag>::EPV;
+#pragma unroll
+  for (int p = 0; p < 8 / EPV; ++p) {
+    float w[EPV];
+#pragma unroll
+    for (int k = 0; k < EPV; ++k) w[k] = v[p * EPV + k];
+    // cached: a non-temporal half line is written by itself, at 3.1 TB/s instead of 5.1
+    __builtin_amdgcn_raw_buffer_store_b128(Pack16<Tag>::pack(w), out, off + 16 * p, soff, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 1");  // as in store_b128_nt
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
 
 // A workgroup: a slab of 4 x VT x 16 weight rows (a wave's own VT x 16 each, in
 // registers) against tile after tile of NT x 16 activation rows (shared, through LDS
@@ -234,11 +253,15 @@ __device__ __forceinline__ void store8(char* row, int64_t n, int64_t N, const fl
 // A wave's weight rows are dealt to its fragments so that the 4 x VT outputs a
 // lane receives are runs of 8 neighbours: fragment i, row 4 b + k is weight row
 // 32 (i / 2) + 8 b + 4 (i % 2) + k of the wave's.
-template <int VT, int NT, bool RESIDENT>
+template <int VT, int NT, int STAGES>
 __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearArgs a) {
   constexpr int kRows = 16 * VT, kSlab = kRows * kLinWaves;
-  __shared__ u32x4 lds_c[2][kStage][NT][64];
-  __shared__ uint32_t lds_a[2][NT][64];
+  constexpr bool RESIDENT = STAGES > 0;
+  const int stages = RESIDENT ? STAGES : a.stages;
+  // with two stages a tile has two buffers, and a barrier serves both
+  constexpr int kBuffers = STAGES == 2 ? 4 : 2;
+  __shared__ u32x4 lds_c[kBuffers][kStage][NT][64];
+  __shared__ uint32_t lds_a[kBuffers][NT][64];
   __shared__ uint32_t lds_w[2][kLinWaves][VT][64];
   const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r16 = lane & 15, blk = lane >> 4;
@@ -250,7 +273,7 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
   const int group = (int)(slot % a.groups);
   const int tile0 = (int)((int64_t)a.tiles * group / a.groups);
   const int tile1 = (int)((int64_t)a.tiles * (group + 1) / a.groups);
-  const int turns = (tile1 - tile0) * a.stages;
+  const int turns = (tile1 - tile0) * stages;
 
   const int64_t P = (int64_t)a.steps * kDepth;
   const uint32_t rows = (uint32_t)min((int64_t)kSlab, a.N - base);
@@ -282,12 +305,12 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
     const __amdgpu_buffer_rsrc_t cr =
         row_rsrc(a.ac + (int64_t)f0 * a.steps * 64, (uint32_t)(count * a.steps) * 1024);
     const __amdgpu_buffer_rsrc_t ar =
-        row_rsrc(a.as + (int64_t)f0 * a.stages * 64, (uint32_t)(count * a.stages) * 256);
+        row_rsrc(a.as + (int64_t)f0 * stages * 64, (uint32_t)(count * stages) * 256);
 #pragma unroll
     for (int j = 0; j < NT; ++j)
       turn_c[j] = __builtin_amdgcn_raw_buffer_load_b128(
           cr, lane * 16, (j * a.steps + min(st * kStage + wv, a.steps - 1)) * 1024, 0);
-    turn_a = __builtin_amdgcn_raw_buffer_load_b32(ar, lane * 4, (af * a.stages + st) * 256, 0);
+    turn_a = __builtin_amdgcn_raw_buffer_load_b32(ar, lane * 4, (af * stages + st) * 256, 0);
   };
   auto fetch_scales = [&](int stage) RRL_INLINE {
     turn_w = __builtin_amdgcn_raw_buffer_load_b128(srsrc, (t % kSlab) * (int)(P / kBlock), stage * 16, 0);
@@ -311,58 +334,89 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
   };
 
   f32x4 acc[VT][NT] = {};
-  int tile = tile0, stage = 0;              // this turn
+  int tile = tile0, stage = 0, half = 0;    // this turn, and its tile's buffers
   int next_tile = tile0, next_stage = 0;    // the one whose loads go out next
   auto advance = [&](int& tl, int& st) RRL_INLINE {
-    const bool wrap = st + 1 == a.stages;
+    const bool wrap = st + 1 == stages;
     st = wrap ? 0 : st + 1;
     tl += wrap;
   };
+  const int64_t size = a.out_dtype == RRL_F32 ? 4 : 2;
+  const int64_t column = base + wv * kRows + 8 * blk;  // of the first of a lane's runs
   auto store = [&]() RRL_INLINE {
-    const int64_t size = a.out_dtype == RRL_F32 ? 4 : 2;
-    const int64_t m0 = (int64_t)tile * (NT * 16) + r16;
-    char* row = a.out + m0 * a.N * size;
+    if (a.aligned) {
+      // no branch: a lane whose row or column is past the end stores past the buffer's
+      const int64_t m0 = (int64_t)tile * (NT * 16);
+      const uint32_t here = (uint32_t)min((int64_t)NT * 16, a.M - m0);
+      const __amdgpu_buffer_rsrc_t out =
+          row_rsrc(a.out + m0 * a.N * size, here * (uint32_t)(a.N * size));
 #pragma unroll
-    for (int j = 0; j < NT; ++j, row += 16 * a.N * size) {
-      if (m0 + 16 * j < a.M) {
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int h = 0; h < VT / 2; ++h) {
-          const int64_t n = base + wv * kRows + 32 * h + 8 * blk;
+          const int64_t n = column + 32 * h;
+          const int off = n < a.N ? (int)((r16 * a.N + n) * size) : -64;
+          const int soff = (int)(16 * j * a.N * size);
           float v[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[k] = acc[2 * h + k / 4][j][k % 4];
-          if (a.out_dtype == RRL_F32) store8<TagF32>(row, n, a.N, v);
-          else if (a.out_dtype == RRL_BF16) store8<TagBF16>(row, n, a.N, v);
-          else store8<TagF16>(row, n, a.N, v);
+          if (a.out_dtype == RRL_F32) store8_buffer<TagF32>(out, off, soff, v);
+          else if (a.out_dtype == RRL_BF16) store8_buffer<TagBF16>(out, off, soff, v);
+          else store8_buffer<TagF16>(out, off, soff, v);
         }
-      }
+    } else {
+      const int64_t m0 = (int64_t)tile * (NT * 16) + r16;
+      char* row = a.out + m0 * a.N * size;
 #pragma unroll
-      for (int i = 0; i < VT; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int j = 0; j < NT; ++j, row += 16 * a.N * size)
+        if (m0 + 16 * j < a.M) {
+#pragma unroll
+          for (int h = 0; h < VT / 2; ++h) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = acc[2 * h + k / 4][j][k % 4];
+            if (a.out_dtype == RRL_F32) store8<TagF32>(row, column + 32 * h, a.N, v);
+            else if (a.out_dtype == RRL_BF16) store8<TagBF16>(row, column + 32 * h, a.N, v);
+            else store8<TagF16>(row, column + 32 * h, a.N, v);
+          }
+        }
+    }
+    if constexpr (!RESIDENT) {  // a resident tile's first products take zeros for it
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < VT; ++i) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
   };
   uint32_t sw[2][VT];
   auto turn = [&](auto bc) RRL_INLINE {
     constexpr int B = decltype(bc)::value;
-    lds_barrier();
+    const int st = STAGES == 2 ? B : (STAGES == 1 ? 0 : stage);
+    // this turn's buffer, and where the data loaded during it go
+    const int from = STAGES == 2 ? 2 * half + B : B, to = STAGES == 2 ? from ^ 2 : from ^ 1;
+    if (STAGES != 2 || B == 0) lds_barrier();
     if constexpr (!RESIDENT) {
 #pragma unroll
       for (int i = 0; i < VT; ++i) sw[B][i] = lds_w[B][wv][i][lane];
     }
     uint32_t sa[NT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) sa[j] = lds_a[B][j][lane];
+    for (int j = 0; j < NT; ++j) sa[j] = lds_a[from][j][lane];
     // a fragment is read while the products of the one before run
-    u32x4 x = lds_c[B][0][0][lane];
+    u32x4 x = lds_c[from][0][0][lane];
     auto step = [&](auto tc) RRL_INLINE {
       constexpr int T = decltype(tc)::value;
-      if (stage * kStage + T < a.steps) {
+      if (st * kStage + T < a.steps) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const u32x4 next = lds_c[B][j + 1 < NT ? T : (T + 1) % kStage][(j + 1) % NT][lane];
+          const u32x4 next = lds_c[from][j + 1 < NT ? T : (T + 1) % kStage][(j + 1) % NT][lane];
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int i = 0; i < VT; ++i)
-            acc[i][j] = mfma_fp4<T>(w[B][T][i], sw[B][i], x, sa[j], acc[i][j]);
+            acc[i][j] = mfma_fp4<T>(w[B][T][i], sw[B][i], x, sa[j],
+                                    RESIDENT && T == 0 && (STAGES == 1 || B == 0)
+                                        ? f32x4{0.0f, 0.0f, 0.0f, 0.0f}
+                                        : acc[i][j]);
           __builtin_amdgcn_sched_barrier(0);
           x = next;
         }
@@ -373,21 +427,22 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
     step(std::integral_constant<int, 1>{});
     step(std::integral_constant<int, 2>{});
     step(std::integral_constant<int, 3>{});
-    // the next turn's data arrived during this one's products
-    put(B ^ 1);
+    // what is in flight arrived during the products
+    put(to);
     if constexpr (!RESIDENT) put_scales(B ^ 1);
     fetch(next_tile, next_stage);
     if constexpr (!RESIDENT) fetch_scales(next_stage);
     advance(next_tile, next_stage);
-    if (stage == a.stages - 1) store();
+    if (st == stages - 1) store();
     advance(tile, stage);
+    if (STAGES == 2 && B == 1) half ^= 1;
   };
 
   const std::integral_constant<int, 0> c0;
   const std::integral_constant<int, 1> c1;
   const std::integral_constant<int, 2> c2;
   const std::integral_constant<int, 3> c3;
-  const int second = a.stages > 1 ? 1 : 0;
+  const int second = stages > 1 ? 1 : 0;
   fetch(tile0, 0);
   fetch_scales(0);
   weights(c0, c0, 0), weights(c0, c1, 0), weights(c0, c2, 0), weights(c0, c3, 0);
@@ -397,6 +452,11 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
   fetch(next_tile, next_stage);
   fetch_scales(second);
   advance(next_tile, next_stage);
+  if constexpr (STAGES == 2) {
+    put(1);
+    fetch(next_tile, next_stage);
+    advance(next_tile, next_stage);
+  }
   weights(c1, c0, second), weights(c1, c1, second), weights(c1, c2, second), weights(c1, c3, second);
   if constexpr (RESIDENT) {
     put_scales(1);
@@ -475,12 +535,10 @@ int launch_linear(LinearArgs a, hipStream_t st) {
   const int64_t blocks = (slabs + 7) / 8 * 8 * a.groups;
   RRL_REQUIRE(blocks < ((int64_t)1 << 32) / (64 * kLinWaves), RRL_EINVAL,
               "rrl_mxfp4_linear: too many weight rows");
-  if (a.stages <= 2)
-    hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT, true>), dim3((uint32_t)blocks),
-                       dim3(64 * kLinWaves), 0, st, a);
-  else
-    hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT, false>), dim3((uint32_t)blocks),
-                       dim3(64 * kLinWaves), 0, st, a);
+  const dim3 grid((uint32_t)blocks), threads(64 * kLinWaves);
+  if (a.stages == 1) hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT, 1>), grid, threads, 0, st, a);
+  else if (a.stages == 2) hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT, 2>), grid, threads, 0, st, a);
+  else hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT, 0>), grid, threads, 0, st, a);
   return check_launch("mxfp4_linear_kernel");
 }
 
@@ -572,6 +630,9 @@ extern "C" int rrl_mxfp4_linear(const void* x, int32_t dtype, int64_t M, int64_t
   a.fragments = (int32_t)l.fragments;
   a.out = static_cast<char*>(out);
   a.out_dtype = out_dtype;
+  // a tile's 64 rows are addressed with 32 bits
+  const int64_t row = N * (int64_t)dtype_size(out_dtype);
+  a.aligned = N % 8 == 0 && (uintptr_t)out % 16 == 0 && row < (1 << 25);
   // 128 weight rows to a workgroup where 256 would not give every CU two
   return N * ((l.fragments + 3) / 4) < 256 * 512 ? launch_linear<2>(a, st) : launch_linear<4>(a, st);
 }
