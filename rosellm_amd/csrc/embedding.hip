@@ -9,12 +9,13 @@
 //
 // Both are bound by memory: the lookup moves N rows in and out, the gradient
 // reads N rows and writes V.  For the gradient the positions are sorted by id
-// (stable least-significant-digit radix passes), so that each row of dW is
-// written once, by one wave, zeros included, and no float is added by an atomic:
-// equal inputs give equal bits.  The runs of frequent ids, which one wave would
-// follow for too long, are cut at multiples of kPiece sorted positions; a piece
-// that holds one id only is summed by waves of its own into a float32 row that
-// the id's wave then adds in place of its positions.
+// (stable least-significant-digit radix passes, in one workgroup's LDS while they
+// fit), so that each row of dW is written once, zeros included, and no float is
+// added by an atomic: equal inputs give equal bits.  A wave takes kRowsWave rows of dW,
+// whose positions are neighbours in the sorted order, and streams through them.  Runs
+// longer than kPiece positions, which one wave would follow for too long, are left to
+// workgroups of their own: the positions are cut at multiples of kPiece, a piece that
+// holds one id only is summed into a float32 row, and the run's workgroup adds those.
 #include "wave_common.hpp"
 #include "rrl_common.hpp"
 
@@ -65,7 +66,9 @@ __device__ __forceinline__ int64_t id_row(const Ids& ids, int64_t i) {
 
 constexpr int kThreads = 256;
 
-// kThreads / LPR rows per workgroup, LPR lanes along a row.
+constexpr int kFwdRows = 4;  // rows that a lane has in flight
+
+// lpr lanes along a row, kThreads / lpr rows at a time.
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(Ids ids, int64_t N,
                                                              const typename T::S* __restrict__ w,
@@ -74,41 +77,173 @@ __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(Ids ids, int64_t N,
                                                              int lpr) {
   typedef Pack<typename T::S, VEC> P;
   const int64_t rows = kThreads / lpr;
-  for (int64_t i = blockIdx.x * rows + threadIdx.x / lpr; i < N; i += gridDim.x * rows) {
-    const int64_t v = id_row(ids, i);
-    typename T::S* dst = out + i * H;
+  for (int64_t i0 = blockIdx.x * rows * kFwdRows + threadIdx.x / lpr; i0 < N;
+       i0 += gridDim.x * rows * kFwdRows) {
+    int64_t v[kFwdRows];
+#pragma unroll
+    for (int r = 0; r < kFwdRows; ++r) v[r] = i0 + r * rows < N ? id_row(ids, i0 + r * rows) : kIsBad;
     for (int64_t c = (int64_t)(threadIdx.x % lpr) * VEC; c < H; c += (int64_t)lpr * VEC) {
-      P o;
-      if (v >= 0) {
-        const P x = *reinterpret_cast<const P*>(w + v * w_ld + c);
+      P x[kFwdRows];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) o.e[k] = T::down(T::up(x.e[k]) * scale);
-      } else {
-        const typename T::S f = T::down(v == kIsPad ? 0.0f : __builtin_nanf(""));
+      for (int r = 0; r < kFwdRows; ++r)
+        if (v[r] >= 0) x[r] = *reinterpret_cast<const P*>(w + v[r] * w_ld + c);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) o.e[k] = f;
+      for (int r = 0; r < kFwdRows; ++r) {
+        if (i0 + r * rows >= N) break;
+        P o;
+        const typename T::S f = T::down(v[r] == kIsPad ? 0.0f : __builtin_nanf(""));
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) o.e[k] = v[r] >= 0 ? T::down(T::up(x[r].e[k]) * scale) : f;
+        *reinterpret_cast<P*>(out + (i0 + r * rows) * H + c) = o;
       }
-      *reinterpret_cast<P*>(dst + c) = o;
     }
   }
 }
 
 // ---- the positions sorted by id ----------------------------------------------------
 
-constexpr int kMaxDigit = 9;               // bits of one pass
+constexpr int kMaxDigit = 9;  // bits of one pass
 constexpr int kBins = 1 << kMaxDigit;
-constexpr int kSortThreads = 512;          // a thread per bin
-constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kRounds = 8;                 // positions per lane in a tile
-constexpr int kTile = kSortThreads * kRounds;
-constexpr int kMaxBlocks = 128;
-static_assert(kBins == kSortThreads, "a thread per bin");
 
 struct SortShape {
-  int passes, digit;   // digit bits of each pass
+  int passes, digit;  // digit bits of each pass
   int blocks;
-  int64_t per;         // positions per block
+  int64_t per;        // positions per block
 };
+
+// Key of position i: from the ids (first pass) or the last pass's order.
+__device__ __forceinline__ uint32_t sort_key(const Ids& ids, const uint32_t* keys, int64_t i) {
+  if (keys) return keys[i];
+  const int64_t v = id_row(ids, i);
+  return (uint32_t)(v >= 0 ? v : ids.V);
+}
+
+// Lanes of equal digit (all lanes that are `on`).
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, int digit, bool on) {
+  uint64_t same = __ballot(on);
+  for (int b = 0; b < digit; ++b) {
+    const uint64_t one = __ballot((d >> b) & 1);
+    same &= ((d >> b) & 1) ? one : ~one;
+  }
+  return same;
+}
+
+// One pass over the ROUNDS x 64 keys that each wave of a workgroup holds, in order:
+// at[r] becomes the place of lane's key r.  base: the place of the workgroup's first
+// key of bin threadIdx.x (first kBins threads), advanced past its last.  Stable: the
+// waves own consecutive stretches, and a wave goes through its own in order, lanes of
+// equal digit ranked by lane.
+template <int WAVES, int ROUNDS>
+__device__ __forceinline__ void places(const uint32_t (&key)[ROUNDS], int count, int shift,
+                                       uint32_t mask, int digit, uint32_t& base,
+                                       uint32_t (&place)[WAVES][kBins], uint32_t (&at)[ROUNDS]) {
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+  for (int k = t; k < WAVES * kBins; k += 64 * WAVES) (&place[0][0])[k] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r)
+    if (r * 64 + lane < count) atomicAdd(&place[wv][(key[r] >> shift) & mask], 1u);
+  __syncthreads();
+  if (t < kBins) {
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) {
+      const uint32_t c = place[k][t];
+      place[k][t] = base;
+      base += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const bool on = r * 64 + lane < count;
+    const uint32_t d = (key[r] >> shift) & mask;
+    const uint64_t same = same_digit(d, digit, on);
+    const uint32_t rank = __popcll(same & (((uint64_t)1 << lane) - 1));
+    at[r] = on ? place[wv][d] + rank : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (on && rank == 0) place[wv][d] += (uint32_t)__popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Exclusive running sum over the first kBins threads of a workgroup.
+__device__ __forceinline__ uint32_t bins_before(uint32_t v, uint32_t* sh) {
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+  uint32_t incl = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += y;
+  }
+  __syncthreads();
+  if (lane == 63 && t < kBins) sh[wv] = incl;
+  __syncthreads();
+  uint32_t before = incl - v;
+  for (int k = 0; k < wv && k < kBins / 64; ++k) before += sh[k];
+  return before;
+}
+
+// Few positions: every pass in one workgroup.
+constexpr int kSmallWaves = 16, kSmallRounds = 8, kSmall = 64 * kSmallWaves * kSmallRounds;
+
+__global__ __launch_bounds__(64 * kSmallWaves) void sort_small_kernel(Ids ids, int N, int passes,
+                                                                      int digit,
+                                                                      uint32_t* __restrict__ keys_out,
+                                                                      uint32_t* __restrict__ pos_out) {
+  __shared__ uint32_t place[kSmallWaves][kBins];
+  __shared__ uint32_t keys[kSmall], pos[kSmall], total[kBins], sh[kBins / 64];
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+  // a wave's stretch: as many rounds as all waves need
+  const int rounds = (N + 64 * kSmallWaves - 1) / (64 * kSmallWaves), first = wv * rounds * 64;
+  const int count = max(0, min(N - first, rounds * 64));
+  const uint32_t mask = ((uint32_t)1 << digit) - 1;
+  uint32_t key[kSmallRounds], p[kSmallRounds], at[kSmallRounds];
+#pragma unroll
+  for (int r = 0; r < kSmallRounds; ++r) {
+    const int i = r * 64 + lane;
+    p[r] = first + i;
+    key[r] = i < count ? sort_key(ids, nullptr, first + i) : 0;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    if (t < kBins) total[t] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; ++r)
+      if (r * 64 + lane < count) atomicAdd(&total[(key[r] >> (pass * digit)) & mask], 1u);
+    __syncthreads();
+    uint32_t base = bins_before(t < kBins ? total[t] : 0, sh);
+    places<kSmallWaves, kSmallRounds>(key, count, pass * digit, mask, digit, base, place, at);
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; ++r)
+      if (r * 64 + lane < count) {
+        keys[at[r]] = key[r];
+        pos[at[r]] = p[r];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSmallRounds; ++r)
+      if (r * 64 + lane < count) {
+        key[r] = keys[first + r * 64 + lane];
+        p[r] = pos[first + r * 64 + lane];
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < kSmallRounds; ++r)
+    if (r * 64 + lane < count) {
+      keys_out[first + r * 64 + lane] = key[r];
+      pos_out[first + r * 64 + lane] = p[r];
+    }
+}
+
+// More: a count, a scan and a scatter per pass.
+constexpr int kSortThreads = 512;  // a thread per bin
+constexpr int kSortWaves = kSortThreads / 64;
+constexpr int kRounds = 2;         // positions per lane in a tile
+constexpr int kTile = kSortThreads * kRounds;
+constexpr int kMaxBlocks = 512;
+static_assert(kBins == kSortThreads, "a thread per bin");
 
 inline SortShape sort_shape(int64_t N, int64_t V) {
   SortShape s;
@@ -123,13 +258,7 @@ inline SortShape sort_shape(int64_t N, int64_t V) {
   return s;
 }
 
-// Key of position i: from the ids (first pass) or the last pass's order.
-__device__ __forceinline__ uint32_t sort_key(const Ids& ids, const uint32_t* keys, int64_t i) {
-  if (keys) return keys[i];
-  const int64_t v = id_row(ids, i);
-  return (uint32_t)(v >= 0 ? v : ids.V);
-}
-
+// hist[bin, block]
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Ids ids,
                                                                   const uint32_t* __restrict__ keys,
                                                                   int64_t N, int64_t per, int shift,
@@ -142,81 +271,65 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Ids ids,
   for (int64_t i = lo + threadIdx.x; i < hi; i += kSortThreads)
     atomicAdd(&cnt[(sort_key(ids, keys, i) >> shift) & mask], 1u);
   __syncthreads();
-  hist[(int64_t)blockIdx.x * kBins + threadIdx.x] = cnt[threadIdx.x];
+  hist[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = cnt[threadIdx.x];
 }
 
-// Moves this block's positions to their places.  Stable: within a tile the
-// waves own consecutive stretches, and a wave goes through its own in order,
-// lanes of equal digit ranked by lane.
-__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(
-    Ids ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t N,
-    int64_t per, int shift, uint32_t mask, int digit, const uint32_t* __restrict__ hist,
-    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out) {
-  __shared__ uint32_t place[kSortWaves][kBins];
-  __shared__ uint32_t wave_total[kSortWaves];
-  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
-  // where this block's first position of bin t goes
-  uint32_t before = 0, total = 0;
-  for (int b = 0; b < (int)gridDim.x; ++b) {
-    const uint32_t h = hist[(int64_t)b * kBins + t];
-    before += b < (int)blockIdx.x ? h : 0;
-    total += h;
-  }
-  uint32_t incl = total;
+// A wave per bin: hist becomes each block's offset within the bin, total its sum.
+__global__ __launch_bounds__(256) void sort_scan_kernel(uint32_t* __restrict__ hist, int blocks,
+                                                        uint32_t* __restrict__ total) {
+  const int lane = threadIdx.x & 63, bin = blockIdx.x * 4 + (threadIdx.x >> 6);
+  uint32_t* row = hist + (int64_t)bin * blocks;
+  constexpr int kEach = kMaxBlocks / 64;
+  uint32_t h[kEach], sum = 0;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) h[k] = lane * kEach + k < blocks ? row[lane * kEach + k] : 0;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) sum += h[k];
+  uint32_t incl = sum;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const uint32_t y = __shfl_up(incl, o, 64);
     if (lane >= o) incl += y;
   }
-  if (lane == 63) wave_total[wv] = incl;
-  __syncthreads();
-  uint32_t base = incl - total + before;
-  for (int k = 0; k < wv; ++k) base += wave_total[k];
+  uint32_t at = incl - sum;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    if (lane * kEach + k < blocks) row[lane * kEach + k] = at;
+    at += h[k];
+  }
+  if (lane == 63) total[bin] = incl;
+}
 
+// Moves a block's positions to their places.
+__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(
+    Ids ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t N,
+    int64_t per, int shift, uint32_t mask, int digit, const uint32_t* __restrict__ hist,
+    const uint32_t* __restrict__ total, uint32_t* __restrict__ keys_out,
+    uint32_t* __restrict__ pos_out) {
+  __shared__ uint32_t place[kSortWaves][kBins];
+  __shared__ uint32_t sh[kBins / 64];
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+  const uint32_t within = hist[(int64_t)t * gridDim.x + blockIdx.x];
+  uint32_t base = bins_before(total[t], sh) + within;
   const int64_t lo = blockIdx.x * per, hi = min(N, lo + per);
   for (int64_t tile = lo; tile < hi; tile += kTile) {
-#pragma unroll
-    for (int k = 0; k < kSortWaves; ++k) place[k][t] = 0;
-    __syncthreads();
-    uint32_t key[kRounds];
-    const int64_t first = tile + (int64_t)wv * 64 * kRounds + lane;
+    const int64_t first = tile + (int64_t)wv * 64 * kRounds;
+    const int count = (int)max((int64_t)0, min((int64_t)64 * kRounds, hi - first));
+    uint32_t key[kRounds], p[kRounds], at[kRounds];
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
-      const int64_t i = first + r * 64;
-      key[r] = i < hi ? sort_key(ids, keys, i) : 0;
-      if (i < hi) atomicAdd(&place[wv][(key[r] >> shift) & mask], 1u);
+      const int64_t i = first + r * 64 + lane;
+      const bool on = r * 64 + lane < count;
+      key[r] = on ? sort_key(ids, keys, i) : 0;
+      p[r] = on && pos ? pos[i] : (uint32_t)i;
     }
-    __syncthreads();
+    places<kSortWaves, kRounds>(key, count, shift, mask, digit, base, place, at);
 #pragma unroll
-    for (int k = 0; k < kSortWaves; ++k) {
-      const uint32_t c = place[k][t];
-      place[k][t] = base;
-      base += c;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-      const int64_t i = first + r * 64;
-      const bool on = i < hi;
-      const uint32_t d = (key[r] >> shift) & mask;
-      uint64_t same = __ballot(on);
-      for (int b = 0; b < digit; ++b) {
-        const uint64_t one = __ballot((d >> b) & 1);
-        same &= ((d >> b) & 1) ? one : ~one;
+    for (int r = 0; r < kRounds; ++r)
+      if (r * 64 + lane < count) {
+        keys_out[at[r]] = key[r];
+        pos_out[at[r]] = p[r];
       }
-      const uint32_t rank = __popcll(same & (((uint64_t)1 << lane) - 1));
-      uint32_t at = 0;
-      if (on) at = place[wv][d];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      if (on && rank == 0) place[wv][d] = at + (uint32_t)__popcll(same);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      if (on) {
-        keys_out[at + rank] = key[r];
-        pos_out[at + rank] = pos ? pos[i] : (uint32_t)i;
-      }
-    }
     __syncthreads();
   }
 }
@@ -260,8 +373,8 @@ __device__ __forceinline__ void add_rows(float (&acc)[U][VEC], const typename T:
   }
 }
 
-// Workgroup (p, chunk): piece p's bounds of runs (chunk 0), and its sum where the
-// piece holds one id only.
+// Piece blockIdx.x: its bounds of runs, and, with `sums`, its sum where it holds one id
+// only (a wave per chunk of columns).
 template <typename T, int VEC, int U>
 __global__ __launch_bounds__(64) void embed_piece_kernel(const uint32_t* __restrict__ keys,
                                                          const uint32_t* __restrict__ pos, int64_t N,
@@ -296,48 +409,13 @@ __global__ __launch_bounds__(64) void embed_piece_kernel(const uint32_t* __restr
   }
 }
 
-constexpr int kRowWaves = 4;
-
-// A wave per (row of dW, chunk of columns).  begin[v] is read before it is known
-// to have been written: the key at its place tells (keys[begin[v]] == v only if
-// v occurs, and then both bounds were written by this call).
 template <typename T, int VEC, int U>
-__global__ __launch_bounds__(64 * kRowWaves) void embed_rows_kernel(
-    const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t N, int64_t V,
-    const typename T::S* __restrict__ g, int64_t g_ld, int64_t H, float scale,
-    const uint32_t* __restrict__ begin, const uint32_t* __restrict__ end,
-    const float* __restrict__ partial, typename T::S* __restrict__ dw, int64_t dw_ld) {
+__device__ __forceinline__ void write_row(const float (&acc)[U][VEC], float scale,
+                                          typename T::S* dst, int64_t c0, int64_t H) {
   typedef Pack<typename T::S, VEC> P;
-  const int lane = threadIdx.x & 63;
-  const int64_t v = (int64_t)blockIdx.x * kRowWaves + (threadIdx.x >> 6);
-  if (v >= V) return;
-  const int64_t c0 = (int64_t)blockIdx.y * (64 * VEC * U);
-  float acc[U][VEC] = {};
-  const int64_t s = begin[v];
-  if (s < N && keys[s] == (uint32_t)v) {
-    const int64_t e = end[v];
-    const int64_t p0 = (s + kPiece - 1) / kPiece, p1 = e / kPiece;
-    if (p0 < p1) {  // whole pieces [p0, p1) within the run
-      add_rows<T, VEC, U>(acc, g, g_ld, pos, s, p0 * kPiece, c0, H);
-      for (int64_t p = p0; p < p1; ++p) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int64_t c = c0 + (int64_t)(u * 64 + lane) * VEC;
-          if (c < H) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) acc[u][k] += partial[p * H + c + k];
-          }
-        }
-      }
-      add_rows<T, VEC, U>(acc, g, g_ld, pos, p1 * kPiece, e, c0, H);
-    } else {
-      add_rows<T, VEC, U>(acc, g, g_ld, pos, s, e, c0, H);
-    }
-  }
-  typename T::S* dst = dw + v * dw_ld;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t c = c0 + (int64_t)(u * 64 + lane) * VEC;
+    const int64_t c = c0 + (int64_t)(u * 64 + (threadIdx.x & 63)) * VEC;
     if (c < H) {
       P o;
 #pragma unroll
@@ -347,12 +425,164 @@ __global__ __launch_bounds__(64 * kRowWaves) void embed_rows_kernel(
   }
 }
 
+constexpr int kRowWaves = 4, kRowsWave = 8;
+
+// A wave per (kRowsWave rows of dW, chunk of columns): zeros, and the runs of up to
+// kPiece positions.  begin[v] is read before it is known to have been written: the key
+// at its place tells (keys[begin[v]] == v only if v occurs, and then both bounds were
+// written by this call).
+template <typename T, int VEC, int U>
+__global__ __launch_bounds__(64 * kRowWaves) void embed_rows_kernel(
+    const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t N, int64_t V,
+    const typename T::S* __restrict__ g, int64_t g_ld, int64_t H, float scale,
+    const uint32_t* __restrict__ begin, const uint32_t* __restrict__ end,
+    typename T::S* __restrict__ dw, int64_t dw_ld) {
+  typedef Pack<typename T::S, VEC> P;
+  const int lane = threadIdx.x & 63;
+  const int64_t v0 = ((int64_t)blockIdx.x * kRowWaves + (threadIdx.x >> 6)) * kRowsWave;
+  if (v0 >= V) return;
+  const int64_t c0 = (int64_t)blockIdx.y * (64 * VEC * U);
+  const int rows = (int)min((int64_t)kRowsWave, V - v0);
+  // lane r: row r's run (an empty one where it does not occur)
+  uint32_t b = 0, e = 0;
+  if (lane < rows) {
+    const uint32_t s = begin[v0 + lane];
+    if (s < N && keys[s] == (uint32_t)(v0 + lane)) {
+      b = s;
+      e = end[v0 + lane];
+    }
+  }
+  const bool longer = e - b > kPiece;
+  const uint32_t occurs = (uint32_t)__ballot(e > b), skip = (uint32_t)__ballot(longer);
+  float acc[U][VEC] = {};
+  int cur = 0;  // the row that acc belongs to; rows before it are written
+  auto finish = [&](int upto) {
+    for (; cur < upto; ++cur) {
+      if ((skip >> cur) & 1) continue;
+      write_row<T, VEC, U>(acc, scale, dw + (v0 + cur) * dw_ld, c0, H);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[u][k] = 0.0f;
+    }
+  };
+  // stretches of neighbouring positions: between runs that are skipped
+  int r = 0;
+  while (r < rows) {
+    const uint32_t ahead = skip >> r;
+    const int r1 = ahead ? r + __ffs(ahead) - 1 : rows;
+    const uint32_t in = occurs & (((uint32_t)1 << r1) - 1) & ~(((uint32_t)1 << r) - 1);
+    if (in) {
+      const uint32_t lo = __builtin_amdgcn_readlane(b, __ffs(in) - 1);
+      const uint32_t hi = __builtin_amdgcn_readlane(e, 31 - __clz(in));
+      for (uint32_t w = lo; w < hi; w += 64) {
+        const int n = (int)min(64u, hi - w);
+        const uint32_t p = lane < n ? pos[w + lane] : 0;
+        const uint32_t k = lane < n ? keys[w + lane] - (uint32_t)v0 : 0;
+        constexpr int kAhead = 8 / U;  // positions in flight
+        for (int i = 0; i < n; i += kAhead) {
+          P x[kAhead][U];
+#pragma unroll
+          for (int a = 0; a < kAhead; ++a) {
+            const typename T::S* row = g + (int64_t)__builtin_amdgcn_readlane(p, min(i + a, n - 1)) * g_ld;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const int64_t c = c0 + (int64_t)(u * 64 + lane) * VEC;
+              if (c < H) x[a][u] = *reinterpret_cast<const P*>(row + c);
+            }
+          }
+#pragma unroll
+          for (int a = 0; a < kAhead; ++a)
+            if (i + a < n) {
+              finish((int)__builtin_amdgcn_readlane(k, i + a));
+#pragma unroll
+              for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[u][j] += T::up(x[a][u].e[j]);
+            }
+        }
+      }
+    }
+    finish(min(r1 + 1, rows));
+    r = r1 + 1;
+  }
+}
+
+constexpr int kLongWaves = 16;
+
+// Workgroup (p, chunk of columns): the run of more than kPiece positions that begins
+// in piece p, if there is one (there is at most one).  Its waves take its pieces, and
+// the positions before the first and behind the last, in turn; their sums are added in
+// the waves' order.
+template <typename T, int VEC, int U>
+__global__ __launch_bounds__(64 * kLongWaves) void embed_long_kernel(
+    const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t N, uint32_t V,
+    const typename T::S* __restrict__ g, int64_t g_ld, int64_t H, float scale,
+    const uint32_t* __restrict__ begin, const uint32_t* __restrict__ end,
+    const float* __restrict__ partial, typename T::S* __restrict__ dw, int64_t dw_ld) {
+  const int64_t lo = (int64_t)blockIdx.x * kPiece;
+  if (lo + kPiece >= N) return;  // a run that begins here is no longer than kPiece
+  const uint32_t v = keys[lo + kPiece - 1];
+  if (v >= V || keys[lo + kPiece] != v) return;
+  const int64_t s = begin[v], e = end[v];
+  if (s < lo || e - s <= kPiece) return;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int64_t c0 = (int64_t)blockIdx.y * (64 * VEC * U);
+  const int64_t p0 = (s + kPiece - 1) / kPiece, p1 = e / kPiece;
+  float acc[U][VEC] = {};
+  if (p0 < p1) {
+    constexpr int kAhead = 4;  // sums in flight
+    for (int64_t p = p0 + wv; p < p1; p += kLongWaves * kAhead) {
+      float x[kAhead][U][VEC] = {};
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t c = c0 + (int64_t)(u * 64 + lane) * VEC;
+          if (p + a * kLongWaves < p1 && c < H) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) x[a][u][k] = partial[(p + a * kLongWaves) * H + c + k];
+          }
+        }
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[u][k] += x[a][u][k];
+    }
+  }
+  // the positions outside whole pieces, fewer than 2 kPiece: a stretch per wave
+  const int64_t head = p0 < p1 ? p0 * kPiece - s : e - s, tail = p0 < p1 ? e - p1 * kPiece : 0;
+  const int64_t each = (head + tail + kLongWaves - 1) / kLongWaves;
+  const int64_t f0 = min(wv * each, head + tail), f1 = min(f0 + each, head + tail);
+  if (f0 < head) add_rows<T, VEC, U>(acc, g, g_ld, pos, s + f0, s + min(f1, head), c0, H);
+  if (f1 > head)
+    add_rows<T, VEC, U>(acc, g, g_ld, pos, p1 * kPiece + max(f0, head) - head,
+                        p1 * kPiece + f1 - head, c0, H);
+  __shared__ float sums[kLongWaves][64 * VEC];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sums[wv][k * 64 + lane] = acc[u][k];
+    __syncthreads();
+    if (wv == 0) {
+      float one[1][VEC] = {};
+      for (int x = 0; x < kLongWaves; ++x)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) one[0][k] += sums[x][k * 64 + lane];
+      write_row<T, VEC, 1>(one, scale, dw + (int64_t)v * dw_ld, c0 + (int64_t)u * 64 * VEC, H);
+    }
+    __syncthreads();
+  }
+}
+
 // ---- host ---------------------------------------------------------------------------
 
 // Bytes of the widest access that every row start of `p` (rows ld elements
 // apart) allows, for rows of H elements.
 inline int access_bytes(const void* p, int64_t ld, int64_t H, size_t size) {
-  for (int b = 16; b > (int)size; b >>= 2)
+  for (int b = 16; b > (int)size; b >>= 1)
     if ((uintptr_t)p % b == 0 && (ld * size) % b == 0 && (H * size) % b == 0) return b;
   return (int)size;
 }
@@ -370,7 +600,7 @@ inline BwdLayout bwd_layout(int64_t N, int64_t V, int64_t H) {
   };
   for (int k = 0; k < 2; ++k) l.keys[k] = take(4 * (size_t)N);
   for (int k = 0; k < 2; ++k) l.pos[k] = take(4 * (size_t)N);
-  l.hist = take(4 * (size_t)kMaxBlocks * kBins);
+  l.hist = take(4 * (size_t)(kMaxBlocks + 1) * kBins);
   l.begin = take(4 * (size_t)V);
   l.end = take(4 * (size_t)V);
   l.partial = take(4 * (size_t)(N / kPiece) * (size_t)H);
@@ -386,7 +616,7 @@ int launch_fwd(const Ids& ids, int64_t N, const void* w, int64_t w_ld, int64_t H
   while (lpr < kThreads && lpr < packs) lpr <<= 1;
   const int64_t rows = kThreads / lpr;
   // a grid's threads are counted in 32 bits: past 2^22 workgroups they take rows in turn
-  const int64_t blocks = min((N + rows - 1) / rows, (int64_t)1 << 22);
+  const int64_t blocks = min((N + rows * kFwdRows - 1) / (rows * kFwdRows), (int64_t)1 << 22);
   hipLaunchKernelGGL((embed_fwd_kernel<T, VEC>), dim3((uint32_t)blocks), dim3(kThreads), 0, st, ids,
                      N, static_cast<const typename T::S*>(w), w_ld, H, scale,
                      static_cast<typename T::S*>(out), lpr);
@@ -411,10 +641,15 @@ int launch_rows(const BwdLayout& l, char* ws, int last, int64_t N, int64_t V, co
     if (int rc = check_launch("embed_piece_kernel")) return rc;
   }
   hipLaunchKernelGGL((embed_rows_kernel<T, VEC, U>),
-                     dim3((uint32_t)((V + kRowWaves - 1) / kRowWaves), chunks), dim3(64 * kRowWaves), 0,
-                     st, keys, pos, N, V, static_cast<const S*>(g), g_ld, H, scale, begin, end, partial,
-                     static_cast<S*>(dw), dw_ld);
-  return check_launch("embed_rows_kernel");
+                     dim3((uint32_t)((V + kRowWaves * kRowsWave - 1) / (kRowWaves * kRowsWave)), chunks),
+                     dim3(64 * kRowWaves), 0, st, keys, pos, N, V, static_cast<const S*>(g), g_ld, H,
+                     scale, begin, end, static_cast<S*>(dw), dw_ld);
+  if (int rc = check_launch("embed_rows_kernel")) return rc;
+  if (N <= kPiece) return RRL_OK;  // no run is longer
+  hipLaunchKernelGGL((embed_long_kernel<T, VEC, U>), dim3((uint32_t)(N / kPiece), chunks),
+                     dim3(64 * kLongWaves), 0, st, keys, pos, N, (uint32_t)V, static_cast<const S*>(g),
+                     g_ld, H, scale, begin, end, partial, static_cast<S*>(dw), dw_ld);
+  return check_launch("embed_long_kernel");
 }
 
 template <typename T, int VEC>
@@ -433,9 +668,9 @@ int check_common(const char* what, int64_t N, int64_t V, int64_t H, int32_t ids_
   RRL_REQUIRE(ids_dtype == RRL_I32 || ids_dtype == RRL_I64, RRL_EDTYPE,
               w + ": ids must be int32 or int64");
   RRL_REQUIRE(N >= 0 && V >= 0 && H >= 0, RRL_EINVAL, w + ": negative size");
-  // sorted positions and the gradient's grid (64 threads a row) are 32-bit
-  RRL_REQUIRE(N < ((int64_t)1 << 31) && V < ((int64_t)1 << 26) && H < ((int64_t)1 << 22), RRL_EINVAL,
-              w + ": at most 2^31 - 1 ids, and 2^26 - 1 rows of 2^22 - 1 elements");
+  // the gradient's grids (16 threads a position, 64 a row) are 32-bit
+  RRL_REQUIRE(N < ((int64_t)1 << 28) && V < ((int64_t)1 << 26) && H < ((int64_t)1 << 22), RRL_EINVAL,
+              w + ": at most 2^28 - 1 ids, and 2^26 - 1 rows of 2^22 - 1 elements");
   return RRL_OK;
 }
 
@@ -464,15 +699,16 @@ extern "C" int rrl_embedding_fwd(const void* ids, int32_t ids_dtype, int64_t N, 
 #define RRL_FWD(T, VEC) return launch_fwd<T, VEC>(d, N, weight, w_ld, H, s, out, st)
   if (dtype == RRL_F32) {
     if (b == 16) RRL_FWD(F32, 4);
+    if (b == 8) RRL_FWD(F32, 2);
     RRL_FWD(F32, 1);
   }
   if (dtype == RRL_BF16) {
     if (b == 16) RRL_FWD(Bf16, 8);
-    if (b == 4) RRL_FWD(Bf16, 2);
+    if (b >= 4) RRL_FWD(Bf16, 2);
     RRL_FWD(Bf16, 1);
   }
   if (b == 16) RRL_FWD(F16, 8);
-  if (b == 4) RRL_FWD(F16, 2);
+  if (b >= 4) RRL_FWD(F16, 2);
   RRL_FWD(F16, 1);
 #undef RRL_FWD
 }
@@ -507,15 +743,24 @@ extern "C" int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, 
     const SortShape s = sort_shape(N, V);
     const uint32_t mask = ((uint32_t)1 << s.digit) - 1;
     uint32_t* hist = reinterpret_cast<uint32_t*>(ws + l.hist);
-    for (int p = 0; p < s.passes; ++p) {
+    uint32_t* total = hist + (size_t)kMaxBlocks * kBins;
+    if (N <= kSmall) {
+      hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(64 * kSmallWaves), 0, st, d, (int)N, s.passes,
+                         s.digit, reinterpret_cast<uint32_t*>(ws + l.keys[0]),
+                         reinterpret_cast<uint32_t*>(ws + l.pos[0]));
+      if (int rc = check_launch("sort_small_kernel")) return rc;
+    }
+    for (int p = 0; p < s.passes && N > kSmall; ++p) {
       const uint32_t* kin = p ? reinterpret_cast<uint32_t*>(ws + l.keys[last]) : nullptr;
       const uint32_t* pin = p ? reinterpret_cast<uint32_t*>(ws + l.pos[last]) : nullptr;
       const int to = p & 1;
       hipLaunchKernelGGL(sort_count_kernel, dim3(s.blocks), dim3(kSortThreads), 0, st, d, kin, N,
                          s.per, p * s.digit, mask, hist);
       if (int rc = check_launch("sort_count_kernel")) return rc;
+      hipLaunchKernelGGL(sort_scan_kernel, dim3(kBins / 4), dim3(256), 0, st, hist, s.blocks, total);
+      if (int rc = check_launch("sort_scan_kernel")) return rc;
       hipLaunchKernelGGL(sort_scatter_kernel, dim3(s.blocks), dim3(kSortThreads), 0, st, d, kin, pin,
-                         N, s.per, p * s.digit, mask, s.digit, hist,
+                         N, s.per, p * s.digit, mask, s.digit, hist, total,
                          reinterpret_cast<uint32_t*>(ws + l.keys[to]),
                          reinterpret_cast<uint32_t*>(ws + l.pos[to]));
       if (int rc = check_launch("sort_scatter_kernel")) return rc;
@@ -527,15 +772,16 @@ extern "C" int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, 
 #define RRL_BWD(T, VEC) return launch_rows_u<T, VEC>(l, ws, last, N, V, grad, g_ld, H, sc, dweight, dw_ld, st)
   if (dtype == RRL_F32) {
     if (b == 16) RRL_BWD(F32, 4);
+    if (b == 8) RRL_BWD(F32, 2);
     RRL_BWD(F32, 1);
   }
   if (dtype == RRL_BF16) {
     if (b == 16) RRL_BWD(Bf16, 8);
-    if (b == 4) RRL_BWD(Bf16, 2);
+    if (b >= 4) RRL_BWD(Bf16, 2);
     RRL_BWD(Bf16, 1);
   }
   if (b == 16) RRL_BWD(F16, 8);
-  if (b == 4) RRL_BWD(F16, 2);
+  if (b >= 4) RRL_BWD(F16, 2);
   RRL_BWD(F16, 1);
 #undef RRL_BWD
 }

@@ -45,7 +45,7 @@ def test_embedding_entry_point_validation(lib):
         assert call(dt=nat.F64) == -2 and b"float32" in lib.rrl_last_error()
         assert call(idt=nat.F32) == -2 and b"int32 or int64" in lib.rrl_last_error()
         assert call(N=-1) == -1 and b"negative" in lib.rrl_last_error()
-        assert call(N=1 << 31) == -1 and b"2^31" in lib.rrl_last_error()
+        assert call(N=1 << 28) == -1 and b"2^28" in lib.rrl_last_error()
         assert call(V=1 << 26) == -1 and b"2^26" in lib.rrl_last_error()
         assert call(ids=None) == -1 and b"null" in lib.rrl_last_error()
         assert call(ids=12) == -4 and b"aligned" in lib.rrl_last_error()
