@@ -66,10 +66,8 @@ __device__ __forceinline__ int64_t id_row(const Ids& ids, int64_t i) {
 
 constexpr int kThreads = 256;
 
-constexpr int kFwdRows = 4;  // rows that a lane has in flight
-
-// lpr lanes along a row, kThreads / lpr rows at a time.
-template <typename T, int VEC>
+// lpr lanes along a row, kThreads / lpr rows at a time, kFwdRows of each lane's in flight.
+template <typename T, int VEC, int kFwdRows>
 __global__ __launch_bounds__(kThreads) void embed_fwd_kernel(Ids ids, int64_t N,
                                                              const typename T::S* __restrict__ w,
                                                              int64_t w_ld, int64_t H, float scale,
@@ -155,6 +153,7 @@ __device__ __forceinline__ void places(const uint32_t (&key)[ROUNDS], int count,
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
+    if (r * 64 >= count) break;
     const bool on = r * 64 + lane < count;
     const uint32_t d = (key[r] >> shift) & mask;
     const uint64_t same = same_digit(d, digit, on);
@@ -345,7 +344,7 @@ __device__ __forceinline__ void add_rows(float (&acc)[U][VEC], const typename T:
                                          int64_t hi, int64_t c0, int64_t H) {
   typedef Pack<typename T::S, VEC> P;
   const int lane = threadIdx.x & 63;
-  constexpr int kAhead = 4;  // rows in flight
+  constexpr int kAhead = 8 / U;  // rows in flight
   for (int64_t b = lo; b < hi; b += 64) {
     const int n = (int)min((int64_t)64, hi - b);
     const uint32_t mine = lane < n ? pos[b + lane] : 0;
@@ -432,16 +431,16 @@ constexpr int kRowWaves = 4, kRowsWave = 8;
 // at its place tells (keys[begin[v]] == v only if v occurs, and then both bounds were
 // written by this call).
 template <typename T, int VEC, int U>
-__global__ __launch_bounds__(64 * kRowWaves) void embed_rows_kernel(
-    const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t N, int64_t V,
+__device__ __forceinline__ void embed_rows(
+    int64_t block, int chunk, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t N, int64_t V,
     const typename T::S* __restrict__ g, int64_t g_ld, int64_t H, float scale,
     const uint32_t* __restrict__ begin, const uint32_t* __restrict__ end,
     typename T::S* __restrict__ dw, int64_t dw_ld) {
   typedef Pack<typename T::S, VEC> P;
   const int lane = threadIdx.x & 63;
-  const int64_t v0 = ((int64_t)blockIdx.x * kRowWaves + (threadIdx.x >> 6)) * kRowsWave;
+  const int64_t v0 = (block * kRowWaves + (threadIdx.x >> 6)) * kRowsWave;
   if (v0 >= V) return;
-  const int64_t c0 = (int64_t)blockIdx.y * (64 * VEC * U);
+  const int64_t c0 = (int64_t)chunk * (64 * VEC * U);
   const int rows = (int)min((int64_t)kRowsWave, V - v0);
   // lane r: row r's run (an empty one where it does not occur)
   uint32_t b = 0, e = 0;
@@ -508,49 +507,48 @@ __global__ __launch_bounds__(64 * kRowWaves) void embed_rows_kernel(
   }
 }
 
-constexpr int kLongWaves = 16;
+constexpr int kLongWaves = kRowWaves;
 
-// Workgroup (p, chunk of columns): the run of more than kPiece positions that begins
-// in piece p, if there is one (there is at most one).  Its waves take its pieces, and
-// the positions before the first and behind the last, in turn; their sums are added in
-// the waves' order.
+// Piece p, chunk of columns: the run of more than kPiece positions that begins in
+// piece p, if there is one (there is at most one).  The waves take the run's pieces, and the
+// positions before the first and behind the last, in turn; their sums are added in the
+// waves' order.
 template <typename T, int VEC, int U>
-__global__ __launch_bounds__(64 * kLongWaves) void embed_long_kernel(
-    const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t N, uint32_t V,
+__device__ __forceinline__ void embed_long(
+    int64_t piece, int chunk, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t N, uint32_t V,
     const typename T::S* __restrict__ g, int64_t g_ld, int64_t H, float scale,
     const uint32_t* __restrict__ begin, const uint32_t* __restrict__ end,
     const float* __restrict__ partial, typename T::S* __restrict__ dw, int64_t dw_ld) {
-  const int64_t lo = (int64_t)blockIdx.x * kPiece;
-  if (lo + kPiece >= N) return;  // a run that begins here is no longer than kPiece
+  __shared__ float sums[kLongWaves][64 * VEC];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int64_t c0 = (int64_t)chunk * (64 * VEC * U);
+  const int64_t lo = piece * kPiece;
+  if (lo + kPiece >= N) return;  // a run that begins in the last piece is no longer
   const uint32_t v = keys[lo + kPiece - 1];
   if (v >= V || keys[lo + kPiece] != v) return;
   const int64_t s = begin[v], e = end[v];
   if (s < lo || e - s <= kPiece) return;
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int64_t c0 = (int64_t)blockIdx.y * (64 * VEC * U);
   const int64_t p0 = (s + kPiece - 1) / kPiece, p1 = e / kPiece;
   float acc[U][VEC] = {};
-  if (p0 < p1) {
-    constexpr int kAhead = 4;  // sums in flight
-    for (int64_t p = p0 + wv; p < p1; p += kLongWaves * kAhead) {
-      float x[kAhead][U][VEC] = {};
+  constexpr int kAhead = 8 / U;  // sums in flight
+  for (int64_t p = p0 + wv; p < p1; p += kLongWaves * kAhead) {
+    float x[kAhead][U][VEC] = {};
 #pragma unroll
-      for (int a = 0; a < kAhead; ++a)
+    for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int64_t c = c0 + (int64_t)(u * 64 + lane) * VEC;
-          if (p + a * kLongWaves < p1 && c < H) {
+      for (int u = 0; u < U; ++u) {
+        const int64_t c = c0 + (int64_t)(u * 64 + lane) * VEC;
+        if (p + a * kLongWaves < p1 && c < H) {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) x[a][u][k] = partial[(p + a * kLongWaves) * H + c + k];
-          }
+          for (int k = 0; k < VEC; ++k) x[a][u][k] = partial[(p + a * kLongWaves) * H + c + k];
         }
+      }
 #pragma unroll
-      for (int a = 0; a < kAhead; ++a)
+    for (int a = 0; a < kAhead; ++a)
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) acc[u][k] += x[a][u][k];
-    }
+        for (int k = 0; k < VEC; ++k) acc[u][k] += x[a][u][k];
   }
   // the positions outside whole pieces, fewer than 2 kPiece: a stretch per wave
   const int64_t head = p0 < p1 ? p0 * kPiece - s : e - s, tail = p0 < p1 ? e - p1 * kPiece : 0;
@@ -560,7 +558,6 @@ __global__ __launch_bounds__(64 * kLongWaves) void embed_long_kernel(
   if (f1 > head)
     add_rows<T, VEC, U>(acc, g, g_ld, pos, p1 * kPiece + max(f0, head) - head,
                         p1 * kPiece + f1 - head, c0, H);
-  __shared__ float sums[kLongWaves][64 * VEC];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -574,6 +571,25 @@ __global__ __launch_bounds__(64 * kLongWaves) void embed_long_kernel(
       write_row<T, VEC, 1>(one, scale, dw + (int64_t)v * dw_ld, c0 + (int64_t)u * 64 * VEC, H);
     }
     __syncthreads();
+  }
+}
+
+// Both, neither waiting for the other: the long runs first, then the rows.
+template <typename T, int VEC, int U>
+__global__ __launch_bounds__(64 * kRowWaves) void embed_grad_kernel(
+    uint32_t pieces, uint32_t narrow, uint32_t chunks, const uint32_t* __restrict__ keys,
+    const uint32_t* __restrict__ pos, int64_t N, int64_t V, const typename T::S* __restrict__ g,
+    int64_t g_ld, int64_t H, float scale, const uint32_t* __restrict__ begin,
+    const uint32_t* __restrict__ end, const float* __restrict__ partial,
+    typename T::S* __restrict__ dw, int64_t dw_ld) {
+  uint32_t id = blockIdx.x;
+  if (id < pieces * narrow) {
+    embed_long<T, VEC, 1>(id / narrow, id % narrow, keys, pos, N, (uint32_t)V, g, g_ld, H, scale, begin,
+                          end, partial, dw, dw_ld);
+  } else {
+    id -= pieces * narrow;
+    embed_rows<T, VEC, U>(id / chunks, id % chunks, keys, pos, N, V, g, g_ld, H, scale, begin, end, dw,
+                          dw_ld);
   }
 }
 
@@ -615,11 +631,21 @@ int launch_fwd(const Ids& ids, int64_t N, const void* w, int64_t w_ld, int64_t H
   int lpr = 1;
   while (lpr < kThreads && lpr < packs) lpr <<= 1;
   const int64_t rows = kThreads / lpr;
-  // a grid's threads are counted in 32 bits: past 2^22 workgroups they take rows in turn
-  const int64_t blocks = min((N + rows * kFwdRows - 1) / (rows * kFwdRows), (int64_t)1 << 22);
-  hipLaunchKernelGGL((embed_fwd_kernel<T, VEC>), dim3((uint32_t)blocks), dim3(kThreads), 0, st, ids,
-                     N, static_cast<const typename T::S*>(w), w_ld, H, scale,
-                     static_cast<typename T::S*>(out), lpr);
+  const typename T::S* src = static_cast<const typename T::S*>(w);
+  typename T::S* dst = static_cast<typename T::S*>(out);
+  // Four rows in flight where there are enough to fill the chip with them (262,144 rows
+  // of 2 KB: 183 us against 197 us with one), one for a decode step's few (320 rows: 2.8
+  // against 4.1 us).  A grid's threads are counted in 32 bits: past 2^22 workgroups they
+  // take rows in turn.
+  const int64_t groups = (N + rows - 1) / rows;
+  if (groups <= 8192) {
+    hipLaunchKernelGGL((embed_fwd_kernel<T, VEC, 1>), dim3((uint32_t)groups), dim3(kThreads), 0, st, ids,
+                       N, src, w_ld, H, scale, dst, lpr);
+  } else {
+    hipLaunchKernelGGL((embed_fwd_kernel<T, VEC, 4>),
+                       dim3((uint32_t)min((groups + 3) / 4, (int64_t)1 << 22)), dim3(kThreads), 0, st,
+                       ids, N, src, w_ld, H, scale, dst, lpr);
+  }
   return check_launch("embed_fwd_kernel");
 }
 
@@ -634,22 +660,20 @@ int launch_rows(const BwdLayout& l, char* ws, int last, int64_t N, int64_t V, co
   float* partial = reinterpret_cast<float*>(ws + l.partial);
   const int64_t chunk = 64 * VEC * U;
   const uint32_t chunks = (uint32_t)((H + chunk - 1) / chunk);
+  const uint32_t narrow = (uint32_t)((H + 64 * VEC - 1) / (64 * VEC));  // more waves for long runs
   if (N > 0) {
-    hipLaunchKernelGGL((embed_piece_kernel<T, VEC, U>), dim3((uint32_t)((N + kPiece - 1) / kPiece), chunks),
+    hipLaunchKernelGGL((embed_piece_kernel<T, VEC, 1>), dim3((uint32_t)((N + kPiece - 1) / kPiece), narrow),
                        dim3(64), 0, st, keys, pos, N, (uint32_t)V, static_cast<const S*>(g), g_ld, H,
                        begin, end, partial);
     if (int rc = check_launch("embed_piece_kernel")) return rc;
   }
-  hipLaunchKernelGGL((embed_rows_kernel<T, VEC, U>),
-                     dim3((uint32_t)((V + kRowWaves * kRowsWave - 1) / (kRowWaves * kRowsWave)), chunks),
-                     dim3(64 * kRowWaves), 0, st, keys, pos, N, V, static_cast<const S*>(g), g_ld, H,
-                     scale, begin, end, static_cast<S*>(dw), dw_ld);
-  if (int rc = check_launch("embed_rows_kernel")) return rc;
-  if (N <= kPiece) return RRL_OK;  // no run is longer
-  hipLaunchKernelGGL((embed_long_kernel<T, VEC, U>), dim3((uint32_t)(N / kPiece), chunks),
-                     dim3(64 * kLongWaves), 0, st, keys, pos, N, (uint32_t)V, static_cast<const S*>(g),
-                     g_ld, H, scale, begin, end, partial, static_cast<S*>(dw), dw_ld);
-  return check_launch("embed_long_kernel");
+  // no run is longer than kPiece where the positions end with the first piece
+  const uint32_t pieces = (uint32_t)(N / kPiece);
+  const int64_t rows = (V + kRowWaves * kRowsWave - 1) / (kRowWaves * kRowsWave);
+  const uint32_t blocks = pieces * narrow + (uint32_t)rows * chunks;  // rrl_embedding_bwd's check
+  hipLaunchKernelGGL((embed_grad_kernel<T, VEC, U>), dim3(blocks), dim3(64 * kRowWaves), 0, st, pieces, narrow,
+                     chunks, keys, pos, N, V, static_cast<const S*>(g), g_ld, H, scale, begin, end, partial, static_cast<S*>(dw), dw_ld);
+  return check_launch("embed_grad_kernel");
 }
 
 template <typename T, int VEC>
@@ -734,6 +758,11 @@ extern "C" int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, 
   RRL_REQUIRE((uintptr_t)grad % size == 0 && (uintptr_t)dweight % size == 0 &&
                   (uintptr_t)ids % dtype_size(ids_dtype) == 0 && (uintptr_t)workspace % 16 == 0,
               RRL_EALIGN, "rrl_embedding_bwd: a pointer is not aligned to its element");
+  const int b = min(access_bytes(grad, g_ld, H, size), access_bytes(dweight, dw_ld, H, size));
+  // a grid's threads are counted in 32 bits
+  const int64_t wide = (H * (int64_t)size + 64 * b - 1) / (64 * b);
+  RRL_REQUIRE((N / kPiece + V / (kRowWaves * kRowsWave) + 1) * wide < ((int64_t)1 << 32) / (64 * kRowWaves),
+              RRL_EINVAL, "rrl_embedding_bwd: too many ids or rows for their length");
   hipStream_t st = as_stream(stream);
   const Ids d{ids, ids_dtype, V, padding_idx, has_padding};
   const BwdLayout l = bwd_layout(N, V, H);
@@ -767,7 +796,6 @@ extern "C" int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, 
       last = to;
     }
   }
-  const int b = min(access_bytes(grad, g_ld, H, size), access_bytes(dweight, dw_ld, H, size));
   const float sc = (float)scale;
 #define RRL_BWD(T, VEC) return launch_rows_u<T, VEC>(l, ws, last, N, V, grad, g_ld, H, sc, dweight, dw_ld, st)
   if (dtype == RRL_F32) {

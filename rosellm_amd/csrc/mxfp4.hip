@@ -102,11 +102,11 @@ __global__ __launch_bounds__(kQT) void mxfp4_quantize_kernel(const char* __restr
                                                              uint8_t* __restrict__ codes,
                                                              uint8_t* __restrict__ scales) {
   constexpr int SZ = 16 / Pack16<Tag>::EPV;
-  const int64_t id = ((int64_t)blockIdx.x * kQT + threadIdx.x) / 4;
+  const uint32_t id = (blockIdx.x * kQT + threadIdx.x) / 4;  // below 2^30 (blocks_fit)
   const int part = threadIdx.x & 3;
   if (id >= R * blocks) return;
   const int64_t r = id / blocks;
-  const uint32_t b = (uint32_t)(id % blocks);
+  const uint32_t b = id % blocks;
   float v[8];
   load8<Tag>(x + r * ld * SZ, (int64_t)b * kBlock + part * 8, H, v);
   uint32_t m = 0;
@@ -119,13 +119,17 @@ __global__ __launch_bounds__(kQT) void mxfp4_quantize_kernel(const char* __restr
   if (part == 0) scales[order.scale(r, b)] = (uint8_t)byte;
 }
 
-// The value of a code times 2^(byte - 127).
-__device__ __forceinline__ float code_value(uint32_t code, uint32_t byte) {
-  const uint32_t mag = code & 7;
-  // e2m1: exponent bias 1, one bit of mantissa; twice the value is a whole number
-  const int twice = mag < 2 ? (int)mag : (2 + (int)(mag & 1)) << ((mag >> 1) - 1);
-  const float v = ldexpf((float)twice, (int)byte - 128);
-  return byte == 255 ? __builtin_nanf("") : ((code & 8) ? -v : v);
+// Eight codes as the numbers they stand for.
+__device__ __forceinline__ void values8(uint32_t word, uint32_t byte, float (&v)[8]) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  // the instruction takes the exponent field; of 255, NaN, it would make an infinity
+  const float unit = __uint_as_float(byte << 23);
+  const f2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, unit, 0),
+                   __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, unit, 1),
+                   __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, unit, 2),
+                   __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, unit, 3)};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = byte == 255 ? __builtin_nanf("") : p[k / 2][k % 2];
 }
 
 template <class Tag>
@@ -134,16 +138,15 @@ __global__ __launch_bounds__(kQT) void mxfp4_dequantize_kernel(const uint8_t* __
                                                                int64_t R, int64_t H, uint32_t blocks,
                                                                char* __restrict__ out, int vec) {
   constexpr int EPV = Pack16<Tag>::EPV, SZ = 16 / EPV;
-  const int64_t id = ((int64_t)blockIdx.x * kQT + threadIdx.x) / 4;
+  const uint32_t id = (blockIdx.x * kQT + threadIdx.x) / 4;
   const int part = threadIdx.x & 3;
   if (id >= R * blocks) return;
-  const int64_t r = id / blocks, c = (id % blocks) * kBlock + part * 8;
+  const int64_t r = id / blocks, c = (int64_t)(id % blocks) * kBlock + part * 8;
   if (c >= H) return;
-  const uint32_t word = reinterpret_cast<const uint32_t*>(codes)[id * 4 + part];
+  const uint32_t word = reinterpret_cast<const uint32_t*>(codes)[(int64_t)id * 4 + part];
   const uint32_t byte = scales[id];
   float v[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = code_value((word >> (4 * k)) & 15, byte);
+  values8(word, byte, v);
   char* dst = out + (r * H + c) * SZ;
   if (vec) {  // whole vectors, every one 16-byte aligned
 #pragma unroll
@@ -633,6 +636,8 @@ extern "C" int rrl_mxfp4_linear(const void* x, int32_t dtype, int64_t M, int64_t
   // a tile's 64 rows are addressed with 32 bits
   const int64_t row = N * (int64_t)dtype_size(out_dtype);
   a.aligned = N % 8 == 0 && (uintptr_t)out % 16 == 0 && row < (1 << 25);
-  // 128 weight rows to a workgroup where 256 would not give every CU two
-  return N * ((l.fragments + 3) / 4) < 256 * 512 ? launch_linear<2>(a, st) : launch_linear<4>(a, st);
+  // 128 weight rows to a workgroup, or 256 where those make work enough for rounds of
+  // them (us with 128 / 256: 8 x 151,936 x 1024 15.2 / 17.3, 130 x 50,257 x 2080
+  // 32 / 42, 2,048 x 151,936 x 1024 288 / 236)
+  return N * ((l.fragments + 3) / 4) < (1 << 20) ? launch_linear<2>(a, st) : launch_linear<4>(a, st);
 }
