@@ -227,7 +227,7 @@ __device__ __forceinline__ void store8(char* row, int64_t n, int64_t N, const fl
     }
 }
 template <class Tag>
-__device__ __forceinline__ void store8_buffer(__amdgpu_buffer_rsrc_t out, int off, int soff,
+__device__ __forceinline__ void store8_buffer(__amdgpu_buffer_rsrc_t out, int off,
                                               const float (&v)[8]) {
   constexpr int EPV = Pack16<Tag>::EPV;
 #pragma unroll
@@ -236,7 +236,7 @@ __device__ __forceinline__ void store8_buffer(__amdgpu_buffer_rsrc_t out, int of
 #pragma unroll
     for (int k = 0; k < EPV; ++k) w[k] = v[p * EPV + k];
     // cached: a non-temporal half line is written by itself, at 3.1 TB/s instead of 5.1
-    __builtin_amdgcn_raw_buffer_store_b128(Pack16<Tag>::pack(w), out, off + 16 * p, soff, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(Pack16<Tag>::pack(w), out, off + 16 * p, 0, 0);
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_nop 1");  // as in store_b128_nt
     __builtin_amdgcn_sched_barrier(0);
@@ -251,8 +251,9 @@ __device__ __forceinline__ void store8_buffer(__amdgpu_buffer_rsrc_t out, int of
 // stages are one sequence of turns with a barrier each, so that loads run ahead over
 // tile borders and a tile's stores leave while the next one's products run; a turn
 // issues its loads before its stores, for a wait on a load waits for what was issued
-// before it.  All loads are unconditional (past an end they read the last row again,
-// or zeros past the buffer): behind a branch the compiler would wait for all of them.
+// before it.  All loads are unconditional (past an end they read the last fragment or
+// step again, or zeros past the buffer; scalar offsets stay within it, for the bounds
+// check subtracts them): behind a branch the compiler would wait for all of them.
 // A wave's weight rows are dealt to its fragments so that the 4 x VT outputs a
 // lane receives are runs of 8 neighbours: fragment i, row 4 b + k is weight row
 // 32 (i / 2) + 8 b + 4 (i % 2) + k of the wave's.
@@ -294,17 +295,19 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
 #pragma unroll
     for (int i = 0; i < VT; ++i)
       w[B][T][i] = __builtin_amdgcn_raw_buffer_load_b128(crsrc, wrow[i],
-                                                         (stage * kStage + T) * (kDepth / 2), 0);
+                                                         min(stage * kStage + T, a.steps - 1) * (kDepth / 2), 0);
   };
 
   // what a turn needs in LDS, through registers: activations (a wave's own step),
   // their scales, and the weights' scales (a thread's own row)
   u32x4 turn_c[NT], turn_w;
-  uint32_t turn_a;
-  const int af = min(wv, NT - 1);  // the fragment whose scales this wave takes along
+  constexpr int kOwn = (NT + kLinWaves - 1) / kLinWaves;
+  uint32_t turn_a[kOwn];
+  // the fragments whose scales this wave takes along
+  auto own = [&](int e) RRL_INLINE { return min(wv + e * kLinWaves, NT - 1); };
   auto fetch = [&](int tl, int st) RRL_INLINE {
-    // fragments and steps past the end are past their buffers' end: they read as zeros
-    const int f0 = tl * NT, count = max(0, min(NT, a.fragments - f0));
+    // past the end the last fragment and step are read again
+    const int f0 = min(tl * NT, a.fragments - 1), count = min(NT, a.fragments - f0);
     const __amdgpu_buffer_rsrc_t cr =
         row_rsrc(a.ac + (int64_t)f0 * a.steps * 64, (uint32_t)(count * a.steps) * 1024);
     const __amdgpu_buffer_rsrc_t ar =
@@ -312,16 +315,24 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
 #pragma unroll
     for (int j = 0; j < NT; ++j)
       turn_c[j] = __builtin_amdgcn_raw_buffer_load_b128(
-          cr, lane * 16, (j * a.steps + min(st * kStage + wv, a.steps - 1)) * 1024, 0);
-    turn_a = __builtin_amdgcn_raw_buffer_load_b32(ar, lane * 4, (af * stages + st) * 256, 0);
+          cr, lane * 16, (min(j, count - 1) * a.steps + min(st * kStage + wv, a.steps - 1)) * 1024, 0);
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e)
+      turn_a[e] = __builtin_amdgcn_raw_buffer_load_b32(
+          ar, lane * 4, (min(own(e), count - 1) * stages + st) * 256, 0);
   };
   auto fetch_scales = [&](int stage) RRL_INLINE {
-    turn_w = __builtin_amdgcn_raw_buffer_load_b128(srsrc, (t % kSlab) * (int)(P / kBlock), stage * 16, 0);
+    // a row's last stage may hold fewer than 16 bytes: a dword past the end reads as zeros
+    const int row = (t % kSlab) * (int)(P / kBlock) + stage * 16;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+      turn_w[d] = __builtin_amdgcn_raw_buffer_load_b32(srsrc, row + 4 * d, 0, 0);
   };
   auto put = [&](int B) RRL_INLINE {
 #pragma unroll
     for (int j = 0; j < NT; ++j) lds_c[B][wv][j][lane] = turn_c[j];
-    lds_a[B][af][lane] = turn_a;
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e) lds_a[B][own(e)][lane] = turn_a[e];
   };
   auto put_scales = [&](int B) RRL_INLINE {
     // byte T of lane 16 b + r's dword: block b of step T
@@ -358,14 +369,14 @@ __global__ __launch_bounds__(64 * kLinWaves, 2) void mxfp4_linear_kernel(LinearA
 #pragma unroll
         for (int h = 0; h < VT / 2; ++h) {
           const int64_t n = column + 32 * h;
-          const int off = n < a.N ? (int)((r16 * a.N + n) * size) : -64;
-          const int soff = (int)(16 * j * a.N * size);
+          const uint32_t row = 16 * j + r16;
+          const int off = n < a.N && row < here ? (int)((row * a.N + n) * size) : -64;
           float v[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[k] = acc[2 * h + k / 4][j][k % 4];
-          if (a.out_dtype == RRL_F32) store8_buffer<TagF32>(out, off, soff, v);
-          else if (a.out_dtype == RRL_BF16) store8_buffer<TagBF16>(out, off, soff, v);
-          else store8_buffer<TagF16>(out, off, soff, v);
+          if (a.out_dtype == RRL_F32) store8_buffer<TagF32>(out, off, v);
+          else if (a.out_dtype == RRL_BF16) store8_buffer<TagBF16>(out, off, v);
+          else store8_buffer<TagF16>(out, off, v);
         }
     } else {
       const int64_t m0 = (int64_t)tile * (NT * 16) + r16;
@@ -540,15 +551,25 @@ int launch_linear(LinearArgs a, hipStream_t st) {
               "rrl_mxfp4_linear: too many weight rows");
   const dim3 grid((uint32_t)blocks), threads(64 * kLinWaves);
   if (a.stages == 1) hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT, 1>), grid, threads, 0, st, a);
-  else if (a.stages == 2) hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT, 2>), grid, threads, 0, st, a);
+  else if (a.stages == 2 && NT <= 4)  // four buffers of more fragments leave room for one workgroup
+    hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT <= 4 ? NT : 1, 2>), grid, threads, 0, st, a);
   else hipLaunchKernelGGL((mxfp4_linear_kernel<VT, NT, 0>), grid, threads, 0, st, a);
   return check_launch("mxfp4_linear_kernel");
 }
 
+// Activation fragments of a tile: with narrow slabs as many as make the tiles even, for
+// each tile reads the slab again (130 x 50,257 x 2080, nine fragments: 64, 46 and 37 us
+// with 1, 2 and 4).
 template <int VT>
 int launch_linear(const LinearArgs& a, hipStream_t st) {
   if (a.fragments <= 1) return launch_linear<VT, 1>(a, st);
   if (a.fragments <= 2) return launch_linear<VT, 2>(a, st);
+  if constexpr (VT == 2) {
+    const int tiles = (a.fragments + 5) / 6, need = (a.fragments + tiles - 1) / tiles;
+    if (need == 3) return launch_linear<VT, 3>(a, st);
+    if (need == 5) return launch_linear<VT, 5>(a, st);
+    if (need == 6) return launch_linear<VT, 6>(a, st);
+  }
   return launch_linear<VT, 4>(a, st);
 }
 

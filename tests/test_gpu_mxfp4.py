@@ -13,6 +13,7 @@ import math
 import pytest
 import torch
 
+from rosellm_amd import _native as nat
 from rosellm_amd import roseinfer as RI
 
 pytestmark = pytest.mark.gpu
@@ -148,6 +149,11 @@ SIZES = [
     (65, 257, 1000),
     (130, 4097, 520),
     (300, 777, 2080),
+    (40, 264, 500),
+    (83, 520, 1024),
+    (90, 1000, 1100),
+    (150, 128, 130),
+    (200, 2008, 900),
     (1, 151936, 64),
 ]
 
@@ -165,6 +171,39 @@ def test_linear(device, M, N, H, dtype):
         assert out.shape == (M, N) and out.dtype == (out_dtype or dtype)
         _check_linear(out, x, q)
     assert torch.equal(RI.mxfp4_linear(x, q, torch.float32), out)
+
+
+def _guarded(rows, cols, dtype, device):
+    """An [rows, cols] view in the middle of a buffer of a pattern, and a check that the rest still holds it."""
+    pad = 4096
+    base = torch.full((rows * cols + 2 * pad,), 77.0, dtype=dtype, device=device)
+    return base[pad:pad + rows * cols].view(rows, cols), lambda: bool((base[:pad] == 77).all()
+                                                                       and (base[pad + rows * cols:] == 77).all())
+
+
+@pytest.mark.parametrize("M,N,H", [(2, 8, 64), (17, 264, 128), (65, 512, 640), (130, 1000, 1000), (250, 136, 1500),
+                                   (1100, 60000, 70), (1100, 60008, 640), (1100, 60000, 1100), (5, 1 << 20, 96),
+                                   (20, (1 << 20) + 8, 600), (9, 1 << 20, 1030), (33, 1 << 20, 40)])
+def test_linear_stays_within_its_output(device, M, N, H):
+    """Partial tiles of whole vectors and the wide slabs: the right values, and nothing beside them."""
+    g = torch.Generator(device=device).manual_seed(M + N + H)
+    x = torch.randn(M, H, generator=g, device=device).to(torch.bfloat16)
+    q = RI.quantize_mxfp4(torch.randn(N, H, generator=g, device=device).to(torch.bfloat16))
+    lib = nat.lib()
+    for dtype, code in ((torch.bfloat16, nat.BF16), (torch.float32, nat.F32)):
+        out, intact = _guarded(M, N, dtype, device)
+        ws = torch.full((lib.rrl_mxfp4_linear_workspace_bytes(M, H),), 255, dtype=torch.uint8, device=device)
+        nat.call("rrl_mxfp4_linear", x.data_ptr(), nat.BF16, M, H, H, q.codes.data_ptr(), q.scales.data_ptr(), N,
+                 out.data_ptr(), code, ws.data_ptr(), nat.stream_ptr(x.device))
+        assert intact()
+        a = RI.dequantize_mxfp4(RI.quantize_mxfp4(x)).double()
+        w = RI.dequantize_mxfp4(q).double()
+        half = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+        for lo in range(0, N, 1 << 16):
+            part = w[lo:lo + (1 << 16)].t()
+            want, mass = a @ part, a.abs() @ part.abs()
+            err = (out[:, lo:lo + (1 << 16)].double() - want).abs()
+            assert (err <= H * 2.0 ** -23 * mass * (1 + half) + half * want.abs()).all(), lo
 
 
 def test_linear_places(device):
