@@ -188,7 +188,7 @@ def test_verify_masked_rows(device):
     for dtype in DTYPES:
         x, d, y, u = _inputs(8, 3, 4500, dtype, device, 41)
         low = torch.finfo(dtype).min
-        keep = torch.rand(4500, device=device) < 0.3
+        keep = (torch.rand(4500, generator=torch.Generator().manual_seed(42)) < 0.3).to(device)
         keep[17] = True
         x[0:2, :, ~keep] = -math.inf
         x[2:4, :, ~keep] = low
@@ -303,7 +303,7 @@ def test_verified_tokens_are_embedded(device):
     """What follows in a rollout: the verified tokens' input rows, the places past them empty."""
     x, d, y, u = _inputs(7, 3, 5000, torch.bfloat16, device, 67)
     out = RI.verify_draft_tokens(x, d, y, u)
-    w = torch.randn(5000, 64, device=device)
+    w = torch.randn(5000, 64, generator=torch.Generator().manual_seed(68)).to(device)
     rows = embedding(out.token_ids, w, scale=8.0, padding_idx=-1)
     want = torch.where((out.token_ids >= 0)[..., None], w[out.token_ids.clamp_min(0)] * 8.0, 0.0)
     assert torch.equal(rows, want)
