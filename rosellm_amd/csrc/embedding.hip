@@ -184,7 +184,7 @@ __device__ __forceinline__ uint32_t bins_before(uint32_t v, uint32_t* sh) {
   return before;
 }
 
-// Few positions: every pass in one workgroup.
+// Few positions: every pass in one workgroup (4,097 of them, two passes: 17 us).
 constexpr int kSmallWaves = 16, kSmallRounds = 8, kSmall = 64 * kSmallWaves * kSmallRounds;
 
 __global__ __launch_bounds__(64 * kSmallWaves) void sort_small_kernel(Ids ids, int N, int passes,
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(64 * kSmallWaves) void sort_small_kernel(Ids ids, i
     }
 }
 
-// More: a count, a scan and a scatter per pass.
+// More: a count, a scan and a scatter per pass (262,144 positions: 5 + 5 + 7 us).
 constexpr int kSortThreads = 512;  // a thread per bin
 constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kRounds = 2;         // positions per lane in a tile
@@ -372,8 +372,9 @@ __device__ __forceinline__ void add_rows(float (&acc)[U][VEC], const typename T:
   }
 }
 
-// Piece blockIdx.x: its bounds of runs, and, with `sums`, its sum where it holds one id
-// only (a wave per chunk of columns).
+// Piece blockIdx.x: its bounds of runs, and its sum where it holds one id only (a wave
+// per chunk of columns).  Bound by reads of rows in no order: 79 us for about 125,000
+// rows of 2 KB (3.2 TB/s).
 template <typename T, int VEC, int U>
 __global__ __launch_bounds__(64) void embed_piece_kernel(const uint32_t* __restrict__ keys,
                                                          const uint32_t* __restrict__ pos, int64_t N,
@@ -426,6 +427,8 @@ __device__ __forceinline__ void write_row(const float (&acc)[U][VEC], float scal
 
 constexpr int kRowWaves = 4, kRowsWave = 8;
 
+// 151,936 rows of 1024 bfloat16 with about 110,000 positions take 188 us with the long
+// runs beside them: 227 MB of rows in no order, and 311 MB of dW.
 // A wave per (kRowsWave rows of dW, chunk of columns): zeros, and the runs of up to
 // kPiece positions.  begin[v] is read before it is known to have been written: the key
 // at its place tells (keys[begin[v]] == v only if v occurs, and then both bounds were
