@@ -524,7 +524,8 @@ RRL_API int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, con
  * token -1 and log-prob NaN.  workspace:
  * rrl_verify_drafts_workspace_bytes(B, K, V, draft != NULL) bytes of caller
  * device memory (16-byte aligned; contents of no meaning; 0 for sizes that
- * rrl_verify_drafts refuses). */
+ * rrl_verify_drafts refuses), which also serve fewer sequences, shorter drafts,
+ * greedy calls and calls without draft logits at the same V. */
 RRL_API size_t rrl_verify_drafts_workspace_bytes(int64_t B, int64_t K, int64_t V,
                     int32_t with_draft_logits);
 RRL_API int rrl_verify_drafts(const void* target, const void* draft, int32_t dtype, int64_t B,

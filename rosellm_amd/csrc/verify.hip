@@ -672,9 +672,19 @@ __global__ __launch_bounds__(kVT) void verify_draw_kernel(VerifyArgs a, Ws ws) {
 // 2048 / 4096 entries: 13.8 / 14.6 / 17.0 us at 12,950 chunks of 1024 (half of them
 // behind a draft's end), 18.5 / 17.4 / 19.2 us at 19,072, 2048 / 4096: 85 / 81 us at
 // 104,896.
+constexpr int64_t kMost1024 = 16384, kMost2048 = 40960;
 inline int chunk_entries(int64_t rows, int64_t V) {
   const int64_t least = rows * ((V + 1023) / 1024);
-  return least <= 16384 ? 1024 : (least <= 40960 ? 2048 : 4096);
+  return least <= kMost1024 ? 1024 : (least <= kMost2048 ? 2048 : 4096);
+}
+
+// Chunks of `rows` rows or of any smaller number of them, of which there may be more, for
+// they may be shorter: a workspace serves every smaller batch, shorter draft, and a call
+// that leaves the draft logits out (greedy decoding among them).
+inline int64_t chunks_at_most(int64_t rows, int64_t V) {
+  const int64_t c1 = (V + 1023) / 1024, c2 = (V + 2047) / 2048, c4 = (V + 4095) / 4096;
+  const int64_t with_c1 = kMost1024 / c1, with_c2 = kMost2048 / c1;  // rows in chunks of 1024, 2048
+  return max(rows * c4, max(min(rows, with_c1) * c1, min(rows, with_c2) * c2));
 }
 
 struct VerifyLayout {
@@ -693,7 +703,7 @@ inline VerifyLayout verify_layout(int64_t B, int64_t K, int64_t V, bool with_dra
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  l.stat = take(sizeof(ChunkStat) * (size_t)(B * l.rows * l.chunks));
+  l.stat = take(sizeof(ChunkStat) * (size_t)chunks_at_most(B * l.rows, V));
   l.row = take(sizeof(RowStat) * (size_t)(B * l.rows));
   l.masses = (V + kMass - 1) / kMass;
   l.mass = take(sizeof(double) * (size_t)(B * l.masses));
