@@ -513,7 +513,8 @@ RRL_API int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, con
  * softmax(draft / T) (one-hot at the draft when draft is NULL), draft j is
  * accepted while u[j] q(d_j) < p(d_j); n = the first that is not, or L.  The next
  * token is the first v whose running sum of rest exceeds u[K] sum(rest), rest =
- * max(p_n - q_n, 0) after a rejection (p_n where that has no mass), p_L else.
+ * max(p_n - q_n, 0) after a rejection (p_n where that has no mass), p_L else; a
+ * difference under 2^-35 of p, which rounding can make, is none.
  * Greedy (do_sample == 0 or temperature <= 0): accepted while d_j is the target's
  * first maximum, the next token is row n's; draft and uniforms are not read and
  * T = 1.  Sums and exponentials are float64 (1.1e-12 relative).

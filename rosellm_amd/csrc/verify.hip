@@ -48,6 +48,12 @@ __device__ __forceinline__ double exp2_poly(double r) {
 // Weights below this count as none.
 constexpr double kNothing = 0x1p-960;
 
+// A probability differs from another by no more than rounding if by less than this of it.
+// Each is off by five exponentials' 1.1e-12 (its weight, the factor of its row, and the
+// row's sum, whose chunks have a factor and are brought to one maximum), so that equal
+// ones lie up to 1.1e-11 apart, however the two rows were shifted or summed.
+constexpr double kSame = 0x1p-35;
+
 // Takes a whole number n, held in the low word of 1.5 2^52 + n, as an exponent.
 __device__ __forceinline__ double with_exponent(double p, double whole) {
   return __hiloint2double(__double2hiint(p) + (int)((uint32_t)__double2loint(whole) << 20),
@@ -366,9 +372,12 @@ struct Rest {
 #pragma unroll
     for (int k = 0; k < EPV; ++k) w[k] = p.template unscaled<DIRECT>(v[k]) * p.template factor<DIRECT>();
     if (y) {
-      const double f = -q.template factor<DIRECT>();
+      const double f = q.template factor<DIRECT>();
 #pragma unroll
-      for (int k = 0; k < EPV; ++k) w[k] = fmax(fma(f, q.template unscaled<DIRECT>(d[k]), w[k]), 0.0);
+      for (int k = 0; k < EPV; ++k) {
+        const double rest = fma(-f, q.template unscaled<DIRECT>(d[k]), w[k]);
+        w[k] = rest > kSame * w[k] ? rest : 0.0;
+      }
     }
 #pragma unroll
     for (int k = 0; k < EPV; ++k)

@@ -48,7 +48,9 @@ def verify_draft_tokens(
     without draft logits), draft j is accepted while ``uniforms[b, j] * q < p``
     at its token.  The next token is drawn with ``uniforms[b, K]`` by inverse CDF
     in vocabulary order, from ``max(p - q, 0)`` after a rejection, else from
-    ``p``.  ``uniforms`` [B, K + 1] are float32 in [0, 1), such as
+    ``p``; also from ``p`` where the two rows are equal (to 2^-35 of ``p``, what
+    rounding can make of equal ones) and the draft has no mass in either.
+    ``uniforms`` [B, K + 1] are float32 in [0, 1), such as
     ``torch.rand``'s.  A negative draft token ends its sequence's draft, so that
     drafts of different lengths can be padded with -1; the logits behind its
     end are not looked at.

@@ -1,7 +1,15 @@
 """Draft verification at the edges of its contract (MI355X): the workspace of
-greedy calls that are given draft logits."""
+greedy calls that are given draft logits, and rows whose difference has no mass.
+
+Tokens have to be those of the 64-bit definition wherever the uniform falls further
+than 1e-9 of the whole from a border between two entries (the kernel's exponentials
+are good to 1.1e-12, its sums of a few thousand terms to 1e-12); the inputs' seeds
+leave no other.
+"""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -47,3 +55,52 @@ def test_verify_greedy_with_draft_logits_stays_within_its_workspace(device, B, K
     want = RI.verify_draft_tokens(x[:B // 2], d[:B // 2], y[:B // 2], u[:B // 2])
     got = _entry_point(x[:B // 2], d[:B // 2], y[:B // 2], u[:B // 2], 1.0, True, (B, K, V, 1))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def _draws(p, u):
+    """The entries that an inverse-CDF draw from p [V] takes for the uniforms u [n]."""
+    run = p.double().cumsum(0)
+    border = u.double() * run[-1]
+    at = torch.searchsorted(run, border, right=True)
+    near = torch.stack([run[(at - 1).clamp_min(0)], run[at]]) - border
+    assert (near.abs() > 1e-9 * run[-1]).all(), "an undecided uniform"
+    return at
+
+
+@pytest.mark.parametrize("with_infs", [False, True])
+@pytest.mark.parametrize("shift", [0.0, 3.0])
+@pytest.mark.parametrize("V", [5000, 40961])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=lambda d: str(d)[6:])
+def test_verify_equal_rows_without_the_draft(device, dtype, V, shift, with_infs):
+    """A draft without mass in two rows that are equal, or equal but for a constant: drawn from the target."""
+    print(f"[verify] equal rows V={V} {dtype} shift={shift} infs={with_infs}", flush=True)
+    g = torch.Generator().manual_seed(V)
+    n = 300
+    row = torch.randint(-32, 33, (V,), generator=g) / 8.0  # whole eighths up to 7: exact in every type
+    row[17] = -math.inf
+    if with_infs:
+        row[torch.rand(V, generator=g) < 0.7] = -math.inf
+    x = row.to(dtype).expand(n, 2, V).to(device)
+    y = (row + shift).to(dtype).expand(n, 1, V).to(device)
+    d = torch.full((n, 1), 17, device=device)
+    u = torch.rand(n, 2, generator=g).to(device)
+    out = RI.verify_draft_tokens(x, d, y, u)
+    assert (out.num_accepted == 0).all()
+    assert torch.equal(out.token_ids[:, 0], _draws(torch.softmax(x[0, 0].double(), 0), u[:, 1]))
+
+
+def test_verify_small_difference_is_kept(device):
+    """Rows that differ in one entry of 1e-12 of the mass only: it is all that the rest holds."""
+    g = torch.Generator().manual_seed(5)
+    n, V = 100, 5000
+    row = torch.randn(V, generator=g)
+    row[17] = row[4321] = -math.inf
+    low = float(torch.logsumexp(row, 0)) - 27.6
+    x = row.clone()
+    x[4321] = low
+    y = row.clone()
+    y[17] = low
+    d = torch.full((n, 1), 17, device=device)
+    u = torch.rand(n, 2, generator=g).to(device)
+    out = RI.verify_draft_tokens(x.expand(n, 2, V).to(device), d, y.expand(n, 1, V).to(device), u)
+    assert (out.num_accepted == 0).all() and (out.token_ids[:, 0] == 4321).all()
