@@ -79,7 +79,8 @@ __device__ __forceinline__ float max2(float a, float b) {
 //   r = c x - rint(c x)       one fma, exact but for its rounding
 // so an entry takes no reduction by its own maximum: 2^(i - c m) goes into k.
 // Outside the range of that (c m past 2^20, or c so small that no float weighs
-// 2^-1000) c (x - m) is formed first.
+// 2^-1000, or so large that only subnormal steps below a maximum next to 0 weigh more)
+// c (x - m) is formed first.
 struct Weight {
   double c, scale, k, m, magic;  // k: scale 2^(i - c m)
   float least;
@@ -88,7 +89,7 @@ struct Weight {
   __device__ __forceinline__ Weight(float max, double c_, double scale_)
       : c(c_), scale(scale_), k(scale_), m(max), magic(0x1.8p52) {
     const double mc = m * c, low = m - 1000.0 / c;
-    direct = fabs(mc) < 0x1p20 && low > -3e38;
+    direct = fabs(mc) < 0x1p20 && low > -3e38 && c < 0x1p100;
     least = (float)low;
     if (direct) {
       const double i = rint(mc);

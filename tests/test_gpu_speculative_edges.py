@@ -1,5 +1,6 @@
 """Draft verification at the edges of its contract (MI355X): the workspace of
-greedy calls that are given draft logits, and rows whose difference has no mass.
+greedy calls that are given draft logits, rows whose difference has no mass, and
+temperatures next to 0 over rows whose maximum is 0.
 
 Tokens have to be those of the 64-bit definition wherever the uniform falls further
 than 1e-9 of the whole from a border between two entries (the kernel's exponentials
@@ -104,3 +105,60 @@ def test_verify_small_difference_is_kept(device):
     u = torch.rand(n, 2, generator=g).to(device)
     out = RI.verify_draft_tokens(x.expand(n, 2, V).to(device), d, y.expand(n, 1, V).to(device), u)
     assert (out.num_accepted == 0).all() and (out.token_ids[:, 0] == 4321).all()
+
+
+@pytest.mark.parametrize("T", [1e-25, 1e-31, 1e-38, 1e-44, 1e-45, 3e-48, 1e-60, 1e-200, 1e-310])
+def test_verify_small_temperatures_at_a_maximum_of_zero(device, T):
+    """Log-probs and shifted logits have 0 as their maximum: all mass is at it, shared by its ties."""
+    print(f"[verify] T={T}", flush=True)
+    g = torch.Generator().manual_seed(7)
+    B, K, V = 9, 2, 5003
+    x = -torch.rand(B, K + 1, V, generator=g) - 0.5
+    top = torch.randint(0, V, (B, K + 1), generator=g)
+    x.scatter_(-1, top[..., None], 0.0)
+    x[8, :, ::2] = -math.inf
+    x[8].scatter_(-1, top[8][:, None], 0.0)
+    x[5, 0, 4999], x[5, 0, 3] = 0.0, 0.0
+    top[5, 0] = 3  # the first of the tied, which the uniform below takes
+    y = -torch.rand(B, K, V, generator=g) - 0.5
+    y.scatter_(-1, top[:, :K, None], 0.0)
+    d = top[:, :K].clone()
+    d[1, 1] = (d[1, 1] + 1) % V
+    d[2, 0] = (d[2, 0] + 7) % V
+    d[3, 0] = -1
+    d[5, 0] = -1
+    u = torch.rand(B, K + 1, generator=g).clamp(0.05, 0.95)
+    u[5, K] = 0.2
+    n = torch.tensor([2, 1, 0, 0, 2, 0, 2, 2, 2])
+    for dtype in (torch.float32, torch.bfloat16):
+        xd, dd, ud = x.to(dtype).to(device), d.to(device), u.to(device)
+        for q in (y.to(dtype).to(device), None):
+            out = RI.verify_draft_tokens(xd, dd, q, ud, T)
+            assert torch.equal(out.num_accepted.cpu(), n), T
+            for b in range(B):
+                j = int(n[b])
+                assert out.token_ids[b].tolist() == top[b, :j + 1].tolist() + [-1] * (K - j), (T, b)
+            want = torch.zeros(B, K + 1)
+            want[5, 0] = -math.log((x[5, 0] == 0).sum())
+            # float64 rounded once, and 1e-11 from the exponentials and sums
+            assert ((out.logprobs.cpu() - want).abs() <= 2.0 ** -24 * want.abs() + 1e-11).all()
+
+
+@pytest.mark.parametrize("T", [1e-44, 1e-46])
+def test_verify_subnormal_logits_at_small_temperatures(device, T):
+    """Subnormal steps below a maximum of 0, in proportion to the temperature, weigh as anywhere else."""
+    g = torch.Generator().manual_seed(11)
+    V, n = 3001, 200
+    step = 2.0 ** -149
+    row = -step * torch.randint(0, 2000, (V,), generator=g).double()
+    row[5] = 0.0
+    x = row.float()
+    assert torch.equal(x.double(), row)
+    u = torch.rand(n, 1, generator=g)
+    out = RI.verify_draft_tokens(x.expand(n, 1, V).to(device), torch.zeros(n, 0, dtype=torch.long, device=device), None,
+                                 u.to(device), T)
+    p = torch.softmax(row / T, 0)
+    want = _draws(p, u[:, 0])
+    assert torch.equal(out.token_ids[:, 0].cpu(), want)
+    lp = torch.log_softmax(row / T, 0)[want]
+    assert ((out.logprobs[:, 0].double().cpu() - lp).abs() <= 2.0 ** -24 * lp.abs() + 1e-11).all()
