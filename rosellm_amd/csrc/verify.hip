@@ -666,7 +666,8 @@ __global__ __launch_bounds__(kVT) void verify_draw_kernel(VerifyArgs a, Ws ws) {
       lp = M<float>::nan();
       if (id >= 0) {
         const double d = (double)load_entry<Tag>(target_row<Tag>(a, b, j), id) - (double)rows[j].m;
-        lp = (float)((d * a.c - log2(rows[j].s)) * 0.69314718055994530942);
+        // the sum, at least 1, may come out 1e-12 under it where one entry holds all mass
+        lp = fminf((float)((d * a.c - log2(rows[j].s)) * 0.69314718055994530942), 0.0f);
       }
     }
     a.token_out[b * (a.K + 1) + j] = id;

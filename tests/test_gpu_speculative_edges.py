@@ -1,6 +1,7 @@
 """Draft verification at the edges of its contract (MI355X): the workspace of
-greedy calls that are given draft logits, rows whose difference has no mass, and
-temperatures next to 0 over rows whose maximum is 0.
+greedy calls that are given draft logits, rows whose difference has no mass,
+temperatures next to 0 over rows whose maximum is 0, and log-probs of tokens that
+hold all mass.
 
 Tokens have to be those of the 64-bit definition wherever the uniform falls further
 than 1e-9 of the whole from a border between two entries (the kernel's exponentials
@@ -162,3 +163,19 @@ def test_verify_subnormal_logits_at_small_temperatures(device, T):
     assert torch.equal(out.token_ids[:, 0].cpu(), want)
     lp = torch.log_softmax(row / T, 0)[want]
     assert ((out.logprobs[:, 0].double().cpu() - lp).abs() <= 2.0 ** -24 * lp.abs() + 1e-11).all()
+
+
+@pytest.mark.parametrize("do_sample", [True, False])
+def test_verify_logprobs_are_at_most_zero(device, do_sample):
+    """A token that holds all mass, or all but 1e-13 of it, whatever the logits' place."""
+    g = torch.Generator().manual_seed(13)
+    n, V = 400, 3000
+    top = torch.randn(n, generator=g) * 10
+    for rest in (-math.inf, 38.0):
+        x = torch.full((n, 1, V), -math.inf) if rest < 0 else (top - rest)[:, None, None].expand(n, 1, V).clone()
+        x[:, 0, 5] = top
+        none = torch.zeros(n, 0, dtype=torch.long, device=device)
+        out = RI.verify_draft_tokens(x.to(device), none, None, torch.full((n, 1), 0.5, device=device), do_sample=do_sample)
+        assert (out.token_ids == 5).all()
+        # 1e-11: the exponentials' and sums' error
+        assert (out.logprobs <= 0).all() and (out.logprobs >= -1e-11).all()
