@@ -268,20 +268,19 @@ __global__ __launch_bounds__(kVT) void verify_stats_kernel(VerifyArgs a, Ws ws) 
   const int64_t b = rid / a.rows;
   const int r = (int)(rid % a.rows);
   if (b >= a.B) return;
-  // target row j serves only if the j drafts before it exist, draft row j also its own
+  // target row j serves only if the j drafts before it exist, draft row j also its own;
+  // a row behind the draft's end may not be there to be read, so the drafts come first
   const bool is_draft = r > a.K;
   const int j = is_draft ? r - (int)a.K - 1 : r;
+  if (draft_ends_before(a, b, j + (is_draft ? 1 : 0))) return;
   const char* row = is_draft ? draft_row<Tag>(a, b, j) : target_row<Tag>(a, b, j);
   const int64_t lo = (int64_t)chunk * (NS * 64 * EPV) + lane * EPV;
   u32x4 raw[NS];
-  const bool whole = (int64_t)(chunk + 1) * (NS * 64 * EPV) <= a.V;
-  if (whole) {
+  if ((int64_t)(chunk + 1) * (NS * 64 * EPV) <= a.V) {
 #pragma unroll
     for (int s = 0; s < NS; ++s)
       raw[s] = reinterpret_cast<const Any16*>(row + (lo + s * 64 * EPV) * (16 / EPV))->v;
-  }
-  if (draft_ends_before(a, b, j + (is_draft ? 1 : 0))) return;
-  if (!whole) {
+  } else {
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       float x[EPV];
@@ -410,18 +409,17 @@ __device__ __forceinline__ Rest<Tag> rest_of(const VerifyArgs& a, const RowStat*
   return r;
 }
 
-// What deciding position j takes from its rows; beyond the draft's end, and
-// where the draft names no entry, only d.
+// What deciding position j takes from its rows, d its draft; beyond the draft's end at
+// L, whose rows may not be there, and where d names no entry, only d.
 struct Position {
   int64_t d;
   float x, y, u;
 };
 template <class Tag>
-__device__ __forceinline__ Position position(const VerifyArgs& a, int64_t b, int64_t j) {
-  Position p{-1, 0.0f, 0.0f, 0.0f};
-  if (j >= a.K) return p;
-  p.d = draft_at(a, b, j);
-  if (p.d < 0 || p.d >= a.V || a.greedy) return p;
+__device__ __forceinline__ Position position(const VerifyArgs& a, int64_t b, int64_t j, int64_t d,
+                                             int L) {
+  Position p{d, 0.0f, 0.0f, 0.0f};
+  if (j >= L || p.d < 0 || p.d >= a.V || a.greedy) return p;
   p.x = load_entry<Tag>(target_row<Tag>(a, b, j), p.d);
   if (a.y) p.y = load_entry<Tag>(draft_row<Tag>(a, b, j), p.d);
   p.u = a.u[b * (a.K + 1) + j];
@@ -471,7 +469,7 @@ __device__ __forceinline__ Plan decide(const VerifyArgs& a, const Ws& ws, int64_
                                        RowStat* held, const RowStat*& rows) {
   const int t = threadIdx.x, lane = t & 63;
   __shared__ int sh_len, sh_n, sh_rest;
-  Position at = position<Tag>(a, b, t);
+  const int64_t d = t < a.K ? draft_at(a, b, t) : -1;
   if (t < 64) {
     int len = (int)a.K;
     for (int k = 0; k < a.K; k += 64) {
@@ -488,6 +486,7 @@ __device__ __forceinline__ Plan decide(const VerifyArgs& a, const Ws& ws, int64_
   }
   __syncthreads();
   const int L = sh_len;
+  Position at = position<Tag>(a, b, t, d, L);  // these loads are under way while the rows are joined
   // in the workspace, the groups of a sequence write equal values
   RowStat* row = a.rows <= kRowsHeld ? held : ws.row + b * a.rows;
   rows = row;
@@ -504,7 +503,7 @@ __device__ __forceinline__ Plan decide(const VerifyArgs& a, const Ws& ws, int64_
   // positions in turn, kVT at a time: the first that does not accept its draft
   for (int j0 = 0; j0 < L && sh_n == L; j0 += kVT) {
     const int j = j0 + t;
-    if (j0 > 0) at = position<Tag>(a, b, j);
+    if (j0 > 0) at = position<Tag>(a, b, j, j < L ? draft_at(a, b, j) : -1, L);
     const int rest = j < L ? judge(a, row, j, at) : -1;
     __syncthreads();
     if (rest >= 0) atomicMin(&sh_n, j);

@@ -1,7 +1,7 @@
 """Draft verification at the edges of its contract (MI355X): the workspace of
 greedy calls that are given draft logits, rows whose difference has no mass,
-temperatures next to 0 over rows whose maximum is 0, and log-probs of tokens that
-hold all mass.
+temperatures next to 0 over rows whose maximum is 0, log-probs of tokens that
+hold all mass, and drafts behind whose end the buffers stop.
 
 Tokens have to be those of the 64-bit definition wherever the uniform falls further
 than 1e-9 of the whole from a border between two entries (the kernel's exponentials
@@ -179,3 +179,25 @@ def test_verify_logprobs_are_at_most_zero(device, do_sample):
         assert (out.token_ids == 5).all()
         # 1e-11: the exponentials' and sums' error
         assert (out.logprobs <= 0).all() and (out.logprobs >= -1e-11).all()
+
+
+@pytest.mark.parametrize("with_q", [True, False])
+@pytest.mark.parametrize("B,K,V", [(1, 5, 151936), (7, 4, 5003), (3, 90, 1001), (2, 300, 130)])
+def test_verify_rows_behind_the_last_end_need_not_exist(device, B, K, V, with_q):
+    """The last sequence's draft is short and the operands stop with the rows it needs (what follows here is NaN);
+    the sequences before it have drafts behind their ends that name entries."""
+    print(f"[verify] short operands B={B} K={K} V={V} q={with_q}", flush=True)
+    g = torch.Generator(device=device).manual_seed(B + K + V)
+    x = torch.randn(B, K + 1, V, generator=g, device=device) * 2
+    y = x[:, :K] + 0.3 * torch.randn(B, K, V, generator=g, device=device)
+    d = torch.randint(0, V, (B, K), generator=g, device=device)
+    d[:, :2] = y[:, :2].argmax(-1)
+    d[:, 2] = -1
+    d[-1, 1] = -1
+    u = torch.rand(B, K + 1, generator=g, device=device) * 0.9
+    want = RI.verify_draft_tokens(x, d, y if with_q else None, u)
+    x.view(B * (K + 1), V)[(B - 1) * (K + 1) + 2:] = math.nan  # the last sequence's rows 0 and 1 are needed
+    y.view(B * K, V)[(B - 1) * K + 1:] = math.nan              # and its draft's row 0
+    got = _entry_point(x, d, y if with_q else None, u, 1.0, True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert not torch.isnan(got[2]).any()
