@@ -547,7 +547,8 @@ RRL_API int rrl_verify_drafts(const void* target, const void* draft, int32_t dty
  * rrl_mxfp4_dequantize: the numbers they stand for, contiguous [R, H].
  * rrl_mxfp4_linear: out[m, n] = sum_k xq[m, k] wq[n, k], contiguous [M, N]; x is
  * quantised as above within the call, products are summed in float32 and rounded
- * once to out_dtype.  workspace: rrl_mxfp4_linear_workspace_bytes(M, H) bytes of
+ * once to out_dtype.  Its weight's scales are read four at a time and are 4-byte
+ * aligned.  workspace: rrl_mxfp4_linear_workspace_bytes(M, H) bytes of
  * caller device memory (16-byte aligned; contents of no meaning).
  * (The reference's heads are F.linear, rosetrainer/model.py:641.) */
 RRL_API int rrl_mxfp4_quantize(const void* x, int32_t dtype, int64_t R, int64_t H, int64_t ld,

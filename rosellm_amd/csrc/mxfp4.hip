@@ -642,8 +642,9 @@ extern "C" int rrl_mxfp4_linear(const void* x, int32_t dtype, int64_t M, int64_t
               RRL_EINVAL, "rrl_mxfp4_linear: null operand");
   RRL_REQUIRE(M <= 1 || x_ld >= 0, RRL_EINVAL, "rrl_mxfp4_linear: negative row stride");
   RRL_REQUIRE((uintptr_t)x % dtype_size(dtype) == 0 && (uintptr_t)out % dtype_size(out_dtype) == 0 &&
-                  (uintptr_t)codes % 16 == 0 && (uintptr_t)workspace % 16 == 0,
-              RRL_EALIGN, "rrl_mxfp4_linear: a pointer is not aligned (codes: 16 bytes)");
+                  (uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 4 == 0 &&
+                  (uintptr_t)workspace % 16 == 0,
+              RRL_EALIGN, "rrl_mxfp4_linear: a pointer is not aligned (codes: 16 bytes, scales: 4)");
   hipStream_t st = as_stream(stream);
   const LinearLayout l = linear_layout(M, H);
   uint8_t* ac = static_cast<uint8_t*>(workspace);

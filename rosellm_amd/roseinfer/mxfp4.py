@@ -124,9 +124,11 @@ def mxfp4_linear(x: Tensor, weight: MxFp4, out_dtype: Optional[torch.dtype] = No
     dev = nat.require_device(x, weight.codes, weight.scales)
     rows, M, ld = _rows(x.detach())
     H, N = weight.cols, weight.codes.shape[0]
+    # the kernel reads four scales at a time: a view at another address is moved
+    scales = weight.scales if weight.scales.data_ptr() % 4 == 0 else weight.scales.clone()
     out = torch.empty(*x.shape[:-1], N, dtype=out_dtype, device=dev)
     ws = torch.empty(nat.lib().rrl_mxfp4_linear_workspace_bytes(M, H), dtype=torch.uint8, device=dev)
     nat.call_on(dev, "rrl_mxfp4_linear", rows.data_ptr(), nat.dtype_code(x.dtype), M, H, ld,
-                weight.codes.data_ptr(), weight.scales.data_ptr(), N, out.data_ptr(),
+                weight.codes.data_ptr(), scales.data_ptr(), N, out.data_ptr(),
                 nat.dtype_code(out_dtype), ws.data_ptr(), nat.stream_ptr(dev))
     return out
