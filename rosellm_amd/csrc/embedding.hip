@@ -652,39 +652,64 @@ int launch_fwd(const Ids& ids, int64_t N, const void* w, int64_t w_ld, int64_t H
   return check_launch("embed_fwd_kernel");
 }
 
+// Elements of an access of `bytes` bytes: 16-bit types have 16-byte, 4-byte and single
+// accesses only.
+inline int access_elements(int bytes, size_t size) {
+  if (size == 4) return bytes / 4;
+  return bytes == 16 ? 8 : (bytes >= 4 ? 2 : 1);
+}
+
+// The gradient's grids with accesses of `vec` elements.
+struct GradGrid {
+  int u;                          // accesses of a lane along a row
+  int64_t narrow, chunks;         // columns' shares for long runs (64 x vec elements), and for rows (u times that)
+  int64_t pieces, rows, blocks;   // of kPiece positions, of a workgroup's rows of dW, and of embed_grad_kernel
+};
+inline GradGrid grad_grid(int64_t N, int64_t V, int64_t H, int vec) {
+  GradGrid g;
+  g.narrow = (H + 64 * vec - 1) / (64 * vec);
+  g.u = g.narrow <= 1 ? 1 : 2;
+  g.chunks = (g.narrow + g.u - 1) / g.u;
+  // no run is longer than kPiece where the positions end with the first piece
+  g.pieces = N / kPiece;
+  g.rows = (V + kRowWaves * kRowsWave - 1) / (kRowWaves * kRowsWave);
+  g.blocks = g.pieces * g.narrow + g.rows * g.chunks;
+  return g;
+}
+// A grid's threads are counted in 32 bits.  (`narrow`, a second dimension, is at most the
+// 2^16 that one may have: rows are shorter than 2^22.)
+inline bool grad_fits(const GradGrid& g) { return g.blocks < ((int64_t)1 << 32) / (64 * kRowWaves); }
+
 template <typename T, int VEC, int U>
 int launch_rows(const BwdLayout& l, char* ws, int last, int64_t N, int64_t V, const void* g,
-                int64_t g_ld, int64_t H, float scale, void* dw, int64_t dw_ld, hipStream_t st) {
+                int64_t g_ld, int64_t H, float scale, void* dw, int64_t dw_ld, const GradGrid& grid,
+                hipStream_t st) {
   typedef typename T::S S;
   const uint32_t* keys = reinterpret_cast<uint32_t*>(ws + l.keys[last]);
   const uint32_t* pos = reinterpret_cast<uint32_t*>(ws + l.pos[last]);
   uint32_t* begin = reinterpret_cast<uint32_t*>(ws + l.begin);
   uint32_t* end = reinterpret_cast<uint32_t*>(ws + l.end);
   float* partial = reinterpret_cast<float*>(ws + l.partial);
-  const int64_t chunk = 64 * VEC * U;
-  const uint32_t chunks = (uint32_t)((H + chunk - 1) / chunk);
-  const uint32_t narrow = (uint32_t)((H + 64 * VEC - 1) / (64 * VEC));  // more waves for long runs
+  const uint32_t narrow = (uint32_t)grid.narrow;
   if (N > 0) {
     hipLaunchKernelGGL((embed_piece_kernel<T, VEC, 1>), dim3((uint32_t)((N + kPiece - 1) / kPiece), narrow),
                        dim3(64), 0, st, keys, pos, N, (uint32_t)V, static_cast<const S*>(g), g_ld, H,
                        begin, end, partial);
     if (int rc = check_launch("embed_piece_kernel")) return rc;
   }
-  // no run is longer than kPiece where the positions end with the first piece
-  const uint32_t pieces = (uint32_t)(N / kPiece);
-  const int64_t rows = (V + kRowWaves * kRowsWave - 1) / (kRowWaves * kRowsWave);
-  const uint32_t blocks = pieces * narrow + (uint32_t)rows * chunks;  // rrl_embedding_bwd's check
-  hipLaunchKernelGGL((embed_grad_kernel<T, VEC, U>), dim3(blocks), dim3(64 * kRowWaves), 0, st, pieces, narrow,
-                     chunks, keys, pos, N, V, static_cast<const S*>(g), g_ld, H, scale, begin, end, partial, static_cast<S*>(dw), dw_ld);
+  hipLaunchKernelGGL((embed_grad_kernel<T, VEC, U>), dim3((uint32_t)grid.blocks), dim3(64 * kRowWaves), 0, st,
+                     (uint32_t)grid.pieces, narrow, (uint32_t)grid.chunks, keys, pos, N, V,
+                     static_cast<const S*>(g), g_ld, H, scale, begin, end, partial, static_cast<S*>(dw), dw_ld);
   return check_launch("embed_grad_kernel");
 }
 
 template <typename T, int VEC>
 int launch_rows_u(const BwdLayout& l, char* ws, int last, int64_t N, int64_t V, const void* g,
-                  int64_t g_ld, int64_t H, float scale, void* dw, int64_t dw_ld, hipStream_t st) {
-  const int64_t packs = (H + 64 * VEC - 1) / (64 * VEC);
-  if (packs <= 1) return launch_rows<T, VEC, 1>(l, ws, last, N, V, g, g_ld, H, scale, dw, dw_ld, st);
-  return launch_rows<T, VEC, 2>(l, ws, last, N, V, g, g_ld, H, scale, dw, dw_ld, st);
+                  int64_t g_ld, int64_t H, float scale, void* dw, int64_t dw_ld, const GradGrid& grid,
+                  hipStream_t st) {
+  if (grid.u == 1)
+    return launch_rows<T, VEC, 1>(l, ws, last, N, V, g, g_ld, H, scale, dw, dw_ld, grid, st);
+  return launch_rows<T, VEC, 2>(l, ws, last, N, V, g, g_ld, H, scale, dw, dw_ld, grid, st);
 }
 
 int check_common(const char* what, int64_t N, int64_t V, int64_t H, int32_t ids_dtype,
@@ -723,19 +748,20 @@ extern "C" int rrl_embedding_fwd(const void* ids, int32_t ids_dtype, int64_t N, 
   const int b = min(access_bytes(weight, w_ld, H, size), access_bytes(out, H, H, size));
   const float s = (float)scale;
   hipStream_t st = as_stream(stream);
+  const int vec = access_elements(b, size);
 #define RRL_FWD(T, VEC) return launch_fwd<T, VEC>(d, N, weight, w_ld, H, s, out, st)
   if (dtype == RRL_F32) {
-    if (b == 16) RRL_FWD(F32, 4);
-    if (b == 8) RRL_FWD(F32, 2);
+    if (vec == 4) RRL_FWD(F32, 4);
+    if (vec == 2) RRL_FWD(F32, 2);
     RRL_FWD(F32, 1);
   }
   if (dtype == RRL_BF16) {
-    if (b == 16) RRL_FWD(Bf16, 8);
-    if (b >= 4) RRL_FWD(Bf16, 2);
+    if (vec == 8) RRL_FWD(Bf16, 8);
+    if (vec == 2) RRL_FWD(Bf16, 2);
     RRL_FWD(Bf16, 1);
   }
-  if (b == 16) RRL_FWD(F16, 8);
-  if (b >= 4) RRL_FWD(F16, 2);
+  if (vec == 8) RRL_FWD(F16, 8);
+  if (vec == 2) RRL_FWD(F16, 2);
   RRL_FWD(F16, 1);
 #undef RRL_FWD
 }
@@ -762,10 +788,9 @@ extern "C" int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, 
                   (uintptr_t)ids % dtype_size(ids_dtype) == 0 && (uintptr_t)workspace % 16 == 0,
               RRL_EALIGN, "rrl_embedding_bwd: a pointer is not aligned to its element");
   const int b = min(access_bytes(grad, g_ld, H, size), access_bytes(dweight, dw_ld, H, size));
-  // a grid's threads are counted in 32 bits
-  const int64_t wide = (H * (int64_t)size + 64 * b - 1) / (64 * b);
-  RRL_REQUIRE((N / kPiece + V / (kRowWaves * kRowsWave) + 1) * wide < ((int64_t)1 << 32) / (64 * kRowWaves),
-              RRL_EINVAL, "rrl_embedding_bwd: too many ids or rows for their length");
+  const int vec = access_elements(b, size);
+  const GradGrid grid = grad_grid(N, V, H, vec);
+  RRL_REQUIRE(grad_fits(grid), RRL_EINVAL, "rrl_embedding_bwd: too many ids or rows for their length");
   hipStream_t st = as_stream(stream);
   const Ids d{ids, ids_dtype, V, padding_idx, has_padding};
   const BwdLayout l = bwd_layout(N, V, H);
@@ -800,19 +825,20 @@ extern "C" int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, 
     }
   }
   const float sc = (float)scale;
-#define RRL_BWD(T, VEC) return launch_rows_u<T, VEC>(l, ws, last, N, V, grad, g_ld, H, sc, dweight, dw_ld, st)
+#define RRL_BWD(T, VEC) \
+  return launch_rows_u<T, VEC>(l, ws, last, N, V, grad, g_ld, H, sc, dweight, dw_ld, grid, st)
   if (dtype == RRL_F32) {
-    if (b == 16) RRL_BWD(F32, 4);
-    if (b == 8) RRL_BWD(F32, 2);
+    if (vec == 4) RRL_BWD(F32, 4);
+    if (vec == 2) RRL_BWD(F32, 2);
     RRL_BWD(F32, 1);
   }
   if (dtype == RRL_BF16) {
-    if (b == 16) RRL_BWD(Bf16, 8);
-    if (b >= 4) RRL_BWD(Bf16, 2);
+    if (vec == 8) RRL_BWD(Bf16, 8);
+    if (vec == 2) RRL_BWD(Bf16, 2);
     RRL_BWD(Bf16, 1);
   }
-  if (b == 16) RRL_BWD(F16, 8);
-  if (b >= 4) RRL_BWD(F16, 2);
+  if (vec == 8) RRL_BWD(F16, 8);
+  if (vec == 2) RRL_BWD(F16, 2);
   RRL_BWD(F16, 1);
 #undef RRL_BWD
 }
