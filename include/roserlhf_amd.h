@@ -483,15 +483,16 @@ RRL_API int rrl_sample_logprobs(const void* logits, int32_t logits_dtype, int64_
                         float* logp_out, float* logq_out, int32_t* status, void* stream);
 
 /* ---- the token embedding ------------------------------------------------------
- * Lookup: out[i] = scale * weight[id_i], rounded once to `dtype` (F32, BF16 or
- * F16; out is contiguous [N, H], the weight's rows w_ld elements apart).  An id
+ * Lookup: out[i] = scale * weight[id_i] in float32, of the float32 scale (a finite
+ * one past float32's range is refused), rounded to `dtype` (F32, BF16 or F16; out
+ * is contiguous [N, H], the weight's rows w_ld elements apart).  An id
  * equal to padding_idx (has_padding != 0; it may be negative) takes a row of
  * zeros; any other id outside [0, V) takes a row of NaN.  ids: I32 or I64,
  * contiguous.
  * Gradient: dweight[v] = scale * sum of grad[i] over id_i = v, every row of
  * dweight written (zeros where v does not occur, padding and out-of-range ids
- * left out), sums in float32 in an order that depends on the ids alone, rounded
- * once.  workspace: rrl_embedding_bwd_workspace_bytes(N, V, H) bytes of caller
+ * left out), sums and their product with the scale in float32, the sums in an order
+ * that depends on the ids alone, rounded once to `dtype`.  workspace: rrl_embedding_bwd_workspace_bytes(N, V, H) bytes of caller
  * device memory (16-byte aligned; contents in and out are of no meaning).
  * (rosetrainer/model.py and qwen3.py look their tokens up with nn.Embedding.) */
 RRL_API int rrl_embedding_fwd(const void* ids, int32_t ids_dtype, int64_t N, const void* weight,

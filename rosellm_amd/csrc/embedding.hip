@@ -713,13 +713,15 @@ int launch_rows_u(const BwdLayout& l, char* ws, int last, int64_t N, int64_t V, 
 }
 
 int check_common(const char* what, int64_t N, int64_t V, int64_t H, int32_t ids_dtype,
-                 int32_t dtype) {
+                 int32_t dtype, double scale) {
   const std::string w(what);
   RRL_REQUIRE(dtype == RRL_F32 || dtype == RRL_BF16 || dtype == RRL_F16, RRL_EDTYPE,
               w + ": the weight must be float32, bfloat16 or float16");
   RRL_REQUIRE(ids_dtype == RRL_I32 || ids_dtype == RRL_I64, RRL_EDTYPE,
               w + ": ids must be int32 or int64");
   RRL_REQUIRE(N >= 0 && V >= 0 && H >= 0, RRL_EINVAL, w + ": negative size");
+  // (its infinity would make NaN of zeros, and of the rows of dW that no id names)
+  RRL_REQUIRE(!isinf((float)scale) || isinf(scale), RRL_EINVAL, w + ": the scale is past float32's range");
   // the gradient's grids (16 threads a position, 64 a row) are 32-bit
   RRL_REQUIRE(N < ((int64_t)1 << 28) && V < ((int64_t)1 << 26) && H < ((int64_t)1 << 22), RRL_EINVAL,
               w + ": at most 2^28 - 1 ids, and 2^26 - 1 rows of 2^22 - 1 elements");
@@ -735,7 +737,7 @@ extern "C" int rrl_embedding_fwd(const void* ids, int32_t ids_dtype, int64_t N, 
                                  int32_t dtype, int64_t V, int64_t H, int64_t w_ld, double scale,
                                  int64_t padding_idx, int32_t has_padding, void* out, void* stream) {
   clear_error();
-  if (int rc = check_common("rrl_embedding_fwd", N, V, H, ids_dtype, dtype)) return rc;
+  if (int rc = check_common("rrl_embedding_fwd", N, V, H, ids_dtype, dtype, scale)) return rc;
   if (N == 0 || H == 0) return RRL_OK;
   RRL_REQUIRE(ids != nullptr && (weight != nullptr || V == 0) && out != nullptr, RRL_EINVAL,
               "rrl_embedding_fwd: null operand");
@@ -776,7 +778,7 @@ extern "C" int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, 
                                  int64_t padding_idx, int32_t has_padding, void* dweight,
                                  int64_t dw_ld, void* workspace, void* stream) {
   clear_error();
-  if (int rc = check_common("rrl_embedding_bwd", N, V, H, ids_dtype, dtype)) return rc;
+  if (int rc = check_common("rrl_embedding_bwd", N, V, H, ids_dtype, dtype, scale)) return rc;
   if (V == 0 || H == 0) return RRL_OK;
   RRL_REQUIRE((N == 0 || (ids != nullptr && grad != nullptr)) && dweight != nullptr &&
                   workspace != nullptr,

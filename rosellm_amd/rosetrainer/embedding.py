@@ -10,6 +10,8 @@ once, with no float atomics, so equal inputs give equal bits
 
 from __future__ import annotations
 
+import ctypes
+import math
 from typing import Optional
 
 import torch
@@ -64,7 +66,9 @@ def embedding(token_ids: Tensor, weight: Tensor, *, scale: float = 1.0,
               padding_idx: Optional[int] = None) -> Tensor:
     """``scale * weight[token_ids]``: [..., H] in the weight's dtype for
     ``token_ids`` [...] (int32 or int64) and ``weight`` [V, H] (float32, bfloat16
-    or float16), each product rounded once.
+    or float16).  The scale is taken as a float32 number (a finite one past
+    float32's range is refused); the products are float32's, rounded to the
+    weight's dtype.
 
     A token equal to ``padding_idx``, which may be negative (the -1 that
     ``roseinfer.verify_draft_tokens`` leaves past the last verified token), takes
@@ -73,7 +77,8 @@ def embedding(token_ids: Tensor, weight: Tensor, *, scale: float = 1.0,
     no gradient.
 
     The gradient of ``weight`` is dense, in its dtype: float32 sums, in an order
-    that the ids alone decide, rounded once.  It is not differentiable again.
+    that the ids alone decide, times the scale, rounded once to the dtype.  It is
+    not differentiable again.
     """
 
     if token_ids.dtype not in (torch.int64, torch.int32):
@@ -86,4 +91,7 @@ def embedding(token_ids: Tensor, weight: Tensor, *, scale: float = 1.0,
         padding_idx = int(padding_idx)
         if not -2 ** 63 <= padding_idx < 2 ** 63:
             raise ValueError("padding_idx must fit an int64")
-    return _Embedding.apply(token_ids, weight, float(scale), padding_idx)
+    scale = float(scale)
+    if math.isinf(ctypes.c_float(scale).value) and not math.isinf(scale):
+        raise ValueError(f"scale {scale} is past float32's range")
+    return _Embedding.apply(token_ids, weight, scale, padding_idx)
