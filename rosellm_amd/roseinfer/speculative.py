@@ -4,10 +4,15 @@ A draft model proposes K tokens per sequence; one pass of the target model gives
 its logits at those K places and one more.  ``verify_draft_tokens`` keeps the
 longest run of drafts that speculative sampling accepts, draws one more token,
 and returns, as ``sample_next_token_batch`` does, the behaviour log-probability
-of every token that it leaves: the tokens are distributed exactly as if the
-target had sampled them one by one, so they are rollout tokens like any others
-(``PolicyAction.old_logprobs``, roserlhf/trajectory.py:15,27-28).  The reference
-decodes one token per step (roseinfer/engine.py:1103-1171) and has no such step.
+of every token that it leaves.  Where the drafts were drawn from the softmax of the
+draft logits that it is given, the tokens are distributed as if the target had
+sampled them one by one, so they are rollout tokens like any others
+(``PolicyAction.old_logprobs``, roserlhf/trajectory.py:15,27-28).
+``sample_next_token_batch`` draws from ``max(q, 1e-9)``, which lies up to V 1e-9 of
+the mass from that (1.5e-4 at 151,936 entries), and so far at most may a token's
+distribution then lie from the target's; the log-probs are the target's all the
+same.  The reference decodes one token per step (roseinfer/engine.py:1103-1171) and
+has no such step.
 """
 
 from __future__ import annotations
