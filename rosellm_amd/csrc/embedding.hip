@@ -2,7 +2,10 @@
 // tokens.
 //
 //   out[i]     = scale * W[id_i]
-//   dW[v]      = scale * sum_{i : id_i = v} g[i]       (float32 sums, i ascending)
+//   dW[v]      = scale * sum_{i : id_i = v} g[i]       (float32 sums)
+//
+// A sum's order is decided by the ids alone: i ascending in runs of up to kPiece
+// positions, and in longer ones within pieces of kPiece, which are then added up.
 //
 // A padding id takes a row of zeros and passes no gradient; any other id outside
 // [0, V) takes a row of NaN (the host is not waited for) and passes none.
@@ -636,10 +639,13 @@ int launch_fwd(const Ids& ids, int64_t N, const void* w, int64_t w_ld, int64_t H
   const int64_t rows = kThreads / lpr;
   const typename T::S* src = static_cast<const typename T::S*>(w);
   typename T::S* dst = static_cast<typename T::S*>(out);
-  // Four rows in flight where there are enough to fill the chip with them (262,144 rows
-  // of 2 KB: 183 us against 197 us with one), one for a decode step's few (320 rows: 2.8
-  // against 4.1 us).  A grid's threads are counted in 32 bits: past 2^22 workgroups they
-  // take rows in turn.
+  // Four rows in flight where there are enough to fill the chip with them, one for a
+  // decode step's few (320 rows of 2 KB: the kernel takes 2.8 against 4.1 us).  Calls of one
+  // / four took, in us: 1024 bfloat16 (the border is at 16,384 rows): 8,192 rows 7.2 / 7.6,
+  // 16,640 11.1 / 11.5, 24,576 14.7 / 14.8, 65,536 44.1 / 43.3, 262,144 208 / 197; 770
+  // float32 (8,192 rows): 2,048 4.2 / 4.4, 8,192 10.8 / 9.4, 16,384 17.7 / 14.8, 65,536
+  // 93.4 / 71.5.  A grid's threads are counted in 32 bits: past 2^22 workgroups they take
+  // rows in turn.
   const int64_t groups = (N + rows - 1) / rows;
   if (groups <= 8192) {
     hipLaunchKernelGGL((embed_fwd_kernel<T, VEC, 1>), dim3((uint32_t)groups), dim3(kThreads), 0, st, ids,

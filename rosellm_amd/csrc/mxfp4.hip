@@ -259,7 +259,7 @@ __device__ __forceinline__ void store8_buffer(__amdgpu_buffer_rsrc_t out, int of
 // before it.  All loads are unconditional (past an end they read the last fragment or
 // step again, or zeros past the buffer; scalar offsets stay within it, for the bounds
 // check subtracts them): behind a branch the compiler would wait for all of them.
-// 2,048 x 151,936 x 1024 bfloat16 takes 220 us: the matrix instructions alone 147, the
+// 2,048 x 151,936 x 1024 bfloat16 takes 217 us: the matrix instructions alone 147, the
 // same without its stores 170, stores like its own alone 122 (5.1 TB/s).  8 rows take
 // 15 us, the head's 83 MB at 5.5 TB/s.
 // A wave's weight rows are dealt to its fragments so that the 4 x VT outputs a
@@ -663,11 +663,15 @@ extern "C" int rrl_mxfp4_linear(const void* x, int32_t dtype, int64_t M, int64_t
   a.fragments = (int32_t)l.fragments;
   a.out = static_cast<char*>(out);
   a.out_dtype = out_dtype;
-  // a tile's 64 rows are addressed with 32 bits
+  // a tile's rows are addressed with 32 bits: up to 64 of these, or up to 96 with slabs of
+  // 128 weight rows, which are taken for tiles of over 64 only while N is under 2^19
   const int64_t row = N * (int64_t)dtype_size(out_dtype);
   a.aligned = N % 8 == 0 && (uintptr_t)out % 16 == 0 && row < (1 << 25);
   // 128 weight rows to a workgroup, or 256 where those make work enough for rounds of
-  // them (us with 128 / 256, when measured: 8 x 151,936 x 1024 15.2 / 17.3, 130 x 50,257 x
-  // 2080 37 / 42, 2,048 x 151,936 x 1024 288 / 250)
+  // them.  Us with 128 / 256, by activation rows: 151,936 x 1024: 16 17.4 / 19.9, 128 32.8 /
+  // 37.0, 256 68.3 / 59.5, 384 87.2 / 68.0, 400 (the border) 96.1 / 73.8, 1024 204 / 128;
+  // 50,257 x 1024: 512 62.8 / 51.8, 2048 171 / 130; 151,936 x 2048, whose weights do not
+  // stay in registers: 64 53.0 / 60.3, 256 116 / 145, 400 168 / 209, 512 203 / 234.  The
+  // border lies late for weights that stay, and early for those that do not.
   return N * ((l.fragments + 3) / 4) < (1 << 20) ? launch_linear<2>(a, st) : launch_linear<4>(a, st);
 }

@@ -13,9 +13,11 @@
 // A token is decided by where a running sum over the vocabulary passes a border,
 // and there are as many borders as entries: float32 sums (1e-7 of the whole) would
 // pass a wrong one every some ten rows of 150,000 entries.  Exponentials and sums
-// are therefore float64, the exponential a polynomial good to 1.1e-12.  What bounds the
-// kernels is its arithmetic: an entry takes 12 float64 instructions and 6 others, 81 us
-// for the 107 M bfloat16 entries of 64 sequences x (6 + 5) rows x 151,936 (2.6 TB/s).
+// are therefore float64, the exponential a polynomial good to 1.1e-12.  An entry takes 12
+// float64 instructions and 6 others.  For the 107 M bfloat16 entries of 64 sequences x
+// (6 + 5) rows x 151,936 that is 49 us of issue at 2.4 GHz, and their bytes are 45 us at a
+// copy's rate; the first launch takes 80 us (2.7 TB/s), for a wave loads its chunk, finds
+// the maximum and forms the sum one after another, and only other waves fill its waits.
 //
 // Rows are cut into chunks, a wave each, so that a single sequence fills the chip:
 //   1. verify_stats: the chunks of every row that may be needed: maximum, sum
@@ -678,10 +680,13 @@ __global__ __launch_bounds__(kVT) void verify_draw_kernel(VerifyArgs a, Ws ws) {
 // ---- host ---------------------------------------------------------------------------------
 
 // Entries of a chunk: as many as leave the 1024 SIMDs enough waves to hide loads
-// behind, for a longer chunk spends less on its sum.  verify_stats took, with 1024 /
-// 2048 / 4096 entries: 13.8 / 14.6 / 17.0 us at 12,950 chunks of 1024 (half of them
-// behind a draft's end), 18.5 / 17.4 / 19.2 us at 19,072, 2048 / 4096: 85 / 81 us at
-// 104,896.
+// behind, for a longer chunk spends less on its sum.  A call took, in us with 1024 / 2048 /
+// 4096 entries, by its chunks of 1024:
+//   5 drafts of 151,936 bfloat16: 6,556 25.0 / 25.2 / 26.6, 14,751 32.7 / 31.8 / 33.1,
+//   18,029 35.3 / 34.5 / 35.4, 39,336 54.2 / 51.2 / 51.5, 42,614 56.9 / 53.2 / 53.8,
+//   78,672 91.1 / 82.7 / 81.3;
+//   3 drafts of 50,257 float32: 14,000 31.1 / 32.4 / 36.9, 21,000 38.2 / 38.5 / 43.7,
+//   38,500 57.2 / 54.8 / 59.7, 45,500 64.0 / 60.6 / 65.6 (the second border is early here).
 constexpr int64_t kMost1024 = 16384, kMost2048 = 40960;
 inline int chunk_entries(int64_t rows, int64_t V) {
   const int64_t least = rows * ((V + 1023) / 1024);
