@@ -492,8 +492,9 @@ RRL_API int rrl_sample_logprobs(const void* logits, int32_t logits_dtype, int64_
  * Gradient: dweight[v] = scale * sum of grad[i] over id_i = v, every row of
  * dweight written (zeros where v does not occur, padding and out-of-range ids
  * left out), sums and their product with the scale in float32, the sums in an order
- * that depends on the ids alone, rounded once to `dtype`.  workspace: rrl_embedding_bwd_workspace_bytes(N, V, H) bytes of caller
- * device memory (16-byte aligned; contents in and out are of no meaning).
+ * that depends on the ids alone, rounded once to `dtype`.  workspace:
+ * rrl_embedding_bwd_workspace_bytes(N, V, H) bytes of caller device memory (16-byte
+ * aligned; contents in and out are of no meaning).
  * (rosetrainer/model.py and qwen3.py look their tokens up with nn.Embedding.) */
 RRL_API int rrl_embedding_fwd(const void* ids, int32_t ids_dtype, int64_t N, const void* weight,
                     int32_t dtype, int64_t V, int64_t H, int64_t w_ld, double scale,
@@ -549,8 +550,8 @@ RRL_API int rrl_verify_drafts(const void* target, const void* draft, int32_t dty
  * rrl_mxfp4_linear: out[m, n] = sum_k xq[m, k] wq[n, k], contiguous [M, N]; x is
  * quantised as above within the call, products are summed in float32 and rounded
  * once to out_dtype.  Its weight's scales are read four at a time and are 4-byte
- * aligned.  workspace: rrl_mxfp4_linear_workspace_bytes(M, H) bytes of
- * caller device memory (16-byte aligned; contents of no meaning).
+ * aligned.  workspace: rrl_mxfp4_linear_workspace_bytes(M, H) bytes of caller device
+ * memory (16-byte aligned; contents of no meaning).
  * (The reference's heads are F.linear, rosetrainer/model.py:641.) */
 RRL_API int rrl_mxfp4_quantize(const void* x, int32_t dtype, int64_t R, int64_t H, int64_t ld,
                     uint8_t* codes, uint8_t* scales, void* stream);
