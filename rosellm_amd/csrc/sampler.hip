@@ -43,31 +43,13 @@
 // the nucleus does, leaves the row to the passes above.
 // Ties at a top-k or top-p threshold are kept lowest index first; they are
 // located with the same vocabulary-order search over 0/1 weights.
+#include "philox.hpp"
 #include "row_common.hpp"
 #include "wave_common.hpp"
 
 #include <type_traits>
 
 namespace rrl {
-
-// Philox4x32-10 (J. Salmon, M. Moraes, R. Dror, D. Shaw, "Parallel random
-// numbers: as easy as 1, 2, 3", SC 2011): ten rounds of two 32x32->64
-// multiplies with the published multipliers and Weyl key increments.
-__host__ __device__ inline void philox4x32_10(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
-  const uint32_t kM0 = 0xD2511F53u, kM1 = 0xCD9E8D57u;
-  const uint32_t kW0 = 0x9E3779B9u, kW1 = 0xBB67AE85u;
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t p0 = (uint64_t)kM0 * c[0];
-    const uint64_t p1 = (uint64_t)kM1 * c[2];
-    const uint32_t n0 = (uint32_t)(p1 >> 32) ^ c[1] ^ k0;
-    const uint32_t n1 = (uint32_t)p1;
-    const uint32_t n2 = (uint32_t)(p0 >> 32) ^ c[3] ^ k1;
-    const uint32_t n3 = (uint32_t)p0;
-    c[0] = n0; c[1] = n1; c[2] = n2; c[3] = n3;
-    k0 += kW0;
-    k1 += kW1;
-  }
-}
 
 namespace {
 
