@@ -505,6 +505,28 @@ RRL_API int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, con
                     int64_t padding_idx, int32_t has_padding, void* dweight, int64_t dw_ld,
                     void* workspace, void* stream);
 
+/* ---- dropout from a counter-based generator ------------------------------------
+ * out = residual + (kept ? x / (1 - p') : 0), contiguous [rows, cols], of x and (or
+ * NULL) residual [rows, cols], rows x_ld and r_ld elements apart, all `dtype` (F32,
+ * BF16 or F16); the sum is float32's, rounded once.  Nothing is stored of the mask: the
+ * gradient of x is the same call on the gradient of out.
+ * The entries of a row are taken in groups of eight, ceil(cols / 8) to a row, numbered
+ * through all rows.  Group i has the four words of Philox4x32-10 (rrl_philox4x32_10) at
+ * counter {i, i >> 32, o, o >> 32} under the key {seed, seed >> 32}; entry j of it the
+ * half j % 2 (0: the low one) of word j / 2, a number under 65536, and is kept where
+ * that is at least round(65536 p) = 65536 p'.  o = offset + *offset_device (modulo
+ * 2^64), so that a captured graph can take another mask at each replay. */
+typedef struct rrl_dropout_params {
+  double p;                      /* in [0, 1] */
+  uint64_t seed;
+  uint64_t offset;
+  const int64_t* offset_device;  /* one int64 in device memory, or NULL for 0 */
+} rrl_dropout_params;
+
+RRL_API int rrl_dropout(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t x_ld,
+                    const void* residual, int64_t r_ld, const rrl_dropout_params* params,
+                    void* out, void* stream);
+
 /* ---- rollout side: verification of drafted tokens ------------------------------
  * Speculative sampling from given uniforms (the reference decodes one token per
  * step, roseinfer/engine.py:1103-1171).  target: logits [B, K + 1, V], draft:
@@ -562,7 +584,7 @@ RRL_API int rrl_mxfp4_linear(const void* x, int32_t dtype, int64_t M, int64_t H,
                     const uint8_t* codes, const uint8_t* scales, int64_t N, void* out,
                     int32_t out_dtype, void* workspace, void* stream);
 
-/* Philox4x32-10 on the host (the generator rrl_sample_logprobs draws from):
+/* Philox4x32-10 on the host (the generator of rrl_sample_logprobs and rrl_dropout):
  * ctr[4] is replaced by the 4 output words. */
 RRL_API void rrl_philox4x32_10(uint32_t ctr[4], const uint32_t key[2]);
 

@@ -83,6 +83,15 @@ class RrlScalars(ctypes.Structure):
     _fields_ = [("ptr", ctypes.c_void_p * 5), ("dtype", ctypes.c_int32 * 5)]
 
 
+class RrlDropoutParams(ctypes.Structure):
+    _fields_ = [
+        ("p", ctypes.c_double),
+        ("seed", ctypes.c_uint64),
+        ("offset", ctypes.c_uint64),
+        ("offset_device", ctypes.c_void_p),
+    ]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -90,6 +99,7 @@ _D = ctypes.c_double
 _V = RrlView
 _PP = ctypes.POINTER(RrlPolicyParams)
 _PS = ctypes.POINTER(RrlScalars)
+_PD = ctypes.POINTER(RrlDropoutParams)
 
 # name -> (restype, argtypes); mirrors include/roserlhf_amd.h
 SIGNATURES = {
@@ -143,6 +153,7 @@ SIGNATURES = {
     "rrl_embedding_fwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _D, _I64, _I32, _P, _P]),
     "rrl_embedding_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
     "rrl_embedding_bwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _D, _I64, _I32, _P, _I64, _P, _P]),
+    "rrl_dropout": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _I64, _PD, _P, _P]),
     "rrl_philox4x32_10": (None, [ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(ctypes.c_uint32)]),
 }
 

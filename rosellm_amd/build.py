@@ -35,6 +35,7 @@ SOURCES = [
     "embedding.hip",
     "verify.hip",
     "mxfp4.hip",
+    "dropout.hip",
 ]
 
 ARCH = os.environ.get("ROSELLM_AMD_ARCH", "gfx950")

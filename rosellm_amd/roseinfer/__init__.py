@@ -1,7 +1,8 @@
 """MI355X-native pieces of ``rosellm.roseinfer`` on the RoseRLHF path: the
 next-token sampler of roseinfer/engine.py:1088-1171, returning the behaviour
 log-probabilities that rollout records need (roserlhf/trajectory.py:15,27-28);
-the verification of drafted tokens, which returns them too; and a draft model's
+the
+verification of drafted tokens, which returns them too; and a draft model's
 head in microscaled 4-bit floating point."""
 
 from .mxfp4 import MxFp4, dequantize_mxfp4, mxfp4_linear, quantize_mxfp4

@@ -39,6 +39,7 @@ import torch
 from torch import Tensor
 
 from .. import _native as nat
+from .._random import draw_seed
 
 __all__ = ["SampleOutput", "sample_next_token", "sample_next_token_batch"]
 
@@ -48,12 +49,6 @@ class SampleOutput(NamedTuple):
     logprobs: Tensor                     # [B] float32, log_softmax(logits / T)[token]
     sampling_logprobs: Optional[Tensor]  # [B] float32, log q(token) of the sampled
                                          # distribution (None when not asked for)
-
-
-def _draw_seed(generator: Optional[torch.Generator]) -> int:
-    """A 63-bit seed from a host generator (no device sync)."""
-
-    return int(torch.randint(0, 2 ** 63 - 1, (1,), generator=generator, dtype=torch.int64).item())
 
 
 def sample_next_token_batch(
@@ -92,7 +87,7 @@ def sample_next_token_batch(
     if V == 0:
         raise ValueError("logits need at least one vocabulary entry")
     if seed is None:
-        seed = _draw_seed(generator)
+        seed = draw_seed(generator)
     tokens = torch.empty(B, dtype=torch.int64, device=dev)
     logp = torch.empty(B, dtype=torch.float32, device=dev)
     logq = torch.empty(B, dtype=torch.float32, device=dev) if sampling_logprobs else None
