@@ -505,6 +505,37 @@ RRL_API int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, con
                     int64_t padding_idx, int32_t has_padding, void* dweight, int64_t dw_ld,
                     void* workspace, void* stream);
 
+/* ---- rollout side: tokens from given uniforms, settings per row ------------------
+ * logits: [B, V] rows of F32, BF16 or F16, row_stride elements apart.  uniforms: B
+ * float32 in [0, 1).  Settings: one for all rows, or (where the array is not NULL) one a
+ * row, contiguous.  Per row, with p = softmax(x / T):
+ *   the top_k largest are left (0 < top_k < V; ties lowest index first);
+ *   of these, in descending order, those whose inclusive sum of p, over the sum of all of
+ *   these, is at most top_p (0 < top_p < 1), the first always;
+ *   of these, those with x - max x >= T log(min(min_p, 1)) (min_p > 0);
+ * token_out (int64 [B]): the first index, in vocabulary order, at which the running sum of
+ * what is left exceeds u times its whole.  logp_out (float32 [B]): log p of it;
+ * logq_out (float32 [B], or NULL): log of its p over what is left.  T <= 0: the first
+ * maximum, with T = 1 and logq 0; u is not looked at.  Exponentials are float64 (1.1e-12)
+ * and summed in units of 2^-44 of the largest (2^-(62 - b) for 2^b > 2^18 entries), and
+ * u times the whole below one unit counts as 0.
+ * A row with NaN or +inf, or with nothing above -inf, and a temperature that is NaN or
+ * +inf give token -1 and NaN log-probs.  (The reference has one setting for all rows and
+ * no min-p, roseinfer/engine.py:1103-1171.) */
+typedef struct rrl_sample_params {
+  double temperature, top_p, min_p;
+  int64_t top_k;
+  const float* temperatures;
+  const float* top_ps;
+  const float* min_ps;
+  const void* top_ks;  /* I32 or I64 */
+  int32_t top_k_dtype;
+} rrl_sample_params;
+
+RRL_API int rrl_sample_tokens(const void* logits, int32_t dtype, int64_t B, int64_t V,
+                    int64_t row_stride, const float* uniforms, const rrl_sample_params* params,
+                    int64_t* token_out, float* logp_out, float* logq_out, void* stream);
+
 /* ---- dropout from a counter-based generator ------------------------------------
  * out = residual + (kept ? x / (1 - p') : 0), contiguous [rows, cols], of x and (or
  * NULL) residual [rows, cols], rows x_ld and r_ld elements apart, all `dtype` (F32,

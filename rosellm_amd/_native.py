@@ -92,6 +92,20 @@ class RrlDropoutParams(ctypes.Structure):
     ]
 
 
+class RrlSampleParams(ctypes.Structure):
+    _fields_ = [
+        ("temperature", ctypes.c_double),
+        ("top_p", ctypes.c_double),
+        ("min_p", ctypes.c_double),
+        ("top_k", ctypes.c_int64),
+        ("temperatures", ctypes.c_void_p),
+        ("top_ps", ctypes.c_void_p),
+        ("min_ps", ctypes.c_void_p),
+        ("top_ks", ctypes.c_void_p),
+        ("top_k_dtype", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -99,6 +113,7 @@ _D = ctypes.c_double
 _V = RrlView
 _PP = ctypes.POINTER(RrlPolicyParams)
 _PS = ctypes.POINTER(RrlScalars)
+_PT = ctypes.POINTER(RrlSampleParams)
 _PD = ctypes.POINTER(RrlDropoutParams)
 
 # name -> (restype, argtypes); mirrors include/roserlhf_amd.h
@@ -153,6 +168,7 @@ SIGNATURES = {
     "rrl_embedding_fwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _D, _I64, _I32, _P, _P]),
     "rrl_embedding_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
     "rrl_embedding_bwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _D, _I64, _I32, _P, _I64, _P, _P]),
+    "rrl_sample_tokens": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _PT, _P, _P, _P, _P]),
     "rrl_dropout": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _I64, _PD, _P, _P]),
     "rrl_philox4x32_10": (None, [ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(ctypes.c_uint32)]),
 }

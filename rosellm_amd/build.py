@@ -35,6 +35,7 @@ SOURCES = [
     "embedding.hip",
     "verify.hip",
     "mxfp4.hip",
+    "choose.hip",
     "dropout.hip",
 ]
 
