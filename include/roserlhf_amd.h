@@ -558,6 +558,46 @@ RRL_API int rrl_dropout(const void* x, int32_t dtype, int64_t rows, int64_t cols
                     const void* residual, int64_t r_ld, const rrl_dropout_params* params,
                     void* out, void* stream);
 
+/* ---- low-rank adapters of many requests beside a shared projection ----------------
+ * out[n] = base[n] + scale_a up_a (down_a drop(x[n])), a = ids[n], contiguous [N, O]; a
+ * negative id: base[n] alone; an id of A or more: NaN.  x [N, H], base [N, O] (or NULL:
+ * zeros), down [A, r, H] (entry (a, r, h) at a * down_sa + r * down_sr + h), up [A, O, r]
+ * (entry (a, o, r) at a * up_sa + o * up_so + r), all `dtype` (F32, BF16 or F16); ids
+ * contiguous I32 or I64 (NULL with A = 1: all 0); scales float32 [A] (NULL: 1); dropout
+ * (or NULL) of x, as rrl_dropout's.  Ranks up to 128, up to 4096 adapters.  Products are
+ * summed in float32; t = down_a drop(x) is float32, taken to 2^-17 by the second product
+ * of 16-bit operands; one rounding to `dtype`.
+ * t_out: NULL, or float32 [N, rrl_adapter_rank_padded(r)] (16-byte aligned), t of the rows
+ * that have an adapter, for the gradient of up.
+ * rrl_adapter_bwd, of grad = d out [N, O]: dx [N, H], ddown [A, r, H], dup [A, O, r], all
+ * contiguous and each NULL where it is not wanted; ddown and dup are written for every
+ * adapter (zeros where a has no row), dx for every row (zeros without an adapter).  x is
+ * read for ddown, t for dup.  Sums over rows are float32's, in an order that the ids and
+ * sizes alone decide, rounded once.  workspace: rrl_adapter_bwd_workspace_bytes(...) bytes
+ * of caller device memory (16-byte aligned; contents of no meaning).
+ * (The reference has no adapters; its projections are F.linear, rosetrainer/model.py.) */
+typedef struct rrl_adapter_params {
+  int32_t dtype;
+  int64_t N, H, O, A, r;
+  const void* down;
+  int64_t down_sa, down_sr;
+  const void* up;
+  int64_t up_sa, up_so;
+  const void* ids;
+  int32_t ids_dtype;
+  const float* scales;
+  const rrl_dropout_params* dropout;
+} rrl_adapter_params;
+
+RRL_API int64_t rrl_adapter_rank_padded(int64_t r);
+RRL_API int rrl_adapter_fwd(const rrl_adapter_params* params, const void* x, int64_t x_ld,
+                    const void* base, int64_t base_ld, void* out, float* t_out, void* stream);
+RRL_API size_t rrl_adapter_bwd_workspace_bytes(int64_t N, int64_t H, int64_t O, int64_t A,
+                    int64_t r, int32_t dtype);
+RRL_API int rrl_adapter_bwd(const rrl_adapter_params* params, const void* x, int64_t x_ld,
+                    const void* grad, int64_t g_ld, const float* t, void* dx, void* ddown,
+                    void* dup, void* workspace, void* stream);
+
 /* ---- rollout side: verification of drafted tokens ------------------------------
  * Speculative sampling from given uniforms (the reference decodes one token per
  * step, roseinfer/engine.py:1103-1171).  target: logits [B, K + 1, V], draft:

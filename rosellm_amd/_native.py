@@ -106,6 +106,27 @@ class RrlSampleParams(ctypes.Structure):
     ]
 
 
+class RrlAdapterParams(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("N", ctypes.c_int64),
+        ("H", ctypes.c_int64),
+        ("O", ctypes.c_int64),
+        ("A", ctypes.c_int64),
+        ("r", ctypes.c_int64),
+        ("down", ctypes.c_void_p),
+        ("down_sa", ctypes.c_int64),
+        ("down_sr", ctypes.c_int64),
+        ("up", ctypes.c_void_p),
+        ("up_sa", ctypes.c_int64),
+        ("up_so", ctypes.c_int64),
+        ("ids", ctypes.c_void_p),
+        ("ids_dtype", ctypes.c_int32),
+        ("scales", ctypes.c_void_p),
+        ("dropout", ctypes.POINTER(RrlDropoutParams)),
+    ]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
@@ -113,6 +134,7 @@ _D = ctypes.c_double
 _V = RrlView
 _PP = ctypes.POINTER(RrlPolicyParams)
 _PS = ctypes.POINTER(RrlScalars)
+_PA = ctypes.POINTER(RrlAdapterParams)
 _PT = ctypes.POINTER(RrlSampleParams)
 _PD = ctypes.POINTER(RrlDropoutParams)
 
@@ -169,6 +191,10 @@ SIGNATURES = {
     "rrl_embedding_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
     "rrl_embedding_bwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _D, _I64, _I32, _P, _I64, _P, _P]),
     "rrl_sample_tokens": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _PT, _P, _P, _P, _P]),
+    "rrl_adapter_rank_padded": (_I64, [_I64]),
+    "rrl_adapter_fwd": (ctypes.c_int, [_PA, _P, _I64, _P, _I64, _P, _P, _P]),
+    "rrl_adapter_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, _I64, _I32]),
+    "rrl_adapter_bwd": (ctypes.c_int, [_PA, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P]),
     "rrl_dropout": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _I64, _PD, _P, _P]),
     "rrl_philox4x32_10": (None, [ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(ctypes.c_uint32)]),
 }

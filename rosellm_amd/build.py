@@ -36,6 +36,7 @@ SOURCES = [
     "verify.hip",
     "mxfp4.hip",
     "choose.hip",
+    "adapters.hip",
     "dropout.hip",
 ]
 

@@ -1,0 +1,980 @@
+// Low-rank updates of many requests' adapters beside a shared projection, and their
+// gradients.
+//
+//   y_n = base_n + scale_a up_a t_n,   t_n = down_a drop(x_n),   a = id_n
+//   s_n = up_a^T g_n
+//   dx_n = scale_a drop'(down_a^T s_n)
+//   d down_a = scale_a sum_n s_n drop(x_n)^T,   d up_a = scale_a sum_n g_n t_n^T
+//
+// down_a [r, H] and up_a [O, r] are thin (r up to 128), so that all of this is bound by
+// reading and writing the rows of N tokens: 2 r operations an entry.
+//
+// Rows of one adapter stand together only within a request, so a workgroup takes a
+// window of 1024 tokens, sorts it by adapter in LDS (a counting sort; a window of one
+// adapter needs none), and its tiles of 16 or 64 rows are of one adapter each, whatever
+// the order of the ids: no other launch, no list kept between calls.
+//
+// The fused kernel forms t of a tile (the depth H split over four waves, their sums
+// joined in LDS in order) and multiplies it by a run of rows of up while it is there, so
+// t makes no way through memory between the two products.  d x is the same kernel on g
+// with the transposes of up and down, which are laid out by a launch of their own.
+//
+// t is float32.  The second product's bfloat16 instruction takes it as the sum of two
+// bfloat16 numbers, to 2^-17: one rounding to bfloat16 (2^-9) would be as large as that
+// of the result.  With float16 operands, whose range t can leave, up is taken as the
+// exact sum of two bfloat16 numbers as well; the product of the two low parts (2^-18)
+// is left out.  float32 operands take the float32 instruction.
+#include "dropout_common.hpp"
+#include "vocab_weights.hpp"
+
+#include <type_traits>
+
+namespace rrl {
+namespace {
+
+constexpr int kAT = 256, kAW = kAT / 64;  // a workgroup's threads and waves
+constexpr int kWindow = 1024;             // tokens that a workgroup sorts
+constexpr int kMostAdapters = 4096, kMostRank = 128;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x4 mma_bf16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                 0, 0);
+}
+
+// Eight consecutive entries as they stand in memory.
+template <class Tag>
+struct Frag {
+  static constexpr int EPV = Pack16<Tag>::EPV, NV = 8 / EPV, SZ = 16 / EPV;
+  u32x4 v[NV];
+  // entries i..i+7 of a row that may start at any element, zeros from n on
+  __device__ __forceinline__ void load(const char* row, int64_t i, int64_t n) {
+    if (i + 8 <= n) {
+#pragma unroll
+      for (int h = 0; h < NV; ++h) v[h] = reinterpret_cast<const Any16*>(row + i * SZ)[h].v;
+      return;
+    }
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = i + k < n ? load_entry<Tag>(row, i + k) : 0.0f;
+    pack(x);
+  }
+  __device__ __forceinline__ void pack(const float (&x)[8]) {
+#pragma unroll
+    for (int h = 0; h < NV; ++h) {
+      float part[EPV];
+#pragma unroll
+      for (int k = 0; k < EPV; ++k) part[k] = x[h * EPV + k];
+      v[h] = Pack16<Tag>::pack(part);
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&x)[8]) const {
+#pragma unroll
+    for (int h = 0; h < NV; ++h) {
+      float part[EPV];
+      Pack16<Tag>::unpack(v[h], part);
+#pragma unroll
+      for (int k = 0; k < EPV; ++k) x[h * EPV + k] = part[k];
+    }
+  }
+  __device__ __forceinline__ void store(char* row, int64_t i, int64_t n) const {
+    if (i + 8 <= n) {
+#pragma unroll
+      for (int h = 0; h < NV; ++h) reinterpret_cast<Any16*>(row + i * SZ)[h].v = v[h];
+      return;
+    }
+    float x[8];
+    unpack(x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (i + k < n) {
+        if constexpr (SZ == 4) reinterpret_cast<float*>(row)[i + k] = x[k];
+        else reinterpret_cast<uint16_t*>(row)[i + k] = (uint16_t)Pack16<Tag>::pack_one(x[k]);
+      }
+  }
+  // zeros where an entry is dropped
+  __device__ __forceinline__ void keep(uint32_t bits) {
+#pragma unroll
+    for (int h = 0; h < NV; ++h)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        if constexpr (SZ == 4) {
+          v[h][d] = bits >> (4 * h + d) & 1 ? v[h][d] : 0u;
+        } else {
+          const uint32_t two = bits >> (2 * d) & 3;
+          v[h][d] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
+        }
+      }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int h = 0; h < NV; ++h) v[h] = u32x4{0, 0, 0, 0};
+  }
+};
+
+// c += a b^T over the 32 entries of depth that the four groups of 16 lanes hold, eight
+// each: rows of the result 4 (lane / 16) + i from a's lanes, columns lane % 16 from b's.
+template <class Tag>
+__device__ __forceinline__ f32x4 mma(const Frag<Tag>& a, const Frag<Tag>& b, f32x4 c) {
+  if constexpr (std::is_same_v<Tag, TagBF16>) {
+    return mma_bf16(a.v[0], b.v[0], c);
+  } else if constexpr (std::is_same_v<Tag, TagF16>) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.v[0]),
+                                                  __builtin_bit_cast(f16x8, b.v[0]), c, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.v[k / 4][k % 4]), __uint_as_float(b.v[k / 4][k % 4]),
+                                               c, 0, 0, 0);
+    return c;
+  }
+}
+
+// Two numbers as sums of two bfloat16 numbers each.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = f32x2_to_bf16x2_bits(a, b);
+  const float ha = __uint_as_float(hi << 16), hb = __uint_as_float(hi & 0xffff0000u);
+  // (an infinity leaves no rest)
+  lo = f32x2_to_bf16x2_bits(a == ha ? 0.0f : a - ha, b == hb ? 0.0f : b - hb);
+}
+__device__ __forceinline__ void split8(const float (&x)[8], u32x4& hi, u32x4& lo) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    uint32_t h, l;
+    split2(x[2 * d], x[2 * d + 1], h, l);
+    hi[d] = h;
+    lo[d] = l;
+  }
+}
+
+// The second product: rows of up against t, depth R = 16 R16.  16-bit operands take 32
+// entries of depth at once: ranks up to 16 hold t's high parts in the first half of them
+// and its low parts in the second, beside up's entries twice.
+template <class Tag, int R16>
+struct Thin {  // t of 16 tokens
+  static constexpr bool F32 = std::is_same_v<Tag, TagF32>, F16 = std::is_same_v<Tag, TagF16>;
+  static constexpr int KS = R16 == 1 ? 1 : R16 / 2;
+  static constexpr int NF = F32 ? 4 * R16 : 0;
+  u32x4 hi[F32 ? 1 : KS], lo[F32 ? 1 : KS];
+  float f[F32 ? NF : 1];
+  __device__ __forceinline__ void load(const float* t, int kb) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int k = 0; k < NF; ++k) f[k] = t[NF * kb + k];
+    } else {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int at = R16 == 1 ? 8 * (kb & 1) : 32 * s + 8 * kb;
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = t[at + k];
+        split8(x, hi[s], lo[s]);
+        if constexpr (R16 == 1) {
+          const u32x4 h = hi[0], l = lo[0], none = {0, 0, 0, 0};
+          hi[0] = kb < 2 ? h : l;
+          lo[0] = kb < 2 ? h : none;  // beside up's low parts
+        }
+      }
+    }
+  }
+};
+template <class Tag, int R16>
+struct UpRow {  // a lane's row of up
+  using T = Thin<Tag, R16>;
+  Frag<Tag> v[T::F32 ? (T::NF + 7) / 8 : T::KS];
+  __device__ __forceinline__ void load(const char* row, int r, int kb) {
+    if constexpr (T::F32) {
+      if constexpr (T::NF >= 8) {
+#pragma unroll
+        for (int s = 0; s < T::NF / 8; ++s) v[s].load(row, T::NF * kb + 8 * s, r);
+      } else {
+        // four entries to a lane
+        v[0].clear();
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (4 * kb + k < r) v[0].v[0][k] = reinterpret_cast<const uint32_t*>(row)[4 * kb + k];
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < T::KS; ++s) v[s].load(row, R16 == 1 ? 8 * (kb & 1) : 32 * s + 8 * kb, r);
+    }
+  }
+};
+template <class Tag, int R16>
+__device__ __forceinline__ f32x4 expand(const UpRow<Tag, R16>& u, const Thin<Tag, R16>& t, f32x4 c) {
+  using T = Thin<Tag, R16>;
+  if constexpr (T::F32) {
+#pragma unroll
+    for (int k = 0; k < T::NF; ++k)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(u.v[k / 8].v[k / 4 % 2][k % 4]), t.f[k], c, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int s = 0; s < T::KS; ++s) {
+      if constexpr (T::F16) {
+        float x[8];
+        u32x4 hi, lo;
+        u.v[s].unpack(x);
+        split8(x, hi, lo);
+        c = mma_bf16(hi, t.hi[s], c);
+        if constexpr (R16 > 1) {
+          c = mma_bf16(hi, t.lo[s], c);
+          c = mma_bf16(lo, t.hi[s], c);
+        } else {
+          c = mma_bf16(lo, t.lo[s], c);
+        }
+      } else {
+        c = mma_bf16(u.v[s].v[0], t.hi[s], c);
+        if constexpr (R16 > 1) c = mma_bf16(u.v[s].v[0], t.lo[s], c);
+      }
+    }
+  }
+  return c;
+}
+
+struct AdapterIds {
+  const void* ids;  // null: adapter 0 everywhere
+  int dt, A;
+  // the adapter, A for none (a negative id), or A + 1 for an id that there is none of
+  __device__ __forceinline__ int at(int64_t n) const {
+    if (!ids) return 0;
+    const int64_t id = load_index(ids, dt, n);
+    return id < 0 ? A : (id < A ? (int)id : A + 1);
+  }
+};
+
+struct FusedArgs {
+  const char *x, *down, *up, *base;  // base may be null
+  int64_t x_ld, d_sa, d_sr, u_sa, u_so, b_ld;
+  AdapterIds ids;
+  const float* scales;  // null: 1
+  char* out;            // contiguous [N, O]; null: t alone
+  float* t;             // [N, 16 R16], or null
+  int64_t N, K, O;
+  int r;
+  int groups;           // workgroups of a window
+  int slabs;            // runs of up's rows that a tile's work is cut into
+  int64_t slab;         // their length
+  Drop drop;
+  int drop_in, drop_out;
+  int nan_rows;         // rows of ids that there are none of: NaN, or zeros
+};
+
+template <class Tag, int R16, int MT>
+__global__ __launch_bounds__(kAT) void adapter_fused_kernel(FusedArgs a) {
+  constexpr int SZ = 16 / Pack16<Tag>::EPV, TM = 16 * MT, R = 16 * R16, kAhead = 4, kChunks = kWindow / kAT;
+  constexpr int kLd = R + 4;  // a row of t in LDS
+  __shared__ uint16_t order[kWindow];
+  __shared__ __attribute__((aligned(16))) float part[kAW][TM][kLd];
+  __shared__ int scan[2][kAW];
+  extern __shared__ int bins[];  // first place and first tile of each adapter, of none and bad, and the ends
+  const int A2 = a.ids.A + 2;
+  int* const start = bins;
+  int* const tiles = start + A2 + 1;
+  uint16_t* const seen = reinterpret_cast<uint16_t*>(tiles + A2 + 1);  // rows of each by wave
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, kb = lane >> 4, q = lane & 15;
+  const int64_t window = blockIdx.x / a.groups;
+  const int group = (int)(blockIdx.x % a.groups);
+  const int64_t n0 = window * kWindow;
+  const int count = (int)min((int64_t)kWindow, a.N - n0);
+
+  // the window's rows by adapter, in order: every workgroup of the window has to come to
+  // the same tiles.  A wave looks at a quarter of them.
+  int code[kChunks];
+  bool same = true;
+  const int first = a.ids.at(n0), i0 = wv * (kWindow / kAW) + lane;
+#pragma unroll
+  for (int k = 0; k < kChunks; ++k) {
+    code[k] = i0 + 64 * k < count ? a.ids.at(n0 + i0 + 64 * k) : first;
+    same &= code[k] == first;
+  }
+  const bool one = __syncthreads_and(same);
+  if (!one) {
+    for (int k = t; k < kAW * A2; k += kAT) seen[k] = 0;
+    __syncthreads();
+    int rank[kChunks];  // among the wave's rows of the same adapter
+    volatile uint16_t* const mine = seen + wv * A2;
+    const int bits = 32 - __clz(A2);
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) {
+      const bool in = i0 + 64 * k < count;
+      uint64_t like = __ballot(in);
+      for (int b = 0; b < bits; ++b) {
+        const uint64_t set = __ballot(code[k] >> b & 1);
+        like &= code[k] >> b & 1 ? set : ~set;
+      }
+      rank[k] = 0;
+      if (in) {
+        rank[k] = mine[code[k]] + __popcll(like & (((uint64_t)1 << lane) - 1));
+        if (lane == 63 - __clzll((long long)like)) mine[code[k]] = (uint16_t)(rank[k] + 1);
+      }
+    }
+    __syncthreads();
+    // exclusive sums of rows and tiles, a run of bins to a thread
+    const int per = (A2 + kAT - 1) / kAT, lo = min(t * per, A2), hi = min(lo + per, A2);
+    int rows = 0, tls = 0;
+    for (int k = lo; k < hi; ++k) {
+      int c = 0;
+      for (int w = 0; w < kAW; ++w) c += seen[w * A2 + k];
+      start[k] = c;
+      rows += c;
+      tls += (c + TM - 1) / TM;
+    }
+    int rsum = rows, tsum = tls;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(rsum, o, 64), z = __shfl_up(tsum, o, 64);
+      if (lane >= o) {
+        rsum += y;
+        tsum += z;
+      }
+    }
+    if (lane == 63) {
+      scan[0][wv] = rsum;
+      scan[1][wv] = tsum;
+    }
+    __syncthreads();
+    rsum -= rows;
+    tsum -= tls;
+    for (int k = 0; k < wv; ++k) {
+      rsum += scan[0][k];
+      tsum += scan[1][k];
+    }
+    for (int k = lo; k < hi; ++k) {
+      const int c = start[k];
+      start[k] = rsum;
+      tiles[k] = tsum;
+      rsum += c;
+      tsum += (c + TM - 1) / TM;
+    }
+    if (hi == A2 && lo < hi) {  // the thread of the last bin
+      start[A2] = rsum;
+      tiles[A2] = tsum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k)
+      if (i0 + 64 * k < count) {
+        int at = start[code[k]] + rank[k];
+        for (int w = 0; w < wv; ++w) at += seen[w * A2 + code[k]];
+        order[at] = (uint16_t)(i0 + 64 * k);
+      }
+    __syncthreads();
+  }
+  const int all = one ? (count + TM - 1) / TM : tiles[A2];
+  const uint64_t at = a.drop_in || a.drop_out ? a.drop.counter() : 0;
+
+  for (int64_t it = group; it < (int64_t)all * a.slabs; it += a.groups) {
+    const int tile = (int)(it / a.slabs), slab = (int)(it % a.slabs);
+    int ad = first, row0 = tile * TM, end = count;
+    if (!one) {  // the last bin that starts at or before the tile and is not empty
+      int lo = 0, hi = A2;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (tiles[mid] <= tile) lo = mid;
+        else hi = mid;
+      }
+      ad = lo;
+      row0 = start[ad] + (tile - tiles[ad]) * TM;
+      end = start[ad + 1];
+    }
+    const int here = min(TM, end - row0);
+    const int64_t c0 = slab * a.slab, c1 = min(c0 + a.slab, a.O);
+    auto token = [&](int i) { return n0 + (one ? row0 + i : (int)order[row0 + i]); };
+
+    if (ad >= a.ids.A) {  // rows without an adapter
+      if (!a.out) continue;
+      const int per = (int)((c1 - c0 + 7) / 8);
+      for (int64_t k = t; k < (int64_t)here * per; k += kAT) {
+        const int64_t n = token((int)(k / per)), c = c0 + k % per * 8;
+        Frag<Tag> v;
+        v.clear();
+        if (ad == a.ids.A) {
+          if (a.base) v.load(a.base + n * a.b_ld * SZ, c, c1);
+        } else if (a.nan_rows) {
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = M<float>::nan();
+          v.pack(x);
+        }
+        v.store(a.out + n * a.O * SZ, c, c1);
+      }
+      continue;
+    }
+
+    // t of the tile's rows: a wave takes a quarter of the depth
+    int64_t n[MT];
+#pragma unroll
+    for (int f = 0; f < MT; ++f) n[f] = token(min(16 * f + q, here - 1));  // past the end the last again
+    {
+      f32x4 acc[MT][R16] = {};
+      const char* down = a.down + ad * a.d_sa * SZ;
+      const int64_t steps = (a.K + 31) / 32, per_row = (a.K + 7) / 8;
+      const int64_t s0 = steps * wv / kAW, s1 = steps * (wv + 1) / kAW;
+      for (int64_t s = s0; s < s1; s += kAhead) {
+        Frag<Tag> xf[kAhead][MT], df[kAhead][R16];
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+          // past the wave's steps: zeros
+          const int64_t k = s + e < s1 ? (s + e) * 32 + kb * 8 : a.K;
+#pragma unroll
+          for (int f = 0; f < MT; ++f) xf[e][f].load(a.x + n[f] * a.x_ld * SZ, k, a.K);
+#pragma unroll
+          for (int j = 0; j < R16; ++j) {
+            const int rr = 16 * j + q;
+            df[e][j].load(down + min(rr, a.r - 1) * a.d_sr * SZ, rr < a.r ? k : a.K, a.K);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+          if (a.drop_in && s + e < s1) {
+#pragma unroll
+            for (int f = 0; f < MT; ++f)
+              xf[e][f].keep(a.drop.keep_bits((uint64_t)(n[f] * per_row + (s + e) * 4 + kb), at));
+          }
+#pragma unroll
+          for (int f = 0; f < MT; ++f)
+#pragma unroll
+            for (int j = 0; j < R16; ++j) acc[f][j] = mma<Tag>(df[e][j], xf[e][f], acc[f][j]);
+        }
+      }
+      __syncthreads();  // the last tile's t is read
+#pragma unroll
+      for (int f = 0; f < MT; ++f)
+#pragma unroll
+        for (int j = 0; j < R16; ++j)
+          *reinterpret_cast<f32x4*>(&part[wv][16 * f + q][16 * j + 4 * kb]) = acc[f][j];
+    }
+    __syncthreads();
+    const float drop_scale = a.drop_in ? a.drop.scale : 1.0f;
+    for (int k = t; k < TM * R; k += kAT) {
+      const int i = k / R, j = k % R;
+      float v = (((part[0][i][j] + part[1][i][j]) + part[2][i][j]) + part[3][i][j]) * drop_scale;
+      if (j >= a.r) v = 0.0f;  // not an infinity of x times a padding's zero
+      part[0][i][j] = v;
+      if (a.t && slab == 0 && i < here) a.t[token(i) * R + j] = v;
+    }
+    __syncthreads();
+    if (!a.out) continue;
+
+    // a wave takes 32 columns at a time
+    Thin<Tag, R16> thin[MT];
+#pragma unroll
+    for (int f = 0; f < MT; ++f) thin[f].load(&part[0][16 * f + q][0], kb);
+    const float scale = a.scales ? a.scales[ad] : 1.0f;
+    const char* up = a.up + ad * a.u_sa * SZ;
+    for (int64_t c = c0 + 32 * wv; c < c1; c += 32 * kAW) {
+      // two tiles of up's rows, in an order that leaves eight consecutive columns to a lane
+      UpRow<Tag, R16> u[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        u[i].load(up + min(c + 8 * (q >> 2) + 4 * i + (q & 3), a.O - 1) * a.u_so * SZ, a.r, kb);
+      const int64_t col = c + 8 * kb;
+#pragma unroll
+      for (int f = 0; f < MT; ++f) {
+        Frag<Tag> b;
+        if (a.base) b.load(a.base + n[f] * a.b_ld * SZ, col, c1);
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const f32x4 d = expand<Tag, R16>(u[i], thin[f], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[4 * i + k] = d[k];
+        }
+        if (a.drop_out) {
+          const uint32_t keep = a.drop.keep_bits((uint64_t)(n[f] * ((a.O + 7) / 8) + col / 8), at);
+          const float s = scale * a.drop.scale;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = keep >> k & 1 ? v[k] * s : 0.0f;
+        } else if (a.base) {
+          float x[8];
+          b.unpack(x);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = __builtin_fmaf(v[k], scale, x[k]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] *= scale;
+        }
+        Frag<Tag> o;
+        o.pack(v);
+        if (16 * f + q < here) o.store(a.out + n[f] * a.O * SZ, col, c1);
+      }
+    }
+  }
+}
+
+// ---- the weights' gradients ------------------------------------------------------------
+
+// part[c, r] of an adapter and a run of tokens: sum over its tokens of wide[n, c] thin[n, r].
+// A lane loads eight columns of eight tokens, which is what eight matrix instructions'
+// fragments hold: the columns 8 (lane % 16) + j make up the j-th.
+struct OuterJob {
+  const char* wide;   // [N, C]; null: no such job
+  int64_t ld, C;
+  const float* thin;  // [N, R]
+  float* part;        // [A, segments, C, R]
+  int32_t* seen;      // [A, segments]: whether the run holds any of its tokens
+  char* out;          // the gradient: entry (a, c, r) at a * o_sa + c * o_sc + r * o_sr
+  int64_t o_sa, o_sc, o_sr;
+  int tiles;          // of kOuterCols columns
+  int drop;
+};
+struct OuterArgs {
+  OuterJob job[2];
+  AdapterIds ids;
+  int64_t N;
+  int r, R;           // R: r rounded up to a multiple of 16
+  int rank_tiles;     // of 16 RT ranks
+  int window, segments;
+  int64_t windows;
+  Drop drop;
+  const float* scales;
+};
+constexpr int kOuterCols = 128 * kAW;
+
+template <class Tag, int RT>
+__global__ __launch_bounds__(kAT) void adapter_outer_kernel(OuterArgs a) {
+  constexpr int SZ = 16 / Pack16<Tag>::EPV;
+  constexpr bool F32 = std::is_same_v<Tag, TagF32>, F16 = std::is_same_v<Tag, TagF16>;
+  __shared__ uint16_t list[kWindow];
+  __shared__ int counts[kAW];
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, kb = lane >> 4, q = lane & 15;
+  uint32_t id = blockIdx.x;
+  const uint32_t per = (uint32_t)((a.job[0].tiles + a.job[1].tiles) * a.rank_tiles);
+  const uint32_t seg = id / per / a.ids.A, ad = id / per % a.ids.A;
+  id %= per;
+  const int rt = (int)(id % a.rank_tiles);
+  int ct = (int)(id / a.rank_tiles);
+  const bool second = ct >= a.job[0].tiles;
+  if (second) ct -= a.job[0].tiles;
+  const OuterJob& j = a.job[second];
+  const int64_t col = (int64_t)ct * kOuterCols + wv * 128 + 8 * q;
+  const int64_t per_row = (j.C + 7) / 8;
+  const uint64_t at = j.drop ? a.drop.counter() : 0;
+  const int r0 = rt * 16 * RT;
+
+  f32x4 acc[8][RT] = {};
+  bool any = false;
+  for (int64_t w = a.windows * seg / a.segments; w < a.windows * (seg + 1) / a.segments; ++w) {
+    // the window's tokens of this adapter, in order: a wave looks at a quarter of it
+    const int64_t n0 = w * a.window;
+    const int count = (int)min((int64_t)a.window, a.N - n0);
+    uint64_t mine[kWindow / kAT];
+    int before = 0, sum = 0;
+#pragma unroll
+    for (int k = 0; k < kWindow / kAT; ++k) {
+      const int i = wv * (kWindow / kAW) + 64 * k + lane;
+      mine[k] = __ballot(i < count && a.ids.at(n0 + min(i, count - 1)) == (int)ad);
+      sum += __popcll(mine[k]);
+    }
+    __syncthreads();  // the last window's list is read
+    if (lane == 0) counts[wv] = sum;
+    __syncthreads();
+    int listed = 0;
+    for (int k = 0; k < kAW; ++k) {
+      if (k < wv) before += counts[k];
+      listed += counts[k];
+    }
+#pragma unroll
+    for (int k = 0; k < kWindow / kAT; ++k) {
+      if (mine[k] >> lane & 1)
+        list[before + __popcll(mine[k] & (((uint64_t)1 << lane) - 1))] =
+            (uint16_t)(wv * (kWindow / kAW) + 64 * k + lane);
+      before += __popcll(mine[k]);
+    }
+    __syncthreads();
+    any |= listed > 0;
+    if (col - 8 * q >= j.C) continue;  // this wave's columns are past the end
+    for (int s = 0; s < listed; s += 32) {
+      Frag<Tag> x[8];
+      float th[8][RT];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int k = s + 8 * kb + i;
+        const bool here = k < listed;
+        const int64_t n = n0 + list[here ? k : listed - 1];
+        x[i].load(j.wide + n * j.ld * SZ, here ? col : j.C, j.C);
+        if (j.drop) x[i].keep(a.drop.keep_bits((uint64_t)(n * per_row + col / 8), at));
+#pragma unroll
+        for (int e = 0; e < RT; ++e) th[i][e] = here ? j.thin[n * a.R + r0 + 16 * e + q] : 0.0f;
+      }
+      if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+#pragma unroll
+            for (int e = 0; e < RT; ++e)
+              acc[c][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x[i].v[c / 4][c % 4]), th[i][e],
+                                                               acc[c][e], 0, 0, 0);
+      } else {
+        u32x4 hi[RT], lo[RT];
+#pragma unroll
+        for (int e = 0; e < RT; ++e) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = th[i][e];
+          split8(v, hi[e], lo[e]);
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          u32x4 wide, rest;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            // column c of tokens 2d and 2d + 1
+            const uint32_t two = __builtin_amdgcn_perm(x[2 * d + 1].v[0][c / 2], x[2 * d].v[0][c / 2],
+                                                       c % 2 ? 0x07060302u : 0x05040100u);
+            if constexpr (F16) {
+              uint32_t h, l;
+              split2(f16_bits_to_f32((uint16_t)two), f16_bits_to_f32((uint16_t)(two >> 16)), h, l);
+              wide[d] = h;
+              rest[d] = l;
+            } else {
+              wide[d] = two;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < RT; ++e) {
+            acc[c][e] = mma_bf16(wide, hi[e], acc[c][e]);
+            acc[c][e] = mma_bf16(wide, lo[e], acc[c][e]);
+            if constexpr (F16) acc[c][e] = mma_bf16(rest, hi[e], acc[c][e]);
+          }
+        }
+      }
+    }
+  }
+  const int64_t slot = (int64_t)ad * a.segments + seg;
+  if (ct == 0 && rt == 0 && t == 0) j.seen[slot] = any;
+  if (!any) return;
+  // a lane's columns are 8 (4 kb + i) + c, its rank q
+  float* part = j.part + slot * j.C * a.R;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t o = (int64_t)ct * kOuterCols + wv * 128 + 8 * (4 * kb + i) + c;
+      if (o < j.C)
+#pragma unroll
+        for (int e = 0; e < RT; ++e) part[o * a.R + r0 + 16 * e + q] = acc[c][e][i];
+    }
+}
+
+// Joins the runs' sums, in order.
+template <class Tag>
+__global__ __launch_bounds__(kAT) void adapter_join_kernel(OuterArgs a) {
+  const int64_t n0 = a.job[0].wide ? a.job[0].C * a.r : 0, n1 = a.job[1].wide ? a.job[1].C * a.r : 0;
+  int64_t k = (int64_t)blockIdx.x * kAT + threadIdx.x;
+  const int64_t ad = k / (n0 + n1);
+  if (ad >= a.ids.A) return;
+  k -= ad * (n0 + n1);
+  const bool second = k >= n0;
+  if (second) k -= n0;
+  const OuterJob& j = a.job[second];
+  // neighbours in the gradient's rows
+  const int64_t c = j.o_sr == 1 ? k / a.r : k % j.C, r = j.o_sr == 1 ? k % a.r : k / j.C;
+  float sum = 0.0f;
+  for (int s = 0; s < a.segments; ++s) {
+    const int64_t slot = ad * a.segments + s;
+    if (j.seen[slot]) sum += j.part[(slot * j.C + c) * a.R + r];
+  }
+  sum *= (a.scales ? a.scales[ad] : 1.0f);
+  if (j.drop) sum *= a.drop.scale;
+  const int64_t o = ad * j.o_sa + c * j.o_sc + r * j.o_sr;
+  if constexpr (std::is_same_v<Tag, TagF32>) reinterpret_cast<float*>(j.out)[o] = sum;
+  else reinterpret_cast<uint16_t*>(j.out)[o] = (uint16_t)Pack16<Tag>::pack_one(sum);
+}
+
+// up [A, O, r] as [A, R, P] (P: O rounded up to a multiple of 8) and down [A, r, H] as
+// [A, H, R], zeros where there is nothing.
+struct TurnArgs {
+  const char *down, *up;
+  int64_t d_sa, d_sr, u_sa, u_so, H, O, P;
+  char *downt, *upt;
+  int A, r, R;
+};
+template <class E>
+__global__ __launch_bounds__(kAT) void adapter_turn_kernel(TurnArgs a) {
+  const int64_t nu = (int64_t)a.R * a.P, nd = a.H * a.R;
+  int64_t k = (int64_t)blockIdx.x * kAT + threadIdx.x;
+  const int64_t ad = k / (nu + nd);
+  if (ad >= a.A) return;
+  k -= ad * (nu + nd);
+  if (k < nu) {
+    const int64_t r = k / a.P, o = k % a.P;
+    reinterpret_cast<E*>(a.upt)[ad * nu + k] =
+        r < a.r && o < a.O ? reinterpret_cast<const E*>(a.up)[ad * a.u_sa + o * a.u_so + r] : (E)0;
+  } else {
+    k -= nu;
+    const int64_t h = k / a.R, r = k % a.R;
+    reinterpret_cast<E*>(a.downt)[ad * nd + k] =
+        r < a.r ? reinterpret_cast<const E*>(a.down)[ad * a.d_sa + r * a.d_sr + h] : (E)0;
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------
+
+inline int rank_padded(int r) { return r <= 16 ? 16 : (r <= 32 ? 32 : (r <= 64 ? 64 : 128)); }
+
+template <class Tag, int R16, int MT>
+int launch_fused(FusedArgs a, hipStream_t st) {
+  const int64_t windows = (a.N + kWindow - 1) / kWindow;
+  const int rows = (int)min(a.N, (int64_t)kWindow);
+  // tiles of a window if it is of one adapter, and at most
+  const int64_t even = (rows + 16 * MT - 1) / (16 * MT), most = min((int64_t)rows, even + a.ids.A + 1);
+  // runs of columns: as many as make a thousand workgroups' work, of 128 columns at least
+  const int64_t cuts = a.out ? max((int64_t)1, min((a.O + 127) / 128, 1024 / max((int64_t)1, windows * even))) : 1;
+  a.slab = a.out ? ((a.O + cuts - 1) / cuts + 127) / 128 * 128 : 1;
+  a.slabs = a.out ? (int)((a.O + a.slab - 1) / a.slab) : 1;
+  a.groups = (int)max((int64_t)1, min(most * a.slabs, max(even * a.slabs, 2048 / windows)));
+  RRL_REQUIRE(windows * a.groups < ((int64_t)1 << 32) / kAT, RRL_EINVAL, "rrl_adapter: too many rows");
+  const size_t lds = (2 * sizeof(int) + kAW * sizeof(uint16_t)) * (size_t)(a.ids.A + 3);
+  hipLaunchKernelGGL((adapter_fused_kernel<Tag, R16, MT>), dim3((uint32_t)(windows * a.groups)), dim3(kAT), lds, st,
+                     a);
+  return check_launch("adapter_fused_kernel");
+}
+template <class Tag, int R16>
+int launch_fused(const FusedArgs& a, hipStream_t st) {
+  constexpr int MT = R16 > 4 ? 2 : 4;
+  return a.N <= 256 ? launch_fused<Tag, R16, 1>(a, st) : launch_fused<Tag, R16, MT>(a, st);
+}
+template <class Tag>
+int launch_fused(const FusedArgs& a, hipStream_t st) {
+  switch (rank_padded(a.r)) {
+    case 16: return launch_fused<Tag, 1>(a, st);
+    case 32: return launch_fused<Tag, 2>(a, st);
+    case 64: return launch_fused<Tag, 4>(a, st);
+    default: return launch_fused<Tag, 8>(a, st);
+  }
+}
+int launch_fused(const FusedArgs& a, int32_t dtype, hipStream_t st) {
+  if (a.N == 0) return RRL_OK;
+  if (dtype == RRL_F32) return launch_fused<TagF32>(a, st);
+  if (dtype == RRL_BF16) return launch_fused<TagBF16>(a, st);
+  return launch_fused<TagF16>(a, st);
+}
+
+template <class Tag>
+int launch_outer(const OuterArgs& a, hipStream_t st) {
+  const int64_t blocks =
+      (int64_t)a.segments * a.ids.A * (a.job[0].tiles + a.job[1].tiles) * a.rank_tiles;
+  const dim3 grid((uint32_t)blocks), threads(kAT);
+  if (a.R == 16) hipLaunchKernelGGL((adapter_outer_kernel<Tag, 1>), grid, threads, 0, st, a);
+  else if (a.R == 32) hipLaunchKernelGGL((adapter_outer_kernel<Tag, 2>), grid, threads, 0, st, a);
+  else hipLaunchKernelGGL((adapter_outer_kernel<Tag, 4>), grid, threads, 0, st, a);
+  return check_launch("adapter_outer_kernel");
+}
+template <class Tag>
+int launch_join(const OuterArgs& a, hipStream_t st) {
+  const int64_t each = (a.job[0].wide ? a.job[0].C * a.r : 0) + (a.job[1].wide ? a.job[1].C * a.r : 0);
+  hipLaunchKernelGGL(adapter_join_kernel<Tag>, dim3((uint32_t)((each * a.ids.A + kAT - 1) / kAT)), dim3(kAT), 0, st,
+                     a);
+  return check_launch("adapter_join_kernel");
+}
+
+struct BackLayout {
+  int R;
+  int64_t P, windows;
+  int window, segments, rank_tiles;
+  size_t upt, downt, s, part[2], seen[2], total;
+};
+inline BackLayout back_layout(int64_t N, int64_t H, int64_t O, int64_t A, int r, size_t size) {
+  BackLayout l;
+  l.R = rank_padded(r);
+  l.P = (O + 7) / 8 * 8;
+  l.rank_tiles = l.R > 64 ? 2 : 1;
+  const int64_t tiles = ((H + kOuterCols - 1) / kOuterCols + (O + kOuterCols - 1) / kOuterCols) * l.rank_tiles;
+  // windows of tokens so that there are a thousand workgroups, of 64 tokens at least
+  const int64_t runs = max((int64_t)1, 1024 / max((int64_t)1, A * tiles));
+  l.window = 64;
+  while (l.window < kWindow && (N + l.window - 1) / l.window > runs) l.window *= 2;
+  l.windows = (N + l.window - 1) / l.window;
+  l.segments = (int)min(l.windows, runs);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  l.upt = take((size_t)(A * l.R * l.P) * size);
+  l.downt = take((size_t)(A * l.R * H) * size);
+  l.s = take((size_t)(N * l.R) * 4);
+  l.part[0] = take((size_t)(A * l.segments * O * l.R) * 4);
+  l.part[1] = take((size_t)(A * l.segments * H * l.R) * 4);
+  l.seen[0] = take((size_t)(A * l.segments) * 4);
+  l.seen[1] = take((size_t)(A * l.segments) * 4);
+  l.total = at;
+  return l;
+}
+
+// Sizes whose index arithmetic and grids fit.
+inline bool adapter_fits(int64_t N, int64_t H, int64_t O, int64_t A, int64_t r) {
+  if (N < 0 || H < 1 || O < 1 || A < 1 || r < 1) return false;
+  if (N > ((int64_t)1 << 30) || H > ((int64_t)1 << 24) || O > ((int64_t)1 << 24) || A > kMostAdapters ||
+      r > kMostRank)
+    return false;
+  return A * rank_padded((int)r) * (H + O + 8) < ((int64_t)1 << 32) - kAT;
+}
+
+int check_adapter(const char* who, int32_t dtype, int64_t N, int64_t H, int64_t O, int64_t A, int64_t r,
+                  const void* ids, int32_t ids_dtype, const void* scales) {
+  const std::string w(who);
+  RRL_REQUIRE(dtype == RRL_F32 || dtype == RRL_BF16 || dtype == RRL_F16, RRL_EDTYPE,
+              w + ": entries must be float32, bfloat16 or float16");
+  RRL_REQUIRE(adapter_fits(N, H, O, A, r), RRL_EINVAL,
+              w + ": a bad size (at most 4096 adapters of rank 1 to 128, 2^30 rows, 2^24 columns, and 2^32 "
+                  "weights with ranks rounded up to 16, 32, 64 or 128)");
+  RRL_REQUIRE(ids != nullptr || A == 1 || N == 0, RRL_EINVAL, w + ": ids are needed where there are several adapters");
+  RRL_REQUIRE(ids == nullptr || ids_dtype == RRL_I32 || ids_dtype == RRL_I64, RRL_EDTYPE,
+              w + ": adapter ids must be int32 or int64");
+  RRL_REQUIRE((ids == nullptr || (uintptr_t)ids % dtype_size(ids_dtype) == 0) && (uintptr_t)scales % 4 == 0,
+              RRL_EALIGN, w + ": a pointer is not aligned to its element");
+  return RRL_OK;
+}
+
+}  // namespace
+}  // namespace rrl
+
+using namespace rrl;
+
+extern "C" int64_t rrl_adapter_rank_padded(int64_t r) {
+  return r < 1 || r > kMostRank ? 0 : rank_padded((int)r);
+}
+
+extern "C" int rrl_adapter_fwd(const rrl_adapter_params* p, const void* x, int64_t x_ld, const void* base,
+                               int64_t base_ld, void* out, float* t_out, void* stream) {
+  clear_error();
+  RRL_REQUIRE(p != nullptr, RRL_EINVAL, "rrl_adapter_fwd: null operand");
+  if (int rc = check_adapter("rrl_adapter_fwd", p->dtype, p->N, p->H, p->O, p->A, p->r, p->ids, p->ids_dtype,
+                             p->scales))
+    return rc;
+  FusedArgs a = {};
+  if (p->dropout)
+    if (int rc = make_drop(p->dropout, a.drop, "rrl_adapter_fwd")) return rc;
+  if (p->N == 0) return RRL_OK;
+  RRL_REQUIRE(x != nullptr && p->down != nullptr && p->up != nullptr && out != nullptr, RRL_EINVAL,
+              "rrl_adapter_fwd: null operand");
+  RRL_REQUIRE(p->N <= 1 || (x_ld >= 0 && base_ld >= 0), RRL_EINVAL, "rrl_adapter_fwd: negative row stride");
+  const size_t size = dtype_size(p->dtype);
+  RRL_REQUIRE((uintptr_t)x % size == 0 && (uintptr_t)p->down % size == 0 && (uintptr_t)p->up % size == 0 &&
+                  (uintptr_t)base % size == 0 && (uintptr_t)out % size == 0 && (uintptr_t)t_out % 16 == 0,
+              RRL_EALIGN, "rrl_adapter_fwd: a pointer is not aligned (t_out: 16 bytes)");
+  a.x = static_cast<const char*>(x);
+  a.x_ld = x_ld;
+  a.down = static_cast<const char*>(p->down);
+  a.d_sa = p->down_sa;
+  a.d_sr = p->down_sr;
+  a.up = static_cast<const char*>(p->up);
+  a.u_sa = p->up_sa;
+  a.u_so = p->up_so;
+  a.base = static_cast<const char*>(base);
+  a.b_ld = base_ld;
+  a.ids = AdapterIds{p->ids, p->ids_dtype, (int)p->A};
+  a.scales = p->scales;
+  a.out = static_cast<char*>(out);
+  a.t = t_out;
+  a.N = p->N;
+  a.K = p->H;
+  a.O = p->O;
+  a.r = (int)p->r;
+  a.drop_in = p->dropout != nullptr;
+  a.nan_rows = 1;
+  return launch_fused(a, p->dtype, as_stream(stream));
+}
+
+extern "C" size_t rrl_adapter_bwd_workspace_bytes(int64_t N, int64_t H, int64_t O, int64_t A, int64_t r,
+                                                  int32_t dtype) {
+  if (!adapter_fits(N, H, O, A, r)) return 0;
+  return back_layout(N, H, O, A, (int)r, dtype_size(dtype)).total;
+}
+
+extern "C" int rrl_adapter_bwd(const rrl_adapter_params* p, const void* x, int64_t x_ld, const void* grad,
+                               int64_t g_ld, const float* t, void* dx, void* ddown, void* dup, void* workspace,
+                               void* stream) {
+  clear_error();
+  RRL_REQUIRE(p != nullptr, RRL_EINVAL, "rrl_adapter_bwd: null operand");
+  if (int rc = check_adapter("rrl_adapter_bwd", p->dtype, p->N, p->H, p->O, p->A, p->r, p->ids, p->ids_dtype,
+                             p->scales))
+    return rc;
+  Drop drop = {};
+  if (p->dropout)
+    if (int rc = make_drop(p->dropout, drop, "rrl_adapter_bwd")) return rc;
+  RRL_REQUIRE(workspace != nullptr && p->down != nullptr && p->up != nullptr &&
+                  (p->N == 0 || (grad != nullptr && (ddown == nullptr || x != nullptr) &&
+                                 (dup == nullptr || t != nullptr))),
+              RRL_EINVAL, "rrl_adapter_bwd: null operand");
+  RRL_REQUIRE(p->N <= 1 || (x_ld >= 0 && g_ld >= 0), RRL_EINVAL, "rrl_adapter_bwd: negative row stride");
+  const size_t size = dtype_size(p->dtype);
+  RRL_REQUIRE((uintptr_t)x % size == 0 && (uintptr_t)p->down % size == 0 && (uintptr_t)p->up % size == 0 &&
+                  (uintptr_t)grad % size == 0 && (uintptr_t)dx % size == 0 && (uintptr_t)ddown % size == 0 &&
+                  (uintptr_t)dup % size == 0 && (uintptr_t)t % 16 == 0 && (uintptr_t)workspace % 16 == 0,
+              RRL_EALIGN, "rrl_adapter_bwd: a pointer is not aligned (t and workspace: 16 bytes)");
+  hipStream_t st = as_stream(stream);
+  const BackLayout l = back_layout(p->N, p->H, p->O, p->A, (int)p->r, size);
+  char* w = static_cast<char*>(workspace);
+  float* s = reinterpret_cast<float*>(w + l.s);
+  const AdapterIds ids{p->ids, p->ids_dtype, (int)p->A};
+  if (p->N > 0 && (dx || ddown)) {
+    TurnArgs ta{static_cast<const char*>(p->down), static_cast<const char*>(p->up), p->down_sa, p->down_sr, p->up_sa,
+                p->up_so, p->H, p->O, l.P, w + l.downt, w + l.upt, (int)p->A, (int)p->r, l.R};
+    const dim3 grid((uint32_t)((p->A * l.R * (l.P + p->H) + kAT - 1) / kAT));
+    if (size == 4) hipLaunchKernelGGL(adapter_turn_kernel<uint32_t>, grid, dim3(kAT), 0, st, ta);
+    else hipLaunchKernelGGL(adapter_turn_kernel<uint16_t>, grid, dim3(kAT), 0, st, ta);
+    if (int rc = check_launch("adapter_turn_kernel")) return rc;
+    FusedArgs a = {};
+    a.x = static_cast<const char*>(grad);
+    a.x_ld = g_ld;
+    a.down = w + l.upt;
+    a.d_sa = l.R * l.P;
+    a.d_sr = l.P;
+    a.up = w + l.downt;
+    a.u_sa = p->H * l.R;
+    a.u_so = l.R;
+    a.ids = ids;
+    a.scales = p->scales;
+    a.out = static_cast<char*>(dx);
+    a.t = ddown ? s : nullptr;
+    a.N = p->N;
+    a.K = p->O;
+    a.O = p->H;
+    a.r = (int)p->r;
+    a.drop = drop;
+    a.drop_out = p->dropout != nullptr;
+    if (int rc = launch_fused(a, p->dtype, st)) return rc;
+  }
+  if (!ddown && !dup) return RRL_OK;
+  OuterArgs o = {};
+  o.ids = ids;
+  o.N = p->N;
+  o.r = (int)p->r;
+  o.R = l.R;
+  o.rank_tiles = l.rank_tiles;
+  o.window = l.window;
+  o.windows = l.windows;
+  o.segments = l.segments;
+  o.drop = drop;
+  o.scales = p->scales;
+  if (dup) {
+    o.job[0] = OuterJob{static_cast<const char*>(grad), g_ld, p->O, t, reinterpret_cast<float*>(w + l.part[0]),
+                        reinterpret_cast<int32_t*>(w + l.seen[0]), static_cast<char*>(dup), p->O * p->r, p->r, 1,
+                        (int)((p->O + kOuterCols - 1) / kOuterCols), 0};
+    o.job[0].wide = p->N ? o.job[0].wide : w;
+  }
+  if (ddown) {
+    o.job[1] = OuterJob{static_cast<const char*>(x), x_ld, p->H, s, reinterpret_cast<float*>(w + l.part[1]),
+                        reinterpret_cast<int32_t*>(w + l.seen[1]), static_cast<char*>(ddown), p->H * p->r, 1, p->H,
+                        (int)((p->H + kOuterCols - 1) / kOuterCols), p->dropout != nullptr};
+    o.job[1].wide = p->N ? o.job[1].wide : w;
+  }
+  if (p->N > 0) {
+    int rc;
+    if (p->dtype == RRL_F32) rc = launch_outer<TagF32>(o, st);
+    else if (p->dtype == RRL_BF16) rc = launch_outer<TagBF16>(o, st);
+    else rc = launch_outer<TagF16>(o, st);
+    if (rc) return rc;
+  }
+  if (p->dtype == RRL_F32) return launch_join<TagF32>(o, st);
+  if (p->dtype == RRL_BF16) return launch_join<TagBF16>(o, st);
+  return launch_join<TagF16>(o, st);
+}
