@@ -521,7 +521,10 @@ RRL_API int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, con
  * u times the whole below one unit counts as 0.
  * A row with NaN or +inf, or with nothing above -inf, and a temperature that is NaN or
  * +inf give token -1 and NaN log-probs.  (The reference has one setting for all rows and
- * no min-p, roseinfer/engine.py:1103-1171.) */
+ * no min-p, roseinfer/engine.py:1103-1171.)  workspace:
+ * rrl_sample_tokens_workspace_bytes(B, V, params) bytes of caller device memory (16-byte
+ * aligned; contents of no meaning; params tell whether there may be a top_k or a top_p,
+ * NULL stands for both). */
 typedef struct rrl_sample_params {
   double temperature, top_p, min_p;
   int64_t top_k;
@@ -532,9 +535,12 @@ typedef struct rrl_sample_params {
   int32_t top_k_dtype;
 } rrl_sample_params;
 
+RRL_API size_t rrl_sample_tokens_workspace_bytes(int64_t B, int64_t V,
+                    const rrl_sample_params* params);
 RRL_API int rrl_sample_tokens(const void* logits, int32_t dtype, int64_t B, int64_t V,
                     int64_t row_stride, const float* uniforms, const rrl_sample_params* params,
-                    int64_t* token_out, float* logp_out, float* logq_out, void* stream);
+                    int64_t* token_out, float* logp_out, float* logq_out, void* workspace,
+                    void* stream);
 
 /* ---- dropout from a counter-based generator ------------------------------------
  * out = residual + (kept ? x / (1 - p') : 0), contiguous [rows, cols], of x and (or

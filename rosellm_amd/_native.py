@@ -190,7 +190,8 @@ SIGNATURES = {
     "rrl_embedding_fwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _D, _I64, _I32, _P, _P]),
     "rrl_embedding_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64]),
     "rrl_embedding_bwd": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I64, _D, _I64, _I32, _P, _I64, _P, _P]),
-    "rrl_sample_tokens": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _PT, _P, _P, _P, _P]),
+    "rrl_sample_tokens_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _PT]),
+    "rrl_sample_tokens": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _PT, _P, _P, _P, _P, _P]),
     "rrl_adapter_rank_padded": (_I64, [_I64]),
     "rrl_adapter_fwd": (ctypes.c_int, [_PA, _P, _I64, _P, _I64, _P, _P, _P]),
     "rrl_adapter_bwd_workspace_bytes": (ctypes.c_size_t, [_I64, _I64, _I64, _I64, _I64, _I32]),

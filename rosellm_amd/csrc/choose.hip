@@ -17,18 +17,40 @@
 // order, so that LDS atomics may form them, and off by 2^-45 an entry, 1e-11 of the
 // whole for 150,000 entries.
 //
-// What is left is always the entries above a place (x, v) in descending order, so a cut
-// is found by histograms of 2048 bins: first of the distance to the maximum, then of the
-// keys within the bin that holds the border, until that is one value; then, if it was
-// only partly taken, of the indexes of its ties.
+// What is left is always the entries above a place (x, v) in descending order.  Rows are
+// cut into parts, a workgroup each, so that a single row fills the chip, and read once a
+// launch (from the caches, but for the first):
+//   1. choose_max: the maximum of each part
+//   2. choose_weigh: each part's sum, and where the row has a top-k or a top-p its
+//      histogram, counts or sums in 1024 bins of 1/16 of a factor of two below m; sums
+//      leave out entries that no nucleus can hold
+//   3. choose_cut (only if there may be a top-k or top-p): a workgroup a row finds the bin
+//      that holds the border, lists its entries, and finds the place among them
+//   4. choose_left (as 3): the sum of what is left, of each quarter of a part
+//   5. choose_draw: a workgroup a row finds the quarter, then the entry
 #include "vocab_weights.hpp"
+
+#include <type_traits>
 
 namespace rrl {
 namespace {
 
-constexpr int kCT = 1024, kCW = kCT / 64;  // a workgroup's threads and waves
-constexpr int kBins = 2048;                // two for each thread
+constexpr int kPT = 256, kPW = kPT / 64;   // threads and waves of a part
+constexpr int kRT = 1024, kRW = kRT / 64;  // of a row
+constexpr int kBins = 1024, kBinBits = 10;
+constexpr int kListed = 4096;              // entries of a bin that are held in LDS
+constexpr int kAhead = 4;                  // 16-byte vectors that a lane loads at once
 constexpr int kNoIndex = 0x7fffffff;
+static_assert(kBins == kRT, "a bin to a thread");
+
+typedef unsigned long long u64;
+
+// Entries are left where x > v, or x == v and their index is below n.
+struct Cut {
+  float v;
+  int n;
+  __device__ __forceinline__ bool keeps(float x, int i) const { return x > v || (x == v && i < n); }
+};
 
 struct ChooseArgs {
   const char* x;
@@ -40,24 +62,20 @@ struct ChooseArgs {
   int top_k_dt;
   double temperature_all, top_p_all, min_p_all;
   int64_t top_k_all;
-  int slabs;     // 16-byte vectors of a lane: a wave's entries stand together
-  double magic;  // 2^(52 - F): a weight added to it stands in the low bits, in units of 2^-F
-  int unit_log2; // F
+  int parts, part;  // parts of a row, and their entries
+  double magic;     // 2^(52 - F): a weight added to it stands in the low bits, in units of 2^-F
+  int unit_log2;    // F
+  float* peak;      // [B, parts] a part's maximum; +inf: it holds NaN or +inf
+  u64* whole;       // [B, parts] sum of all entries
+  u64* left;        // [B, parts, kPW] of those that are left, a wave's run of a part each
+  u64* sums;        // [B, parts, kBins], where there may be a top-p
+  uint32_t* counts; // [B, parts, kBins], where there may be a top-k
+  Cut* cut;         // [B], where there may be either
   int64_t* token_out;
   float *logp_out, *logq_out;  // logq_out may be null
 };
 
-typedef unsigned long long u64;
-
-// Entries are left where x > v, or x == v and their index is below n.
-struct Cut {
-  float v;
-  int n;
-  __device__ __forceinline__ bool keeps(float x, int i) const { return x > v || (x == v && i < n); }
-};
-
-// Order of floats as that of unsigned numbers (-0 below +0, which are brought together
-// before).
+// Order of floats as that of unsigned numbers (-0 as +0).
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
@@ -66,7 +84,8 @@ __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
-template <class T, class Op>
+// `sh` holds a value for each of the NW waves.
+template <int NW, class T, class Op>
 __device__ __forceinline__ T block_reduce(T v, T* sh, Op op) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
@@ -75,84 +94,247 @@ __device__ __forceinline__ T block_reduce(T v, T* sh, Op op) {
   __syncthreads();
   v = sh[0];
 #pragma unroll
-  for (int k = 1; k < kCW; ++k) v = op(v, sh[k]);
+  for (int k = 1; k < NW; ++k) v = op(v, sh[k]);
   return v;
 }
-__device__ __forceinline__ u64 block_sum_u64(u64 v, u64* sh) {
-  return block_reduce(v, sh, [](u64 a, u64 b) { return a + b; });
-}
-
-struct ChooseShared {
-  u64 hist[kBins];
-  u64 wave[kCW];
-  u64 above;  // of the bins before the one that holds the border
-  int bin;
-  int slot;
+struct Add {
+  __device__ __forceinline__ u64 operator()(u64 a, u64 b) const { return a + b; }
+};
+struct Max {
+  template <class T>
+  __device__ __forceinline__ T operator()(T a, T b) const { return a > b ? a : b; }
+};
+struct Min {
+  template <class T>
+  __device__ __forceinline__ T operator()(T a, T b) const { return a < b ? a : b; }
 };
 
-template <class Tag>
-struct Row {
-  static constexpr int EPV = Pack16<Tag>::EPV;
-  const char* p;
-  int64_t V;
-  int slabs;
-  // f(value, index) for every entry of this lane that is above -inf
-  template <class F>
-  __device__ __forceinline__ void each(F f) const {
-    const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int s = 0; s < slabs; ++s) {
-      const int64_t i = (((int64_t)wv * slabs + s) * 64 + lane) * EPV;
-      if (i >= V) break;
-      float x[EPV];
-      load_entries<Tag>(p, i, V, x);
-#pragma unroll
-      for (int k = 0; k < EPV; ++k)
-        if (x[k] != -M<float>::inf()) f(x[k], (int)i + k);
-    }
+// A row's settings.
+struct Settings {
+  double T, top_p, min_p;
+  int64_t top_k;  // 0: none
+  bool greedy, bad, filtered;
+  __device__ __forceinline__ Settings(const ChooseArgs& a, int64_t b) {
+    T = a.temperature ? (double)a.temperature[b] : a.temperature_all;
+    top_p = a.top_p ? (double)a.top_p[b] : a.top_p_all;
+    min_p = a.min_p ? (double)a.min_p[b] : a.min_p_all;
+    top_k = a.top_k ? load_index(a.top_k, a.top_k_dt, b) : a.top_k_all;
+    greedy = T <= 0.0;
+    bad = !(T < M<double>::inf());
+    if (greedy) T = 1.0;
+    if (T < 1e-290) T = 1e-290;  // has the distribution's limit already
+    if (top_k < 0 || top_k >= a.V) top_k = 0;
+    if (!(top_p > 0.0 && top_p < 1.0)) top_p = 0.0;
+    filtered = !greedy && (top_k > 0 || top_p > 0.0);
+  }
+  __device__ __forceinline__ double c() const { return 1.4426950408889634074 / T; }
+  // bins of 1/16 of a factor of two, by the distance to the maximum
+  __device__ __forceinline__ float scale() const { return (float)fmin(16.0 * c(), 3e38); }
+  // what min_p alone leaves
+  __device__ __forceinline__ Cut least(float m) const {
+    if (!(min_p > 0.0)) return Cut{-M<float>::inf(), 0};
+    // the least float at no more than that distance, a step or two from this one
+    const double far = T * log(fmin(min_p, 1.0));
+    uint32_t k = key_of((float)((double)m + far));
+    for (int n = 0; n < 4 && (double)value_of(k) - (double)m < far; ++n) ++k;
+    for (int n = 0; n < 4 && (double)value_of(k - 1) - (double)m >= far; ++n) --k;
+    return Cut{value_of(k), kNoIndex};
   }
 };
+__device__ __forceinline__ int bin_of(float x, float m, float scale) {
+  return (int)fminf((m - x) * scale, (float)(kBins - 1));
+}
+
+// The row's maximum; +inf where it has no distribution.
+template <int NW>
+__device__ __forceinline__ float row_peak(const ChooseArgs& a, int64_t b, float* sh) {
+  float m = -M<float>::inf();
+  for (int k = threadIdx.x; k < a.parts; k += NW * 64) m = fmaxf(m, a.peak[b * a.parts + k]);
+  m = block_reduce<NW>(m, sh, Max());
+  return m == -M<float>::inf() ? M<float>::inf() : m;
+}
 
 // The integer mass of an entry.
 struct Mass {
   Weight w;
   double magic;
   u64 zero;  // the bits of magic
-  __device__ __forceinline__ Mass(const Weight& weight, double magic_)
-      : w(weight), magic(magic_), zero((u64)__double_as_longlong(magic_)) {}
-  __device__ __forceinline__ u64 operator()(float x) const {
-    const double v = w.direct ? fma(w.template unscaled<true>(x), w.k, magic) : w.template unscaled<false>(x) + magic;
+  __device__ __forceinline__ Mass(float m, double c, double magic_)
+      : w(m, c, 1.0), magic(magic_), zero((u64)__double_as_longlong(magic_)) {}
+  template <bool DIRECT>
+  __device__ __forceinline__ u64 of(float x) const {
+    const double v = DIRECT ? fma(w.template unscaled<DIRECT>(x), w.k, magic) : w.template unscaled<DIRECT>(x) + magic;
     return (u64)__double_as_longlong(v) - zero;
   }
+  __device__ __forceinline__ u64 operator()(float x) const { return w.direct ? of<true>(x) : of<false>(x); }
 };
 
-// Clears the histogram; the workgroup may add to it afterwards.
-__device__ __forceinline__ void clear_bins(ChooseShared& sh) {
-  __syncthreads();
-  for (int k = threadIdx.x; k < kBins; k += kCT) sh.hist[k] = 0;
-  __syncthreads();
+// f(values, index of the first) for the 16-byte vectors of entries lo..hi-1 of a row, by
+// NT threads of which this is the t-th; past the end of them -inf.
+template <class Tag, int NT, class F>
+__device__ __forceinline__ void sweep(const char* row, int64_t lo, int64_t hi, int t, F f) {
+  constexpr int EPV = Pack16<Tag>::EPV, SZ = 16 / EPV;
+  for (int64_t i0 = lo + t * EPV; i0 < hi; i0 += kAhead * NT * EPV) {
+    u32x4 raw[kAhead];
+    if (i0 + (int64_t)((kAhead - 1) * NT + 1) * EPV <= hi) {
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s)
+        raw[s] = reinterpret_cast<const Any16*>(row + (i0 + s * NT * EPV) * SZ)->v;
+    } else {
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        float x[EPV];
+        load_entries<Tag>(row, i0 + s * NT * EPV, hi, x);
+        raw[s] = Pack16<Tag>::pack(x);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      float x[EPV];
+      Pack16<Tag>::unpack(raw[s], x);
+      f(x, (int)(i0 + s * NT * EPV));
+    }
+  }
+}
+// The same by a wave over its quarter of a part.
+template <class Tag, class F>
+__device__ __forceinline__ void sweep_part(const ChooseArgs& a, const char* row, int64_t part, F f) {
+  const int64_t lo = part * a.part + (threadIdx.x >> 6) * (a.part / kPW);
+  sweep<Tag, 64>(row, lo, min(lo + a.part / kPW, a.V), threadIdx.x & 63, f);
+}
+template <class Tag>
+__device__ __forceinline__ const char* row_at(const ChooseArgs& a, int64_t b) {
+  return a.x + b * a.ld * (16 / Pack16<Tag>::EPV);
 }
 
-// The bin at which the running sum, `above` before the first, exceeds target: -1 if none
-// does.  `above` becomes the sum before that bin.
-__device__ __forceinline__ int find_bin(ChooseShared& sh, u64& above, u64 target) {
-  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+// ---- 1 ---------------------------------------------------------------------------------
+
+template <class Tag>
+__global__ __launch_bounds__(kPT) void choose_max_kernel(ChooseArgs a) {
+  constexpr int EPV = Pack16<Tag>::EPV;
+  const int64_t b = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  __shared__ float sh[kPW];
+  float m = -M<float>::inf();
+  bool nan = false;
+  sweep_part<Tag>(a, row_at<Tag>(a, b), part, [&](const float (&x)[EPV], int) {
+#pragma unroll
+    for (int k = 0; k < EPV; k += 2) {
+      // with NaN among them the result is not used
+      asm("v_max3_f32 %0, %1, %2, %0" : "+v"(m) : "v"(x[k]), "v"(x[k + 1]));
+      nan |= __builtin_isunordered(x[k], x[k + 1]);
+    }
+  });
+  m = block_reduce<kPW>(nan ? M<float>::inf() : m, sh, Max());
+  if (threadIdx.x == 0) a.peak[blockIdx.x] = m;
+}
+
+// ---- 2 ---------------------------------------------------------------------------------
+
+template <class Tag, bool DIRECT>
+__device__ __forceinline__ void weigh(const ChooseArgs& a, const Settings& set, const Mass& mass, float m, int64_t b,
+                                      int64_t part, u64* sums, uint32_t* counts, u64& whole, u64& left) {
+  constexpr int EPV = Pack16<Tag>::EPV;
+  const char* row = row_at<Tag>(a, b);
+  if (set.filtered) {
+    const float scale = set.scale();
+    // Entries of at most (1 - top_p) / V of the largest make up no more than 1 - top_p of
+    // the whole, so that the border lies above them.  What top_k leaves has a whole of its
+    // own, for which the sums are needed down to it.
+    const u64 floor = set.top_p == 0.0 ? ~(u64)0
+                                       : (set.top_k > 0 ? 0 : (u64)ldexp((1.0 - set.top_p) / (double)a.V, a.unit_log2));
+    sweep_part<Tag>(a, row, part, [&](const float (&x)[EPV], int) {
+#pragma unroll
+      for (int k = 0; k < EPV; ++k) {
+        const u64 w = mass.of<DIRECT>(x[k]);
+        whole += w;
+        if (w > floor) atomicAdd(&sums[bin_of(x[k], m, scale)], w);
+        if (set.top_k > 0 && x[k] != -M<float>::inf()) atomicAdd(&counts[bin_of(x[k], m, scale)], 1u);
+      }
+    });
+  } else {
+    const Cut cut = set.least(m);
+    sweep_part<Tag>(a, row, part, [&](const float (&x)[EPV], int) {
+#pragma unroll
+      for (int k = 0; k < EPV; ++k) {
+        const u64 w = mass.of<DIRECT>(x[k]);
+        whole += w;
+        left += x[k] >= cut.v ? w : 0;
+      }
+    });
+  }
+}
+__device__ __forceinline__ u64 wave_total(u64 v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+template <class Tag>
+__global__ __launch_bounds__(kPT) void choose_weigh_kernel(ChooseArgs a) {
+  const int64_t b = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  const int t = threadIdx.x;
+  __shared__ u64 sums[kBins];
+  __shared__ uint32_t counts[kBins];
+  __shared__ u64 sh[kPW];
+  const Settings set(a, b);
+  const float m = row_peak<kPW>(a, b, reinterpret_cast<float*>(sh));
+  if (set.bad || !(m < M<float>::inf())) return;
+  if (set.filtered) {
+    for (int k = t; k < kBins; k += kPT) {
+      sums[k] = 0;
+      counts[k] = 0;
+    }
+  }
   __syncthreads();
-  const u64 a = sh.hist[2 * t], b = sh.hist[2 * t + 1];
-  u64 v = a + b;
+  const Mass mass(m, set.c(), a.magic);
+  u64 whole = 0, left = 0;
+  if (mass.w.direct) weigh<Tag, true>(a, set, mass, m, b, part, sums, counts, whole, left);
+  else weigh<Tag, false>(a, set, mass, m, b, part, sums, counts, whole, left);
+  whole = block_reduce<kPW>(whole, sh, Add());
+  if (t == 0) a.whole[blockIdx.x] = whole;
+  if (set.filtered) {
+    __syncthreads();
+    const int64_t to = (int64_t)blockIdx.x * kBins;
+    if (set.top_p > 0.0)
+      for (int k = t; k < kBins; k += kPT) a.sums[to + k] = sums[k];
+    if (set.top_k > 0)
+      for (int k = t; k < kBins; k += kPT) a.counts[to + k] = counts[k];
+  } else {
+    left = wave_total(left);
+    if ((t & 63) == 0) a.left[blockIdx.x * kPW + (t >> 6)] = left;
+  }
+}
+
+// ---- 3 ---------------------------------------------------------------------------------
+
+struct CutShared {
+  u64 hist[kBins];
+  u64 wave[kRW];
+  u64 above;  // of the bins before the one that holds the border
+  float list_x[kListed];
+  int list_i[kListed];
+  int bin, listed;
+};
+
+// The bin at which the running sum, `above` before the first, exceeds target: -1 if none
+// does.  `mine` is this thread's bin; `above` becomes the sum before that bin.
+__device__ __forceinline__ int find_bin(CutShared& sh, u64 mine, u64& above, u64 target) {
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+  u64 v = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const u64 y = __shfl_up(v, o, 64);
     if (lane >= o) v += y;
   }
+  __syncthreads();
   if (t == 0) sh.bin = -1;
   if (lane == 63) sh.wave[wv] = v;
   __syncthreads();
-  u64 before = above;
-  for (int k = 0; k < wv; ++k) before += sh.wave[k];
-  const u64 end = before + v, mid = end - b, start = mid - a;
-  if (start <= target && end > target) {  // one thread's
-    sh.bin = mid > target ? 2 * t : 2 * t + 1;
-    sh.above = mid > target ? start : mid;
+  u64 end = above + v;
+  for (int k = 0; k < wv; ++k) end += sh.wave[k];
+  if (end - mine <= target && end > target) {  // one thread's
+    sh.bin = t;
+    sh.above = end - mine;
   }
   __syncthreads();
   const int bin = sh.bin;
@@ -162,42 +344,94 @@ __device__ __forceinline__ int find_bin(ChooseShared& sh, u64& above, u64 target
 
 __device__ __forceinline__ int bits_over(uint32_t n) {  // bits to drop so that numbers up to n fit the bins
   const int bits = 32 - __clz((int)n);
-  return bits > 11 ? bits - 11 : 0;
+  return bits > kBinBits ? bits - kBinBits : 0;
 }
 
-// The longest run of the entries that `cut` leaves, in descending order, ties lowest
-// index first, whose measure (1 or a mass) sums to no more than target; at least one entry.
-template <class R, class Measure>
-__device__ Cut select(const R& row, const Cut& cut, float m, float scale, u64 target, Measure measure,
-                      ChooseShared& sh) {
-  u64 above = 0;
-  clear_bins(sh);
-  auto bin_of = [&](float x) { return (int)fminf((m - x) * scale, (float)(kBins - 1)); };
-  row.each([&](float x, int i) {
-    if (cut.keeps(x, i)) atomicAdd(&sh.hist[bin_of(x)], measure(x));
-  });
-  const int bin = find_bin(sh, above, target);
-  if (bin < 0) return cut;
-  // the keys of that bin
-  uint32_t lo = 0xffffffffu, hi = 0;
-  row.each([&](float x, int i) {
-    if (cut.keeps(x, i) && bin_of(x) == bin) {
-      const uint32_t k = key_of(x);
-      lo = min(lo, k);
-      hi = max(hi, k);
+// The least float (by its key) that falls into a bin up to `bin`; the whole workgroup
+// looks for the same.
+__device__ __forceinline__ float bin_floor(int bin, float m, float scale) {
+  uint32_t lo = key_of(-__FLT_MAX__), hi = key_of(m);  // hi does
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (bin_of(value_of(mid), m, scale) <= bin) hi = mid;
+    else lo = mid + 1;
+  }
+  return value_of(hi);
+}
+
+// The entries of one bin that a cut leaves: listed in LDS, or, if they are too many for
+// that, looked for in the row each time.
+template <class Tag>
+struct BinEntries {
+  const char* row;
+  int64_t V;
+  float lo, hi;  // entries lo <= x < hi (hi: +inf for the first bin)
+  Cut cut;
+  CutShared* sh;
+  int listed;
+  __device__ __forceinline__ BinEntries(const ChooseArgs& a, int64_t b, float m, float scale, int bin, const Cut& cut_,
+                                        CutShared& sh_)
+      : row(row_at<Tag>(a, b)), V(a.V), cut(cut_), sh(&sh_), listed(kListed + 1) {
+    lo = bin_floor(bin, m, scale);
+    hi = bin > 0 ? bin_floor(bin - 1, m, scale) : M<float>::inf();
+    __syncthreads();
+    if (threadIdx.x == 0) sh->listed = 0;
+    __syncthreads();
+    each([&](float x, int i) {  // in any order: what follows does not depend on it
+      const int at = atomicAdd(&sh->listed, 1);
+      if (at < kListed) {
+        sh->list_x[at] = x;
+        sh->list_i[at] = i;
+      }
+    });
+    __syncthreads();
+    listed = sh->listed;
+  }
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    if (listed <= kListed) {
+      for (int k = threadIdx.x; k < listed; k += kRT) f(sh->list_x[k], sh->list_i[k]);
+    } else {
+      constexpr int EPV = Pack16<Tag>::EPV;
+      sweep<Tag, kRT>(row, 0, V, threadIdx.x, [&](const float (&x)[EPV], int i) {
+        uint32_t in = 0;
+#pragma unroll
+        for (int k = 0; k < EPV; ++k) in |= (x[k] >= lo && x[k] < hi ? 1u : 0u) << k;
+        if (!in) return;
+#pragma unroll
+        for (int k = 0; k < EPV; ++k)
+          if ((in >> k & 1) && cut.keeps(x[k], i + k)) f(x[k], i + k);
+      });
     }
+  }
+};
+
+// The longest run of these entries, in descending order, ties lowest index first, whose
+// measure (1 or a mass), with `above` before them, sums to no more than target, which all
+// of them exceed; at least one entry where nothing is above.
+template <class Entries, class Measure>
+__device__ Cut select(const Entries& in, u64 above, u64 target, Measure measure, CutShared& sh) {
+  const int t = threadIdx.x;
+  uint32_t lo = 0xffffffffu, hi = 0;
+  in.each([&](float x, int) {
+    const uint32_t k = key_of(x);
+    lo = min(lo, k);
+    hi = max(hi, k);
   });
   uint32_t* sh32 = reinterpret_cast<uint32_t*>(sh.wave);
-  lo = block_reduce(lo, sh32, [](uint32_t a, uint32_t b) { return min(a, b); });
-  hi = block_reduce(hi, sh32, [](uint32_t a, uint32_t b) { return max(a, b); });
+  lo = block_reduce<kRW>(lo, sh32, Min());
+  hi = block_reduce<kRW>(hi, sh32, Max());
   while (lo < hi) {
     const int shift = bits_over(hi - lo);
-    clear_bins(sh);
-    row.each([&](float x, int i) {
+    __syncthreads();
+    sh.hist[t] = 0;
+    __syncthreads();
+    in.each([&](float x, int) {
       const uint32_t k = key_of(x);
-      if (k >= lo && k <= hi && cut.keeps(x, i)) atomicAdd(&sh.hist[(hi - k) >> shift], measure(x));
+      if (k >= lo && k <= hi) atomicAdd(&sh.hist[(hi - k) >> shift], measure(x));
     });
-    const int b = find_bin(sh, above, target);
+    __syncthreads();
+    const int b = max(find_bin(sh, sh.hist[t], above, target), 0);
     hi -= (uint32_t)b << shift;
     lo = max(lo, shift ? hi - ((1u << shift) - 1) : hi);
   }
@@ -206,47 +440,181 @@ __device__ Cut select(const R& row, const Cut& cut, float m, float scale, u64 ta
   const u64 each = measure(v);
   const u64 room = each ? (target - above) / each : ~(u64)0;
   const u64 take = above == 0 && room == 0 ? 1 : room;
-  u64 seen = 0;
-  int ilo = 0, ihi = (int)min(row.V, (int64_t)kNoIndex - 1);  // the place of the first that is not taken
   if (take == 0) return Cut{v, 0};
+  u64 seen = 0;
+  int ilo = 0, ihi = (int)in.V;  // the place of the first that is not taken
   while (ilo < ihi) {
     const int shift = bits_over((uint32_t)(ihi - ilo));
-    clear_bins(sh);
-    row.each([&](float x, int i) {
-      if (x == v && i >= ilo && i <= ihi && cut.keeps(x, i)) atomicAdd(&sh.hist[(i - ilo) >> shift], (u64)1);
+    __syncthreads();
+    sh.hist[t] = 0;
+    __syncthreads();
+    in.each([&](float x, int i) {
+      if (x == v && i >= ilo && i <= ihi) atomicAdd(&sh.hist[(i - ilo) >> shift], (u64)1);
     });
-    const int b = find_bin(sh, seen, take);
-    if (b < 0) return Cut{v, cut.v == v ? cut.n : kNoIndex};  // all of them
+    __syncthreads();
+    const int b = find_bin(sh, sh.hist[t], seen, take);
+    if (b < 0) return Cut{v, in.cut.v == v ? in.cut.n : kNoIndex};  // all of them
     ilo += b << shift;
     ihi = min(ihi, ilo + (1 << shift) - 1);
   }
   return Cut{v, ilo};
 }
 
+// One bin of every part.
+template <class T>
+__device__ __forceinline__ u64 over_parts(const T* bins, int parts) {
+  constexpr int kTogether = 10;
+  u64 sum = 0;
+  for (int k0 = 0; k0 < parts; k0 += kTogether) {
+    T v[kTogether];
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) v[k] = bins[(int64_t)min(k0 + k, parts - 1) * kBins];
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) sum += k0 + k < parts ? v[k] : 0;
+  }
+  return sum;
+}
+
 template <class Tag>
-__global__ __launch_bounds__(kCT) void choose_kernel(ChooseArgs a) {
-  __shared__ ChooseShared sh;
+__global__ __launch_bounds__(kRT) void choose_cut_kernel(ChooseArgs a) {
+  __shared__ CutShared sh;
+  const int64_t b = blockIdx.x;
+  const int t = threadIdx.x;
+  const Settings set(a, b);
+  if (!set.filtered || set.bad) return;
+  const float m = row_peak<kRW>(a, b, reinterpret_cast<float*>(sh.wave));
+  if (!(m < M<float>::inf())) return;
+  const float scale = set.scale();
+  const Mass mass(m, set.c(), a.magic);
+  Cut cut{-M<float>::inf(), 0};
+  u64 sum = 0, count = 0;  // this thread's bin
+  if (set.top_p > 0.0)
+    sum = over_parts(a.sums + (int64_t)b * a.parts * kBins + t, a.parts);
+  if (set.top_k > 0) {
+    count = over_parts(a.counts + (int64_t)b * a.parts * kBins + t, a.parts);
+    u64 above = 0;
+    const int bin = find_bin(sh, count, above, (u64)set.top_k);
+    if (bin >= 0) {
+      const BinEntries<Tag> in(a, b, m, scale, bin, cut, sh);
+      cut = select(in, above, (u64)set.top_k, [](float) { return (u64)1; }, sh);
+      if (set.top_p > 0.0) {  // what is left of that bin, and nothing below it
+        u64 rest = 0;
+        in.each([&](float x, int i) { rest += cut.keeps(x, i) ? mass(x) : 0; });
+        rest = block_reduce<kRW>(rest, sh.wave, Add());
+        sum = t < bin ? sum : (t == bin ? rest : 0);
+      }
+    }
+  }
+  if (set.top_p > 0.0) {
+    u64 all = 0;
+    if (set.top_k > 0) all = sum;
+    else
+      for (int k = t; k < a.parts; k += kRT) all += a.whole[b * a.parts + k];
+    all = block_reduce<kRW>(all, sh.wave, Add());
+    const u64 target = (u64)(set.top_p * (double)all);
+    u64 above = 0;
+    const int bin = find_bin(sh, sum, above, target);
+    if (bin >= 0) {
+      const BinEntries<Tag> in(a, b, m, scale, bin, cut, sh);
+      cut = select(in, above, target, mass, sh);
+    }
+  }
+  const Cut least = set.least(m);
+  if (least.v > cut.v) cut = least;
+  if (t == 0) a.cut[b] = cut;
+}
+
+// ---- 4 ---------------------------------------------------------------------------------
+
+// A nucleus is a few entries in a hundred, so a lane first marks those of its vectors,
+// then weighs its marked ones, read again, one after another: as many turns as the lane
+// with most of them has.  Where some lane has over a quarter, all are weighed in place.
+template <class Tag, bool DIRECT>
+__device__ __forceinline__ u64 weigh_left(const ChooseArgs& a, const char* row, int64_t part, const Cut& cut,
+                                          const Mass& mass) {
+  constexpr int EPV = Pack16<Tag>::EPV;
+  u64 left = 0;
+  const int64_t quarter = a.part / kPW, lo = part * a.part + (threadIdx.x >> 6) * quarter;
+  const int64_t hi = min(lo + quarter, a.V);
+  const int lane = threadIdx.x & 63;
+  for (int64_t i0 = lo; i0 < hi; i0 += kAhead * 64 * EPV) {
+    u32x4 raw[kAhead];
+    if (i0 + kAhead * 64 * EPV <= hi) {
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s)
+        raw[s] = reinterpret_cast<const Any16*>(row + (i0 + (s * 64 + lane) * EPV) * (16 / EPV))->v;
+    } else {
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        float x[EPV];
+        load_entries<Tag>(row, i0 + (s * 64 + lane) * EPV, hi, x);
+        raw[s] = Pack16<Tag>::pack(x);
+      }
+    }
+    uint32_t marks = 0;
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      float x[EPV];
+      Pack16<Tag>::unpack(raw[s], x);
+#pragma unroll
+      for (int k = 0; k < EPV; ++k)
+        marks |= (cut.keeps(x[k], (int)(i0 + (s * 64 + lane) * EPV) + k) ? 1u : 0u) << (s * EPV + k);
+    }
+    if (__any(__popc(marks) > kAhead * EPV / 4)) {
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        float x[EPV];
+        Pack16<Tag>::unpack(raw[s], x);
+#pragma unroll
+        for (int k = 0; k < EPV; ++k) left += marks >> (s * EPV + k) & 1 ? mass.of<DIRECT>(x[k]) : 0;
+      }
+    } else {
+      while (__any(marks != 0)) {
+        if (marks) {
+          const int k = __ffs((int)marks) - 1;
+          marks &= marks - 1;
+          left += mass.of<DIRECT>(load_entry<Tag>(row, i0 + (k / EPV * 64 + lane) * EPV + k % EPV));
+        }
+      }
+    }
+  }
+  return left;
+}
+
+template <class Tag>
+__global__ __launch_bounds__(kPT) void choose_left_kernel(ChooseArgs a) {
+  const int64_t b = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  __shared__ float sh[kPW];
+  const Settings set(a, b);
+  if (!set.filtered || set.bad) return;
+  const float m = row_peak<kPW>(a, b, sh);
+  if (!(m < M<float>::inf())) return;
+  const Cut cut = a.cut[b];
+  u64 left = 0;
+  if (a.peak[blockIdx.x] >= cut.v) {
+    const Mass mass(m, set.c(), a.magic);
+    const char* row = row_at<Tag>(a, b);
+    left = mass.w.direct ? weigh_left<Tag, true>(a, row, part, cut, mass) : weigh_left<Tag, false>(a, row, part, cut, mass);
+    left = wave_total(left);
+  }
+  if ((threadIdx.x & 63) == 0) a.left[blockIdx.x * kPW + (threadIdx.x >> 6)] = left;
+}
+
+// ---- 5 ---------------------------------------------------------------------------------
+
+template <class Tag>
+__global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
+  constexpr int EPV = Pack16<Tag>::EPV;
   const int64_t b = blockIdx.x;
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
-  const Row<Tag> row{a.x + b * a.ld * (16 / Pack16<Tag>::EPV), a.V, a.slabs};
-  double T = a.temperature ? (double)a.temperature[b] : a.temperature_all;
-  const double top_p = a.top_p ? (double)a.top_p[b] : a.top_p_all;
-  const double min_p = a.min_p ? (double)a.min_p[b] : a.min_p_all;
-  const int64_t top_k = a.top_k ? load_index(a.top_k, a.top_k_dt, b) : a.top_k_all;
-  const bool greedy = T <= 0.0;
-  if (greedy) T = 1.0;
-
-  float m = -M<float>::inf();
-  int nan = 0;
-  row.each([&](float x, int) {
-    m = fmaxf(m, x);
-    nan |= x != x;
-  });
-  float* shf = reinterpret_cast<float*>(sh.wave);
-  m = block_reduce(m, shf, [](float p, float q) { return fmaxf(p, q); });
-  nan = block_reduce(nan, reinterpret_cast<int*>(sh.wave), [](int p, int q) { return p | q; });
-  // a row or a temperature without a distribution
-  if (nan || !(fabsf(m) < M<float>::inf()) || !(T < M<double>::inf())) {
+  __shared__ u64 sh[kPW], sh_before;
+  __shared__ int sh_quarter;
+  int* const shi = reinterpret_cast<int*>(sh);
+  const char* row = row_at<Tag>(a, b);
+  const float* peak = a.peak + b * a.parts;
+  const Settings set(a, b);
+  const float m = row_peak<kPW>(a, b, reinterpret_cast<float*>(sh));
+  if (set.bad || !(m < M<float>::inf())) {  // a row or a temperature without a distribution
     if (t == 0) {
       a.token_out[b] = -1;
       a.logp_out[b] = M<float>::nan();
@@ -254,139 +622,215 @@ __global__ __launch_bounds__(kCT) void choose_kernel(ChooseArgs a) {
     }
     return;
   }
-  if (T < 1e-290) T = 1e-290;  // has the distribution's limit already
-  const Weight weight(m, 1.4426950408889634074 / T, 1.0);
-  const Mass mass(weight, a.magic);
-
-  u64 whole = 0;
-  row.each([&](float x, int) { whole += mass(x); });
+  u64 whole = 0, left = 0;
+  for (int p = t; p < a.parts; p += kPT) whole += a.whole[b * a.parts + p];
+  // sums of what is left in their order, a run of quarters to a thread
+  const int quarters = a.parts * kPW, run = (quarters + kPT - 1) / kPT;
+  const int p0 = min(t * run, quarters), p1 = min(p0 + run, quarters);
+  const u64* const lefts = a.left + b * quarters;
+  if (!set.greedy)
+    for (int p = p0; p < p1; ++p) left += lefts[p];
   const double unit = ldexp(1.0, -a.unit_log2);
-  const double norm = log((double)block_sum_u64(whole, sh.wave) * unit);
-
-  int64_t token;
+  const double norm = log((double)block_reduce<kPW>(whole, sh, Add()) * unit);
+  int token = kNoIndex;
   double logq = 0.0;
-  if (greedy) {
-    int first = kNoIndex;
-    row.each([&](float x, int i) { first = x == m ? min(first, i) : first; });
-    token = block_reduce(first, reinterpret_cast<int*>(sh.wave), [](int p, int q) { return min(p, q); });
-  } else {
-    Cut cut{-M<float>::inf(), 0};
-    // bins of 1/32 of a factor of two
-    const float scale = (float)fmin(32.0 * weight.c, 3e38);
-    if (top_k > 0 && top_k < a.V)
-      cut = select(row, cut, m, scale, (u64)top_k, [](float) { return (u64)1; }, sh);
-    if (top_p > 0.0 && top_p < 1.0) {
-      u64 left = 0;
-      row.each([&](float x, int i) { left += cut.keeps(x, i) ? mass(x) : 0; });
-      left = block_sum_u64(left, sh.wave);
-      cut = select(row, cut, m, scale, (u64)(top_p * (double)left), mass, sh);
-    }
-    if (min_p > 0.0) {
-      const double far = T * log(fmin(min_p, 1.0));
-      // the least float at no more than that distance, a step or two from this one
-      uint32_t k = key_of((float)((double)m + far));
-      for (int n = 0; n < 4 && (double)value_of(k) - (double)m < far; ++n) ++k;
-      for (int n = 0; n < 4 && (double)value_of(k - 1) - (double)m >= far; ++n) --k;
-      const float least = value_of(k);
-      if (least > cut.v) cut = Cut{least, kNoIndex};
-    }
-    u64 mine = 0;
-    row.each([&](float x, int i) { mine += cut.keeps(x, i) ? mass(x) : 0; });
-    u64 sum = mine;
+  auto span = [&](int64_t lo, int64_t n, auto f) {
+    sweep<Tag, kPT>(row, lo, min(lo + n, a.V), t, [&](const float (&x)[EPV], int i) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+      for (int k = 0; k < EPV; ++k) f(x[k], i + k);
+    });
+  };
+  if (set.greedy) {
+    int first = kNoIndex;
+    for (int p = t; p < a.parts; p += kPT)
+      if (peak[p] == m) first = min(first, p);
+    first = block_reduce<kPW>(first, shi, Min());
+    span((int64_t)first * a.part, a.part, [&](float x, int i) { token = x == m ? min(token, i) : token; });
+    token = block_reduce<kPW>(token, shi, Min());
+  } else {
+    const Mass mass(m, set.c(), a.magic);
+    const Cut cut = set.filtered ? a.cut[b] : set.least(m);
+    u64 upto = left;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const u64 y = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += y;
+    }
     __syncthreads();
-    if (lane == 0) sh.wave[wv] = sum;
-    if (t == 0) sh.slot = kNoIndex;
+    if (lane == 63) sh[wv] = upto;
     __syncthreads();
-    u64 total = 0, before = 0;
-    for (int k = 0; k < kCW; ++k) {
-      if (k < wv) before += sh.wave[k];
-      total += sh.wave[k];
+    u64 total = 0;
+    for (int k = 0; k < kPW; ++k) {
+      if (k < wv) upto += sh[k];
+      total += sh[k];
     }
     const double u = (double)a.u[b];
     const u64 border = u > 0.0 ? (u64)(fmin(u, 1.0) * (double)total) : 0;
-    int found = kNoIndex;
     if (border == 0) {  // the first entry with any mass, be it less than a unit
-      row.each([&](float x, int i) {
-        if (cut.keeps(x, i) && ((double)x - (double)m) * weight.c > -1000.0) found = min(found, i);
-      });
+      for (int p = 0; p < a.parts && token == kNoIndex; ++p) {
+        if (peak[p] < cut.v) continue;
+        span((int64_t)p * a.part, a.part, [&](float x, int i) {
+          if (x != -M<float>::inf() && cut.keeps(x, i) && ((double)x - (double)m) * mass.w.c > -1000.0)
+            token = min(token, i);
+        });
+        token = block_reduce<kPW>(token, shi, Min());
+      }
     } else if (border >= total) {  // a uniform of 1: the last with any
       int last = -1;
-      row.each([&](float x, int i) {
-        if (cut.keeps(x, i) && mass(x)) last = max(last, i);
+      for (int p = p0; p < p1; ++p)
+        if (lefts[p]) last = p;
+      last = block_reduce<kPW>(last, shi, Max());
+      token = -1;
+      span((int64_t)last * (a.part / kPW), a.part / kPW, [&](float x, int i) {
+        if (cut.keeps(x, i) && mass(x)) token = max(token, i);
       });
-      found = block_reduce(last, reinterpret_cast<int*>(sh.wave), [](int p, int q) { return max(p, q); });
-    } else if (before <= border && before + sum > border) {  // one wave's
-      for (int s = 0; s < a.slabs; ++s) {
-        constexpr int EPV = Row<Tag>::EPV;
-        const int64_t i = (((int64_t)wv * a.slabs + s) * 64 + lane) * EPV;
+      token = block_reduce<kPW>(token, shi, Max());
+    } else {
+      if (upto > border && upto - left <= border) {  // one thread's
+        u64 at = upto - left;
+        int p = p0;
+        for (; p < p1 - 1; ++p) {
+          const u64 w = lefts[p];
+          if (at + w > border) break;
+          at += w;
+        }
+        sh_quarter = p;
+        sh_before = at;
+      }
+      __syncthreads();
+      // a run of the quarter's vectors to a thread
+      const int vectors = a.part / (kPW * EPV * kPT) > 0 ? a.part / (kPW * EPV * kPT) : 1;
+      const int64_t lo = (int64_t)sh_quarter * (a.part / kPW), hi = min(lo + a.part / kPW, a.V);
+      const int64_t i0 = lo + (int64_t)t * vectors * EPV;
+      auto weights = [&](int64_t i, u64 (&w)[EPV]) {
         float x[EPV];
+        load_entries<Tag>(row, i, hi, x);
 #pragma unroll
-        for (int k = 0; k < EPV; ++k) x[k] = -M<float>::inf();
-        if (i < a.V) load_entries<Tag>(row.p, i, a.V, x);
-        u64 w[EPV], here = 0;
+        for (int k = 0; k < EPV; ++k) w[k] = cut.keeps(x[k], (int)i + k) ? mass(x[k]) : 0;
+      };
+      u64 here = 0;
+      for (int s = 0; s < vectors; ++s) {
+        u64 w[EPV];
+        weights(i0 + s * EPV, w);
 #pragma unroll
-        for (int k = 0; k < EPV; ++k) {
-          w[k] = x[k] != -M<float>::inf() && cut.keeps(x[k], (int)i + k) ? mass(x[k]) : 0;
-          here += w[k];
-        }
-        u64 upto = here;
+        for (int k = 0; k < EPV; ++k) here += w[k];
+      }
+      u64 end = here;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const u64 y = __shfl_up(upto, o, 64);
-          if (lane >= o) upto += y;
-        }
-        u64 at = before + upto - here;
-        if (at <= border && at + here > border) {
+      for (int o = 1; o < 64; o <<= 1) {
+        const u64 y = __shfl_up(end, o, 64);
+        if (lane >= o) end += y;
+      }
+      if (lane == 63) sh[wv] = end;
+      __syncthreads();
+      for (int k = 0; k < wv; ++k) end += sh[k];
+      u64 at = sh_before + end - here;
+      if (at <= border && at + here > border) {  // one thread's
+        for (int s = 0; s < vectors; ++s) {
+          u64 w[EPV];
+          weights(i0 + s * EPV, w);
 #pragma unroll
           for (int k = 0; k < EPV; ++k) {
             at += w[k];
-            if (at > border) found = min(found, (int)i + k);
+            if (at > border) token = min(token, (int)(i0 + s * EPV) + k);
           }
         }
-        before += __shfl(upto, 63, 64);
-        if (before > border) break;
       }
+      token = block_reduce<kPW>(token, shi, Min());
     }
-    token = block_reduce(found, reinterpret_cast<int*>(sh.wave), [](int p, int q) { return min(p, q); });
     logq = log((double)total * unit);
   }
   if (t == 0) {
-    const double d = ((double)load_entry<Tag>(row.p, token) - (double)m) / T;
+    const double d = ((double)load_entry<Tag>(row, token) - (double)m) / set.T;
     a.token_out[b] = token;
     a.logp_out[b] = fminf((float)(d - norm), 0.0f);
-    if (a.logq_out) a.logq_out[b] = greedy ? 0.0f : fminf((float)(d - logq), 0.0f);
+    if (a.logq_out) a.logq_out[b] = set.greedy ? 0.0f : fminf((float)(d - logq), 0.0f);
   }
 }
 
-template <class Tag>
-int launch_choose(ChooseArgs a, int64_t B, hipStream_t st) {
-  constexpr int64_t step = (int64_t)kCT * Pack16<Tag>::EPV;
-  a.slabs = (int)((a.V + step - 1) / step);
-  hipLaunchKernelGGL(choose_kernel<Tag>, dim3((uint32_t)B), dim3(kCT), 0, st, a);
-  return check_launch("choose_kernel");
+// ---- host ------------------------------------------------------------------------------
+
+// Entries of a part: as many as leave a thousand workgroups.
+inline int part_entries(int64_t B, int64_t V) {
+  int part = 8192;
+  while (part < 65536 && B * ((V + 2 * part - 1) / (2 * part)) >= 1024) part *= 2;
+  return part;
 }
+
+struct ChooseLayout {
+  int part;
+  int64_t parts;
+  size_t peak, whole, left, sums, counts, cut, total;
+};
+inline ChooseLayout choose_layout(int64_t B, int64_t V, bool top_k, bool top_p) {
+  ChooseLayout l;
+  l.part = part_entries(B, V);
+  l.parts = (V + l.part - 1) / l.part;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  const size_t n = (size_t)(B * l.parts);
+  l.peak = take(4 * n);
+  l.whole = take(8 * n);
+  l.left = take(8 * n * kPW);
+  l.sums = take(top_p ? 8 * n * kBins : 0);
+  l.counts = take(top_k ? 4 * n * kBins : 0);
+  l.cut = take(sizeof(Cut) * (size_t)B);
+  l.total = at;
+  return l;
+}
+
+template <class Tag>
+int launch_choose(const ChooseArgs& a, int64_t B, bool filters, hipStream_t st) {
+  const dim3 parts((uint32_t)(B * a.parts)), rows((uint32_t)B);
+  hipLaunchKernelGGL(choose_max_kernel<Tag>, parts, dim3(kPT), 0, st, a);
+  if (int rc = check_launch("choose_max_kernel")) return rc;
+  hipLaunchKernelGGL(choose_weigh_kernel<Tag>, parts, dim3(kPT), 0, st, a);
+  if (int rc = check_launch("choose_weigh_kernel")) return rc;
+  if (filters) {
+    hipLaunchKernelGGL(choose_cut_kernel<Tag>, rows, dim3(kRT), 0, st, a);
+    if (int rc = check_launch("choose_cut_kernel")) return rc;
+    hipLaunchKernelGGL(choose_left_kernel<Tag>, parts, dim3(kPT), 0, st, a);
+    if (int rc = check_launch("choose_left_kernel")) return rc;
+  }
+  hipLaunchKernelGGL(choose_draw_kernel<Tag>, rows, dim3(kPT), 0, st, a);
+  return check_launch("choose_draw_kernel");
+}
+
+// Sizes whose index arithmetic and grids fit (a grid's threads are counted in 32 bits).
+inline bool choose_fits(int64_t B, int64_t V) {
+  return B >= 0 && V >= 1 && B < ((int64_t)1 << 22) && V <= ((int64_t)1 << 30) &&
+         B * ((V + part_entries(B, V) - 1) / part_entries(B, V)) < ((int64_t)1 << 24);
+}
+inline bool may_top_k(const rrl_sample_params& p, int64_t V) { return p.top_ks || (p.top_k > 0 && p.top_k < V); }
+inline bool may_top_p(const rrl_sample_params& p) { return p.top_ps || (p.top_p > 0.0 && p.top_p < 1.0); }
 
 }  // namespace
 }  // namespace rrl
 
 using namespace rrl;
 
+extern "C" size_t rrl_sample_tokens_workspace_bytes(int64_t B, int64_t V, const rrl_sample_params* params) {
+  if (!choose_fits(B, V)) return 0;
+  return choose_layout(B, V, !params || may_top_k(*params, V), !params || may_top_p(*params)).total;
+}
+
 extern "C" int rrl_sample_tokens(const void* logits, int32_t dtype, int64_t B, int64_t V, int64_t row_stride,
                                  const float* uniforms, const rrl_sample_params* params, int64_t* token_out,
-                                 float* logp_out, float* logq_out, void* stream) {
+                                 float* logp_out, float* logq_out, void* workspace, void* stream) {
   clear_error();
   RRL_REQUIRE(dtype == RRL_F32 || dtype == RRL_BF16 || dtype == RRL_F16, RRL_EDTYPE,
               "rrl_sample_tokens: logits must be float32, bfloat16 or float16");
   RRL_REQUIRE(B >= 0, RRL_EINVAL, "rrl_sample_tokens: negative size");
   if (B == 0) return RRL_OK;
   RRL_REQUIRE(V >= 1, RRL_EINVAL, "rrl_sample_tokens: logits need at least one vocabulary entry");
-  // a grid's threads are counted in 32 bits, and an index with its bins in 31
-  RRL_REQUIRE(B < ((int64_t)1 << 22) && V <= ((int64_t)1 << 30), RRL_EINVAL,
-              "rrl_sample_tokens: 2^22 rows or more, or rows of over 2^30 entries");
+  RRL_REQUIRE(choose_fits(B, V), RRL_EINVAL,
+              "rrl_sample_tokens: 2^22 rows or more, rows of over 2^30 entries, or 2^24 parts of them or more");
   RRL_REQUIRE(logits != nullptr && uniforms != nullptr && params != nullptr && token_out != nullptr &&
-                  logp_out != nullptr,
+                  logp_out != nullptr && workspace != nullptr,
               RRL_EINVAL, "rrl_sample_tokens: null operand");
   RRL_REQUIRE(B <= 1 || row_stride >= 0, RRL_EINVAL, "rrl_sample_tokens: negative row stride");
   const rrl_sample_params& p = *params;
@@ -394,9 +838,9 @@ extern "C" int rrl_sample_tokens(const void* logits, int32_t dtype, int64_t B, i
               "rrl_sample_tokens: top_k must be int32 or int64");
   RRL_REQUIRE((uintptr_t)logits % dtype_size(dtype) == 0 && (uintptr_t)uniforms % 4 == 0 &&
                   (uintptr_t)p.temperatures % 4 == 0 && (uintptr_t)p.top_ps % 4 == 0 &&
-                  (uintptr_t)p.min_ps % 4 == 0 &&
+                  (uintptr_t)p.min_ps % 4 == 0 && (uintptr_t)workspace % 16 == 0 &&
                   (p.top_ks == nullptr || (uintptr_t)p.top_ks % dtype_size(p.top_k_dtype) == 0),
-              RRL_EALIGN, "rrl_sample_tokens: a pointer is not aligned to its element");
+              RRL_EALIGN, "rrl_sample_tokens: a pointer is not aligned (workspace: 16 bytes)");
   ChooseArgs a;
   a.x = static_cast<const char*>(logits);
   a.ld = row_stride;
@@ -415,11 +859,22 @@ extern "C" int rrl_sample_tokens(const void* logits, int32_t dtype, int64_t B, i
   while (((int64_t)1 << bits) < V) ++bits;
   a.unit_log2 = bits > 18 ? 62 - bits : 44;
   a.magic = ldexp(1.0, 52 - a.unit_log2);
+  const bool top_k = may_top_k(p, V), top_p = may_top_p(p);
+  const ChooseLayout l = choose_layout(B, V, top_k, top_p);
+  char* w = static_cast<char*>(workspace);
+  a.part = l.part;
+  a.parts = (int)l.parts;
+  a.peak = reinterpret_cast<float*>(w + l.peak);
+  a.whole = reinterpret_cast<u64*>(w + l.whole);
+  a.left = reinterpret_cast<u64*>(w + l.left);
+  a.sums = reinterpret_cast<u64*>(w + l.sums);
+  a.counts = reinterpret_cast<uint32_t*>(w + l.counts);
+  a.cut = reinterpret_cast<Cut*>(w + l.cut);
   a.token_out = token_out;
   a.logp_out = logp_out;
   a.logq_out = logq_out;
   hipStream_t st = as_stream(stream);
-  if (dtype == RRL_F32) return launch_choose<TagF32>(a, B, st);
-  if (dtype == RRL_BF16) return launch_choose<TagBF16>(a, B, st);
-  return launch_choose<TagF16>(a, B, st);
+  if (dtype == RRL_F32) return launch_choose<TagF32>(a, B, top_k || top_p, st);
+  if (dtype == RRL_BF16) return launch_choose<TagBF16>(a, B, top_k || top_p, st);
+  return launch_choose<TagF16>(a, B, top_k || top_p, st);
 }

@@ -98,7 +98,8 @@ def sample_tokens(
     tokens = torch.empty(B, dtype=torch.int64, device=dev)
     logp = torch.empty(B, dtype=torch.float32, device=dev)
     logq = torch.empty(B, dtype=torch.float32, device=dev) if sampling_logprobs else None
+    ws = torch.empty(nat.lib().rrl_sample_tokens_workspace_bytes(B, V, params), dtype=torch.uint8, device=dev)
     nat.call_on(dev, "rrl_sample_tokens", x.data_ptr(), nat.dtype_code(x.dtype), B, V,
                 x.stride(0) if B > 1 else V, u.data_ptr(), params, tokens.data_ptr(), logp.data_ptr(),
-                nat.ptr(logq), nat.stream_ptr(dev))
+                nat.ptr(logq), ws.data_ptr(), nat.stream_ptr(dev))
     return SampleOutput(tokens, logp, logq)

@@ -63,19 +63,24 @@ def lib():
 
 def test_entry_point_validation(lib):
     def call(x=16, dt=nat.BF16, B=2, V=8, ld=8, u=16, T=None, tp=None, mp=None, k=None, kdt=nat.I32, tok=16, lp=16,
-             params=True):
+             ws=16, params=True):
         p = nat.RrlSampleParams(1.0, 1.0, 0.0, 0, T, tp, mp, k, kdt) if params else None
-        return lib.rrl_sample_tokens(x, dt, B, V, ld, u, p, tok, lp, None, None)
+        return lib.rrl_sample_tokens(x, dt, B, V, ld, u, p, tok, lp, None, ws, None)
 
     assert call(B=0) == 0
     assert call(dt=nat.F64) == -2 and b"float32" in lib.rrl_last_error()
     assert call(B=-1) == -1 and b"negative" in lib.rrl_last_error()
     assert call(V=0) == -1 and b"vocabulary" in lib.rrl_last_error()
     assert call(B=1 << 22) == -1 and call(V=(1 << 30) + 1) == -1 and b"2^30" in lib.rrl_last_error()
-    for missing in ("x", "u", "tok", "lp"):
+    for missing in ("x", "u", "tok", "lp", "ws"):
         assert call(**{missing: None}) == -1 and b"null" in lib.rrl_last_error()
     assert call(params=False) == -1
     assert call(ld=-8) == -1
     assert call(k=16, kdt=nat.F32) == -2 and b"top_k" in lib.rrl_last_error()
     assert call(x=17) == -4 and call(u=18) == -4 and call(T=2) == -4 and call(tp=2) == -4 and call(mp=2) == -4
-    assert call(k=2) == -4 and call(k=12, kdt=nat.I64) == -4 and b"aligned" in lib.rrl_last_error()
+    assert call(ws=8) == -4 and call(k=2) == -4 and call(k=12, kdt=nat.I64) == -4 and b"aligned" in lib.rrl_last_error()
+    size = lib.rrl_sample_tokens_workspace_bytes
+    assert size(-1, 8, None) == 0 and size(1, 0, None) == 0 and size(1 << 22, 8, None) == 0
+    none, both = nat.RrlSampleParams(1.0, 1.0, 0.0, 0), nat.RrlSampleParams(1.0, 0.9, 0.0, 5)
+    # histograms of 1024 sums and counts a part of 4096 entries, where there may be a cut
+    assert size(4, 8192, both) == size(4, 8192, None) >= 4 * 2 * 1024 * 12 > size(4, 8192, none) > 0
