@@ -573,8 +573,8 @@ RRL_API int rrl_dropout(const void* x, int32_t dtype, int64_t rows, int64_t cols
  * (or NULL) of x, as rrl_dropout's.  Ranks up to 128, up to 4096 adapters.  Products are
  * summed in float32; t = down_a drop(x) is float32, taken to 2^-17 by the second product
  * of 16-bit operands; one rounding to `dtype`.
- * t_out: NULL, or float32 [N, rrl_adapter_rank_padded(r)] (16-byte aligned), t of the rows
- * that have an adapter, for the gradient of up.
+ * t_out: float32 [N, rrl_adapter_rank_padded(r)] (16-byte aligned), t of the rows that
+ * have an adapter (the others are not written), also for the gradient of up.
  * rrl_adapter_bwd, of grad = d out [N, O]: dx [N, H], ddown [A, r, H], dup [A, O, r], all
  * contiguous and each NULL where it is not wanted; ddown and dup are written for every
  * adapter (zeros where a has no row), dx for every row (zeros without an adapter).  x is

@@ -251,7 +251,7 @@ struct FusedArgs {
   AdapterIds ids;
   const float* scales;  // null: 1
   char* out;            // contiguous [N, O]; null: t alone
-  float* t;             // [N, 16 R16], or null
+  float* t;             // [N, 16 R16]
   int64_t N, K, O;
   int r;
   int groups;           // workgroups of a window
@@ -262,12 +262,15 @@ struct FusedArgs {
   int nan_rows;         // rows of ids that there are none of: NaN, or zeros
 };
 
-template <class Tag, int R16, int MT>
+enum Phase { BOTH, SHRINK, EXPAND };
+
+template <class Tag, int R16, int MT, int PHASE>
 __global__ __launch_bounds__(kAT) void adapter_fused_kernel(FusedArgs a) {
-  constexpr int SZ = 16 / Pack16<Tag>::EPV, TM = 16 * MT, R = 16 * R16, kAhead = 4, kChunks = kWindow / kAT;
+  constexpr int SZ = 16 / Pack16<Tag>::EPV, TM = 16 * MT, R = 16 * R16, kChunks = kWindow / kAT;
+  constexpr int kAhead = R16 > 2 || std::is_same_v<Tag, TagF32> ? 4 : 8, NC = 4;
   constexpr int kLd = R + 4;  // a row of t in LDS
   __shared__ uint16_t order[kWindow];
-  __shared__ __attribute__((aligned(16))) float part[kAW][TM][kLd];
+  __shared__ __attribute__((aligned(16))) float part[PHASE == EXPAND ? 1 : kAW][TM][kLd];
   __shared__ int scan[2][kAW];
   extern __shared__ int bins[];  // first place and first tile of each adapter, of none and bad, and the ends
   const int A2 = a.ids.A + 2;
@@ -385,7 +388,7 @@ __global__ __launch_bounds__(kAT) void adapter_fused_kernel(FusedArgs a) {
     auto token = [&](int i) { return n0 + (one ? row0 + i : (int)order[row0 + i]); };
 
     if (ad >= a.ids.A) {  // rows without an adapter
-      if (!a.out) continue;
+      if (PHASE == SHRINK || !a.out) continue;
       const int per = (int)((c1 - c0 + 7) / 8);
       for (int64_t k = t; k < (int64_t)here * per; k += kAT) {
         const int64_t n = token((int)(k / per)), c = c0 + k % per * 8;
@@ -404,102 +407,116 @@ __global__ __launch_bounds__(kAT) void adapter_fused_kernel(FusedArgs a) {
       continue;
     }
 
-    // t of the tile's rows: a wave takes a quarter of the depth
+    // t of the tile's rows; past its end the last again
+    auto n_of = [&](int f) { return token(min(16 * f + q, here - 1)); };
     int64_t n[MT];
 #pragma unroll
-    for (int f = 0; f < MT; ++f) n[f] = token(min(16 * f + q, here - 1));  // past the end the last again
-    {
-      f32x4 acc[MT][R16] = {};
+    for (int f = 0; f < MT; ++f) n[f] = n_of(f);
+    if constexpr (PHASE != EXPAND) {
+      __syncthreads();  // the last tile's t is read
       const char* down = a.down + ad * a.d_sa * SZ;
       const int64_t steps = (a.K + 31) / 32, per_row = (a.K + 7) / 8;
-      const int64_t s0 = steps * wv / kAW, s1 = steps * (wv + 1) / kAW;
-      for (int64_t s = s0; s < s1; s += kAhead) {
-        Frag<Tag> xf[kAhead][MT], df[kAhead][R16];
+      // Four sums over quarters of the depth, which are added in order.  With few rows a
+      // wave takes a quarter of all of them, else all quarters of 16 rows, each wave and
+      // tile starting at another one: rows a power of two apart lie on few of the memory's
+      // channels at one column.
+      for (int turn = 0; turn < (MT == 1 ? 1 : kAW); ++turn) {
+        if (MT > 1 && wv >= MT) break;
+        const int quarter = MT == 1 ? wv : (turn + wv + tile) % kAW;
+        const int64_t nf = MT == 1 ? n[0] : n_of(wv);
+        const char* xrow = a.x + nf * a.x_ld * SZ;
+        f32x4 acc[R16] = {};
+        const int64_t s0 = steps * quarter / kAW, s1 = steps * (quarter + 1) / kAW;
+        for (int64_t s = s0; s < s1; s += kAhead) {
+          Frag<Tag> xf[kAhead], df[kAhead][R16];
 #pragma unroll
-        for (int e = 0; e < kAhead; ++e) {
-          // past the wave's steps: zeros
-          const int64_t k = s + e < s1 ? (s + e) * 32 + kb * 8 : a.K;
+          for (int e = 0; e < kAhead; ++e) {
+            // past the quarter's steps: zeros
+            const int64_t k = s + e < s1 ? (s + e) * 32 + kb * 8 : a.K;
+            xf[e].load(xrow, k, a.K);
 #pragma unroll
-          for (int f = 0; f < MT; ++f) xf[e][f].load(a.x + n[f] * a.x_ld * SZ, k, a.K);
+            for (int j = 0; j < R16; ++j) {
+              const int rr = 16 * j + q;
+              df[e][j].load(down + min(rr, a.r - 1) * a.d_sr * SZ, rr < a.r ? k : a.K, a.K);
+            }
+          }
 #pragma unroll
-          for (int j = 0; j < R16; ++j) {
-            const int rr = 16 * j + q;
-            df[e][j].load(down + min(rr, a.r - 1) * a.d_sr * SZ, rr < a.r ? k : a.K, a.K);
+          for (int e = 0; e < kAhead; ++e) {
+            if (a.drop_in && s + e < s1) xf[e].keep(a.drop.keep_bits((uint64_t)(nf * per_row + (s + e) * 4 + kb), at));
+#pragma unroll
+            for (int j = 0; j < R16; ++j) acc[j] = mma<Tag>(df[e][j], xf[e], acc[j]);
           }
         }
-#pragma unroll
-        for (int e = 0; e < kAhead; ++e) {
-          if (a.drop_in && s + e < s1) {
-#pragma unroll
-            for (int f = 0; f < MT; ++f)
-              xf[e][f].keep(a.drop.keep_bits((uint64_t)(n[f] * per_row + (s + e) * 4 + kb), at));
-          }
-#pragma unroll
-          for (int f = 0; f < MT; ++f)
-#pragma unroll
-            for (int j = 0; j < R16; ++j) acc[f][j] = mma<Tag>(df[e][j], xf[e][f], acc[f][j]);
-        }
-      }
-      __syncthreads();  // the last tile's t is read
-#pragma unroll
-      for (int f = 0; f < MT; ++f)
 #pragma unroll
         for (int j = 0; j < R16; ++j)
-          *reinterpret_cast<f32x4*>(&part[wv][16 * f + q][16 * j + 4 * kb]) = acc[f][j];
+          *reinterpret_cast<f32x4*>(&part[quarter][(MT == 1 ? 0 : 16 * wv) + q][16 * j + 4 * kb]) = acc[j];
+      }
+      __syncthreads();
+      const float drop_scale = a.drop_in ? a.drop.scale : 1.0f;
+      for (int k = t; k < TM * R; k += kAT) {
+        const int i = k / R, j = k % R;
+        float v = (((part[0][i][j] + part[1][i][j]) + part[2][i][j]) + part[3][i][j]) * drop_scale;
+        if (j >= a.r) v = 0.0f;  // not an infinity of x times a padding's zero
+        part[0][i][j] = v;
+        if (slab == 0 && i < here) a.t[token(i) * R + j] = v;
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    const float drop_scale = a.drop_in ? a.drop.scale : 1.0f;
-    for (int k = t; k < TM * R; k += kAT) {
-      const int i = k / R, j = k % R;
-      float v = (((part[0][i][j] + part[1][i][j]) + part[2][i][j]) + part[3][i][j]) * drop_scale;
-      if (j >= a.r) v = 0.0f;  // not an infinity of x times a padding's zero
-      part[0][i][j] = v;
-      if (a.t && slab == 0 && i < here) a.t[token(i) * R + j] = v;
-    }
-    __syncthreads();
-    if (!a.out) continue;
+    if (PHASE == SHRINK || !a.out) continue;
 
-    // a wave takes 32 columns at a time
+    // a wave takes 16 NC columns at a time
     Thin<Tag, R16> thin[MT];
 #pragma unroll
-    for (int f = 0; f < MT; ++f) thin[f].load(&part[0][16 * f + q][0], kb);
+    for (int f = 0; f < MT; ++f) thin[f].load(PHASE == EXPAND ? a.t + n[f] * R : &part[0][16 * f + q][0], kb);
     const float scale = a.scales ? a.scales[ad] : 1.0f;
     const char* up = a.up + ad * a.u_sa * SZ;
-    for (int64_t c = c0 + 32 * wv; c < c1; c += 32 * kAW) {
-      // two tiles of up's rows, in an order that leaves eight consecutive columns to a lane
-      UpRow<Tag, R16> u[2];
+    // a run of them each, and each wave and tile from another place on, as above
+    const int groups = (int)((c1 - c0 + 16 * NC - 1) / (16 * NC));
+    const int g0 = groups * wv / kAW, g1 = groups * (wv + 1) / kAW;
+    for (int g = g0; g < g1; ++g) {
+      const int64_t c = c0 + 16 * NC * (g0 + (g - g0 + tile) % (g1 - g0));
+      Frag<Tag> b[MT][NC / 2];
+      UpRow<Tag, R16> u[NC];
+      if (a.base) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        u[i].load(up + min(c + 8 * (q >> 2) + 4 * i + (q & 3), a.O - 1) * a.u_so * SZ, a.r, kb);
-      const int64_t col = c + 8 * kb;
+        for (int f = 0; f < MT; ++f)
 #pragma unroll
-      for (int f = 0; f < MT; ++f) {
-        Frag<Tag> b;
-        if (a.base) b.load(a.base + n[f] * a.b_ld * SZ, col, c1);
-        float v[8];
+          for (int p = 0; p < NC / 2; ++p) b[f][p].load(a.base + n[f] * a.b_ld * SZ, c + 32 * p + 8 * kb, c1);
+      }
+      // pairs of tiles of up's rows, in an order that leaves eight consecutive columns to a lane
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const f32x4 d = expand<Tag, R16>(u[i], thin[f], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+      for (int i = 0; i < NC; ++i)
+        u[i].load(up + min(c + 16 * (i & ~1) + 8 * (q >> 2) + 4 * (i & 1) + (q & 3), a.O - 1) * a.u_so * SZ, a.r, kb);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[4 * i + k] = d[k];
+      for (int p = 0; p < NC / 2; ++p) {
+        const int64_t col = c + 32 * p + 8 * kb;
+#pragma unroll
+        for (int f = 0; f < MT; ++f) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const f32x4 d = expand<Tag, R16>(u[2 * p + i], thin[f], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[4 * i + k] = d[k];
+          }
+          if (a.drop_out) {
+            const uint32_t keep = a.drop.keep_bits((uint64_t)(n[f] * ((a.O + 7) / 8) + col / 8), at);
+            const float s = scale * a.drop.scale;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = keep >> k & 1 ? v[k] * s : 0.0f;
+          } else if (a.base) {
+            float x[8];
+            b[f][p].unpack(x);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = __builtin_fmaf(v[k], scale, x[k]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= scale;
+          }
+          Frag<Tag> o;
+          o.pack(v);
+          if (16 * f + q < here) o.store(a.out + n[f] * a.O * SZ, col, c1);
         }
-        if (a.drop_out) {
-          const uint32_t keep = a.drop.keep_bits((uint64_t)(n[f] * ((a.O + 7) / 8) + col / 8), at);
-          const float s = scale * a.drop.scale;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = keep >> k & 1 ? v[k] * s : 0.0f;
-        } else if (a.base) {
-          float x[8];
-          b.unpack(x);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = __builtin_fmaf(v[k], scale, x[k]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] *= scale;
-        }
-        Frag<Tag> o;
-        o.pack(v);
-        if (16 * f + q < here) o.store(a.out + n[f] * a.O * SZ, col, c1);
       }
     }
   }
@@ -514,7 +531,7 @@ struct OuterJob {
   const char* wide;   // [N, C]; null: no such job
   int64_t ld, C;
   const float* thin;  // [N, R]
-  float* part;        // [A, segments, C, R]
+  float* part;        // [A, segments], each [C, R], or [R, C] where the gradient's rows are along C
   int32_t* seen;      // [A, segments]: whether the run holds any of its tokens
   char* out;          // the gradient: entry (a, c, r) at a * o_sa + c * o_sc + r * o_sr
   int64_t o_sa, o_sc, o_sr;
@@ -527,12 +544,18 @@ struct OuterArgs {
   int64_t N;
   int r, R;           // R: r rounded up to a multiple of 16
   int rank_tiles;     // of 16 RT ranks
-  int window, segments;
-  int64_t windows;
+  int segments;
   Drop drop;
   const float* scales;
 };
 constexpr int kOuterCols = 128 * kAW;
+
+// What a lane holds of 32 tokens: eight columns and RT ranks of eight of them.
+template <class Tag, int RT>
+struct OuterStep {
+  Frag<Tag> x[8];
+  float th[8][RT];
+};
 
 template <class Tag, int RT>
 __global__ __launch_bounds__(kAT) void adapter_outer_kernel(OuterArgs a) {
@@ -557,10 +580,12 @@ __global__ __launch_bounds__(kAT) void adapter_outer_kernel(OuterArgs a) {
 
   f32x4 acc[8][RT] = {};
   bool any = false;
-  for (int64_t w = a.windows * seg / a.segments; w < a.windows * (seg + 1) / a.segments; ++w) {
+  // a run of tokens, from a multiple of 64 on
+  const int64_t begin = a.N * seg / a.segments / 64 * 64;
+  const int64_t end = seg + 1 == (uint32_t)a.segments ? a.N : a.N * (seg + 1) / a.segments / 64 * 64;
+  for (int64_t n0 = begin; n0 < end; n0 += kWindow) {
     // the window's tokens of this adapter, in order: a wave looks at a quarter of it
-    const int64_t n0 = w * a.window;
-    const int count = (int)min((int64_t)a.window, a.N - n0);
+    const int count = (int)min((int64_t)kWindow, end - n0);
     uint64_t mine[kWindow / kAT];
     int before = 0, sum = 0;
 #pragma unroll
@@ -586,19 +611,24 @@ __global__ __launch_bounds__(kAT) void adapter_outer_kernel(OuterArgs a) {
     }
     __syncthreads();
     any |= listed > 0;
-    if (col - 8 * q >= j.C) continue;  // this wave's columns are past the end
+    if (listed == 0 || col - 8 * q >= j.C) continue;  // or this wave's columns are past the end
     for (int s = 0; s < listed; s += 32) {
-      Frag<Tag> x[8];
-      float th[8][RT];
+      OuterStep<Tag, RT> in;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int k = s + 8 * kb + i;
         const bool here = k < listed;
         const int64_t n = n0 + list[here ? k : listed - 1];
-        x[i].load(j.wide + n * j.ld * SZ, here ? col : j.C, j.C);
-        if (j.drop) x[i].keep(a.drop.keep_bits((uint64_t)(n * per_row + col / 8), at));
+        in.x[i].load(j.wide + n * j.ld * SZ, here ? col : j.C, j.C);
 #pragma unroll
-        for (int e = 0; e < RT; ++e) th[i][e] = here ? j.thin[n * a.R + r0 + 16 * e + q] : 0.0f;
+        for (int e = 0; e < RT; ++e) in.th[i][e] = here ? j.thin[n * a.R + r0 + 16 * e + q] : 0.0f;
+      }
+      if (j.drop) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int64_t n = n0 + list[min(s + 8 * kb + i, listed - 1)];
+          in.x[i].keep(a.drop.keep_bits((uint64_t)(n * per_row + col / 8), at));
+        }
       }
       if constexpr (F32) {
 #pragma unroll
@@ -607,7 +637,7 @@ __global__ __launch_bounds__(kAT) void adapter_outer_kernel(OuterArgs a) {
           for (int c = 0; c < 8; ++c)
 #pragma unroll
             for (int e = 0; e < RT; ++e)
-              acc[c][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x[i].v[c / 4][c % 4]), th[i][e],
+              acc[c][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(in.x[i].v[c / 4][c % 4]), in.th[i][e],
                                                                acc[c][e], 0, 0, 0);
       } else {
         u32x4 hi[RT], lo[RT];
@@ -615,7 +645,7 @@ __global__ __launch_bounds__(kAT) void adapter_outer_kernel(OuterArgs a) {
         for (int e = 0; e < RT; ++e) {
           float v[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = th[i][e];
+          for (int i = 0; i < 8; ++i) v[i] = in.th[i][e];
           split8(v, hi[e], lo[e]);
         }
 #pragma unroll
@@ -624,7 +654,7 @@ __global__ __launch_bounds__(kAT) void adapter_outer_kernel(OuterArgs a) {
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
             // column c of tokens 2d and 2d + 1
-            const uint32_t two = __builtin_amdgcn_perm(x[2 * d + 1].v[0][c / 2], x[2 * d].v[0][c / 2],
+            const uint32_t two = __builtin_amdgcn_perm(in.x[2 * d + 1].v[0][c / 2], in.x[2 * d].v[0][c / 2],
                                                        c % 2 ? 0x07060302u : 0x05040100u);
             if constexpr (F16) {
               uint32_t h, l;
@@ -648,37 +678,65 @@ __global__ __launch_bounds__(kAT) void adapter_outer_kernel(OuterArgs a) {
   const int64_t slot = (int64_t)ad * a.segments + seg;
   if (ct == 0 && rt == 0 && t == 0) j.seen[slot] = any;
   if (!any) return;
-  // a lane's columns are 8 (4 kb + i) + c, its rank q
+  // a lane's columns are 8 (4 kb + i) + c, its rank q; neighbours as in the gradient
   float* part = j.part + slot * j.C * a.R;
+  const int64_t p_sc = j.o_sr == 1 ? a.R : 1, p_sr = j.o_sr == 1 ? 1 : j.C;
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
+  for (int i = 0; i < 4; ++i) {
+    const int64_t o = (int64_t)ct * kOuterCols + wv * 128 + 8 * (4 * kb + i);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t o = (int64_t)ct * kOuterCols + wv * 128 + 8 * (4 * kb + i) + c;
-      if (o < j.C)
+    for (int e = 0; e < RT; ++e) {
+      float* at = part + o * p_sc + (r0 + 16 * e + q) * p_sr;
+      if (p_sc == 1) {
+        Frag<TagF32> v;
+        float x[8];
 #pragma unroll
-        for (int e = 0; e < RT; ++e) part[o * a.R + r0 + 16 * e + q] = acc[c][e][i];
+        for (int c = 0; c < 8; ++c) x[c] = acc[c][e][i];
+        v.pack(x);
+        v.store(reinterpret_cast<char*>(at), 0, j.C - o);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (o + c < j.C) at[c * p_sc] = acc[c][e][i];
+      }
     }
+  }
 }
 
-// Joins the runs' sums, in order.
+// Joins the runs' sums, in order: a workgroup takes 64 entries, a wave a quarter of the runs.
 template <class Tag>
 __global__ __launch_bounds__(kAT) void adapter_join_kernel(OuterArgs a) {
+  __shared__ float quarter[kAW][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int64_t n0 = a.job[0].wide ? a.job[0].C * a.r : 0, n1 = a.job[1].wide ? a.job[1].C * a.r : 0;
-  int64_t k = (int64_t)blockIdx.x * kAT + threadIdx.x;
-  const int64_t ad = k / (n0 + n1);
-  if (ad >= a.ids.A) return;
-  k -= ad * (n0 + n1);
-  const bool second = k >= n0;
-  if (second) k -= n0;
+  const int64_t b0 = (n0 + 63) / 64, b1 = (n1 + 63) / 64;
+  const int64_t ad = blockIdx.x / (b0 + b1);
+  const bool second = blockIdx.x % (b0 + b1) >= b0;
+  const int64_t k = (blockIdx.x % (b0 + b1) - (second ? b0 : 0)) * 64 + lane;
   const OuterJob& j = a.job[second];
+  const bool in = k < (second ? n1 : n0);
   // neighbours in the gradient's rows
   const int64_t c = j.o_sr == 1 ? k / a.r : k % j.C, r = j.o_sr == 1 ? k % a.r : k / j.C;
+  const int64_t size = j.C * a.R, slot0 = ad * a.segments;
+  const float* part = j.part + slot0 * size + (j.o_sr == 1 ? c * a.R + r : r * j.C + c);
+  const int begin = a.segments * wv / kAW, end = a.segments * (wv + 1) / kAW;
+  constexpr int kTogether = 8;
   float sum = 0.0f;
-  for (int s = 0; s < a.segments; ++s) {
-    const int64_t slot = ad * a.segments + s;
-    if (j.seen[slot]) sum += j.part[(slot * j.C + c) * a.R + r];
+  for (int s64 = begin; s64 < end; s64 += 64) {
+    const uint64_t seen = __ballot(s64 + lane < end && j.seen[slot0 + min(s64 + lane, end - 1)]);
+    for (int s0 = 0; s0 < 64 && seen >> s0; s0 += kTogether) {
+      float v[kTogether];
+#pragma unroll
+      for (int s = 0; s < kTogether; ++s)
+        v[s] = in && (seen >> (s0 + s) & 1) ? part[(s64 + s0 + s) * size] : 0.0f;
+#pragma unroll
+      for (int s = 0; s < kTogether; ++s) sum += v[s];
+    }
   }
+  quarter[wv][lane] = sum;
+  __syncthreads();
+  if (wv != 0 || !in) return;
+  sum = ((quarter[0][lane] + quarter[1][lane]) + quarter[2][lane]) + quarter[3][lane];
   sum *= (a.scales ? a.scales[ad] : 1.0f);
   if (j.drop) sum *= a.drop.scale;
   const int64_t o = ad * j.o_sa + c * j.o_sc + r * j.o_sr;
@@ -717,27 +775,32 @@ __global__ __launch_bounds__(kAT) void adapter_turn_kernel(TurnArgs a) {
 
 inline int rank_padded(int r) { return r <= 16 ? 16 : (r <= 32 ? 32 : (r <= 64 ? 64 : 128)); }
 
-template <class Tag, int R16, int MT>
+template <class Tag, int R16, int MT, int PHASE>
 int launch_fused(FusedArgs a, hipStream_t st) {
   const int64_t windows = (a.N + kWindow - 1) / kWindow;
   const int rows = (int)min(a.N, (int64_t)kWindow);
   // tiles of a window if it is of one adapter, and at most
   const int64_t even = (rows + 16 * MT - 1) / (16 * MT), most = min((int64_t)rows, even + a.ids.A + 1);
-  // runs of columns: as many as make a thousand workgroups' work, of 128 columns at least
-  const int64_t cuts = a.out ? max((int64_t)1, min((a.O + 127) / 128, 1024 / max((int64_t)1, windows * even))) : 1;
-  a.slab = a.out ? ((a.O + cuts - 1) / cuts + 127) / 128 * 128 : 1;
-  a.slabs = a.out ? (int)((a.O + a.slab - 1) / a.slab) : 1;
+  // runs of columns: as many as make a thousand workgroups' work, of 256 columns at least
+  const bool wide = PHASE != SHRINK && a.out;
+  const int64_t cuts = wide ? max((int64_t)1, min((a.O + 255) / 256, 1024 / max((int64_t)1, windows * even))) : 1;
+  a.slab = wide ? ((a.O + cuts - 1) / cuts + 255) / 256 * 256 : 1;
+  a.slabs = wide ? (int)((a.O + a.slab - 1) / a.slab) : 1;
   a.groups = (int)max((int64_t)1, min(most * a.slabs, max(even * a.slabs, 2048 / windows)));
   RRL_REQUIRE(windows * a.groups < ((int64_t)1 << 32) / kAT, RRL_EINVAL, "rrl_adapter: too many rows");
   const size_t lds = (2 * sizeof(int) + kAW * sizeof(uint16_t)) * (size_t)(a.ids.A + 3);
-  hipLaunchKernelGGL((adapter_fused_kernel<Tag, R16, MT>), dim3((uint32_t)(windows * a.groups)), dim3(kAT), lds, st,
-                     a);
+  hipLaunchKernelGGL((adapter_fused_kernel<Tag, R16, MT, PHASE>), dim3((uint32_t)(windows * a.groups)), dim3(kAT), lds,
+                     st, a);
   return check_launch("adapter_fused_kernel");
 }
+// Few rows: both products in one launch.
+constexpr int64_t kFusedRows = 256;
 template <class Tag, int R16>
 int launch_fused(const FusedArgs& a, hipStream_t st) {
   constexpr int MT = R16 > 4 ? 2 : 4;
-  return a.N <= 256 ? launch_fused<Tag, R16, 1>(a, st) : launch_fused<Tag, R16, MT>(a, st);
+  if (a.N <= kFusedRows) return launch_fused<Tag, R16, 1, BOTH>(a, st);
+  if (int rc = launch_fused<Tag, R16, MT, SHRINK>(a, st)) return rc;
+  return a.out ? launch_fused<Tag, R16, MT, EXPAND>(a, st) : RRL_OK;
 }
 template <class Tag>
 int launch_fused(const FusedArgs& a, hipStream_t st) {
@@ -767,16 +830,15 @@ int launch_outer(const OuterArgs& a, hipStream_t st) {
 }
 template <class Tag>
 int launch_join(const OuterArgs& a, hipStream_t st) {
-  const int64_t each = (a.job[0].wide ? a.job[0].C * a.r : 0) + (a.job[1].wide ? a.job[1].C * a.r : 0);
-  hipLaunchKernelGGL(adapter_join_kernel<Tag>, dim3((uint32_t)((each * a.ids.A + kAT - 1) / kAT)), dim3(kAT), 0, st,
-                     a);
+  const int64_t each = ((a.job[0].wide ? a.job[0].C * a.r : 0) + 63) / 64 + ((a.job[1].wide ? a.job[1].C * a.r : 0) + 63) / 64;
+  hipLaunchKernelGGL(adapter_join_kernel<Tag>, dim3((uint32_t)(each * a.ids.A)), dim3(kAT), 0, st, a);
   return check_launch("adapter_join_kernel");
 }
 
 struct BackLayout {
   int R;
-  int64_t P, windows;
-  int window, segments, rank_tiles;
+  int64_t P;
+  int segments, rank_tiles;
   size_t upt, downt, s, part[2], seen[2], total;
 };
 inline BackLayout back_layout(int64_t N, int64_t H, int64_t O, int64_t A, int r, size_t size) {
@@ -785,12 +847,8 @@ inline BackLayout back_layout(int64_t N, int64_t H, int64_t O, int64_t A, int r,
   l.P = (O + 7) / 8 * 8;
   l.rank_tiles = l.R > 64 ? 2 : 1;
   const int64_t tiles = ((H + kOuterCols - 1) / kOuterCols + (O + kOuterCols - 1) / kOuterCols) * l.rank_tiles;
-  // windows of tokens so that there are a thousand workgroups, of 64 tokens at least
-  const int64_t runs = max((int64_t)1, 1024 / max((int64_t)1, A * tiles));
-  l.window = 64;
-  while (l.window < kWindow && (N + l.window - 1) / l.window > runs) l.window *= 2;
-  l.windows = (N + l.window - 1) / l.window;
-  l.segments = (int)min(l.windows, runs);
+  // runs of tokens so that there are four workgroups to each of the 256 CUs, of 64 tokens at least
+  l.segments = (int)min((N + 63) / 64, max((int64_t)1, 1024 / (A * tiles)));
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -853,7 +911,7 @@ extern "C" int rrl_adapter_fwd(const rrl_adapter_params* p, const void* x, int64
   if (p->dropout)
     if (int rc = make_drop(p->dropout, a.drop, "rrl_adapter_fwd")) return rc;
   if (p->N == 0) return RRL_OK;
-  RRL_REQUIRE(x != nullptr && p->down != nullptr && p->up != nullptr && out != nullptr, RRL_EINVAL,
+  RRL_REQUIRE(x != nullptr && p->down != nullptr && p->up != nullptr && out != nullptr && t_out != nullptr, RRL_EINVAL,
               "rrl_adapter_fwd: null operand");
   RRL_REQUIRE(p->N <= 1 || (x_ld >= 0 && base_ld >= 0), RRL_EINVAL, "rrl_adapter_fwd: negative row stride");
   const size_t size = dtype_size(p->dtype);
@@ -934,7 +992,7 @@ extern "C" int rrl_adapter_bwd(const rrl_adapter_params* p, const void* x, int64
     a.ids = ids;
     a.scales = p->scales;
     a.out = static_cast<char*>(dx);
-    a.t = ddown ? s : nullptr;
+    a.t = s;
     a.N = p->N;
     a.K = p->O;
     a.O = p->H;
@@ -950,8 +1008,6 @@ extern "C" int rrl_adapter_bwd(const rrl_adapter_params* p, const void* x, int64
   o.r = (int)p->r;
   o.R = l.R;
   o.rank_tiles = l.rank_tiles;
-  o.window = l.window;
-  o.windows = l.windows;
   o.segments = l.segments;
   o.drop = drop;
   o.scales = p->scales;

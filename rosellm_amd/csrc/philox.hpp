@@ -13,6 +13,7 @@ namespace rrl {
 __host__ __device__ inline void philox4x32_10(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
   const uint32_t kM0 = 0xD2511F53u, kM1 = 0xCD9E8D57u;
   const uint32_t kW0 = 0x9E3779B9u, kW1 = 0xBB67AE85u;
+#pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t p0 = (uint64_t)kM0 * c[0];
     const uint64_t p1 = (uint64_t)kM1 * c[2];

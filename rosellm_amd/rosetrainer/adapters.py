@@ -57,13 +57,12 @@ class _Adapter(torch.autograd.Function):
         up = up if up.stride(2) == 1 or up.shape[2] == 1 else up.contiguous()
         b, b_ld = (None, 0) if base is None else _rows(base)
         out = torch.empty(*x.shape[:-1], up.shape[1], dtype=x.dtype, device=dev)
-        t = None
-        if ctx.needs_input_grad[2]:
-            t = torch.empty(N, nat.lib().rrl_adapter_rank_padded(down.shape[1]), dtype=torch.float32, device=dev)
+        t = torch.empty(N, nat.lib().rrl_adapter_rank_padded(down.shape[1]), dtype=torch.float32, device=dev)
         drop = dropout_params(p, seed, offset, at) if draw is not None else None
         nat.call_on(dev, "rrl_adapter_fwd", _params(x.dtype, N, down, up, flat, scales, drop), rows.data_ptr(), ld,
-                    nat.ptr(b), b_ld, out.data_ptr(), nat.ptr(t), nat.stream_ptr(dev))
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, down, up, ids, scales, t, at)
+                    nat.ptr(b), b_ld, out.data_ptr(), t.data_ptr(), nat.stream_ptr(dev))
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, down, up, ids, scales,
+                              t if ctx.needs_input_grad[2] else None, at)
         ctx.args = (x.shape, None if draw is None else (p, seed, offset))
         return out
 

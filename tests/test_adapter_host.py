@@ -67,13 +67,13 @@ def test_entry_point_validation(lib):
     def params(dt=nat.BF16, N=4, H=8, O=6, A=2, r=3, down=16, up=16, ids=16, idt=nat.I64, scales=None, drop=None):
         return nat.RrlAdapterParams(dt, N, H, O, A, r, down, 24, 8, up, 18, 3, ids, idt, scales, drop)
 
-    def fwd(x=16, ld=8, base=None, bld=0, out=16, t=None, **kw):
+    def fwd(x=16, ld=8, base=None, bld=0, out=16, t=16, **kw):
         return lib.rrl_adapter_fwd(params(**kw), x, ld, base, bld, out, t, None)
 
     def bwd(x=16, ld=8, g=16, gld=6, t=16, dx=16, dd=16, du=16, ws=16, **kw):
         return lib.rrl_adapter_bwd(params(**kw), x, ld, g, gld, t, dx, dd, du, ws, None)
 
-    assert fwd(N=0) == 0 and lib.rrl_adapter_fwd(None, 16, 8, None, 0, 16, None, None) == -1
+    assert fwd(N=0) == 0 and lib.rrl_adapter_fwd(None, 16, 8, None, 0, 16, 16, None) == -1
     assert lib.rrl_adapter_bwd(None, 16, 8, 16, 6, 16, 16, 16, 16, 16, None) == -1
     for call in (fwd, bwd):
         assert call(dt=nat.F64) == -2 and b"float32" in lib.rrl_last_error()
@@ -89,7 +89,7 @@ def test_entry_point_validation(lib):
 
         drop = nat.RrlDropoutParams(2.0, 0, 0, None)
         assert call(drop=ctypes.pointer(drop)) == -1 and b"probability" in lib.rrl_last_error()
-    assert fwd(x=None) == -1 and fwd(out=None) == -1 and fwd(out=17) == -4 and fwd(t=24) == -4
+    assert fwd(x=None) == -1 and fwd(out=None) == -1 and fwd(t=None) == -1 and fwd(out=17) == -4 and fwd(t=24) == -4
     assert fwd(base=17) == -4 and fwd(base=16, bld=-1) == -1
     assert bwd(g=None) == -1 and bwd(x=None) == -1 and bwd(t=None) == -1 and bwd(ws=None) == -1
     assert bwd(g=17) == -4 and bwd(dx=17) == -4 and bwd(dd=17) == -4 and bwd(du=17) == -4
