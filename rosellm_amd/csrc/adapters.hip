@@ -45,22 +45,69 @@ __device__ __forceinline__ f32x4 mma_bf16(const u32x4& a, const u32x4& b, const 
                                                  0, 0);
 }
 
+// Keeps the two arms of a choice between kinds of access from becoming one.
+__device__ __forceinline__ void apart() { asm volatile("" ::: "memory"); }
+
+// 16 bytes at any element's address.
+typedef uint32_t AnyVec __attribute__((ext_vector_type(4), aligned(2)));
+
+// The first n of 16 bytes' entries, zeros behind them; and their store.
+template <class Tag>
+__device__ __forceinline__ u32x4 load_part(const char* from, int64_t n) {
+  constexpr int EPV = Pack16<Tag>::EPV;
+  float x[EPV];
+#pragma unroll
+  for (int k = 0; k < EPV; ++k) x[k] = k < n ? load_entry<Tag>(from, k) : 0.0f;
+  return Pack16<Tag>::pack(x);
+}
+template <class Tag>
+__device__ __forceinline__ void store_part(char* to, const u32x4& v, int64_t n) {
+  constexpr int EPV = Pack16<Tag>::EPV;
+  float x[EPV];
+  Pack16<Tag>::unpack(v, x);
+#pragma unroll
+  for (int k = 0; k < EPV; ++k)
+    if (k < n) {
+      if constexpr (EPV == 4) reinterpret_cast<float*>(to)[k] = x[k];
+      else reinterpret_cast<uint16_t*>(to)[k] = (uint16_t)Pack16<Tag>::pack_one(x[k]);
+    }
+}
+
+// Zeros where an entry's bit is not set.
+template <class Tag>
+__device__ __forceinline__ void keep_entries(u32x4& v, uint32_t bits) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    if constexpr (Pack16<Tag>::EPV == 4) {
+      v[d] = bits >> d & 1 ? v[d] : 0u;
+    } else {
+      const uint32_t two = bits >> (2 * d) & 3;
+      v[d] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
+    }
+  }
+}
+
 // Eight consecutive entries as they stand in memory.
 template <class Tag>
 struct Frag {
   static constexpr int EPV = Pack16<Tag>::EPV, NV = 8 / EPV, SZ = 16 / EPV;
   u32x4 v[NV];
-  // entries i..i+7 of a row that may start at any element, zeros from n on
+  // entries i..i+7 of a row that may start at any element, zeros from n on (WHOLE: there are
+  // eight)
+  template <bool WHOLE = false>
   __device__ __forceinline__ void load(const char* row, int64_t i, int64_t n) {
-    if (i + 8 <= n) {
+    if (WHOLE || i + 8 <= n) {
 #pragma unroll
-      for (int h = 0; h < NV; ++h) v[h] = reinterpret_cast<const Any16*>(row + i * SZ)[h].v;
+      for (int h = 0; h < NV; ++h) v[h] = reinterpret_cast<const AnyVec*>(row + i * SZ)[h];
       return;
     }
-    float x[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = i + k < n ? load_entry<Tag>(row, i + k) : 0.0f;
-    pack(x);
+    for (int h = 0; h < NV; ++h) v[h] = load_part<Tag>(row + (i + h * EPV) * SZ, n - i - h * EPV);
+  }
+  // the same within the row, past the caches
+  __device__ __forceinline__ void stream(const char* row, int64_t i) {
+#pragma unroll
+    for (int h = 0; h < NV; ++h) v[h] = __builtin_nontemporal_load(reinterpret_cast<const AnyVec*>(row + i * SZ) + h);
   }
   __device__ __forceinline__ void pack(const float (&x)[8]) {
 #pragma unroll
@@ -83,31 +130,16 @@ struct Frag {
   __device__ __forceinline__ void store(char* row, int64_t i, int64_t n) const {
     if (i + 8 <= n) {
 #pragma unroll
-      for (int h = 0; h < NV; ++h) reinterpret_cast<Any16*>(row + i * SZ)[h].v = v[h];
+      for (int h = 0; h < NV; ++h) reinterpret_cast<AnyVec*>(row + i * SZ)[h] = v[h];
       return;
     }
-    float x[8];
-    unpack(x);
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (i + k < n) {
-        if constexpr (SZ == 4) reinterpret_cast<float*>(row)[i + k] = x[k];
-        else reinterpret_cast<uint16_t*>(row)[i + k] = (uint16_t)Pack16<Tag>::pack_one(x[k]);
-      }
+    for (int h = 0; h < NV; ++h) store_part<Tag>(row + (i + h * EPV) * SZ, v[h], n - i - h * EPV);
   }
   // zeros where an entry is dropped
   __device__ __forceinline__ void keep(uint32_t bits) {
 #pragma unroll
-    for (int h = 0; h < NV; ++h)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        if constexpr (SZ == 4) {
-          v[h][d] = bits >> (4 * h + d) & 1 ? v[h][d] : 0u;
-        } else {
-          const uint32_t two = bits >> (2 * d) & 3;
-          v[h][d] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
-        }
-      }
+    for (int h = 0; h < NV; ++h) keep_entries<Tag>(v[h], bits >> (EPV * h));
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -182,14 +214,17 @@ struct Thin {  // t of 16 tokens
   }
 };
 template <class Tag, int R16>
-struct UpRow {  // a lane's row of up
+struct UpRow {  // a lane's row of up; WHOLE: r is 16 R16
   using T = Thin<Tag, R16>;
   Frag<Tag> v[T::F32 ? (T::NF + 7) / 8 : T::KS];
+  template <bool WHOLE = false>
   __device__ __forceinline__ void load(const char* row, int r, int kb) {
     if constexpr (T::F32) {
       if constexpr (T::NF >= 8) {
 #pragma unroll
-        for (int s = 0; s < T::NF / 8; ++s) v[s].load(row, T::NF * kb + 8 * s, r);
+        for (int s = 0; s < T::NF / 8; ++s) v[s].template load<WHOLE>(row, T::NF * kb + 8 * s, r);
+      } else if constexpr (WHOLE) {
+        v[0].v[0] = reinterpret_cast<const AnyVec*>(row)[kb];
       } else {
         // four entries to a lane
         v[0].clear();
@@ -199,7 +234,7 @@ struct UpRow {  // a lane's row of up
       }
     } else {
 #pragma unroll
-      for (int s = 0; s < T::KS; ++s) v[s].load(row, R16 == 1 ? 8 * (kb & 1) : 32 * s + 8 * kb, r);
+      for (int s = 0; s < T::KS; ++s) v[s].template load<WHOLE>(row, R16 == 1 ? 8 * (kb & 1) : 32 * s + 8 * kb, r);
     }
   }
 };
@@ -260,41 +295,63 @@ struct FusedArgs {
   Drop drop;
   int drop_in, drop_out;
   int nan_rows;         // rows of ids that there are none of: NaN, or zeros
+  int stream_x, stream_out;  // x, and base and out, are larger than the memory-side cache
 };
 
-enum Phase { BOTH, SHRINK, EXPAND };
+// The row of up that lane q holds of the i-th of tiles of 16 from column c on: pairs of
+// tiles in an order that leaves eight consecutive columns to a lane of the result.
+__device__ __forceinline__ int64_t up_row(int64_t c, int i, int q, int64_t O) {
+  return min(c + 16 * (i & ~1) + 8 * (q >> 2) + 4 * (i & 1) + (q & 3), O - 1);
+}
 
-template <class Tag, int R16, int MT, int PHASE>
-__global__ __launch_bounds__(kAT) void adapter_fused_kernel(FusedArgs a) {
-  constexpr int SZ = 16 / Pack16<Tag>::EPV, TM = 16 * MT, R = 16 * R16, kChunks = kWindow / kAT;
-  constexpr int kAhead = R16 > 2 || std::is_same_v<Tag, TagF32> ? 4 : 8, NC = 4;
-  constexpr int kLd = R + 4;  // a row of t in LDS
-  __shared__ uint16_t order[kWindow];
-  __shared__ __attribute__((aligned(16))) float part[PHASE == EXPAND ? 1 : kAW][TM][kLd];
-  __shared__ int scan[2][kAW];
-  extern __shared__ int bins[];  // first place and first tile of each adapter, of none and bad, and the ends
-  const int A2 = a.ids.A + 2;
-  int* const start = bins;
-  int* const tiles = start + A2 + 1;
-  uint16_t* const seen = reinterpret_cast<uint16_t*>(tiles + A2 + 1);  // rows of each by wave
-  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, kb = lane >> 4, q = lane & 15;
-  const int64_t window = blockIdx.x / a.groups;
-  const int group = (int)(blockIdx.x % a.groups);
-  const int64_t n0 = window * kWindow;
-  const int count = (int)min((int64_t)kWindow, a.N - n0);
+// A wave's exchange through LDS that is its own: the order of its accesses stays as written.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
-  // the window's rows by adapter, in order: every workgroup of the window has to come to
-  // the same tiles.  A wave looks at a quarter of them.
-  int code[kChunks];
-  bool same = true;
-  const int first = a.ids.at(n0), i0 = wv * (kWindow / kAW) + lane;
+// The rows of a window of 1024 tokens by adapter, in order, as tiles of up to TM rows of
+// one: every workgroup of a window comes to the same tiles.  The whole workgroup takes part.
+template <int TM>
+struct Window {
+  struct Tile {
+    int ad, row0, here;  // ad: A for rows without an adapter, A + 1 for ids that there are none of
+  };
+  int64_t n0;
+  int count, first, A2;
+  bool one;  // one adapter's
+  const uint16_t* order;
+  const int *start, *tiles;
+  int all;  // tiles
+
+  static size_t lds(int A) { return (2 * sizeof(int) + kAW * sizeof(uint16_t)) * (size_t)(A + 3); }
+
+  __device__ __forceinline__ Window(const FusedArgs& a, uint16_t* order_, int* scan, int* bins) {
+    constexpr int kChunks = kWindow / kAT;
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+    n0 = (int64_t)(blockIdx.x / a.groups) * kWindow;
+    count = (int)min((int64_t)kWindow, a.N - n0);
+    A2 = a.ids.A + 2;
+    int* const start_ = bins;                // first place of each adapter, of none and bad, and the end
+    int* const tiles_ = start_ + A2 + 1;     // first tile
+    uint16_t* const seen = reinterpret_cast<uint16_t*>(tiles_ + A2 + 1);  // rows of each by wave
+    order = order_;
+    start = start_;
+    tiles = tiles_;
+    // a wave looks at a quarter of the rows
+    int code[kChunks];
+    bool same = true;
+    const int i0 = wv * (kWindow / kAW) + lane;
+    first = a.ids.at(n0);
 #pragma unroll
-  for (int k = 0; k < kChunks; ++k) {
-    code[k] = i0 + 64 * k < count ? a.ids.at(n0 + i0 + 64 * k) : first;
-    same &= code[k] == first;
-  }
-  const bool one = __syncthreads_and(same);
-  if (!one) {
+    for (int k = 0; k < kChunks; ++k) {
+      code[k] = i0 + 64 * k < count ? a.ids.at(n0 + i0 + 64 * k) : first;
+      same &= code[k] == first;
+    }
+    one = __syncthreads_and(same);
+    all = (count + TM - 1) / TM;
+    if (one) return;
     for (int k = t; k < kAW * A2; k += kAT) seen[k] = 0;
     __syncthreads();
     int rank[kChunks];  // among the wave's rows of the same adapter
@@ -321,7 +378,7 @@ __global__ __launch_bounds__(kAT) void adapter_fused_kernel(FusedArgs a) {
     for (int k = lo; k < hi; ++k) {
       int c = 0;
       for (int w = 0; w < kAW; ++w) c += seen[w * A2 + k];
-      start[k] = c;
+      start_[k] = c;
       rows += c;
       tls += (c + TM - 1) / TM;
     }
@@ -335,189 +392,416 @@ __global__ __launch_bounds__(kAT) void adapter_fused_kernel(FusedArgs a) {
       }
     }
     if (lane == 63) {
-      scan[0][wv] = rsum;
-      scan[1][wv] = tsum;
+      scan[wv] = rsum;
+      scan[kAW + wv] = tsum;
     }
     __syncthreads();
     rsum -= rows;
     tsum -= tls;
     for (int k = 0; k < wv; ++k) {
-      rsum += scan[0][k];
-      tsum += scan[1][k];
+      rsum += scan[k];
+      tsum += scan[kAW + k];
     }
     for (int k = lo; k < hi; ++k) {
-      const int c = start[k];
-      start[k] = rsum;
-      tiles[k] = tsum;
+      const int c = start_[k];
+      start_[k] = rsum;
+      tiles_[k] = tsum;
       rsum += c;
       tsum += (c + TM - 1) / TM;
     }
     if (hi == A2 && lo < hi) {  // the thread of the last bin
-      start[A2] = rsum;
-      tiles[A2] = tsum;
+      start_[A2] = rsum;
+      tiles_[A2] = tsum;
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kChunks; ++k)
       if (i0 + 64 * k < count) {
-        int at = start[code[k]] + rank[k];
+        int at = start_[code[k]] + rank[k];
         for (int w = 0; w < wv; ++w) at += seen[w * A2 + code[k]];
-        order[at] = (uint16_t)(i0 + 64 * k);
+        order_[at] = (uint16_t)(i0 + 64 * k);
       }
     __syncthreads();
+    all = tiles_[A2];
   }
-  const int all = one ? (count + TM - 1) / TM : tiles[A2];
-  const uint64_t at = a.drop_in || a.drop_out ? a.drop.counter() : 0;
-
-  for (int64_t it = group; it < (int64_t)all * a.slabs; it += a.groups) {
-    const int tile = (int)(it / a.slabs), slab = (int)(it % a.slabs);
-    int ad = first, row0 = tile * TM, end = count;
-    if (!one) {  // the last bin that starts at or before the tile and is not empty
-      int lo = 0, hi = A2;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (tiles[mid] <= tile) lo = mid;
-        else hi = mid;
-      }
-      ad = lo;
-      row0 = start[ad] + (tile - tiles[ad]) * TM;
-      end = start[ad + 1];
+  __device__ __forceinline__ Tile tile(int k) const {
+    if (one) return Tile{first, k * TM, min(TM, count - k * TM)};
+    // the last bin that starts at or before the tile and is not empty
+    int lo = 0, hi = A2;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (tiles[mid] <= k) lo = mid;
+      else hi = mid;
     }
-    const int here = min(TM, end - row0);
-    const int64_t c0 = slab * a.slab, c1 = min(c0 + a.slab, a.O);
-    auto token = [&](int i) { return n0 + (one ? row0 + i : (int)order[row0 + i]); };
+    const int row0 = start[lo] + (k - tiles[lo]) * TM;
+    return Tile{lo, row0, min(TM, start[lo + 1] - row0)};
+  }
+  // the i-th row of a tile, from the window's first; past its end the last again
+  __device__ __forceinline__ int row(const Tile& k, int i) const {
+    const int at = k.row0 + min(i, k.here - 1);
+    return one ? at : (int)order[at];
+  }
+  __device__ __forceinline__ int64_t token(const Tile& k, int i) const { return n0 + row(k, i); }
+};
 
-    if (ad >= a.ids.A) {  // rows without an adapter
-      if (PHASE == SHRINK || !a.out) continue;
-      const int per = (int)((c1 - c0 + 7) / 8);
-      for (int64_t k = t; k < (int64_t)here * per; k += kAT) {
-        const int64_t n = token((int)(k / per)), c = c0 + k % per * 8;
-        Frag<Tag> v;
-        v.clear();
-        if (ad == a.ids.A) {
-          if (a.base) v.load(a.base + n * a.b_ld * SZ, c, c1);
-        } else if (a.nan_rows) {
-          float x[8];
+// Columns c0..c1-1 of rows without an adapter.
+template <class Tag, int TM>
+__device__ __forceinline__ void plain_rows(const FusedArgs& a, const Window<TM>& w,
+                                           const typename Window<TM>::Tile& tile, int64_t c0, int64_t c1) {
+  constexpr int SZ = Frag<Tag>::SZ;
+  const int per = (int)((c1 - c0 + 7) / 8);
+  for (int64_t k = threadIdx.x; k < (int64_t)tile.here * per; k += kAT) {
+    const int64_t n = w.token(tile, (int)(k / per)), c = c0 + k % per * 8;
+    Frag<Tag> v;
+    v.clear();
+    if (tile.ad == a.ids.A) {
+      if (a.base) v.load(a.base + n * a.b_ld * SZ, c, c1);
+    } else if (a.nan_rows) {
+      float x[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = M<float>::nan();
-          v.pack(x);
-        }
-        v.store(a.out + n * a.O * SZ, c, c1);
-      }
+      for (int j = 0; j < 8; ++j) x[j] = M<float>::nan();
+      v.pack(x);
+    }
+    v.store(a.out + n * a.O * SZ, c, c1);
+  }
+}
+
+// Eight consecutive columns of a row: the product, scaled and dropped or added to base's.
+template <class Tag>
+__device__ __forceinline__ void finish(const FusedArgs& a, const f32x4& d0, const f32x4& d1, int64_t n, int64_t col,
+                                       float scale, uint64_t at, Frag<Tag>& b) {
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[k] = d0[k];
+    v[4 + k] = d1[k];
+  }
+  if (a.drop_out) {
+    const uint32_t keep = a.drop.keep_bits((uint64_t)(n * ((a.O + 7) / 8) + col / 8), at);
+    const float s = scale * a.drop.scale;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = keep >> k & 1 ? v[k] * s : 0.0f;
+  } else if (a.base) {
+    float x[8];
+    b.unpack(x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = __builtin_fmaf(v[k], scale, x[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= scale;
+  }
+  b.pack(v);
+}
+
+// Few rows, in tiles of 16: t with the depth split over the four waves, and (where out is
+// not null) its product with a run of up's rows, 64 to a wave at a time.
+template <class Tag, int R16>
+__global__ __launch_bounds__(kAT) void adapter_fused_kernel(FusedArgs a) {
+  constexpr int SZ = Frag<Tag>::SZ, R = 16 * R16, kAhead = 4, NC = 4;
+  __shared__ uint16_t order[kWindow];
+  __shared__ __attribute__((aligned(16))) float part[kAW][16][R + 4];
+  __shared__ int scan[2 * kAW];
+  extern __shared__ int bins[];
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, kb = lane >> 4, q = lane & 15;
+  const Window<16> w(a, order, scan, bins);
+  const uint64_t at = a.drop_in || a.drop_out ? a.drop.counter() : 0;
+  for (int64_t it = blockIdx.x % a.groups; it < (int64_t)w.all * a.slabs; it += a.groups) {
+    const Window<16>::Tile tile = w.tile((int)(it / a.slabs));
+    const int slab = (int)(it % a.slabs);
+    const int64_t c0 = slab * a.slab, c1 = min(c0 + a.slab, a.O);
+    if (tile.ad >= a.ids.A) {
+      if (a.out) plain_rows<Tag, 16>(a, w, tile, c0, c1);
       continue;
     }
-
-    // t of the tile's rows; past its end the last again
-    auto n_of = [&](int f) { return token(min(16 * f + q, here - 1)); };
-    int64_t n[MT];
+    const int64_t n = w.token(tile, q);
+    const char* xrow = a.x + n * a.x_ld * SZ;
+    const char* down = a.down + tile.ad * a.d_sa * SZ;
+    const int64_t steps = (a.K + 31) / 32, per_row = (a.K + 7) / 8;
+    const int64_t s0 = steps * wv / kAW, s1 = steps * (wv + 1) / kAW;
+    f32x4 acc[R16] = {};
+    for (int64_t s = s0; s < s1; s += kAhead) {
+      Frag<Tag> xf[kAhead], df[kAhead][R16];
 #pragma unroll
-    for (int f = 0; f < MT; ++f) n[f] = n_of(f);
-    if constexpr (PHASE != EXPAND) {
-      __syncthreads();  // the last tile's t is read
-      const char* down = a.down + ad * a.d_sa * SZ;
-      const int64_t steps = (a.K + 31) / 32, per_row = (a.K + 7) / 8;
-      // Four sums over quarters of the depth, which are added in order.  With few rows a
-      // wave takes a quarter of all of them, else all quarters of 16 rows, each wave and
-      // tile starting at another one: rows a power of two apart lie on few of the memory's
-      // channels at one column.
-      for (int turn = 0; turn < (MT == 1 ? 1 : kAW); ++turn) {
-        if (MT > 1 && wv >= MT) break;
-        const int quarter = MT == 1 ? wv : (turn + wv + tile) % kAW;
-        const int64_t nf = MT == 1 ? n[0] : n_of(wv);
-        const char* xrow = a.x + nf * a.x_ld * SZ;
-        f32x4 acc[R16] = {};
-        const int64_t s0 = steps * quarter / kAW, s1 = steps * (quarter + 1) / kAW;
-        for (int64_t s = s0; s < s1; s += kAhead) {
-          Frag<Tag> xf[kAhead], df[kAhead][R16];
+      for (int e = 0; e < kAhead; ++e) {
+        // past the wave's steps: zeros
+        const int64_t k = s + e < s1 ? (s + e) * 32 + kb * 8 : a.K;
+        xf[e].load(xrow, k, a.K);
 #pragma unroll
-          for (int e = 0; e < kAhead; ++e) {
-            // past the quarter's steps: zeros
-            const int64_t k = s + e < s1 ? (s + e) * 32 + kb * 8 : a.K;
-            xf[e].load(xrow, k, a.K);
-#pragma unroll
-            for (int j = 0; j < R16; ++j) {
-              const int rr = 16 * j + q;
-              df[e][j].load(down + min(rr, a.r - 1) * a.d_sr * SZ, rr < a.r ? k : a.K, a.K);
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < kAhead; ++e) {
-            if (a.drop_in && s + e < s1) xf[e].keep(a.drop.keep_bits((uint64_t)(nf * per_row + (s + e) * 4 + kb), at));
-#pragma unroll
-            for (int j = 0; j < R16; ++j) acc[j] = mma<Tag>(df[e][j], xf[e], acc[j]);
-          }
+        for (int j = 0; j < R16; ++j) {
+          const int rr = 16 * j + q;
+          df[e][j].load(down + min(rr, a.r - 1) * a.d_sr * SZ, rr < a.r ? k : a.K, a.K);
         }
+      }
 #pragma unroll
-        for (int j = 0; j < R16; ++j)
-          *reinterpret_cast<f32x4*>(&part[quarter][(MT == 1 ? 0 : 16 * wv) + q][16 * j + 4 * kb]) = acc[j];
+      for (int e = 0; e < kAhead; ++e) {
+        if (a.drop_in && s + e < s1) xf[e].keep(a.drop.keep_bits((uint64_t)(n * per_row + (s + e) * 4 + kb), at));
+#pragma unroll
+        for (int j = 0; j < R16; ++j) acc[j] = mma<Tag>(df[e][j], xf[e], acc[j]);
       }
-      __syncthreads();
-      const float drop_scale = a.drop_in ? a.drop.scale : 1.0f;
-      for (int k = t; k < TM * R; k += kAT) {
-        const int i = k / R, j = k % R;
-        float v = (((part[0][i][j] + part[1][i][j]) + part[2][i][j]) + part[3][i][j]) * drop_scale;
-        if (j >= a.r) v = 0.0f;  // not an infinity of x times a padding's zero
-        part[0][i][j] = v;
-        if (slab == 0 && i < here) a.t[token(i) * R + j] = v;
-      }
-      __syncthreads();
     }
-    if (PHASE == SHRINK || !a.out) continue;
-
-    // a wave takes 16 NC columns at a time
-    Thin<Tag, R16> thin[MT];
+    __syncthreads();  // the last tile's t is read
 #pragma unroll
-    for (int f = 0; f < MT; ++f) thin[f].load(PHASE == EXPAND ? a.t + n[f] * R : &part[0][16 * f + q][0], kb);
-    const float scale = a.scales ? a.scales[ad] : 1.0f;
-    const char* up = a.up + ad * a.u_sa * SZ;
-    // a run of them each, and each wave and tile from another place on, as above
-    const int groups = (int)((c1 - c0 + 16 * NC - 1) / (16 * NC));
-    const int g0 = groups * wv / kAW, g1 = groups * (wv + 1) / kAW;
-    for (int g = g0; g < g1; ++g) {
-      const int64_t c = c0 + 16 * NC * (g0 + (g - g0 + tile) % (g1 - g0));
-      Frag<Tag> b[MT][NC / 2];
+    for (int j = 0; j < R16; ++j) *reinterpret_cast<f32x4*>(&part[wv][q][16 * j + 4 * kb]) = acc[j];
+    __syncthreads();
+    const float drop_scale = a.drop_in ? a.drop.scale : 1.0f;
+    for (int k = t; k < 16 * R; k += kAT) {
+      const int i = k / R, j = k % R;
+      float v = (((part[0][i][j] + part[1][i][j]) + part[2][i][j]) + part[3][i][j]) * drop_scale;
+      if (j >= a.r) v = 0.0f;  // not an infinity of x times a padding's zero
+      part[0][i][j] = v;
+      if (slab == 0 && i < tile.here) a.t[w.token(tile, i) * R + j] = v;
+    }
+    __syncthreads();
+    if (!a.out) continue;
+    Thin<Tag, R16> thin;
+    thin.load(&part[0][q][0], kb);
+    const float scale = a.scales ? a.scales[tile.ad] : 1.0f;
+    const char* up = a.up + tile.ad * a.u_sa * SZ;
+    for (int64_t c = c0 + 16 * NC * wv; c < c1; c += 16 * NC * kAW) {
+      Frag<Tag> b[NC / 2];
       UpRow<Tag, R16> u[NC];
       if (a.base) {
 #pragma unroll
-        for (int f = 0; f < MT; ++f)
-#pragma unroll
-          for (int p = 0; p < NC / 2; ++p) b[f][p].load(a.base + n[f] * a.b_ld * SZ, c + 32 * p + 8 * kb, c1);
+        for (int p = 0; p < NC / 2; ++p) b[p].load(a.base + n * a.b_ld * SZ, c + 32 * p + 8 * kb, c1);
       }
-      // pairs of tiles of up's rows, in an order that leaves eight consecutive columns to a lane
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
-        u[i].load(up + min(c + 16 * (i & ~1) + 8 * (q >> 2) + 4 * (i & 1) + (q & 3), a.O - 1) * a.u_so * SZ, a.r, kb);
+      for (int i = 0; i < NC; ++i) u[i].load(up + up_row(c, i, q, a.O) * a.u_so * SZ, a.r, kb);
 #pragma unroll
       for (int p = 0; p < NC / 2; ++p) {
+        const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
         const int64_t col = c + 32 * p + 8 * kb;
+        finish<Tag>(a, expand<Tag, R16>(u[2 * p], thin, none), expand<Tag, R16>(u[2 * p + 1], thin, none), n, col, scale,
+                    at, b[p]);
+        if (q < tile.here) b[p].store(a.out + n * a.O * SZ, col, c1);
+      }
+    }
+  }
+}
+
+// Eight KB of a matrix, ROWS rows of 8192 / ROWS bytes, staged in LDS by a wave: loaded and
+// stored as whole 128-byte lines, read and written as the products hold them (16 rows of 64
+// bytes to an instruction).  Matrices that are larger than the 256 MB memory-side cache are
+// streamed past it, which only whole lines bear: 537 MB are read at 4.5 instead of 3.4 TB/s,
+// and leave what other passes read again in it.
+template <class Tag, int ROWS, bool WHOLE>
+struct Stage {
+  static constexpr int EPV = Pack16<Tag>::EPV, SZ = 16 / EPV, kBytes = 8192 / ROWS, kCols = kBytes / SZ;
+  static constexpr int kPieces = kBytes / 16, kTogether = 64 / kPieces, kRow = kBytes + 16;  // rows to an instruction
+  u32x4 raw[8];
+  static __device__ __forceinline__ int piece() { return (threadIdx.x & 63) % kPieces; }
+  static __device__ __forceinline__ int row(int i) { return kTogether * i + (threadIdx.x & 63) / kPieces; }
+  // columns from c on of rows n[i], zeros from `end` on
+  __device__ __forceinline__ void load(const char* base, int64_t ld, const int (&n)[8], int64_t c, int64_t end,
+                                       bool stream) {
+    const int64_t col = c + piece() * EPV;
+    if (WHOLE || col + EPV <= end) {
+      if (stream) {
+        apart();
 #pragma unroll
-        for (int f = 0; f < MT; ++f) {
-          float v[8];
+        for (int i = 0; i < 8; ++i)
+          raw[i] = __builtin_nontemporal_load(reinterpret_cast<const AnyVec*>(base + ((int64_t)n[i] * ld + col) * SZ));
+        apart();
+      } else {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const f32x4 d = expand<Tag, R16>(u[2 * p + i], thin[f], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+        for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const AnyVec*>(base + ((int64_t)n[i] * ld + col) * SZ);
+      }
+    } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[4 * i + k] = d[k];
-          }
-          if (a.drop_out) {
-            const uint32_t keep = a.drop.keep_bits((uint64_t)(n[f] * ((a.O + 7) / 8) + col / 8), at);
-            const float s = scale * a.drop.scale;
+      for (int i = 0; i < 8; ++i) raw[i] = load_part<Tag>(base + ((int64_t)n[i] * ld + col) * SZ, end - col);
+    }
+  }
+  __device__ __forceinline__ void put(char* stage) const {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = keep >> k & 1 ? v[k] * s : 0.0f;
-          } else if (a.base) {
-            float x[8];
-            b[f][p].unpack(x);
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<u32x4*>(stage + row(i) * kRow + piece() * 16) = raw[i];
+  }
+  __device__ __forceinline__ void get(const char* stage) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = __builtin_fmaf(v[k], scale, x[k]);
-          } else {
+    for (int i = 0; i < 8; ++i) raw[i] = *reinterpret_cast<const u32x4*>(stage + row(i) * kRow + piece() * 16);
+  }
+  // the first `rows` of them
+  __device__ __forceinline__ void store(char* base, int64_t ld, const int (&n)[8], int rows, int64_t c, int64_t end,
+                                        bool stream) const {
+    const int64_t col = c + piece() * EPV;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] *= scale;
-          }
-          Frag<Tag> o;
-          o.pack(v);
-          if (16 * f + q < here) o.store(a.out + n[f] * a.O * SZ, col, c1);
+    for (int i = 0; i < 8; ++i) {
+      if (row(i) >= rows) continue;
+      char* to = base + ((int64_t)n[i] * ld + col) * SZ;
+      if (WHOLE || col + EPV <= end) {
+        if (stream) {
+          apart();
+          __builtin_nontemporal_store(raw[i], reinterpret_cast<AnyVec*>(to));
+          apart();
+        } else {
+          *reinterpret_cast<AnyVec*>(to) = raw[i];
+        }
+      } else {
+        store_part<Tag>(to, raw[i], end - col);
+      }
+    }
+  }
+  // eight columns of a row as the products hold them
+  static __device__ __forceinline__ void read(const char* stage, int r, int col, Frag<Tag>& f) {
+#pragma unroll
+    for (int h = 0; h < Frag<Tag>::NV; ++h)
+      f.v[h] = *reinterpret_cast<const u32x4*>(stage + r * kRow + col * SZ + 16 * h);
+  }
+  static __device__ __forceinline__ void write(char* stage, int r, int col, const Frag<Tag>& f) {
+#pragma unroll
+    for (int h = 0; h < Frag<Tag>::NV; ++h)
+      *reinterpret_cast<u32x4*>(stage + r * kRow + col * SZ + 16 * h) = f.v[h];
+  }
+};
+
+// t of many rows: 16 to a wave, over the whole depth.  WHOLE: the depth is stages, and r is
+// 16 R16, so that no load looks for an end.
+template <class Tag, int R16, bool WHOLE>
+__global__ __launch_bounds__(kAT) void adapter_shrink_kernel(FusedArgs a) {
+  using S = Stage<Tag, 16, WHOLE>;
+  constexpr int SZ = S::SZ, R = 16 * R16;
+  __shared__ uint16_t order[kWindow];
+  __shared__ __attribute__((aligned(16))) char stages[kAW][16 * S::kRow];
+  __shared__ int scan[2 * kAW];
+  extern __shared__ int bins[];
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, kb = lane >> 4, q = lane & 15;
+  char* const stage = stages[wv];
+  const Window<64> w(a, order, scan, bins);
+  const uint64_t at = a.drop_in ? a.drop.counter() : 0;
+  const float drop_scale = a.drop_in ? a.drop.scale : 1.0f;
+  const char* const x0 = a.x + w.n0 * a.x_ld * SZ;
+  for (int it = (int)(blockIdx.x % a.groups); it < w.all; it += a.groups) {
+    const Window<64>::Tile tile = w.tile(it);
+    if (tile.ad >= a.ids.A || 16 * wv >= tile.here) continue;
+    const int64_t n = w.token(tile, 16 * wv + q);
+    int rows[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rows[i] = w.row(tile, 16 * wv + S::row(i));
+    const char* down = a.down + tile.ad * a.d_sa * SZ;
+    f32x4 acc[R16] = {};
+    S in;
+    in.load(x0, a.x_ld, rows, 0, a.K, a.stream_x);
+    for (int64_t c = 0; c < a.K; c += S::kCols) {
+      if (a.drop_in) {
+        const int64_t col = c + S::piece() * S::EPV, per_row = (a.K + 7) / 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t bits = a.drop.keep_bits((uint64_t)((w.n0 + rows[i]) * per_row + col / 8), at);
+          if constexpr (SZ == 4) bits >>= col & 4;
+          keep_entries<Tag>(in.raw[i], bits);
         }
       }
+      wave_fence();
+      in.put(stage);
+      wave_fence();
+      if (c + S::kCols < a.K) in.load(x0, a.x_ld, rows, c + S::kCols, a.K, a.stream_x);
+      constexpr int kSteps = S::kCols / 32, kAhead = R16 > 2 ? 2 : 4;
+#pragma unroll
+      for (int s0 = 0; s0 < kSteps; s0 += kAhead) {
+        Frag<Tag> df[kAhead][R16];
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e)
+#pragma unroll
+          for (int j = 0; j < R16; ++j) {
+            const int rr = 16 * j + q;
+            const int64_t k = c + (s0 + e) * 32 + 8 * kb;
+            if constexpr (WHOLE) df[e][j].template load<true>(down + rr * a.d_sr * SZ, k, a.K);
+            else df[e][j].load(down + min(rr, a.r - 1) * a.d_sr * SZ, rr < a.r ? k : a.K, a.K);
+          }
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+          Frag<Tag> xf;
+          S::read(stage, q, (s0 + e) * 32 + 8 * kb, xf);
+#pragma unroll
+          for (int j = 0; j < R16; ++j) acc[j] = mma<Tag>(df[e][j], xf, acc[j]);
+        }
+      }
+    }
+    if (16 * wv + q < tile.here) {
+#pragma unroll
+      for (int j = 0; j < R16; ++j) {
+        f32x4 v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // padding: not an infinity of x times its zero
+          v[k] = 16 * j + 4 * kb + k < a.r ? acc[j][k] * drop_scale : 0.0f;
+        *reinterpret_cast<f32x4*>(a.t + n * R + 16 * j + 4 * kb) = v;
+      }
+    }
+  }
+}
+
+// base + scale up t, a stage of all rows of a tile to a wave at a time, the waves side by
+// side.  WHOLE: the columns are stages, and r is 16 R16.
+template <class Tag, int R16, int TM, bool WHOLE>
+__global__ __launch_bounds__(kAT, R16 <= 2 ? 3 : 2) void adapter_expand_kernel(FusedArgs a) {
+  using S = Stage<Tag, TM, WHOLE>;
+  constexpr int SZ = S::SZ, R = 16 * R16, MT = TM / 16;
+  __shared__ uint16_t order[kWindow];
+  __shared__ __attribute__((aligned(16))) char stages[kAW][TM * S::kRow];
+  __shared__ int scan[2 * kAW];
+  extern __shared__ int bins[];
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, kb = lane >> 4, q = lane & 15;
+  char* const stage = stages[wv];
+  const Window<TM> w(a, order, scan, bins);
+  const uint64_t at = a.drop_out ? a.drop.counter() : 0;
+  const char* const base0 = a.base + w.n0 * a.b_ld * SZ;
+  char* const out0 = a.out + w.n0 * a.O * SZ;
+  for (int64_t it = blockIdx.x % a.groups; it < (int64_t)w.all * a.slabs; it += a.groups) {
+    const typename Window<TM>::Tile tile = w.tile((int)(it / a.slabs));
+    const int slab = (int)(it % a.slabs);
+    const int64_t c0 = slab * a.slab, c1 = min(c0 + a.slab, a.O);
+    if (tile.ad >= a.ids.A) {
+      plain_rows<Tag, TM>(a, w, tile, c0, c1);
+      continue;
+    }
+    const int chunks = (int)((c1 - c0 + S::kCols - 1) / S::kCols);
+    if (wv >= chunks) continue;
+    int n[MT], rows[8];
+    Thin<Tag, R16> thin[MT];
+#pragma unroll
+    for (int f = 0; f < MT; ++f) {
+      n[f] = w.row(tile, 16 * f + q);
+      thin[f].load(a.t + (w.n0 + n[f]) * R, kb);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rows[i] = w.row(tile, S::row(i));
+    const float scale = a.scales ? a.scales[tile.ad] : 1.0f;
+    const char* up = a.up + tile.ad * a.u_sa * SZ;
+    S in;
+    if (a.base) in.load(base0, a.b_ld, rows, c0 + wv * S::kCols, c1, a.stream_out);
+    for (int chunk = wv; chunk < chunks; chunk += kAW) {
+      const int64_t c = c0 + chunk * S::kCols;
+      if (a.base) {
+        wave_fence();
+        in.put(stage);
+        if (chunk + kAW < chunks) in.load(base0, a.b_ld, rows, c + kAW * S::kCols, c1, a.stream_out);
+      }
+      wave_fence();
+      constexpr int NC = S::kCols / 16 < 4 ? S::kCols / 16 : 4;  // tiles of up's rows at once
+#pragma unroll 1
+      for (int i0 = 0; i0 < S::kCols / 16; i0 += NC) {
+        if (c + 16 * i0 >= c1) break;
+        UpRow<Tag, R16> u[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+          u[i].template load<WHOLE>(up + up_row(c + 16 * i0, i, q, a.O) * a.u_so * SZ, a.r, kb);
+#pragma unroll
+        for (int p = 0; p < NC / 2; ++p)
+#pragma unroll
+          for (int f = 0; f < MT; ++f) {
+            const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+            const int col = 16 * i0 + 32 * p + 8 * kb;
+            Frag<Tag> b;
+            if (a.base) S::read(stage, 16 * f + q, col, b);
+            finish<Tag>(a, expand<Tag, R16>(u[2 * p], thin[f], none), expand<Tag, R16>(u[2 * p + 1], thin[f], none),
+                        w.n0 + n[f], c + col, scale, at, b);
+            S::write(stage, 16 * f + q, col, b);
+            // side by side, these would take the registers of more waves
+            __builtin_amdgcn_sched_barrier(0);
+          }
+      }
+      wave_fence();
+      S out;
+      out.get(stage);
+      out.store(out0, a.O, rows, tile.here, c, c1, a.stream_out);
     }
   }
 }
@@ -536,7 +820,7 @@ struct OuterJob {
   char* out;          // the gradient: entry (a, c, r) at a * o_sa + c * o_sc + r * o_sr
   int64_t o_sa, o_sc, o_sr;
   int tiles;          // of kOuterCols columns
-  int drop;
+  int drop, stream;
 };
 struct OuterArgs {
   OuterJob job[2];
@@ -558,7 +842,7 @@ struct OuterStep {
 };
 
 template <class Tag, int RT>
-__global__ __launch_bounds__(kAT) void adapter_outer_kernel(OuterArgs a) {
+__global__ __launch_bounds__(kAT, RT <= 2 ? 3 : 2) void adapter_outer_kernel(OuterArgs a) {
   constexpr int SZ = 16 / Pack16<Tag>::EPV;
   constexpr bool F32 = std::is_same_v<Tag, TagF32>, F16 = std::is_same_v<Tag, TagF16>;
   __shared__ uint16_t list[kWindow];
@@ -574,6 +858,7 @@ __global__ __launch_bounds__(kAT) void adapter_outer_kernel(OuterArgs a) {
   if (second) ct -= a.job[0].tiles;
   const OuterJob& j = a.job[second];
   const int64_t col = (int64_t)ct * kOuterCols + wv * 128 + 8 * q;
+  const bool whole = __all(col + 8 <= j.C);
   const int64_t per_row = (j.C + 7) / 8;
   const uint64_t at = j.drop ? a.drop.counter() : 0;
   const int r0 = rt * 16 * RT;
@@ -614,14 +899,24 @@ __global__ __launch_bounds__(kAT) void adapter_outer_kernel(OuterArgs a) {
     if (listed == 0 || col - 8 * q >= j.C) continue;  // or this wave's columns are past the end
     for (int s = 0; s < listed; s += 32) {
       OuterStep<Tag, RT> in;
+      const char* row[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int k = s + 8 * kb + i;
         const bool here = k < listed;
-        const int64_t n = n0 + list[here ? k : listed - 1];
-        in.x[i].load(j.wide + n * j.ld * SZ, here ? col : j.C, j.C);
+        const int64_t n = n0 + list[min(k, listed - 1)];
+        row[i] = j.wide + n * j.ld * SZ;
 #pragma unroll
         for (int e = 0; e < RT; ++e) in.th[i][e] = here ? j.thin[n * a.R + r0 + 16 * e + q] : 0.0f;
+      }
+      if (j.stream && s + 32 <= listed && whole) {
+        apart();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) in.x[i].stream(row[i], col);
+        apart();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) in.x[i].load(row[i], s + 8 * kb + i < listed ? col : j.C, j.C);
       }
       if (j.drop) {
 #pragma unroll
@@ -775,32 +1070,65 @@ __global__ __launch_bounds__(kAT) void adapter_turn_kernel(TurnArgs a) {
 
 inline int rank_padded(int r) { return r <= 16 ? 16 : (r <= 32 ? 32 : (r <= 64 ? 64 : 128)); }
 
-template <class Tag, int R16, int MT, int PHASE>
-int launch_fused(FusedArgs a, hipStream_t st) {
+// The grid of tiles of TM rows, and with `wide` runs of columns: as many as make a thousand
+// workgroups' work, of `least` columns at least.
+template <int TM>
+int tile_grid(FusedArgs& a, bool wide, int64_t least, dim3& grid) {
   const int64_t windows = (a.N + kWindow - 1) / kWindow;
   const int rows = (int)min(a.N, (int64_t)kWindow);
   // tiles of a window if it is of one adapter, and at most
-  const int64_t even = (rows + 16 * MT - 1) / (16 * MT), most = min((int64_t)rows, even + a.ids.A + 1);
-  // runs of columns: as many as make a thousand workgroups' work, of 256 columns at least
-  const bool wide = PHASE != SHRINK && a.out;
-  const int64_t cuts = wide ? max((int64_t)1, min((a.O + 255) / 256, 1024 / max((int64_t)1, windows * even))) : 1;
-  a.slab = wide ? ((a.O + cuts - 1) / cuts + 255) / 256 * 256 : 1;
+  const int64_t even = (rows + TM - 1) / TM, most = min((int64_t)rows, even + a.ids.A + 1);
+  const int64_t cuts = wide ? max((int64_t)1, min((a.O + least - 1) / least, 1024 / max((int64_t)1, windows * even))) : 1;
+  a.slab = wide ? ((a.O + cuts - 1) / cuts + least - 1) / least * least : 1;
   a.slabs = wide ? (int)((a.O + a.slab - 1) / a.slab) : 1;
   a.groups = (int)max((int64_t)1, min(most * a.slabs, max(even * a.slabs, 2048 / windows)));
   RRL_REQUIRE(windows * a.groups < ((int64_t)1 << 32) / kAT, RRL_EINVAL, "rrl_adapter: too many rows");
-  const size_t lds = (2 * sizeof(int) + kAW * sizeof(uint16_t)) * (size_t)(a.ids.A + 3);
-  hipLaunchKernelGGL((adapter_fused_kernel<Tag, R16, MT, PHASE>), dim3((uint32_t)(windows * a.groups)), dim3(kAT), lds,
-                     st, a);
-  return check_launch("adapter_fused_kernel");
+  grid = dim3((uint32_t)(windows * a.groups));
+  return RRL_OK;
 }
+
+template <class Tag, int R16, int TM>
+int launch_expand(FusedArgs a, int64_t least, size_t lds, hipStream_t st) {
+  dim3 grid;
+  if (int rc = tile_grid<TM>(a, true, least, grid)) return rc;
+  if (a.r == 16 * R16 && a.O % Stage<Tag, TM, true>::kCols == 0)
+    hipLaunchKernelGGL((adapter_expand_kernel<Tag, R16, TM, true>), grid, dim3(kAT), lds, st, a);
+  else hipLaunchKernelGGL((adapter_expand_kernel<Tag, R16, TM, false>), grid, dim3(kAT), lds, st, a);
+  return check_launch("adapter_expand_kernel");
+}
+
 // Few rows: both products in one launch.
-constexpr int64_t kFusedRows = 256;
+constexpr int64_t kFewRows = 256, kFusedColumns = 8192;
+constexpr int64_t kStreamed = (int64_t)128 << 20;  // half the memory-side cache
+inline int larger_than_cache(int64_t rows, int64_t cols, size_t size) {
+  return rows * cols * (int64_t)size > kStreamed;
+}
+
 template <class Tag, int R16>
-int launch_fused(const FusedArgs& a, hipStream_t st) {
-  constexpr int MT = R16 > 4 ? 2 : 4;
-  if (a.N <= kFusedRows) return launch_fused<Tag, R16, 1, BOTH>(a, st);
-  if (int rc = launch_fused<Tag, R16, MT, SHRINK>(a, st)) return rc;
-  return a.out ? launch_fused<Tag, R16, MT, EXPAND>(a, st) : RRL_OK;
+int launch_fused(FusedArgs a, hipStream_t st) {
+  constexpr int TM = R16 > 4 ? 32 : 64;  // (t of 64 rows of rank 128 would not stay in registers)
+  a.stream_x = larger_than_cache(a.N, a.K, Frag<Tag>::SZ);
+  a.stream_out = larger_than_cache(a.N, a.O, Frag<Tag>::SZ);
+  const size_t lds = Window<64>::lds(a.ids.A);
+  dim3 grid;
+  const bool few = a.N <= kFewRows, together = few && a.O <= kFusedColumns;
+  if (few) {
+    char* const out = a.out;
+    if (!together) a.out = nullptr;
+    if (int rc = tile_grid<16>(a, a.out != nullptr, 256, grid)) return rc;
+    hipLaunchKernelGGL((adapter_fused_kernel<Tag, R16>), grid, dim3(kAT), lds, st, a);
+    if (int rc = check_launch("adapter_fused_kernel")) return rc;
+    a.out = out;
+  } else {
+    if (int rc = tile_grid<64>(a, false, 256, grid)) return rc;
+    if (a.r == 16 * R16 && a.K % Stage<Tag, 16, true>::kCols == 0)
+      hipLaunchKernelGGL((adapter_shrink_kernel<Tag, R16, true>), grid, dim3(kAT), lds, st, a);
+    else hipLaunchKernelGGL((adapter_shrink_kernel<Tag, R16, false>), grid, dim3(kAT), lds, st, a);
+    if (int rc = check_launch("adapter_shrink_kernel")) return rc;
+  }
+  if (together || !a.out) return RRL_OK;
+  if (few) return launch_expand<Tag, R16, 16>(a, 1024, lds, st);
+  return launch_expand<Tag, R16, TM>(a, 256, lds, st);
 }
 template <class Tag>
 int launch_fused(const FusedArgs& a, hipStream_t st) {
@@ -1014,13 +1342,14 @@ extern "C" int rrl_adapter_bwd(const rrl_adapter_params* p, const void* x, int64
   if (dup) {
     o.job[0] = OuterJob{static_cast<const char*>(grad), g_ld, p->O, t, reinterpret_cast<float*>(w + l.part[0]),
                         reinterpret_cast<int32_t*>(w + l.seen[0]), static_cast<char*>(dup), p->O * p->r, p->r, 1,
-                        (int)((p->O + kOuterCols - 1) / kOuterCols), 0};
+                        (int)((p->O + kOuterCols - 1) / kOuterCols), 0, larger_than_cache(p->N, p->O, size)};
     o.job[0].wide = p->N ? o.job[0].wide : w;
   }
   if (ddown) {
     o.job[1] = OuterJob{static_cast<const char*>(x), x_ld, p->H, s, reinterpret_cast<float*>(w + l.part[1]),
                         reinterpret_cast<int32_t*>(w + l.seen[1]), static_cast<char*>(ddown), p->H * p->r, 1, p->H,
-                        (int)((p->H + kOuterCols - 1) / kOuterCols), p->dropout != nullptr};
+                        (int)((p->H + kOuterCols - 1) / kOuterCols), p->dropout != nullptr,
+                        larger_than_cache(p->N, p->H, size)};
     o.job[1].wide = p->N ? o.job[1].wide : w;
   }
   if (p->N > 0) {
