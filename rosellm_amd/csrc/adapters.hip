@@ -731,7 +731,7 @@ __global__ __launch_bounds__(kAT) void adapter_shrink_kernel(FusedArgs a) {
 // base + scale up t, a stage of all rows of a tile to a wave at a time, the waves side by
 // side.  WHOLE: the columns are stages, and r is 16 R16.
 template <class Tag, int R16, int TM, bool WHOLE>
-__global__ __launch_bounds__(kAT, R16 <= 2 ? 3 : 2) void adapter_expand_kernel(FusedArgs a) {
+__global__ __launch_bounds__(kAT, R16 <= 2 && TM > 16 ? 3 : 2) void adapter_expand_kernel(FusedArgs a) {
   using S = Stage<Tag, TM, WHOLE>;
   constexpr int SZ = S::SZ, R = 16 * R16, MT = TM / 16;
   __shared__ uint16_t order[kWindow];
@@ -775,7 +775,9 @@ __global__ __launch_bounds__(kAT, R16 <= 2 ? 3 : 2) void adapter_expand_kernel(F
         if (chunk + kAW < chunks) in.load(base0, a.b_ld, rows, c + kAW * S::kCols, c1, a.stream_out);
       }
       wave_fence();
-      constexpr int NC = S::kCols / 16 < 4 ? S::kCols / 16 : 4;  // tiles of up's rows at once
+      // tiles of up's rows at once: with 16 rows of t, as many as 64 registers hold
+      constexpr int kMost = TM > 16 ? 4 : (std::is_same_v<Tag, TagF32> || R16 > 2 ? 32 / R16 : 16);
+      constexpr int NC = S::kCols / 16 < kMost ? S::kCols / 16 : kMost;
 #pragma unroll 1
       for (int i0 = 0; i0 < S::kCols / 16; i0 += NC) {
         if (c + 16 * i0 >= c1) break;
