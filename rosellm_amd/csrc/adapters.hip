@@ -1100,7 +1100,7 @@ int launch_expand(FusedArgs a, int64_t least, size_t lds, hipStream_t st) {
 }
 
 // Few rows: both products in one launch.
-constexpr int64_t kFewRows = 256, kFusedColumns = 8192;
+constexpr int64_t kFusedColumns = 8192;
 constexpr int64_t kStreamed = (int64_t)128 << 20;  // half the memory-side cache
 inline int larger_than_cache(int64_t rows, int64_t cols, size_t size) {
   return rows * cols * (int64_t)size > kStreamed;
@@ -1113,7 +1113,7 @@ int launch_fused(FusedArgs a, hipStream_t st) {
   a.stream_out = larger_than_cache(a.N, a.O, Frag<Tag>::SZ);
   const size_t lds = Window<64>::lds(a.ids.A);
   dim3 grid;
-  const bool few = a.N <= kFewRows, together = few && a.O <= kFusedColumns;
+  const bool few = a.N <= (R16 <= 2 ? 1024 : 256), together = few && a.O <= kFusedColumns;
   if (few) {
     char* const out = a.out;
     if (!together) a.out = nullptr;

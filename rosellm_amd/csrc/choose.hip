@@ -22,8 +22,8 @@
 // launch (from the caches, but for the first):
 //   1. choose_max: the maximum of each part
 //   2. choose_weigh: each part's sum, and where the row has a top-k or a top-p its
-//      histogram, counts or sums in 1024 bins of 1/16 of a factor of two below m; sums
-//      leave out entries that no nucleus can hold
+//      histogram, counts or sums in 1024 bins of 1/16 of a factor of two below m, of the
+//      entries that a nucleus or the top k can hold at all; the latter are listed as well
 //   3. choose_cut (only if there may be a top-k or top-p): a workgroup a row finds the bin
 //      that holds the border, lists its entries, and finds the place among them
 //   4. choose_left (as 3): the sum of what is left, of each quarter of a part
@@ -38,7 +38,7 @@ namespace {
 constexpr int kPT = 256, kPW = kPT / 64;   // threads and waves of a part
 constexpr int kRT = 1024, kRW = kRT / 64;  // of a row
 constexpr int kBins = 1024, kBinBits = 10;
-constexpr int kListed = 4096;              // entries of a bin that are held in LDS
+constexpr int kListed = 4096, kPartListed = 2048;  // entries that are held in LDS
 constexpr int kAhead = 4;                  // 16-byte vectors that a lane loads at once
 constexpr int kNoIndex = 0x7fffffff;
 static_assert(kBins == kRT, "a bin to a thread");
@@ -71,6 +71,10 @@ struct ChooseArgs {
   u64* sums;        // [B, parts, kBins], where there may be a top-p
   uint32_t* counts; // [B, parts, kBins], where there may be a top-k
   Cut* cut;         // [B], where there may be either
+  float* tops;      // [B, parts, kPT] a lane's maximum, where there may be a top-k
+  float* reach;     // [B] the least value that the top k can hold
+  float* list_x;    // [B, kListed] entries that the top k can hold, in any order
+  int *list_i, *listed;  // their places, and [B] their number (over kListed: not all are there)
   int64_t* token_out;
   float *logp_out, *logq_out;  // logq_out may be null
 };
@@ -82,6 +86,20 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
+// The bits of a key that a type's values differ in: bfloat16's lower 16 and float16's lower
+// 13 are all zeros, or all ones below 0.
+template <class Tag> constexpr int kKeyShift = 0;
+template <> constexpr int kKeyShift<TagBF16> = 16;
+template <> constexpr int kKeyShift<TagF16> = 13;
+template <class Tag>
+__device__ __forceinline__ uint32_t short_key(float x) { return key_of(x) >> kKeyShift<Tag>; }
+template <class Tag>
+__device__ __forceinline__ float short_value(uint32_t k) {
+  constexpr int S = kKeyShift<Tag>;
+  k <<= S;
+  return value_of(k >> 31 ? k : k | ((1u << S) - 1u));
 }
 
 // `sh` holds a value for each of the NW waves.
@@ -143,6 +161,28 @@ struct Settings {
 };
 __device__ __forceinline__ int bin_of(float x, float m, float scale) {
   return (int)fminf((m - x) * scale, (float)(kBins - 1));
+}
+
+// The least float (by its key) that falls into a bin up to `bin`.  Whole waves look for the
+// same, 64 places at a time.
+__device__ __forceinline__ float bin_floor(int bin, float m, float scale) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t lo = key_of(-__FLT_MAX__), hi = key_of(m);  // hi does
+  while (lo < hi) {
+    const uint32_t step = (hi - lo) / 64 + 1;
+    const uint32_t at = hi - lo > lane * step ? lo + lane * step : hi;
+    const uint64_t in = __ballot(bin_of(value_of(at), m, scale) <= bin);
+    if (in) {
+      const uint32_t first = (uint32_t)__ffsll((unsigned long long)in) - 1;
+      const uint32_t found = hi - lo > first * step ? lo + first * step : hi;
+      if (first > 0) lo += (first - 1) * step + 1;
+      hi = found;
+      if (first == 0) lo = hi;
+    } else {
+      lo += 63 * step + 1;
+    }
+  }
+  return value_of(hi);
 }
 
 // The row's maximum; +inf where it has no distribution.
@@ -224,34 +264,108 @@ __global__ __launch_bounds__(kPT) void choose_max_kernel(ChooseArgs a) {
       nan |= __builtin_isunordered(x[k], x[k + 1]);
     }
   });
+  if (a.tops) {
+    a.tops[(int64_t)blockIdx.x * kPT + threadIdx.x] = m;
+    if (part == 0 && threadIdx.x == 0) a.listed[b] = 0;
+  }
   m = block_reduce<kPW>(nan ? M<float>::inf() : m, sh, Max());
   if (threadIdx.x == 0) a.peak[blockIdx.x] = m;
 }
 
 // ---- 2 ---------------------------------------------------------------------------------
 
+struct WeighShared {
+  u64 sums[kBins];
+  uint32_t counts[kBins];
+  float list_x[kPartListed];
+  int list_i[kPartListed];
+  u64 wave[kPW];
+  int listed, bin, base;
+};
+
+// The last bin that the top k reach at most: k lanes' maxima are that large or larger.
+__device__ __forceinline__ int top_bin(const ChooseArgs& a, const Settings& set, float m, int64_t b, WeighShared& sh) {
+  const int t = threadIdx.x, lane = t & 63, wv = t >> 6, n = a.parts * kPT;
+  if (set.top_k > n) return kBins - 1;
+  const float scale = set.scale();
+  constexpr int kTogether = 8;
+  for (int k0 = t; k0 < n; k0 += kTogether * kPT) {
+    float x[kTogether];
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k) x[k] = a.tops[b * n + min(k0 + k * kPT, n - 1)];
+#pragma unroll
+    for (int k = 0; k < kTogether; ++k)
+      if (k0 + k * kPT < n && x[k] != -M<float>::inf()) atomicAdd(&sh.counts[bin_of(x[k], m, scale)], 1u);
+  }
+  if (t == 0) sh.bin = kBins - 1;
+  __syncthreads();
+  constexpr int kEach = kBins / kPT;
+  uint32_t mine[kEach], sum = 0;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    mine[k] = sh.counts[t * kEach + k];
+    sum += mine[k];
+  }
+  uint32_t upto = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += y;
+  }
+  uint32_t* const sums = reinterpret_cast<uint32_t*>(sh.wave);
+  if (lane == 63) sums[wv] = upto;
+  __syncthreads();
+  for (int k = 0; k < wv; ++k) upto += sums[k];
+  uint32_t at = upto - sum;
+  if (at < set.top_k && upto >= set.top_k) {  // one thread's
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      if (at < set.top_k && at + mine[k] >= set.top_k) sh.bin = t * kEach + k;
+      at += mine[k];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) sh.counts[t * kEach + k] = 0;
+  __syncthreads();
+  return sh.bin;
+}
+
 template <class Tag, bool DIRECT>
 __device__ __forceinline__ void weigh(const ChooseArgs& a, const Settings& set, const Mass& mass, float m, int64_t b,
-                                      int64_t part, u64* sums, uint32_t* counts, u64& whole, u64& left) {
+                                      int64_t part, float reach, WeighShared& sh, u64& whole, u64& left) {
   constexpr int EPV = Pack16<Tag>::EPV;
   const char* row = row_at<Tag>(a, b);
-  if (set.filtered) {
-    const float scale = set.scale();
+  const float scale = set.scale();
+  if (set.filtered && set.top_k > 0) {
+    sweep_part<Tag>(a, row, part, [&](const float (&x)[EPV], int i) {
+#pragma unroll
+      for (int k = 0; k < EPV; ++k) {
+        const u64 w = mass.of<DIRECT>(x[k]);
+        whole += w;
+        if (x[k] >= reach) {
+          const int bin = bin_of(x[k], m, scale), at = atomicAdd(&sh.listed, 1);
+          atomicAdd(&sh.counts[bin], 1u);
+          if (set.top_p > 0.0) atomicAdd(&sh.sums[bin], w);
+          if (at < kPartListed) {
+            sh.list_x[at] = x[k];
+            sh.list_i[at] = i + k;
+          }
+        }
+      }
+    });
+  } else if (set.filtered) {
     // Entries of at most (1 - top_p) / V of the largest make up no more than 1 - top_p of
-    // the whole, so that the border lies above them.  What top_k leaves has a whole of its
-    // own, for which the sums are needed down to it.
-    const u64 floor = set.top_p == 0.0 ? ~(u64)0
-                                       : (set.top_k > 0 ? 0 : (u64)ldexp((1.0 - set.top_p) / (double)a.V, a.unit_log2));
+    // the whole, so that the border lies above them.
+    const u64 floor = (u64)ldexp((1.0 - set.top_p) / (double)a.V, a.unit_log2);
     sweep_part<Tag>(a, row, part, [&](const float (&x)[EPV], int) {
 #pragma unroll
       for (int k = 0; k < EPV; ++k) {
         const u64 w = mass.of<DIRECT>(x[k]);
         whole += w;
-        if (w > floor) atomicAdd(&sums[bin_of(x[k], m, scale)], w);
-        if (set.top_k > 0 && x[k] != -M<float>::inf()) atomicAdd(&counts[bin_of(x[k], m, scale)], 1u);
+        if (w > floor) atomicAdd(&sh.sums[bin_of(x[k], m, scale)], w);
       }
     });
-  } else {
+  } else if (set.min_p > 0.0) {
     const Cut cut = set.least(m);
     sweep_part<Tag>(a, row, part, [&](const float (&x)[EPV], int) {
 #pragma unroll
@@ -261,6 +375,12 @@ __device__ __forceinline__ void weigh(const ChooseArgs& a, const Settings& set, 
         left += x[k] >= cut.v ? w : 0;
       }
     });
+  } else {
+    sweep_part<Tag>(a, row, part, [&](const float (&x)[EPV], int) {
+#pragma unroll
+      for (int k = 0; k < EPV; ++k) whole += mass.of<DIRECT>(x[k]);
+    });
+    left = whole;
   }
 }
 __device__ __forceinline__ u64 wave_total(u64 v) {
@@ -273,32 +393,41 @@ template <class Tag>
 __global__ __launch_bounds__(kPT) void choose_weigh_kernel(ChooseArgs a) {
   const int64_t b = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   const int t = threadIdx.x;
-  __shared__ u64 sums[kBins];
-  __shared__ uint32_t counts[kBins];
-  __shared__ u64 sh[kPW];
+  __shared__ WeighShared sh;
   const Settings set(a, b);
-  const float m = row_peak<kPW>(a, b, reinterpret_cast<float*>(sh));
+  const float m = row_peak<kPW>(a, b, reinterpret_cast<float*>(sh.wave));
   if (set.bad || !(m < M<float>::inf())) return;
+  float reach = 0.0f;
   if (set.filtered) {
     for (int k = t; k < kBins; k += kPT) {
-      sums[k] = 0;
-      counts[k] = 0;
+      sh.sums[k] = 0;
+      sh.counts[k] = 0;
     }
+    if (t == 0) sh.listed = 0;
+    __syncthreads();
+    if (set.top_k > 0) reach = bin_floor(top_bin(a, set, m, b, sh), m, set.scale());
   }
-  __syncthreads();
   const Mass mass(m, set.c(), a.magic);
   u64 whole = 0, left = 0;
-  if (mass.w.direct) weigh<Tag, true>(a, set, mass, m, b, part, sums, counts, whole, left);
-  else weigh<Tag, false>(a, set, mass, m, b, part, sums, counts, whole, left);
-  whole = block_reduce<kPW>(whole, sh, Add());
+  if (mass.w.direct) weigh<Tag, true>(a, set, mass, m, b, part, reach, sh, whole, left);
+  else weigh<Tag, false>(a, set, mass, m, b, part, reach, sh, whole, left);
+  whole = block_reduce<kPW>(whole, sh.wave, Add());
   if (t == 0) a.whole[blockIdx.x] = whole;
   if (set.filtered) {
-    __syncthreads();
     const int64_t to = (int64_t)blockIdx.x * kBins;
     if (set.top_p > 0.0)
-      for (int k = t; k < kBins; k += kPT) a.sums[to + k] = sums[k];
-    if (set.top_k > 0)
-      for (int k = t; k < kBins; k += kPT) a.counts[to + k] = counts[k];
+      for (int k = t; k < kBins; k += kPT) a.sums[to + k] = sh.sums[k];
+    if (set.top_k > 0) {
+      for (int k = t; k < kBins; k += kPT) a.counts[to + k] = sh.counts[k];
+      if (part == 0 && t == 0) a.reach[b] = reach;
+      // a run of the row's list; beyond its end, or this part's, nothing is listed
+      if (t == 0) sh.base = atomicAdd(&a.listed[b], min(sh.listed, kListed + 1) + (sh.listed > kPartListed ? kListed + 1 : 0));
+      __syncthreads();
+      for (int k = t; k < min(sh.listed, kPartListed) && sh.base + k < kListed; k += kPT) {
+        a.list_x[b * kListed + sh.base + k] = sh.list_x[k];
+        a.list_i[b * kListed + sh.base + k] = sh.list_i[k];
+      }
+    }
   } else {
     left = wave_total(left);
     if ((t & 63) == 0) a.left[blockIdx.x * kPW + (t >> 6)] = left;
@@ -331,7 +460,8 @@ __device__ __forceinline__ int find_bin(CutShared& sh, u64 mine, u64& above, u64
   if (lane == 63) sh.wave[wv] = v;
   __syncthreads();
   u64 end = above + v;
-  for (int k = 0; k < wv; ++k) end += sh.wave[k];
+#pragma unroll
+  for (int k = 0; k < kRW; ++k) end += k < wv ? sh.wave[k] : 0;  // all read at once
   if (end - mine <= target && end > target) {  // one thread's
     sh.bin = t;
     sh.above = end - mine;
@@ -347,20 +477,8 @@ __device__ __forceinline__ int bits_over(uint32_t n) {  // bits to drop so that 
   return bits > kBinBits ? bits - kBinBits : 0;
 }
 
-// The least float (by its key) that falls into a bin up to `bin`; the whole workgroup
-// looks for the same.
-__device__ __forceinline__ float bin_floor(int bin, float m, float scale) {
-  uint32_t lo = key_of(-__FLT_MAX__), hi = key_of(m);  // hi does
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (bin_of(value_of(mid), m, scale) <= bin) hi = mid;
-    else lo = mid + 1;
-  }
-  return value_of(hi);
-}
-
-// The entries of one bin that a cut leaves: listed in LDS, or, if they are too many for
-// that, looked for in the row each time.
+// The entries of one bin that a cut leaves: in a list in LDS, or, if they are too many for
+// that, looked for in the row each time.  The list is the row's if that is whole.
 template <class Tag>
 struct BinEntries {
   const char* row;
@@ -370,94 +488,169 @@ struct BinEntries {
   CutShared* sh;
   int listed;
   __device__ __forceinline__ BinEntries(const ChooseArgs& a, int64_t b, float m, float scale, int bin, const Cut& cut_,
-                                        CutShared& sh_)
+                                        bool have_list, CutShared& sh_)
       : row(row_at<Tag>(a, b)), V(a.V), cut(cut_), sh(&sh_), listed(kListed + 1) {
     lo = bin_floor(bin, m, scale);
-    hi = bin > 0 ? bin_floor(bin - 1, m, scale) : M<float>::inf();
+    hi = bin > 0 ? bin_floor(bin - 1, m, scale) : M<float>::inf();  // (its key lies above all others)
+    if (have_list) {
+      listed = sh->listed;
+      return;
+    }
     __syncthreads();
     if (threadIdx.x == 0) sh->listed = 0;
     __syncthreads();
-    each([&](float x, int i) {  // in any order: what follows does not depend on it
-      const int at = atomicAdd(&sh->listed, 1);
-      if (at < kListed) {
-        sh->list_x[at] = x;
-        sh->list_i[at] = i;
+    constexpr int EPV = Pack16<Tag>::EPV;
+    // a lane marks its entries, then lists them one after another, all lanes' at once
+    for (int64_t base = 0; base < V; base += kAhead * kRT * EPV) {
+      const int64_t i0 = base + threadIdx.x * EPV;
+      uint32_t marks = 0;
+      u32x4 raw[kAhead];
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        const int64_t i = i0 + (int64_t)s * kRT * EPV;
+        if (i + EPV <= V) {
+          raw[s] = reinterpret_cast<const Any16*>(row + i * (16 / EPV))->v;
+        } else {
+          float x[EPV];
+          load_entries<Tag>(row, i, V, x);
+          raw[s] = Pack16<Tag>::pack(x);
+        }
       }
-    });
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        float x[EPV];
+        Pack16<Tag>::unpack(raw[s], x);
+#pragma unroll
+        for (int k = 0; k < EPV; ++k)
+          marks |= (x[k] >= lo && x[k] < hi && x[k] != -M<float>::inf() ? 1u : 0u) << (s * EPV + k);
+      }
+      while (__any(marks != 0)) {
+        const int k = __ffs((int)marks) - 1;
+        const int64_t i = marks ? i0 + (int64_t)(k / EPV) * kRT * EPV + k % EPV : 0;
+        const float x = marks ? load_entry<Tag>(row, i) : 0.0f;
+        const bool in = marks && cut.keeps(x, (int)i);
+        const uint64_t all = __ballot(in);
+        int from = 0;
+        if ((threadIdx.x & 63) == 0 && all) from = atomicAdd(&sh->listed, (int)__popcll(all));
+        from = __builtin_amdgcn_readfirstlane(from);
+        const int at = from + __popcll(all & (((uint64_t)1 << (threadIdx.x & 63)) - 1));
+        if (in && at < kListed) {  // in any order: what follows does not depend on it
+          sh->list_x[at] = x;
+          sh->list_i[at] = (int)i;
+        }
+        marks &= marks - 1;
+      }
+    }
     __syncthreads();
     listed = sh->listed;
   }
+  // f(whether there is one, value, index) with whole waves.  One loop for both kinds, and one
+  // call of f: this kernel runs once over long code, which has to come from memory.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    if (listed <= kListed) {
-      for (int k = threadIdx.x; k < listed; k += kRT) f(sh->list_x[k], sh->list_i[k]);
-    } else {
-      constexpr int EPV = Pack16<Tag>::EPV;
-      sweep<Tag, kRT>(row, 0, V, threadIdx.x, [&](const float (&x)[EPV], int i) {
-        uint32_t in = 0;
+    constexpr int EPV = Pack16<Tag>::EPV;
+    const bool list = listed <= kListed;
+    const int per = list ? kRT : kRT * EPV;
+    const int64_t n = list ? listed : V;
+    for (int64_t base = 0; base < n; base += per) {
+      const int64_t i0 = base + (int64_t)threadIdx.x * (list ? 1 : EPV);
+      uint32_t marks = 0;
+      if (list) {
+        marks = i0 < n && sh->list_x[i0] >= lo && sh->list_x[i0] < hi ? 1u : 0u;
+      } else {
+        float x[EPV];
+        load_entries<Tag>(row, i0, V, x);
 #pragma unroll
-        for (int k = 0; k < EPV; ++k) in |= (x[k] >= lo && x[k] < hi ? 1u : 0u) << k;
-        if (!in) return;
-#pragma unroll
-        for (int k = 0; k < EPV; ++k)
-          if ((in >> k & 1) && cut.keeps(x[k], i + k)) f(x[k], i + k);
-      });
+        for (int k = 0; k < EPV; ++k) marks |= (x[k] >= lo && x[k] < hi && x[k] != -M<float>::inf() ? 1u : 0u) << k;
+      }
+      while (__any(marks != 0)) {
+        const int64_t at = marks ? i0 + __ffs((int)marks) - 1 : 0;
+        const float x = list ? sh->list_x[at] : load_entry<Tag>(row, at);
+        const int i = list ? sh->list_i[at] : (int)at;
+        f(marks && cut.keeps(x, i), x, i);
+        marks &= marks - 1;
+      }
     }
   }
 };
 
+// Adds v to bins that hold equal values of v each; whole waves call it.  An LDS atomic on one
+// address takes some 28 cycles a lane, and the entries of one bin have few values, so that
+// up to eight of them are counted over the wave first.
+__device__ __forceinline__ void add_equal(u64* hist, bool in, int bin, u64 v) {
+  for (int k = 0; k < 8; ++k) {
+    const uint64_t left = __ballot(in);
+    if (!left) return;
+    const bool mine = in && bin == __builtin_amdgcn_readlane(bin, __ffsll((unsigned long long)left) - 1);
+    const uint64_t like = __ballot(mine);
+    if (mine && (int)(threadIdx.x & 63) == __ffsll((unsigned long long)like) - 1)
+      atomicAdd(&hist[bin], v * (u64)__popcll(like));
+    in = in && !mine;
+  }
+  if (in) atomicAdd(&hist[bin], v);
+}
+
 // The longest run of these entries, in descending order, ties lowest index first, whose
 // measure (1 or a mass), with `above` before them, sums to no more than target, which all
 // of them exceed; at least one entry where nothing is above.
-template <class Entries, class Measure>
-__device__ Cut select(const Entries& in, u64 above, u64 target, Measure measure, CutShared& sh) {
+// With `want_rest`, `rest` becomes this thread's part of their masses.
+template <class Tag>
+__device__ __forceinline__ Cut select(const BinEntries<Tag>& in, bool by_mass, u64 above, u64 target, const Mass& mass,
+                                      bool want_rest, u64& rest, CutShared& sh) {
   const int t = threadIdx.x;
-  uint32_t lo = 0xffffffffu, hi = 0;
-  in.each([&](float x, int) {
-    const uint32_t k = key_of(x);
-    lo = min(lo, k);
-    hi = max(hi, k);
-  });
-  uint32_t* sh32 = reinterpret_cast<uint32_t*>(sh.wave);
-  lo = block_reduce<kRW>(lo, sh32, Min());
-  hi = block_reduce<kRW>(hi, sh32, Max());
-  while (lo < hi) {
-    const int shift = bits_over(hi - lo);
+  enum { KEYS, TIES, REST } phase = KEYS;
+  uint32_t lo = short_key<Tag>(in.lo), hi = short_key<Tag>(in.hi);  // the border lies among these keys,
+  uint32_t ilo = 0, ihi = (uint32_t)in.V;                           // the first that is not taken among these places
+  u64 take = 0, seen = 0;
+  float v = 0.0f;
+  Cut out{0.0f, 0};
+  for (;;) {
+    const int shift = phase == KEYS ? bits_over(hi - lo) : bits_over(ihi - ilo);
     __syncthreads();
     sh.hist[t] = 0;
     __syncthreads();
-    in.each([&](float x, int) {
-      const uint32_t k = key_of(x);
-      if (k >= lo && k <= hi) atomicAdd(&sh.hist[(hi - k) >> shift], measure(x));
+    in.each([&](bool is, float x, int i) {
+      if (phase == REST) {
+        rest += is && out.keeps(x, i) ? mass(x) : 0;
+        return;
+      }
+      const uint32_t at = phase == KEYS ? short_key<Tag>(x) : (uint32_t)i;
+      const uint32_t from = phase == KEYS ? lo : ilo, to = phase == KEYS ? hi : ihi;
+      is = is && at >= from && at <= to && (phase == KEYS || x == v);
+      const int bin = (int)((phase == KEYS ? to - at : at - from) >> shift);
+      const u64 w = !is ? 0 : (phase == KEYS && by_mass ? mass(x) : 1);
+      if (phase == KEYS && shift == 0) add_equal(sh.hist, is, bin, w);
+      else if (is) atomicAdd(&sh.hist[bin], w);
     });
+    if (phase == REST) return out;
     __syncthreads();
-    const int b = max(find_bin(sh, sh.hist[t], above, target), 0);
-    hi -= (uint32_t)b << shift;
-    lo = max(lo, shift ? hi - ((1u << shift) - 1) : hi);
+    const int b = find_bin(sh, sh.hist[t], phase == KEYS ? above : seen, phase == KEYS ? target : take);
+    if (phase == KEYS) {
+      const u64 here = sh.hist[max(b, 0)];
+      hi -= (uint32_t)max(b, 0) << shift;
+      lo = max(lo, shift ? hi - ((1u << shift) - 1) : hi);
+      if (lo < hi) continue;
+      // the ties at that value: as many as the rest of the target holds
+      v = short_value<Tag>(hi);
+      const u64 each = by_mass ? mass(v) : 1;
+      const u64 room = each ? (target - above) / each : ~(u64)0;
+      take = above == 0 && room == 0 ? 1 : room;
+      out = Cut{v, in.cut.v == v ? in.cut.n : kNoIndex};  // all of them
+      if (take == 0) {
+        out.n = 0;
+      } else if (each != 0 && take * each < here) {
+        phase = TIES;
+        continue;
+      }
+    } else if (b >= 0) {
+      ilo += (uint32_t)b << shift;
+      ihi = min(ihi, ilo + (1u << shift) - 1);
+      if (ilo < ihi) continue;
+      out.n = (int)ilo;
+    }
+    if (!want_rest) return out;
+    phase = REST;
   }
-  // the ties at that value: as many as the rest of the target holds
-  const float v = value_of(hi);
-  const u64 each = measure(v);
-  const u64 room = each ? (target - above) / each : ~(u64)0;
-  const u64 take = above == 0 && room == 0 ? 1 : room;
-  if (take == 0) return Cut{v, 0};
-  u64 seen = 0;
-  int ilo = 0, ihi = (int)in.V;  // the place of the first that is not taken
-  while (ilo < ihi) {
-    const int shift = bits_over((uint32_t)(ihi - ilo));
-    __syncthreads();
-    sh.hist[t] = 0;
-    __syncthreads();
-    in.each([&](float x, int i) {
-      if (x == v && i >= ilo && i <= ihi) atomicAdd(&sh.hist[(i - ilo) >> shift], (u64)1);
-    });
-    __syncthreads();
-    const int b = find_bin(sh, sh.hist[t], seen, take);
-    if (b < 0) return Cut{v, in.cut.v == v ? in.cut.n : kNoIndex};  // all of them
-    ilo += b << shift;
-    ihi = min(ihi, ilo + (1 << shift) - 1);
-  }
-  return Cut{v, ilo};
 }
 
 // One bin of every part.
@@ -487,36 +680,43 @@ __global__ __launch_bounds__(kRT) void choose_cut_kernel(ChooseArgs a) {
   const float scale = set.scale();
   const Mass mass(m, set.c(), a.magic);
   Cut cut{-M<float>::inf(), 0};
-  u64 sum = 0, count = 0;  // this thread's bin
-  if (set.top_p > 0.0)
-    sum = over_parts(a.sums + (int64_t)b * a.parts * kBins + t, a.parts);
+  u64 sum = 0;  // of this thread's bin
+  if (set.top_p > 0.0) sum = over_parts(a.sums + (int64_t)b * a.parts * kBins + t, a.parts);
+  bool have_list = false;
   if (set.top_k > 0) {
-    count = over_parts(a.counts + (int64_t)b * a.parts * kBins + t, a.parts);
-    u64 above = 0;
-    const int bin = find_bin(sh, count, above, (u64)set.top_k);
-    if (bin >= 0) {
-      const BinEntries<Tag> in(a, b, m, scale, bin, cut, sh);
-      cut = select(in, above, (u64)set.top_k, [](float) { return (u64)1; }, sh);
-      if (set.top_p > 0.0) {  // what is left of that bin, and nothing below it
-        u64 rest = 0;
-        in.each([&](float x, int i) { rest += cut.keeps(x, i) ? mass(x) : 0; });
-        rest = block_reduce<kRW>(rest, sh.wave, Add());
-        sum = t < bin ? sum : (t == bin ? rest : 0);
+    const int n = a.listed[b];
+    have_list = n <= kListed;
+    if (have_list) {
+      for (int k = t; k < n; k += kRT) {
+        sh.list_x[k] = a.list_x[b * kListed + k];
+        sh.list_i[k] = a.list_i[b * kListed + k];
       }
+      if (t == 0) sh.listed = n;
     }
+    __syncthreads();
   }
-  if (set.top_p > 0.0) {
-    u64 all = 0;
-    if (set.top_k > 0) all = sum;
-    else
-      for (int k = t; k < a.parts; k += kRT) all += a.whole[b * a.parts + k];
-    all = block_reduce<kRW>(all, sh.wave, Add());
-    const u64 target = (u64)(set.top_p * (double)all);
-    u64 above = 0;
-    const int bin = find_bin(sh, sum, above, target);
-    if (bin >= 0) {
-      const BinEntries<Tag> in(a, b, m, scale, bin, cut, sh);
-      cut = select(in, above, target, mass, sh);
+#pragma unroll 1
+  for (int stage = set.top_k > 0 ? 0 : 1; stage < (set.top_p > 0.0 ? 2 : 1); ++stage) {
+    const bool by_mass = stage == 1, both = stage == 0 && set.top_p > 0.0;
+    u64 mine = sum, target = (u64)set.top_k, above = 0;
+    if (by_mass) {
+      u64 all = 0;
+      if (set.top_k > 0) all = sum;
+      else
+        for (int k = t; k < a.parts; k += kRT) all += a.whole[b * a.parts + k];
+      target = (u64)(set.top_p * (double)block_reduce<kRW>(all, sh.wave, Add()));
+    } else {
+      mine = over_parts(a.counts + (int64_t)b * a.parts * kBins + t, a.parts);
+      cut = Cut{a.reach[b], kNoIndex};  // if these are k
+    }
+    const int bin = find_bin(sh, mine, above, target);
+    if (bin < 0) continue;
+    const BinEntries<Tag> in(a, b, m, scale, bin, by_mass ? cut : Cut{-M<float>::inf(), 0}, have_list, sh);
+    u64 rest = 0;
+    cut = select(in, by_mass, above, target, mass, both, rest, sh);
+    if (both) {  // what is left of that bin, and nothing below it
+      rest = block_reduce<kRW>(rest, sh.wave, Add());
+      sum = t < bin ? sum : (t == bin ? rest : 0);
     }
   }
   const Cut least = set.least(m);
@@ -644,7 +844,7 @@ __global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
     int first = kNoIndex;
     for (int p = t; p < a.parts; p += kPT)
       if (peak[p] == m) first = min(first, p);
-    first = block_reduce<kPW>(first, shi, Min());
+    first = min(block_reduce<kPW>(first, shi, Min()), a.parts - 1);
     span((int64_t)first * a.part, a.part, [&](float x, int i) { token = x == m ? min(token, i) : token; });
     token = block_reduce<kPW>(token, shi, Min());
   } else {
@@ -679,7 +879,7 @@ __global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
       int last = -1;
       for (int p = p0; p < p1; ++p)
         if (lefts[p]) last = p;
-      last = block_reduce<kPW>(last, shi, Max());
+      last = max(block_reduce<kPW>(last, shi, Max()), 0);
       token = -1;
       span((int64_t)last * (a.part / kPW), a.part / kPW, [&](float x, int i) {
         if (cut.keeps(x, i) && mass(x)) token = max(token, i);
@@ -741,10 +941,12 @@ __global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
     logq = log((double)total * unit);
   }
   if (t == 0) {
-    const double d = ((double)load_entry<Tag>(row, token) - (double)m) / set.T;
-    a.token_out[b] = token;
-    a.logp_out[b] = fminf((float)(d - norm), 0.0f);
-    if (a.logq_out) a.logq_out[b] = set.greedy ? 0.0f : fminf((float)(d - logq), 0.0f);
+    // (there is a token, unless the logits changed meanwhile; then none is read for it)
+    const bool some = token >= 0 && token < a.V;
+    const double d = some ? ((double)load_entry<Tag>(row, token) - (double)m) / set.T : M<double>::nan();
+    a.token_out[b] = some ? token : -1;
+    a.logp_out[b] = some ? fminf((float)(d - norm), 0.0f) : M<float>::nan();
+    if (a.logq_out) a.logq_out[b] = set.greedy && some ? 0.0f : (some ? fminf((float)(d - logq), 0.0f) : M<float>::nan());
   }
 }
 
@@ -760,7 +962,7 @@ inline int part_entries(int64_t B, int64_t V) {
 struct ChooseLayout {
   int part;
   int64_t parts;
-  size_t peak, whole, left, sums, counts, cut, total;
+  size_t peak, whole, left, sums, counts, cut, tops, reach, list_x, list_i, listed, total;
 };
 inline ChooseLayout choose_layout(int64_t B, int64_t V, bool top_k, bool top_p) {
   ChooseLayout l;
@@ -779,6 +981,11 @@ inline ChooseLayout choose_layout(int64_t B, int64_t V, bool top_k, bool top_p) 
   l.sums = take(top_p ? 8 * n * kBins : 0);
   l.counts = take(top_k ? 4 * n * kBins : 0);
   l.cut = take(sizeof(Cut) * (size_t)B);
+  l.tops = take(top_k ? 4 * n * kPT : 0);
+  l.reach = take(top_k ? 4 * (size_t)B : 0);
+  l.list_x = take(top_k ? 4 * (size_t)B * kListed : 0);
+  l.list_i = take(top_k ? 4 * (size_t)B * kListed : 0);
+  l.listed = take(top_k ? 4 * (size_t)B : 0);
   l.total = at;
   return l;
 }
@@ -870,6 +1077,11 @@ extern "C" int rrl_sample_tokens(const void* logits, int32_t dtype, int64_t B, i
   a.sums = reinterpret_cast<u64*>(w + l.sums);
   a.counts = reinterpret_cast<uint32_t*>(w + l.counts);
   a.cut = reinterpret_cast<Cut*>(w + l.cut);
+  a.tops = top_k ? reinterpret_cast<float*>(w + l.tops) : nullptr;
+  a.reach = reinterpret_cast<float*>(w + l.reach);
+  a.list_x = reinterpret_cast<float*>(w + l.list_x);
+  a.list_i = reinterpret_cast<int*>(w + l.list_i);
+  a.listed = reinterpret_cast<int*>(w + l.listed);
   a.token_out = token_out;
   a.logp_out = logp_out;
   a.logq_out = logq_out;
