@@ -62,7 +62,7 @@ __global__ __launch_bounds__(kDT) void dropout_kernel(DropArgs a) {
   constexpr int SZ = 16 / Pack16<Tag>::EPV;
   const int64_t g = (int64_t)blockIdx.x * kDT + threadIdx.x;
   if (g >= a.groups) return;
-  const int64_t row = a.groups < ((int64_t)1 << 32) ? (uint32_t)g / (uint32_t)a.per_row : g / a.per_row;
+  const int64_t row = (uint32_t)g / (uint32_t)a.per_row;  // there are fewer than 2^32
   const int64_t i = (g - row * a.per_row) * 8;
   float v[8];
   load_group<Tag>(a.x + row * a.x_ld * SZ, i, a.cols, v);

@@ -58,8 +58,9 @@ def _reference(x, base, down, up, ids, g, scales, mask=None, factor=1.0):
     N, A = x.shape[0], down.shape[0]
     H, r, O = dd.shape[2], dd.shape[1], ud.shape[1]
     low = 0.0 if x.dtype == torch.float32 else 2.0 ** -16
-    y = torch.zeros(N, O, dtype=torch.float64) if base is None else base.double().clone()
-    ey, dx, edx = torch.zeros(N, O).double(), torch.zeros(N, H).double(), torch.zeros(N, H).double()
+    new = lambda c: torch.zeros(N, c, dtype=torch.float64, device=x.device)
+    y = new(O) if base is None else base.double().clone()
+    ey, dx, edx = new(O), new(H), new(H)
     ddown, eddown, dup, edup = (torch.zeros_like(v) for v in (dd, dd, ud, ud))
     for a in range(A):
         n = (ids == a).nonzero().flatten()
@@ -406,3 +407,70 @@ def test_rollout_and_training_of_adapter_policies(device):
                                       policy.reshape(-1).cpu(), dl.view(-1, V).cpu(), None)
     _close(dd, *want_d, "ddown")
     _close(du, *want_u, "dup")
+
+
+@pytest.mark.parametrize("N,A,r", [(300, 4096, 4), (1300, 4096, 3), (20, 4000, 128)])
+def test_most_adapters(device, N, A, r):
+    gen = torch.Generator().manual_seed(A)
+    H, O = 24, 40
+    x, base, down, up, ids, g = _make(N, A, H, O, r, torch.bfloat16, gen)
+    ids[0], ids[1] = A - 1, 0
+    out = _run(device, x, base, down, up, ids, g, None)
+    want = _reference(x, base, down, up, ids, g, None)
+    for got, (w, e), what in zip(out, want, ("y", "dx", "ddown", "dup")):
+        _close(got, w, e, what)
+
+
+@pytest.mark.parametrize("dtype,N,H,O,r", [(torch.bfloat16, 70000, 1024, 1088, 16), (torch.float32, 40000, 1000, 896, 9)],
+                         ids=["bfloat16", "float32"])
+def test_matrices_larger_than_the_caches(device, dtype, N, H, O, r):
+    """Operands that are streamed, whole and not whole sizes: some rows, and the factors' gradients over all."""
+    gen = torch.Generator(device="cuda").manual_seed(N)
+    x, g, base = (torch.randn(N, c, generator=gen, device=device).to(dtype) for c in (H, O, O))
+    down = (torch.randn(2, r, H, generator=gen, device=device) * H ** -0.5).to(dtype)
+    up = torch.randn(2, O, r, generator=gen, device=device).to(dtype)
+    ids = (torch.arange(N, device=device) // 5000) % 2
+    ids[777:900] = -1
+    leaves = [v.requires_grad_() for v in (x, down, up)]
+    y = adapter_linear(*leaves, ids, base=base, dropout_p=0.1, seed=4)
+    dx, dd, du = torch.autograd.grad(y, leaves, g)
+    mask, factor = keep(N, H, 0.1, 4, 0)
+    want = _reference(x.detach(), base, down.detach(), up.detach(), ids, g, None, mask.to(device), factor)
+    some = torch.randint(0, N, (400,), generator=gen, device=device)
+    some[:4] = torch.tensor([0, N - 1, 777, 4999], device=device)
+    for got, (w, e), what in ((y[some], [v[some] for v in want[0]], "y"), (dx[some], [v[some] for v in want[1]], "dx"),
+                              (dd, want[2], "ddown"), (du, want[3], "dup")):
+        _close(got, w.cpu(), e.cpu(), what)
+
+
+def test_two_threads(device):
+    """Steps from two host threads on streams of their own give the bits of steps in turn."""
+    import threading
+
+    gen = torch.Generator().manual_seed(15)
+    sets = [[v.to(device) for v in _make(600, 3, 80, 72, 12, torch.bfloat16, gen, 7)] for _ in range(2)]
+
+    def step(x, base, down, up, ids, g):
+        leaves = [v.detach().requires_grad_() for v in (x, down, up)]
+        y = adapter_linear(*leaves, ids, base=base, dropout_p=0.1, seed=1)
+        return (y.detach(), *torch.autograd.grad(y, leaves, g))
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                got = step(*sets[i])
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

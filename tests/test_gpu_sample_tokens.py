@@ -118,7 +118,7 @@ def test_settings_of_their_own_for_every_row(device, B, V, dtype):
 
 @pytest.mark.parametrize("V", [300001, 1 << 20])
 def test_long_rows(device, V):
-    """Rows past every register-held length, and with fewer bits to a weight."""
+    """Rows of more parts than others, of which the longer has fewer bits to a weight."""
     gen = torch.Generator().manual_seed(1)
     for dtype in (torch.float32, torch.bfloat16):
         x = _logits(2, V, gen, dtype, "normal")
@@ -276,3 +276,49 @@ def test_drafts_drawn_by_it_are_verified(device):
     assert torch.equal(out.token_ids[:, K], last.token_ids)
     assert torch.equal(out.token_ids[:, :K], drafts)
     assert ((out.logprobs[:, K] - last.logprobs).abs() <= 2.0 ** -23 * last.logprobs.abs()).all()
+
+
+@pytest.mark.parametrize("B,V", [(1100, 70001), (3000, 9), (700, 16385)])
+def test_large_batches(device, B, V):
+    """Longer parts where there are rows enough: some rows against 64 bits, all against calls of fewer rows."""
+    gen = torch.Generator().manual_seed(B)
+    x = _logits(B, V, gen, torch.bfloat16, "normal")
+    kw = _mixed(B, gen)
+    u = torch.rand(B, generator=gen)
+    xd, ud, kd = x.to(device), u.to(device), {k: v.to(device) for k, v in kw.items()}
+    whole = sample_tokens(xd, ud, **kd)
+    for i in range(0, B, B // 3):
+        n = min(B, i + 40)
+        some = sample_tokens(xd[i:n], ud[i:n], **{k: v[i:n] for k, v in kd.items()})
+        for a, b in zip(some, whole):
+            assert torch.equal(a, b[i:n])
+    pick = torch.arange(0, B, max(1, B // 8))
+    _check(x[pick], u[pick], device, **{k: v[pick] for k, v in kw.items()})
+
+
+def test_two_threads(device):
+    """Calls from two host threads on streams of their own give the bits of calls in turn."""
+    import threading
+
+    gen = torch.Generator().manual_seed(5)
+    xs = [_logits(20, 30000, gen, torch.bfloat16, "normal").to(device) for _ in range(2)]
+    u = torch.rand(20, generator=gen).to(device)
+    want = [sample_tokens(x, u, top_k=300, top_p=0.9) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                got = sample_tokens(xs[i], u, top_k=300, top_p=0.9)
+                stream.synchronize()
+                if not (torch.equal(got.token_ids, want[i].token_ids) and torch.equal(got.logprobs, want[i].logprobs)):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
