@@ -731,7 +731,7 @@ __global__ __launch_bounds__(kAT) void adapter_shrink_kernel(FusedArgs a) {
 // base + scale up t, a stage of all rows of a tile to a wave at a time, the waves side by
 // side.  WHOLE: the columns are stages, and r is 16 R16.
 template <class Tag, int R16, int TM, bool WHOLE>
-__global__ __launch_bounds__(kAT, R16 <= 2 && TM > 16 ? 3 : 2) void adapter_expand_kernel(FusedArgs a) {
+__global__ __launch_bounds__(kAT, 2) void adapter_expand_kernel(FusedArgs a) {
   using S = Stage<Tag, TM, WHOLE>;
   constexpr int SZ = S::SZ, R = 16 * R16, MT = TM / 16;
   __shared__ uint16_t order[kWindow];
@@ -1072,15 +1072,15 @@ __global__ __launch_bounds__(kAT) void adapter_turn_kernel(TurnArgs a) {
 
 inline int rank_padded(int r) { return r <= 16 ? 16 : (r <= 32 ? 32 : (r <= 64 ? 64 : 128)); }
 
-// The grid of tiles of TM rows, and with `wide` runs of columns: as many as make a thousand
-// workgroups' work, of `least` columns at least.
+// The grid of tiles of TM rows, and with `wide` runs of columns: as many as make two
+// workgroups to each of the 256 CUs, of `least` columns at least.
 template <int TM>
 int tile_grid(FusedArgs& a, bool wide, int64_t least, dim3& grid) {
   const int64_t windows = (a.N + kWindow - 1) / kWindow;
   const int rows = (int)min(a.N, (int64_t)kWindow);
   // tiles of a window if it is of one adapter, and at most
   const int64_t even = (rows + TM - 1) / TM, most = min((int64_t)rows, even + a.ids.A + 1);
-  const int64_t cuts = wide ? max((int64_t)1, min((a.O + least - 1) / least, 1024 / max((int64_t)1, windows * even))) : 1;
+  const int64_t cuts = wide ? max((int64_t)1, min((a.O + least - 1) / least, 512 / max((int64_t)1, windows * even))) : 1;
   a.slab = wide ? ((a.O + cuts - 1) / cuts + least - 1) / least * least : 1;
   a.slabs = wide ? (int)((a.O + a.slab - 1) / a.slab) : 1;
   a.groups = (int)max((int64_t)1, min(most * a.slabs, max(even * a.slabs, 2048 / windows)));
