@@ -14,10 +14,17 @@
 // adapter needs none), and its tiles of 16 or 64 rows are of one adapter each, whatever
 // the order of the ids: no other launch, no list kept between calls.
 //
-// The fused kernel forms t of a tile (the depth H split over four waves, their sums
-// joined in LDS in order) and multiplies it by a run of rows of up while it is there, so
-// t makes no way through memory between the two products.  d x is the same kernel on g
-// with the transposes of up and down, which are laid out by a launch of their own.
+//   adapter_fused   few rows: t of 16 rows, the depth H split over four waves, and its product
+//                   with a run of rows of up while it is there (64 rows of 16 adapters, 1024
+//                   to 2048, rank 16: 9.5 us, a chain of four dependent loads)
+//   adapter_shrink  t of many rows (131,072 x 1024 bfloat16: 57 us, 4.7 TB/s; with dropout 67,
+//                   of which the generator's issue is 51)
+//   adapter_expand  base + scale up t (131,072 x 2048 bfloat16: 246 us, 4.4 TB/s; a copy of
+//                   that size reaches 4.7; dx, written only, 56 us, 4.8 TB/s)
+//   adapter_outer   the factors' gradients over runs of tokens (g and x of the above: 148 us,
+//                   5.4 TB/s; with dropout 164), adapter_join adds the runs (9 us)
+// d x is adapter_shrink and adapter_expand on g with the transposes of up and down, which
+// adapter_turn lays out.
 //
 // t is float32.  The second product's bfloat16 instruction takes it as the sum of two
 // bfloat16 numbers, to 2^-17: one rounding to bfloat16 (2^-9) would be as large as that
@@ -1072,6 +1079,9 @@ __global__ __launch_bounds__(kAT) void adapter_turn_kernel(TurnArgs a) {
 
 inline int rank_padded(int r) { return r <= 16 ? 16 : (r <= 32 ? 32 : (r <= 64 ? 64 : 128)); }
 
+// Kernels for whole sizes leave out the looks for a row's end (131,072 rows of 1024 by rank
+// 16: t 57 us instead of 64; sizes and ranks that are not whole take the others).
+//
 // The grid of tiles of TM rows, and with `wide` runs of columns: as many as make two
 // workgroups to each of the 256 CUs, of `least` columns at least.
 template <int TM>
@@ -1099,9 +1109,19 @@ int launch_expand(FusedArgs a, int64_t least, size_t lds, hipStream_t st) {
   return check_launch("adapter_expand_kernel");
 }
 
-// Few rows: both products in one launch.
-constexpr int64_t kFusedColumns = 8192;
-constexpr int64_t kStreamed = (int64_t)128 << 20;  // half the memory-side cache
+// Few rows take tiles of 16 with the depth split over the waves, and both products in one
+// launch unless every workgroup would form t again for too few columns.  us with one / two
+// launches: 64 rows of 16 adapters, 1024 to 2048 9.5 / 17.3, 4096 9.7 / 16.5, 8192 11.1 /
+// 17.4, 16,384 17.8 / 17.7, 32,768 25.7 / 23.1; 320 rows, 1024 to 2048 11.1 / 21.8, 512 rows
+// to 4096 15.7 / 24.7, 1000 rows to 2048 13.9 / 24.4; at rank 64 256 rows to 2048 15.2 / 33.5,
+// 512 21.2 / 35.0, 1000 to 4096 42.5 / 39.9.
+template <int R16> constexpr int64_t kFewRows = R16 <= 2 ? 1024 : 512;
+constexpr int64_t kFusedColumns = 16384;
+// Matrices of over half the memory-side cache are streamed past it: 268 and 537 MB are read
+// in 65 and 118 us instead of 65 and 151, and what other passes read again stays in it (the
+// factors' gradients over both: 147 us instead of 194).  67 MB, which stay there, are read in
+// 52.8 us streamed and in 49.6 not.
+constexpr int64_t kStreamed = (int64_t)128 << 20;
 inline int larger_than_cache(int64_t rows, int64_t cols, size_t size) {
   return rows * cols * (int64_t)size > kStreamed;
 }
@@ -1113,7 +1133,7 @@ int launch_fused(FusedArgs a, hipStream_t st) {
   a.stream_out = larger_than_cache(a.N, a.O, Frag<Tag>::SZ);
   const size_t lds = Window<64>::lds(a.ids.A);
   dim3 grid;
-  const bool few = a.N <= (R16 <= 2 ? 1024 : 256), together = few && a.O <= kFusedColumns;
+  const bool few = a.N <= kFewRows<R16>, together = few && a.O <= kFusedColumns;
   if (few) {
     char* const out = a.out;
     if (!together) a.out = nullptr;
