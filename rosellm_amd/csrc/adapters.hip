@@ -30,7 +30,8 @@
 // bfloat16 numbers, to 2^-17: one rounding to bfloat16 (2^-9) would be as large as that
 // of the result.  With float16 operands, whose range t can leave, up is taken as the
 // exact sum of two bfloat16 numbers as well; the product of the two low parts (2^-18)
-// is left out.  float32 operands take the float32 instruction.
+// is left out.  float32 operands take the float32 instruction.  An infinity times a part
+// that is zero is NaN, which is what such a sum may become instead of infinite.
 #include "dropout_common.hpp"
 #include "vocab_weights.hpp"
 

@@ -6,7 +6,7 @@
 // under the key `seed`, 16 bits an entry, the low half of a word first.  An entry is
 // kept where its number is at least cut = round(65536 p), and scaled by
 // 65536 / (65536 - cut): the probability is p to 2^-17, and the expectation exact.
-// With 32 bits an entry the generator alone (140 issue slots a call, most of them the
+// With 32 bits an entry the generator alone (about 120 issue slots a call, most of them the
 // quarter-rate multiplications) would take longer than the entries' bytes.
 #pragma once
 

@@ -19,6 +19,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
+from .._graph import recorded
 from .._random import dropout_arguments, dropout_params
 
 __all__ = ["adapter_linear"]
@@ -36,6 +37,10 @@ def _rows(x: Tensor):
     return y, (y.stride(0) if y.shape[0] > 1 else H)
 
 
+def _factor(w: Tensor) -> Tensor:
+    return w if w.stride(2) == 1 or w.shape[2] == 1 else w.contiguous()
+
+
 def _params(dtype, N, down, up, ids, scales, drop):
     A, r, H = down.shape
     return nat.RrlAdapterParams(
@@ -44,26 +49,32 @@ def _params(dtype, N, down, up, ids, scales, drop):
         nat.ptr(scales), ctypes.pointer(drop) if drop is not None else None)
 
 
+def _adapt(x, down, up, base, ids, scales, draw):
+    """The result, and the rows' ``down x``."""
+
+    p, seed, offset, at = draw if draw is not None else (0.0, 0, 0, None)
+    dev = nat.require_device(x, down, up, base, ids, scales, at)
+    rows, ld = _rows(x)
+    N = rows.shape[0]
+    flat = None if ids is None else ids.reshape(-1).contiguous()
+    scales = None if scales is None else scales.contiguous()
+    down, up = _factor(down), _factor(up)
+    b, b_ld = (None, 0) if base is None else _rows(base)
+    out = torch.empty(*x.shape[:-1], up.shape[1], dtype=x.dtype, device=dev)
+    t = torch.empty(N, nat.lib().rrl_adapter_rank_padded(down.shape[1]), dtype=torch.float32, device=dev)
+    drop = dropout_params(p, seed, offset, at) if draw is not None else None
+    nat.call_on(dev, "rrl_adapter_fwd", _params(x.dtype, N, down, up, flat, scales, drop), rows.data_ptr(), ld,
+                nat.ptr(b), b_ld, out.data_ptr(), t.data_ptr(), nat.stream_ptr(dev))
+    return out, t
+
+
 class _Adapter(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, down, up, base, ids, scales, draw):
-        p, seed, offset, at = draw if draw is not None else (0.0, 0, 0, None)
-        dev = nat.require_device(x, down, up, base, ids, scales, at)
-        rows, ld = _rows(x)
-        N = rows.shape[0]
-        flat = None if ids is None else ids.reshape(-1).contiguous()
-        scales = None if scales is None else scales.contiguous()
-        down = down if down.stride(2) == 1 or down.shape[2] == 1 else down.contiguous()
-        up = up if up.stride(2) == 1 or up.shape[2] == 1 else up.contiguous()
-        b, b_ld = (None, 0) if base is None else _rows(base)
-        out = torch.empty(*x.shape[:-1], up.shape[1], dtype=x.dtype, device=dev)
-        t = torch.empty(N, nat.lib().rrl_adapter_rank_padded(down.shape[1]), dtype=torch.float32, device=dev)
-        drop = dropout_params(p, seed, offset, at) if draw is not None else None
-        nat.call_on(dev, "rrl_adapter_fwd", _params(x.dtype, N, down, up, flat, scales, drop), rows.data_ptr(), ld,
-                    nat.ptr(b), b_ld, out.data_ptr(), t.data_ptr(), nat.stream_ptr(dev))
+        out, t = _adapt(x, down, up, base, ids, scales, draw)
         ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, down, up, ids, scales,
-                              t if ctx.needs_input_grad[2] else None, at)
-        ctx.args = (x.shape, None if draw is None else (p, seed, offset))
+                              t if ctx.needs_input_grad[2] else None, None if draw is None else draw[3])
+        ctx.args = (x.shape, None if draw is None else draw[:3])
         return out
 
     @staticmethod
@@ -75,6 +86,8 @@ class _Adapter(torch.autograd.Function):
         dx = ddown = dup = None
         if need_x or need_down or need_up:
             dev = g.device
+            down, up = _factor(down), _factor(up)
+            scales = None if scales is None else scales.contiguous()
             rows, ld = _rows(g)
             N = rows.shape[0]
             A, r, H = down.shape
@@ -116,7 +129,8 @@ def adapter_linear(x: Tensor, down: Tensor, up: Tensor, adapter_ids: Optional[Te
     Products are summed in float32, with ``down[a] @ x`` held to 2^-17 or better between
     the two, and the result is rounded once.  x, ``down``, ``up`` and ``base`` have
     gradients, the factors' over all their rows in float32, in an order that the ids and
-    sizes alone decide; they are not differentiable again.
+    sizes alone decide; they are not differentiable again.  An infinity among the operands
+    stays in the sums that it enters, but as a NaN where a product was formed in parts.
     """
 
     if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
@@ -153,4 +167,6 @@ def adapter_linear(x: Tensor, down: Tensor, up: Tensor, adapter_ids: Optional[Te
             raise ValueError("scales have no gradient: detach them")
     dropout_p = float(dropout_p)
     draw = dropout_arguments(dropout_p, seed, offset, generator, "dropout_p") if dropout_p != 0.0 else None
+    if not recorded(x, down, up, base):
+        return _adapt(x, down, up, base, adapter_ids, scales, draw)[0]
     return _Adapter.apply(x, down, up, base, adapter_ids, scales, draw)

@@ -16,6 +16,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from .. import _native as nat
+from .._graph import recorded
 from .._random import dropout_arguments, dropout_params
 
 __all__ = ["dropout"]
@@ -89,4 +90,6 @@ def dropout(x: Tensor, p: float, *, seed: Optional[int] = None, offset: Union[in
         if residual.dtype != x.dtype:
             raise TypeError("residual must have the dtype of x")
     draw = dropout_arguments(p, seed, offset, generator, "p")
+    if not recorded(x, residual):
+        return _drop(x, residual, draw)
     return _Dropout.apply(x, residual, *draw)

@@ -474,3 +474,43 @@ def test_two_threads(device):
     for t in threads:
         t.join()
     assert not bad
+
+
+def test_without_a_graph(device):
+    """A call that nothing differentiates gives the recorded call's bits; forward mode is refused."""
+    gen = torch.Generator().manual_seed(16)
+    for N in (5, 1200):
+        x, base, down, up, ids, _ = (v.to(device) for v in _make(N, 3, 40, 48, 8, torch.float16, gen))
+        kw = dict(base=base, dropout_p=0.2, seed=3)
+        y = adapter_linear(x, down, up, ids, **kw)
+        assert y.grad_fn is None
+        for k in range(3):
+            leaves = [x, down, up]
+            leaves[k] = leaves[k].clone().requires_grad_()
+            z = adapter_linear(*leaves, ids, **kw)
+            assert z.grad_fn is not None and torch.equal(y, z)
+            with torch.no_grad():
+                z = adapter_linear(*leaves, ids, **kw)
+            assert z.grad_fn is None and torch.equal(y, z)
+        z = adapter_linear(x, down, up, ids, base=base.clone().requires_grad_(), dropout_p=0.2, seed=3)
+        assert z.grad_fn is not None and torch.equal(y, z)
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        adapter_linear(fwd.make_dual(x, torch.ones_like(x)), down, up, ids)
+
+
+def test_gradients_of_transposed_factors(device):
+    """Factors that are kept transposed: the gradients are those of their copies."""
+    gen = torch.Generator().manual_seed(17)
+    for dtype in (torch.bfloat16, torch.float32):
+        x, base, down, up, ids, g = (v.to(device) for v in _make(70, 3, 40, 32, 8, dtype, gen))
+        scales = torch.tensor([0.5, 9.0, 2.0, 9.0, 1.5, 9.0], device=device)[::2]
+        turned = [v.transpose(1, 2).contiguous().transpose(1, 2).requires_grad_() for v in (down, up)]
+        plain = [v.clone().requires_grad_() for v in (down, up)]
+        grads = []
+        for d, u in (turned, plain):
+            xr = x.clone().requires_grad_()
+            y = adapter_linear(xr, d, u, ids, base=base, scales=scales, dropout_p=0.1, seed=2)
+            grads.append(torch.autograd.grad(y, [xr, d, u], g))
+        for p, q in zip(*grads):
+            assert torch.equal(p, q)

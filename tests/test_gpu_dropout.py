@@ -189,3 +189,19 @@ def test_after_the_embedding(device):
     dropped = dropout(g, 0.1, seed=7)
     (want,) = torch.autograd.grad(embedding(ids, w, scale=2.0), w, dropped)
     assert torch.equal(dw, want)
+
+
+def test_without_a_graph(device):
+    """A call that nothing differentiates gives the recorded call's bits; forward mode is refused."""
+    x, r = torch.randn(9, 50, device=device), torch.randn(9, 50, device=device)
+    y = dropout(x, 0.3, seed=1, residual=r)
+    assert y.grad_fn is None
+    for a, b in ((x.clone().requires_grad_(), r), (x, r.clone().requires_grad_())):
+        z = dropout(a, 0.3, seed=1, residual=b)
+        assert z.grad_fn is not None and torch.equal(y, z)
+        with torch.no_grad():
+            z = dropout(a, 0.3, seed=1, residual=b)
+        assert z.grad_fn is None and torch.equal(y, z)
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        dropout(fwd.make_dual(x, torch.ones_like(x)), 0.3, seed=1)
