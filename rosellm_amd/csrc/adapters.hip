@@ -298,6 +298,7 @@ struct FusedArgs {
   int64_t N, K, O;
   int r;
   int groups;           // workgroups of a window
+  int in_turn;          // 0: a window's workgroups are neighbours, else the windows, which take turns
   int slabs;            // runs of up's rows that a tile's work is cut into
   int64_t slab;         // their length
   Drop drop;
@@ -305,6 +306,15 @@ struct FusedArgs {
   int nan_rows;         // rows of ids that there are none of: NaN, or zeros
   int stream_x, stream_out;  // x, and base and out, are larger than the memory-side cache
 };
+
+// The window that a workgroup belongs to, and which of the window's it is.  Windows that take
+// turns start each turn one further, so that they do not stay on an XCD.
+__device__ __forceinline__ int group_of(const FusedArgs& a) {
+  return (int)(a.in_turn ? blockIdx.x / a.in_turn : blockIdx.x % a.groups);
+}
+__device__ __forceinline__ int64_t window_of(const FusedArgs& a) {
+  return a.in_turn ? (blockIdx.x + blockIdx.x / a.in_turn) % a.in_turn : blockIdx.x / a.groups;
+}
 
 // The row of up that lane q holds of the i-th of tiles of 16 from column c on: pairs of
 // tiles in an order that leaves eight consecutive columns to a lane of the result.
@@ -338,7 +348,7 @@ struct Window {
   __device__ __forceinline__ Window(const FusedArgs& a, uint16_t* order_, int* scan, int* bins) {
     constexpr int kChunks = kWindow / kAT;
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
-    n0 = (int64_t)(blockIdx.x / a.groups) * kWindow;
+    n0 = window_of(a) * kWindow;
     count = (int)min((int64_t)kWindow, a.N - n0);
     A2 = a.ids.A + 2;
     int* const start_ = bins;                // first place of each adapter, of none and bad, and the end
@@ -513,7 +523,7 @@ __global__ __launch_bounds__(kAT) void adapter_fused_kernel(FusedArgs a) {
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, kb = lane >> 4, q = lane & 15;
   const Window<16> w(a, order, scan, bins);
   const uint64_t at = a.drop_in || a.drop_out ? a.drop.counter() : 0;
-  for (int64_t it = blockIdx.x % a.groups; it < (int64_t)w.all * a.slabs; it += a.groups) {
+  for (int64_t it = group_of(a); it < (int64_t)w.all * a.slabs; it += a.groups) {
     const Window<16>::Tile tile = w.tile((int)(it / a.slabs));
     const int slab = (int)(it % a.slabs);
     const int64_t c0 = slab * a.slab, c1 = min(c0 + a.slab, a.O);
@@ -676,7 +686,7 @@ __global__ __launch_bounds__(kAT) void adapter_shrink_kernel(FusedArgs a) {
   const uint64_t at = a.drop_in ? a.drop.counter() : 0;
   const float drop_scale = a.drop_in ? a.drop.scale : 1.0f;
   const char* const x0 = a.x + w.n0 * a.x_ld * SZ;
-  for (int it = (int)(blockIdx.x % a.groups); it < w.all; it += a.groups) {
+  for (int it = group_of(a); it < w.all; it += a.groups) {
     const Window<64>::Tile tile = w.tile(it);
     if (tile.ad >= a.ids.A || 16 * wv >= tile.here) continue;
     const int64_t n = w.token(tile, 16 * wv + q);
@@ -752,7 +762,7 @@ __global__ __launch_bounds__(kAT, 2) void adapter_expand_kernel(FusedArgs a) {
   const uint64_t at = a.drop_out ? a.drop.counter() : 0;
   const char* const base0 = a.base + w.n0 * a.b_ld * SZ;
   char* const out0 = a.out + w.n0 * a.O * SZ;
-  for (int64_t it = blockIdx.x % a.groups; it < (int64_t)w.all * a.slabs; it += a.groups) {
+  for (int64_t it = group_of(a); it < (int64_t)w.all * a.slabs; it += a.groups) {
     const typename Window<TM>::Tile tile = w.tile((int)(it / a.slabs));
     const int slab = (int)(it % a.slabs);
     const int64_t c0 = slab * a.slab, c1 = min(c0 + a.slab, a.O);
@@ -1085,6 +1095,15 @@ inline int rank_padded(int r) { return r <= 16 ? 16 : (r <= 32 ? 32 : (r <= 64 ?
 //
 // The grid of tiles of TM rows, and with `wide` runs of columns: as many as make two
 // workgroups to each of the 256 CUs, of `least` columns at least.
+//
+// How many tiles a window has its ids decide.  Up to a thousand workgroups each possible one
+// gets its own; beyond that those that find nothing cost more (a window is sorted first) than
+// the rounds of two workgroups to a CU: 16 rows of the LM head 26 -> 19 us, 8192 rows of 16
+// adapters in any order, 1024 to 1024, 24 -> 18; with such rounds always, 8192 rows in runs of
+// 700, 1024 to 4096, 37 -> 44.  Where workgroups may find nothing and a tile is not cut by
+// columns, windows take turns, so that those come last: 32,768 rows of 4 adapters, 1024 to
+// 2048, rank 64, a direction's two kernels 74 -> 57 us on average; with tiles that are cut,
+// the 37 us above would be 47.
 template <int TM>
 int tile_grid(FusedArgs& a, bool wide, int64_t least, dim3& grid) {
   const int64_t windows = (a.N + kWindow - 1) / kWindow;
@@ -1094,7 +1113,9 @@ int tile_grid(FusedArgs& a, bool wide, int64_t least, dim3& grid) {
   const int64_t cuts = wide ? max((int64_t)1, min((a.O + least - 1) / least, 512 / max((int64_t)1, windows * even))) : 1;
   a.slab = wide ? ((a.O + cuts - 1) / cuts + least - 1) / least * least : 1;
   a.slabs = wide ? (int)((a.O + a.slab - 1) / a.slab) : 1;
-  a.groups = (int)max((int64_t)1, min(most * a.slabs, max(even * a.slabs, 2048 / windows)));
+  a.groups = (int)(windows * most * a.slabs <= 1024 ? most * a.slabs
+                                                    : min(most * a.slabs, max(even * a.slabs, 512 / windows)));
+  a.in_turn = a.slabs == 1 && a.groups > even ? (int)windows : 0;
   RRL_REQUIRE(windows * a.groups < ((int64_t)1 << 32) / kAT, RRL_EINVAL, "rrl_adapter: too many rows");
   grid = dim3((uint32_t)(windows * a.groups));
   return RRL_OK;
