@@ -809,6 +809,15 @@ __global__ __launch_bounds__(kPT) void choose_left_kernel(ChooseArgs a) {
 
 // ---- 5 ---------------------------------------------------------------------------------
 
+// The log of an entry's share of a sum that holds it.  From the rest beside it where that is
+// less than half, so that it is 0 where there is none.
+__device__ __forceinline__ float log_share(const Mass& mass, float x, u64 sum, int unit_log2) {
+  const double far = ((double)x - mass.w.m) * mass.w.c;  // log2 of its weight
+  const u64 own = far > -1.0 ? mass(x) : 0;
+  if (own > sum - own) return (float)(0.0 - log1p((double)(sum - own) / (double)own));
+  return fminf((float)(far * 0.69314718055994530942 - log(ldexp((double)sum, -unit_log2))), 0.0f);
+}
+
 template <class Tag>
 __global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
   constexpr int EPV = Pack16<Tag>::EPV;
@@ -837,10 +846,10 @@ __global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
   const u64* const lefts = a.left + b * quarters;
   if (!set.greedy)
     for (int p = p0; p < p1; ++p) left += lefts[p];
-  const double unit = ldexp(1.0, -a.unit_log2);
-  const double norm = log((double)block_reduce<kPW>(whole, sh, Add()) * unit);
+  whole = block_reduce<kPW>(whole, sh, Add());
+  const Mass mass(m, set.c(), a.magic);
   int token = kNoIndex;
-  double logq = 0.0;
+  u64 total = 0;  // of what is left
   auto span = [&](int64_t lo, int64_t n, auto f) {
     sweep<Tag, kPT>(row, lo, min(lo + n, a.V), t, [&](const float (&x)[EPV], int i) {
 #pragma unroll
@@ -855,7 +864,6 @@ __global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
     span((int64_t)first * a.part, a.part, [&](float x, int i) { token = x == m ? min(token, i) : token; });
     token = block_reduce<kPW>(token, shi, Min());
   } else {
-    const Mass mass(m, set.c(), a.magic);
     const Cut cut = set.filtered ? a.cut[b] : set.least(m);
     u64 upto = left;
 #pragma unroll
@@ -866,7 +874,6 @@ __global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
     __syncthreads();
     if (lane == 63) sh[wv] = upto;
     __syncthreads();
-    u64 total = 0;
     for (int k = 0; k < kPW; ++k) {
       if (k < wv) upto += sh[k];
       total += sh[k];
@@ -945,15 +952,15 @@ __global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
       }
       token = block_reduce<kPW>(token, shi, Min());
     }
-    logq = log((double)total * unit);
   }
   if (t == 0) {
     // (there is a token, unless the logits changed meanwhile; then none is read for it)
     const bool some = token >= 0 && token < a.V;
-    const double d = some ? ((double)load_entry<Tag>(row, token) - (double)m) / set.T : M<double>::nan();
+    const float x = some ? load_entry<Tag>(row, token) : m;
     a.token_out[b] = some ? token : -1;
-    a.logp_out[b] = some ? fminf((float)(d - norm), 0.0f) : M<float>::nan();
-    if (a.logq_out) a.logq_out[b] = set.greedy && some ? 0.0f : (some ? fminf((float)(d - logq), 0.0f) : M<float>::nan());
+    a.logp_out[b] = some ? log_share(mass, x, whole, a.unit_log2) : M<float>::nan();
+    if (a.logq_out)
+      a.logq_out[b] = !some ? M<float>::nan() : (set.greedy ? 0.0f : log_share(mass, x, total, a.unit_log2));
   }
 }
 
