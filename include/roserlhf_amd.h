@@ -571,8 +571,8 @@ RRL_API int rrl_dropout(const void* x, int32_t dtype, int64_t rows, int64_t cols
  * (entry (a, o, r) at a * up_sa + o * up_so + r), all `dtype` (F32, BF16 or F16); ids
  * contiguous I32 or I64 (NULL with A = 1: all 0); scales float32 [A] (NULL: 1); dropout
  * (or NULL) of x, as rrl_dropout's.  Ranks up to 128, up to 4096 adapters.  Products are
- * summed in float32; t = down_a drop(x) is float32, taken to 2^-17 by the second product
- * of 16-bit operands; one rounding to `dtype`.
+ * summed in float32; t = down_a drop(x) is float32 between them; one rounding to
+ * `dtype`.
  * t_out: float32 [N, rrl_adapter_rank_padded(r)] (16-byte aligned), t of the rows that
  * have an adapter (the others are not written), also for the gradient of up.
  * rrl_adapter_bwd, of grad = d out [N, O]: dx [N, H], ddown [A, r, H], dup [A, O, r], all

@@ -26,12 +26,11 @@
 // d x is adapter_shrink and adapter_expand on g with the transposes of up and down, which
 // adapter_turn lays out.
 //
-// t is float32.  The second product's bfloat16 instruction takes it as the sum of two
-// bfloat16 numbers, to 2^-17: one rounding to bfloat16 (2^-9) would be as large as that
-// of the result.  With float16 operands, whose range t can leave, up is taken as the
-// exact sum of two bfloat16 numbers as well; the product of the two low parts (2^-18)
-// is left out.  float32 operands take the float32 instruction.  An infinity times a part
-// that is zero is NaN, which is what such a sum may become instead of infinite.
+// t is float32, and stays it: the second product's bfloat16 instruction takes it as the
+// exact sum of three bfloat16 numbers of eight bits each.  With float16 operands, whose
+// range t can leave, up is taken as the exact sum of two as well.  float32 operands take
+// the float32 instruction.  An infinity times a part that is zero is NaN, which is what
+// such a sum may become instead of infinite.
 #include "dropout_common.hpp"
 #include "vocab_weights.hpp"
 
@@ -173,32 +172,36 @@ __device__ __forceinline__ f32x4 mma(const Frag<Tag>& a, const Frag<Tag>& b, f32
   }
 }
 
-// Two numbers as sums of two bfloat16 numbers each.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = f32x2_to_bf16x2_bits(a, b);
-  const float ha = __uint_as_float(hi << 16), hb = __uint_as_float(hi & 0xffff0000u);
-  // (an infinity leaves no rest)
-  lo = f32x2_to_bf16x2_bits(a == ha ? 0.0f : a - ha, b == hb ? 0.0f : b - hb);
+// The upper halves of two numbers, cut off: bfloat16 numbers of their first eight bits, and
+// what is left of them.  (Rounded, the largest would overflow.  An infinity leaves no rest.)
+__device__ __forceinline__ uint32_t cut2(float& a, float& b) {
+  const uint32_t bits = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  const float ha = __uint_as_float(bits << 16), hb = __uint_as_float(bits & 0xffff0000u);
+  a = a == ha ? 0.0f : a - ha;
+  b = b == hb ? 0.0f : b - hb;
+  return bits;
 }
-__device__ __forceinline__ void split8(const float (&x)[8], u32x4& hi, u32x4& lo) {
+// Eight numbers as exact sums of bfloat16 numbers: of N, which hold 8 N bits.
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&part)[N]) {
 #pragma unroll
   for (int d = 0; d < 4; ++d) {
-    uint32_t h, l;
-    split2(x[2 * d], x[2 * d + 1], h, l);
-    hi[d] = h;
-    lo[d] = l;
+    float a = x[2 * d], b = x[2 * d + 1];
+#pragma unroll
+    for (int k = 0; k < N; ++k) part[k][d] = cut2(a, b);
   }
 }
 
 // The second product: rows of up against t, depth R = 16 R16.  16-bit operands take 32
-// entries of depth at once: ranks up to 16 hold t's high parts in the first half of them
-// and its low parts in the second, beside up's entries twice.
+// entries of depth at once: ranks up to 16 hold t's first parts in the first half of them
+// and its second parts in the second, beside up's entries twice; then its last parts,
+// beside both parts of a float16 up.
 template <class Tag, int R16>
 struct Thin {  // t of 16 tokens
   static constexpr bool F32 = std::is_same_v<Tag, TagF32>, F16 = std::is_same_v<Tag, TagF16>;
   static constexpr int KS = R16 == 1 ? 1 : R16 / 2;
   static constexpr int NF = F32 ? 4 * R16 : 0;
-  u32x4 hi[F32 ? 1 : KS], lo[F32 ? 1 : KS];
+  u32x4 part[F32 ? 1 : KS][3];
   float f[F32 ? NF : 1];
   __device__ __forceinline__ void load(const float* t, int kb) {
     if constexpr (F32) {
@@ -211,11 +214,11 @@ struct Thin {  // t of 16 tokens
         float x[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] = t[at + k];
-        split8(x, hi[s], lo[s]);
+        split8(x, part[s]);
         if constexpr (R16 == 1) {
-          const u32x4 h = hi[0], l = lo[0], none = {0, 0, 0, 0};
-          hi[0] = kb < 2 ? h : l;
-          lo[0] = kb < 2 ? h : none;  // beside up's low parts
+          const u32x4 none = {0, 0, 0, 0};
+          part[0][0] = kb < 2 ? part[0][0] : part[0][1];
+          if constexpr (!F16) part[0][2] = kb < 2 ? part[0][2] : none;
         }
       }
     }
@@ -258,19 +261,24 @@ __device__ __forceinline__ f32x4 expand(const UpRow<Tag, R16>& u, const Thin<Tag
     for (int s = 0; s < T::KS; ++s) {
       if constexpr (T::F16) {
         float x[8];
-        u32x4 hi, lo;
+        u32x4 up[2];
         u.v[s].unpack(x);
-        split8(x, hi, lo);
-        c = mma_bf16(hi, t.hi[s], c);
+        split8(x, up);
+        c = mma_bf16(up[0], t.part[s][0], c);
+        c = mma_bf16(up[1], t.part[s][0], c);
         if constexpr (R16 > 1) {
-          c = mma_bf16(hi, t.lo[s], c);
-          c = mma_bf16(lo, t.hi[s], c);
+#pragma unroll
+          for (int k = 1; k < 3; ++k) {
+            c = mma_bf16(up[0], t.part[s][k], c);
+            c = mma_bf16(up[1], t.part[s][k], c);
+          }
         } else {
-          c = mma_bf16(lo, t.lo[s], c);
+          c = mma_bf16((threadIdx.x & 63) < 32 ? up[0] : up[1], t.part[s][2], c);
         }
       } else {
-        c = mma_bf16(u.v[s].v[0], t.hi[s], c);
-        if constexpr (R16 > 1) c = mma_bf16(u.v[s].v[0], t.lo[s], c);
+        c = mma_bf16(u.v[s].v[0], t.part[s][0], c);
+        if constexpr (R16 > 1) c = mma_bf16(u.v[s].v[0], t.part[s][1], c);
+        c = mma_bf16(u.v[s].v[0], t.part[s][2], c);
       }
     }
   }
@@ -793,8 +801,11 @@ __global__ __launch_bounds__(kAT, 2) void adapter_expand_kernel(FusedArgs a) {
         if (chunk + kAW < chunks) in.load(base0, a.b_ld, rows, c + kAW * S::kCols, c1, a.stream_out);
       }
       wave_fence();
-      // tiles of up's rows at once: with 16 rows of t, as many as 64 registers hold
-      constexpr int kMost = TM > 16 ? 4 : (std::is_same_v<Tag, TagF32> || R16 > 2 ? 32 / R16 : 16);
+      // tiles of up's rows at once: with 16 rows of t, as many as 64 registers hold; with more
+      // rows of a t of over 32 ranks in parts, two (four spill: 32,768 rows, 1024 to 2048, rank
+      // 128, float16, both directions 1135 us instead of 1045)
+      constexpr bool F32 = std::is_same_v<Tag, TagF32>;
+      constexpr int kMost = TM > 16 ? (!F32 && R16 > 2 ? 2 : 4) : (F32 || R16 > 2 ? 32 / R16 : 16);
       constexpr int NC = S::kCols / 16 < kMost ? S::kCols / 16 : kMost;
 #pragma unroll 1
       for (int i0 = 0; i0 < S::kCols / 16; i0 += NC) {
@@ -955,37 +966,37 @@ __global__ __launch_bounds__(kAT, RT <= 2 ? 3 : 2) void adapter_outer_kernel(Out
               acc[c][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(in.x[i].v[c / 4][c % 4]), in.th[i][e],
                                                                acc[c][e], 0, 0, 0);
       } else {
-        u32x4 hi[RT], lo[RT];
+        u32x4 thin[RT][3];
 #pragma unroll
         for (int e = 0; e < RT; ++e) {
           float v[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[i] = in.th[i][e];
-          split8(v, hi[e], lo[e]);
+          split8(v, thin[e]);
         }
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          u32x4 wide, rest;
+          u32x4 wide[F16 ? 2 : 1];
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
             // column c of tokens 2d and 2d + 1
             const uint32_t two = __builtin_amdgcn_perm(in.x[2 * d + 1].v[0][c / 2], in.x[2 * d].v[0][c / 2],
                                                        c % 2 ? 0x07060302u : 0x05040100u);
             if constexpr (F16) {
-              uint32_t h, l;
-              split2(f16_bits_to_f32((uint16_t)two), f16_bits_to_f32((uint16_t)(two >> 16)), h, l);
-              wide[d] = h;
-              rest[d] = l;
+              float p = f16_bits_to_f32((uint16_t)two), q = f16_bits_to_f32((uint16_t)(two >> 16));
+              wide[0][d] = cut2(p, q);
+              wide[1][d] = cut2(p, q);
             } else {
-              wide[d] = two;
+              wide[0][d] = two;
             }
           }
 #pragma unroll
-          for (int e = 0; e < RT; ++e) {
-            acc[c][e] = mma_bf16(wide, hi[e], acc[c][e]);
-            acc[c][e] = mma_bf16(wide, lo[e], acc[c][e]);
-            if constexpr (F16) acc[c][e] = mma_bf16(rest, hi[e], acc[c][e]);
-          }
+          for (int e = 0; e < RT; ++e)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+              acc[c][e] = mma_bf16(wide[0], thin[e][k], acc[c][e]);
+              if constexpr (F16) acc[c][e] = mma_bf16(wide[1], thin[e][k], acc[c][e]);
+            }
         }
       }
     }

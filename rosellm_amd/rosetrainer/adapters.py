@@ -126,11 +126,11 @@ def adapter_linear(x: Tensor, down: Tensor, up: Tensor, adapter_ids: Optional[Te
 
     ``dropout_p``, ``seed``, ``offset`` and ``generator`` are ``dropout``'s: x is dropped
     out within the product, as ``dropout(x, dropout_p, ...)`` of the same arguments would.
-    Products are summed in float32, with ``down[a] @ x`` held to 2^-17 or better between
-    the two, and the result is rounded once.  x, ``down``, ``up`` and ``base`` have
-    gradients, the factors' over all their rows in float32, in an order that the ids and
-    sizes alone decide; they are not differentiable again.  An infinity among the operands
-    stays in the sums that it enters, but as a NaN where a product was formed in parts.
+    Products are summed in float32, ``down[a] @ x`` is float32 between the two, and the
+    result is rounded once.  x, ``down``, ``up`` and ``base`` have gradients, the factors'
+    over all their rows in float32, in an order that the ids and sizes alone decide; they
+    are not differentiable again.  An infinity among the operands stays in the sums that
+    it enters, but as a NaN where a product was formed in parts.
     """
 
     if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
