@@ -56,7 +56,7 @@ def sample_tokens(
     distribution that was drawn from (0 where greedy).  The call does not wait for the
     device, so a row that has no distribution (a NaN or +inf among its logits or as its
     temperature, or nothing above -inf) cannot raise: its token is -1 and its log-probs
-    are NaN.
+    are NaN.  It cannot be traced by ``torch.jit.trace``; a graph captures it.
     """
 
     if logits.dim() != 2:
@@ -84,6 +84,8 @@ def sample_tokens(
         if value.dtype not in dtypes:
             raise TypeError(f"{name} must be " + " or ".join(str(d)[6:] for d in dtypes))
         rows[name] = value
+    if torch.jit.is_tracing():
+        raise RuntimeError("sample_tokens cannot be traced: a trace would not hold the kernels that write its results")
     dev = nat.require_device(logits, uniforms, *rows.values())
 
     x = logits if logits.stride(1) == 1 or V == 1 else logits.contiguous()

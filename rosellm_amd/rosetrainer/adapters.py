@@ -49,10 +49,9 @@ def _params(dtype, N, down, up, ids, scales, drop):
         nat.ptr(scales), ctypes.pointer(drop) if drop is not None else None)
 
 
-def _adapt(x, down, up, base, ids, scales, draw):
+def _adapt(x, down, up, base, ids, scales, at, draw):
     """The result, and the rows' ``down x``."""
 
-    p, seed, offset, at = draw if draw is not None else (0.0, 0, 0, None)
     dev = nat.require_device(x, down, up, base, ids, scales, at)
     rows, ld = _rows(x)
     N = rows.shape[0]
@@ -62,7 +61,7 @@ def _adapt(x, down, up, base, ids, scales, draw):
     b, b_ld = (None, 0) if base is None else _rows(base)
     out = torch.empty(*x.shape[:-1], up.shape[1], dtype=x.dtype, device=dev)
     t = torch.empty(N, nat.lib().rrl_adapter_rank_padded(down.shape[1]), dtype=torch.float32, device=dev)
-    drop = dropout_params(p, seed, offset, at) if draw is not None else None
+    drop = dropout_params(*draw, at) if draw is not None else None
     nat.call_on(dev, "rrl_adapter_fwd", _params(x.dtype, N, down, up, flat, scales, drop), rows.data_ptr(), ld,
                 nat.ptr(b), b_ld, out.data_ptr(), t.data_ptr(), nat.stream_ptr(dev))
     return out, t
@@ -70,11 +69,11 @@ def _adapt(x, down, up, base, ids, scales, draw):
 
 class _Adapter(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, down, up, base, ids, scales, draw):
-        out, t = _adapt(x, down, up, base, ids, scales, draw)
+    def forward(ctx, x, down, up, base, ids, scales, at, draw):
+        out, t = _adapt(x, down, up, base, ids, scales, at, draw)
         ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, down, up, ids, scales,
-                              t if ctx.needs_input_grad[2] else None, None if draw is None else draw[3])
-        ctx.args = (x.shape, None if draw is None else draw[:3])
+                              t if ctx.needs_input_grad[2] else None, at)
+        ctx.args = (x.shape, draw)
         return out
 
     @staticmethod
@@ -105,7 +104,7 @@ class _Adapter(torch.autograd.Function):
             nat.call_on(dev, "rrl_adapter_bwd", _params(g.dtype, N, down, up, flat, scales, drop), nat.ptr(xr), x_ld,
                         rows.data_ptr(), ld, nat.ptr(t), nat.ptr(dx), nat.ptr(ddown), nat.ptr(dup), ws.data_ptr(),
                         nat.stream_ptr(dev))
-        return dx, ddown, dup, (g if need_base else None), None, None, None
+        return dx, ddown, dup, (g if need_base else None), None, None, None, None
 
 
 def adapter_linear(x: Tensor, down: Tensor, up: Tensor, adapter_ids: Optional[Tensor] = None, *,
@@ -166,7 +165,9 @@ def adapter_linear(x: Tensor, down: Tensor, up: Tensor, adapter_ids: Optional[Te
         if scales.requires_grad:
             raise ValueError("scales have no gradient: detach them")
     dropout_p = float(dropout_p)
-    draw = dropout_arguments(dropout_p, seed, offset, generator, "dropout_p") if dropout_p != 0.0 else None
+    draw = at = None
+    if dropout_p != 0.0:
+        *draw, at = dropout_arguments(dropout_p, seed, offset, generator, "dropout_p")
     if not recorded(x, down, up, base):
-        return _adapt(x, down, up, base, adapter_ids, scales, draw)[0]
-    return _Adapter.apply(x, down, up, base, adapter_ids, scales, draw)
+        return _adapt(x, down, up, base, adapter_ids, scales, at, draw)[0]
+    return _Adapter.apply(x, down, up, base, adapter_ids, scales, at, draw)
