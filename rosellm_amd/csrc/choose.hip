@@ -14,8 +14,11 @@
 // A cut and a token are decided by where a running sum passes a border, so weights are
 // formed in float64 (1.1e-12) and added as integers, in units of 2^-44 of the largest
 // one (2^-(62 - b) for rows of 2^b > 2^18 entries): integer sums are the same in any
-// order, so that LDS atomics may form them, and off by 2^-45 an entry, 1e-11 of the
-// whole for 150,000 entries.
+// order, so that LDS atomics may form them.  An entry is off by up to half a unit, and
+// entries below that count as none, so that a sum may be off by 2^-45 V of the largest
+// weight (a border by 4.3e-9 for 150,000 entries that all are rounded the same way, 1e-11 where
+// they are not); an error that a log-prob next to 0 would show.  Log-probs are formed from
+// sums of the same weights in float64, which are the same in any order of a row's chunks too.
 //
 // What is left is always the entries above a place (x, v) in descending order.  Rows are
 // cut into parts, a workgroup each, so that a single row fills the chip, and read once a
@@ -73,8 +76,10 @@ struct ChooseArgs {
   double magic;     // 2^(52 - F): a weight added to it stands in the low bits, in units of 2^-F
   int unit_log2;    // F
   float* peak;      // [B, parts] a part's maximum; +inf: it holds NaN or +inf
-  u64* whole;       // [B, parts] sum of all entries
+  u64* whole;       // [B, parts] sum of all entries, where there is a top-p and no top-k
   u64* left;        // [B, parts, kPW] of those that are left, a wave's run of a part each
+  struct Exact* all;   // [B, parts, kPW] the same two sums for log-probs; kept only where
+  struct Exact* kept;  // a setting leaves out entries
   u64* sums;        // [B, parts, kBins], where there may be a top-p
   uint32_t* counts; // [B, parts, kBins], where there may be a top-k
   Cut* cut;         // [B], where there may be either
@@ -208,22 +213,46 @@ struct Mass {
   u64 zero;  // the bits of magic
   __device__ __forceinline__ Mass(float m, double c, double magic_)
       : w(m, c, 1.0), magic(magic_), zero((u64)__double_as_longlong(magic_)) {}
+  // of w.unscaled(x)
   template <bool DIRECT>
-  __device__ __forceinline__ u64 of(float x) const {
-    const double v = DIRECT ? fma(w.template unscaled<DIRECT>(x), w.k, magic) : w.template unscaled<DIRECT>(x) + magic;
-    return (u64)__double_as_longlong(v) - zero;
+  __device__ __forceinline__ u64 of(double v) const {
+    return (u64)__double_as_longlong(DIRECT ? fma(v, w.k, magic) : v + magic) - zero;
   }
-  __device__ __forceinline__ u64 operator()(float x) const { return w.direct ? of<true>(x) : of<false>(x); }
+  __device__ __forceinline__ u64 operator()(float x) const {
+    return w.direct ? of<true>(w.unscaled<true>(x)) : of<false>(w.unscaled<false>(x));
+  }
+};
+
+// A sum of weights in units of 2^-90 of the largest, as two integers.
+struct Exact {
+  u64 coarse = 0, fine = 0;  // units of 2^-40; of 2^-90, signed
+  // A chunk's sum, of at most 2^11 weights.  Its last bits are those of a 64-bit number of
+  // its size, and nothing else is rounded: the order of the chunks changes nothing.
+  __device__ __forceinline__ void add(double s) {
+#pragma clang fp contract(off)  // s is a rounded product, as log_share's
+    const double near = s + 0x1p12, rest = s - (near - 0x1p12);  // |rest| <= 2^-41
+    coarse += (u64)__double_as_longlong(near) - (u64)__double_as_longlong(0x1p12);
+    fine += (u64)__double_as_longlong(rest + 0x1.8p-38) - (u64)__double_as_longlong(0x1.8p-38);
+  }
+  __device__ __forceinline__ double value() const {
+    return fma((double)(int64_t)fine, 0x1p-90, (double)coarse * 0x1p-40);
+  }
 };
 
 // f(values, index of the first) for the 16-byte vectors of entries lo..hi-1 of a row, by
-// NT threads of which this is the t-th; past the end of them -inf.
-template <class Tag, int NT, class F>
-__device__ __forceinline__ void sweep(const char* row, int64_t lo, int64_t hi, int t, F f) {
+// NT threads of which this is the t-th; past the end of them -inf.  done() after each chunk
+// of kAhead vectors a thread, by all of them.
+struct Nothing {
+  __device__ __forceinline__ void operator()() const {}
+};
+template <class Tag, int NT, class F, class D = Nothing>
+__device__ __forceinline__ void sweep(const char* row, int64_t lo, int64_t hi, int t, F f, D done = D()) {
   constexpr int EPV = Pack16<Tag>::EPV, SZ = 16 / EPV;
-  for (int64_t i0 = lo + t * EPV; i0 < hi; i0 += kAhead * NT * EPV) {
+  static_assert(kAhead * 64 * EPV <= 2048, "a chunk of a wave is one of Exact's");
+  for (int64_t base = lo; base < hi; base += kAhead * NT * EPV) {
+    const int64_t i0 = base + t * EPV;
     u32x4 raw[kAhead];
-    if (i0 + (int64_t)((kAhead - 1) * NT + 1) * EPV <= hi) {
+    if (base + kAhead * NT * EPV <= hi) {
 #pragma unroll
       for (int s = 0; s < kAhead; ++s)
         raw[s] = reinterpret_cast<const Any16*>(row + (i0 + s * NT * EPV) * SZ)->v;
@@ -241,13 +270,14 @@ __device__ __forceinline__ void sweep(const char* row, int64_t lo, int64_t hi, i
       Pack16<Tag>::unpack(raw[s], x);
       f(x, (int)(i0 + s * NT * EPV));
     }
+    done();
   }
 }
-// The same by a wave over its quarter of a part.
-template <class Tag, class F>
-__device__ __forceinline__ void sweep_part(const ChooseArgs& a, const char* row, int64_t part, F f) {
+// The same by a wave over its quarter of a part, which starts with a chunk.
+template <class Tag, class F, class D = Nothing>
+__device__ __forceinline__ void sweep_part(const ChooseArgs& a, const char* row, int64_t part, F f, D done = D()) {
   const int64_t lo = part * a.part + (threadIdx.x >> 6) * (a.part / kPW);
-  sweep<Tag, 64>(row, lo, min(lo + a.part / kPW, a.V), threadIdx.x & 63, f);
+  sweep<Tag, 64>(row, lo, min(lo + a.part / kPW, a.V), threadIdx.x & 63, f, done);
 }
 template <class Tag>
 __device__ __forceinline__ const char* row_at(const ChooseArgs& a, int64_t b) {
@@ -337,29 +367,36 @@ __device__ __forceinline__ int top_bin(const ChooseArgs& a, const Settings& set,
   return sh.bin;
 }
 
+// whole and left are this thread's, all and kept the wave's.
 template <class Tag, bool DIRECT>
 __device__ __forceinline__ void weigh(const ChooseArgs& a, const Settings& set, const Mass& mass, float m, int64_t b,
-                                      int64_t part, float reach, WeighShared& sh, u64& whole, u64& left) {
+                                      int64_t part, float reach, WeighShared& sh, u64& whole, u64& left, Exact& all,
+                                      Exact& kept) {
   constexpr int EPV = Pack16<Tag>::EPV;
   const char* row = row_at<Tag>(a, b);
   const float scale = set.scale();
+  double sum = 0.0, some = 0.0;
+  auto add = [&] {
+    all.add(wave_sum_d(sum) * mass.w.template factor<DIRECT>());
+    sum = 0.0;
+  };
   if (set.filtered && set.top_k > 0) {
     sweep_part<Tag>(a, row, part, [&](const float (&x)[EPV], int i) {
 #pragma unroll
       for (int k = 0; k < EPV; ++k) {
-        const u64 w = mass.of<DIRECT>(x[k]);
-        whole += w;
+        const double v = mass.w.template unscaled<DIRECT>(x[k]);
+        sum += v;
         if (x[k] >= reach) {
           const int bin = bin_of(x[k], m, scale), at = atomicAdd(&sh.listed, 1);
           atomicAdd(&sh.counts[bin], 1u);
-          if (set.top_p > 0.0) atomicAdd(&sh.sums[bin], w);
+          if (set.top_p > 0.0) atomicAdd(&sh.sums[bin], mass.of<DIRECT>(v));
           if (at < kPartListed) {
             sh.list_x[at] = x[k];
             sh.list_i[at] = i + k;
           }
         }
       }
-    });
+    }, add);
   } else if (set.filtered) {
     // Entries of at most (1 - top_p) / V of the largest make up no more than 1 - top_p of
     // the whole, so that the border lies above them.
@@ -367,27 +404,38 @@ __device__ __forceinline__ void weigh(const ChooseArgs& a, const Settings& set, 
     sweep_part<Tag>(a, row, part, [&](const float (&x)[EPV], int) {
 #pragma unroll
       for (int k = 0; k < EPV; ++k) {
-        const u64 w = mass.of<DIRECT>(x[k]);
+        const double v = mass.w.template unscaled<DIRECT>(x[k]);
+        const u64 w = mass.of<DIRECT>(v);
+        sum += v;
         whole += w;
         if (w > floor) atomicAdd(&sh.sums[bin_of(x[k], m, scale)], w);
       }
-    });
+    }, add);
   } else if (set.min_p > 0.0) {
     const Cut cut = set.least(m);
     sweep_part<Tag>(a, row, part, [&](const float (&x)[EPV], int) {
 #pragma unroll
       for (int k = 0; k < EPV; ++k) {
-        const u64 w = mass.of<DIRECT>(x[k]);
-        whole += w;
-        left += x[k] >= cut.v ? w : 0;
+        const double v = mass.w.template unscaled<DIRECT>(x[k]);
+        const bool in = x[k] >= cut.v;
+        sum += v;
+        some += in ? v : 0.0;
+        left += in ? mass.of<DIRECT>(v) : 0;
       }
+    }, [&] {
+      add();
+      kept.add(wave_sum_d(some) * mass.w.template factor<DIRECT>());
+      some = 0.0;
     });
   } else {
     sweep_part<Tag>(a, row, part, [&](const float (&x)[EPV], int) {
 #pragma unroll
-      for (int k = 0; k < EPV; ++k) whole += mass.of<DIRECT>(x[k]);
-    });
-    left = whole;
+      for (int k = 0; k < EPV; ++k) {
+        const double v = mass.w.template unscaled<DIRECT>(x[k]);
+        sum += v;
+        left += mass.of<DIRECT>(v);
+      }
+    }, add);
   }
 }
 __device__ __forceinline__ u64 wave_total(u64 v) {
@@ -416,11 +464,14 @@ __global__ __launch_bounds__(kPT) void choose_weigh_kernel(ChooseArgs a) {
   }
   const Mass mass(m, set.c(), a.magic);
   u64 whole = 0, left = 0;
-  if (mass.w.direct) weigh<Tag, true>(a, set, mass, m, b, part, reach, sh, whole, left);
-  else weigh<Tag, false>(a, set, mass, m, b, part, reach, sh, whole, left);
-  whole = block_reduce<kPW>(whole, sh.wave, Add());
-  if (t == 0) a.whole[blockIdx.x] = whole;
+  Exact all, kept;
+  if (mass.w.direct) weigh<Tag, true>(a, set, mass, m, b, part, reach, sh, whole, left, all, kept);
+  else weigh<Tag, false>(a, set, mass, m, b, part, reach, sh, whole, left, all, kept);
+  const int64_t wave = (int64_t)blockIdx.x * kPW + (t >> 6);
+  if ((t & 63) == 0) a.all[wave] = all;
   if (set.filtered) {
+    whole = block_reduce<kPW>(whole, sh.wave, Add());
+    if (t == 0) a.whole[blockIdx.x] = whole;
     const int64_t to = (int64_t)blockIdx.x * kBins;
     if (set.top_p > 0.0)
       for (int k = t; k < kBins; k += kPT) a.sums[to + k] = sh.sums[k];
@@ -437,7 +488,10 @@ __global__ __launch_bounds__(kPT) void choose_weigh_kernel(ChooseArgs a) {
     }
   } else {
     left = wave_total(left);
-    if ((t & 63) == 0) a.left[blockIdx.x * kPW + (t >> 6)] = left;
+    if ((t & 63) == 0) {
+      a.left[wave] = left;
+      if (set.min_p > 0.0) a.kept[wave] = kept;
+    }
   }
 }
 
@@ -738,7 +792,7 @@ __global__ __launch_bounds__(kRT) void choose_cut_kernel(ChooseArgs a) {
 // with most of them has.  Where some lane has over a quarter, all are weighed in place.
 template <class Tag, bool DIRECT>
 __device__ __forceinline__ u64 weigh_left(const ChooseArgs& a, const char* row, int64_t part, const Cut& cut,
-                                          const Mass& mass) {
+                                          const Mass& mass, Exact& kept) {
   constexpr int EPV = Pack16<Tag>::EPV;
   u64 left = 0;
   const int64_t quarter = a.part / kPW, lo = part * a.part + (threadIdx.x >> 6) * quarter;
@@ -767,23 +821,33 @@ __device__ __forceinline__ u64 weigh_left(const ChooseArgs& a, const char* row, 
       for (int k = 0; k < EPV; ++k)
         marks |= (cut.keeps(x[k], (int)(i0 + (s * 64 + lane) * EPV) + k) ? 1u : 0u) << (s * EPV + k);
     }
+    if (!__any(marks != 0)) continue;
+    double sum = 0.0;  // in the same order either way
     if (__any(__popc(marks) > kAhead * EPV / 4)) {
 #pragma unroll
       for (int s = 0; s < kAhead; ++s) {
         float x[EPV];
         Pack16<Tag>::unpack(raw[s], x);
 #pragma unroll
-        for (int k = 0; k < EPV; ++k) left += marks >> (s * EPV + k) & 1 ? mass.of<DIRECT>(x[k]) : 0;
+        for (int k = 0; k < EPV; ++k) {
+          const double v = marks >> (s * EPV + k) & 1 ? mass.w.template unscaled<DIRECT>(x[k]) : 0.0;
+          sum += v;
+          left += mass.of<DIRECT>(v);
+        }
       }
     } else {
       while (__any(marks != 0)) {
         if (marks) {
           const int k = __ffs((int)marks) - 1;
           marks &= marks - 1;
-          left += mass.of<DIRECT>(load_entry<Tag>(row, i0 + (k / EPV * 64 + lane) * EPV + k % EPV));
+          const double v =
+              mass.w.template unscaled<DIRECT>(load_entry<Tag>(row, i0 + (k / EPV * 64 + lane) * EPV + k % EPV));
+          sum += v;
+          left += mass.of<DIRECT>(v);
         }
       }
     }
+    kept.add(wave_sum_d(sum) * mass.w.template factor<DIRECT>());
   }
   return left;
 }
@@ -798,24 +862,30 @@ __global__ __launch_bounds__(kPT) void choose_left_kernel(ChooseArgs a) {
   if (!(m < M<float>::inf())) return;
   const Cut cut = a.cut[b];
   u64 left = 0;
+  Exact kept;
   if (a.peak[blockIdx.x] >= cut.v) {
     const Mass mass(m, set.c(), a.magic);
     const char* row = row_at<Tag>(a, b);
-    left = mass.w.direct ? weigh_left<Tag, true>(a, row, part, cut, mass) : weigh_left<Tag, false>(a, row, part, cut, mass);
+    left = mass.w.direct ? weigh_left<Tag, true>(a, row, part, cut, mass, kept)
+                         : weigh_left<Tag, false>(a, row, part, cut, mass, kept);
     left = wave_total(left);
   }
-  if ((threadIdx.x & 63) == 0) a.left[blockIdx.x * kPW + (threadIdx.x >> 6)] = left;
+  if ((threadIdx.x & 63) == 0) {
+    const int64_t wave = (int64_t)blockIdx.x * kPW + (threadIdx.x >> 6);
+    a.left[wave] = left;
+    a.kept[wave] = kept;
+  }
 }
 
 // ---- 5 ---------------------------------------------------------------------------------
 
 // The log of an entry's share of a sum that holds it.  From the rest beside it where that is
 // less than half, so that it is 0 where there is none.
-__device__ __forceinline__ float log_share(const Mass& mass, float x, u64 sum, int unit_log2) {
-  const double far = ((double)x - mass.w.m) * mass.w.c;  // log2 of its weight
-  const u64 own = far > -1.0 ? mass(x) : 0;
-  if (own > sum - own) return (float)(0.0 - log1p((double)(sum - own) / (double)own));
-  return fminf((float)(far * 0.69314718055994530942 - log(ldexp((double)sum, -unit_log2))), 0.0f);
+__device__ __forceinline__ float log_share(const Weight& w, float x, double sum) {
+#pragma clang fp contract(off)
+  const double own = w.one(x);
+  if (own > sum - own) return fminf((float)(0.0 - log1p((sum - own) / own)), 0.0f);
+  return fminf((float)(((double)x - w.m) * w.c * 0.69314718055994530942 - log(sum)), 0.0f);
 }
 
 template <class Tag>
@@ -838,18 +908,30 @@ __global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
     }
     return;
   }
-  u64 whole = 0, left = 0;
-  for (int p = t; p < a.parts; p += kPT) whole += a.whole[b * a.parts + p];
+  u64 left = 0;
   // sums of what is left in their order, a run of quarters to a thread
   const int quarters = a.parts * kPW, run = (quarters + kPT - 1) / kPT;
   const int p0 = min(t * run, quarters), p1 = min(p0 + run, quarters);
   const u64* const lefts = a.left + b * quarters;
   if (!set.greedy)
     for (int p = p0; p < p1; ++p) left += lefts[p];
-  whole = block_reduce<kPW>(whole, sh, Add());
+  double all = 0.0, kept = 0.0;  // the first wave's: for log-probs
+  if (wv == 0) {
+    auto row_sum = [&](const Exact* sums) {
+      Exact s;
+      for (int p = lane; p < quarters; p += 64) {
+        s.coarse += sums[b * quarters + p].coarse;
+        s.fine += sums[b * quarters + p].fine;
+      }
+      s.coarse = wave_total(s.coarse);
+      s.fine = wave_total(s.fine);
+      return s.value();
+    };
+    all = row_sum(a.all);
+    kept = set.filtered || (!set.greedy && set.min_p > 0.0) ? row_sum(a.kept) : all;
+  }
   const Mass mass(m, set.c(), a.magic);
   int token = kNoIndex;
-  u64 total = 0;  // of what is left
   auto span = [&](int64_t lo, int64_t n, auto f) {
     sweep<Tag, kPT>(row, lo, min(lo + n, a.V), t, [&](const float (&x)[EPV], int i) {
 #pragma unroll
@@ -874,6 +956,7 @@ __global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
     __syncthreads();
     if (lane == 63) sh[wv] = upto;
     __syncthreads();
+    u64 total = 0;
     for (int k = 0; k < kPW; ++k) {
       if (k < wv) upto += sh[k];
       total += sh[k];
@@ -958,9 +1041,8 @@ __global__ __launch_bounds__(kPT) void choose_draw_kernel(ChooseArgs a) {
     const bool some = token >= 0 && token < a.V;
     const float x = some ? load_entry<Tag>(row, token) : m;
     a.token_out[b] = some ? token : -1;
-    a.logp_out[b] = some ? log_share(mass, x, whole, a.unit_log2) : M<float>::nan();
-    if (a.logq_out)
-      a.logq_out[b] = !some ? M<float>::nan() : (set.greedy ? 0.0f : log_share(mass, x, total, a.unit_log2));
+    a.logp_out[b] = some ? log_share(mass.w, x, all) : M<float>::nan();
+    if (a.logq_out) a.logq_out[b] = !some ? M<float>::nan() : (set.greedy ? 0.0f : log_share(mass.w, x, kept));
   }
 }
 
@@ -976,7 +1058,7 @@ inline int part_entries(int64_t B, int64_t V) {
 struct ChooseLayout {
   int part;
   int64_t parts;
-  size_t peak, whole, left, sums, counts, cut, tops, reach, list_x, list_i, listed, total;
+  size_t peak, whole, left, all, kept, sums, counts, cut, tops, reach, list_x, list_i, listed, total;
 };
 inline ChooseLayout choose_layout(int64_t B, int64_t V, bool top_k, bool top_p) {
   ChooseLayout l;
@@ -992,6 +1074,8 @@ inline ChooseLayout choose_layout(int64_t B, int64_t V, bool top_k, bool top_p) 
   l.peak = take(4 * n);
   l.whole = take(8 * n);
   l.left = take(8 * n * kPW);
+  l.all = take(sizeof(Exact) * n * kPW);
+  l.kept = take(sizeof(Exact) * n * kPW);
   l.sums = take(top_p ? 8 * n * kBins : 0);
   l.counts = take(top_k ? 4 * n * kBins : 0);
   l.cut = take(sizeof(Cut) * (size_t)B);
@@ -1088,6 +1172,8 @@ extern "C" int rrl_sample_tokens(const void* logits, int32_t dtype, int64_t B, i
   a.peak = reinterpret_cast<float*>(w + l.peak);
   a.whole = reinterpret_cast<u64*>(w + l.whole);
   a.left = reinterpret_cast<u64*>(w + l.left);
+  a.all = reinterpret_cast<Exact*>(w + l.all);
+  a.kept = reinterpret_cast<Exact*>(w + l.kept);
   a.sums = reinterpret_cast<u64*>(w + l.sums);
   a.counts = reinterpret_cast<uint32_t*>(w + l.counts);
   a.cut = reinterpret_cast<Cut*>(w + l.cut);

@@ -73,9 +73,10 @@ def dropout(x: Tensor, p: float, *, seed: Optional[int] = None, offset: Union[in
     whatever the strides, and the gradient draws the forward's mask again.  Give each
     call of a step a seed or an offset of its own.  With ``seed=None`` a seed is drawn
     from ``generator`` (a CPU ``torch.Generator``, default: torch's global one), on the
-    host: a captured graph replays it, and a trace keeps it.  For another mask at each replay, ``offset`` can
-    be an int64 tensor of one element on x's device, which the kernel reads; it must
-    stay as it was until the backward has run (changing it in place before raises there).
+    host: a captured graph replays it, and a trace keeps it.  For another mask at each
+    replay, ``offset`` can be an int64 tensor of one element on x's device, which the
+    kernel reads; it must stay as it was until the backward has run (changing it in place
+    before raises there).
 
     The mask is drawn in groups of eight entries along the last dimension, which are
     numbered through all rows; ``adapter_linear`` drops its input with the same one.  The
