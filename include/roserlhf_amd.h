@@ -516,9 +516,11 @@ RRL_API int rrl_embedding_bwd(const void* ids, int32_t ids_dtype, int64_t N, con
  * token_out (int64 [B]): the first index, in vocabulary order, at which the running sum of
  * what is left exceeds u times its whole.  logp_out (float32 [B]): log p of it;
  * logq_out (float32 [B], or NULL): log of its p over what is left.  T <= 0: the first
- * maximum, with T = 1 and logq 0; u is not looked at.  Exponentials are float64 (1.1e-12)
- * and summed in units of 2^-44 of the largest (2^-(62 - b) for 2^b > 2^18 entries), and
- * u times the whole below one unit counts as 0.
+ * maximum, with T = 1 and logq 0; u is not looked at.  Exponentials are float64 (1.1e-12).
+ * For cuts and tokens they are summed in units of 2^-44 of the largest (2^-(62 - b) for
+ * 2^b > 2^18 entries), so that a sum is off by up to V 2^-45 of the largest (2^-27 for
+ * 2^18 entries, 2^-23 for 2^20), and u times the whole below one unit counts as 0; for
+ * logp and logq in float64.  V is at most 2^20.
  * A row with NaN or +inf, or with nothing above -inf, and a temperature that is NaN or
  * +inf give token -1 and NaN log-probs.  (The reference has one setting for all rows and
  * no min-p, roseinfer/engine.py:1103-1171.)  workspace:

@@ -1105,9 +1105,13 @@ int launch_choose(const ChooseArgs& a, int64_t B, bool filters, hipStream_t st) 
   return check_launch("choose_draw_kernel");
 }
 
-// Sizes whose index arithmetic and grids fit (a grid's threads are counted in 32 bits).
+// Sizes whose index arithmetic and grids fit (a grid's threads are counted in 32 bits), and
+// of rows whose sums are good enough to draw from: those of 2^20 entries, in units of 2^-42,
+// are off by up to 2^-23 of the largest weight, a step or two of a float32 uniform; those of
+// 2^30 would be by an eighth of it.
+constexpr int64_t kMostEntries = (int64_t)1 << 20;
 inline bool choose_fits(int64_t B, int64_t V) {
-  return B >= 0 && V >= 1 && B < ((int64_t)1 << 22) && V <= ((int64_t)1 << 30) &&
+  return B >= 0 && V >= 1 && B < ((int64_t)1 << 22) && V <= kMostEntries &&
          B * ((V + part_entries(B, V) - 1) / part_entries(B, V)) < ((int64_t)1 << 24);
 }
 inline bool may_top_k(const rrl_sample_params& p, int64_t V) { return p.top_ks || (p.top_k > 0 && p.top_k < V); }
@@ -1133,7 +1137,8 @@ extern "C" int rrl_sample_tokens(const void* logits, int32_t dtype, int64_t B, i
   if (B == 0) return RRL_OK;
   RRL_REQUIRE(V >= 1, RRL_EINVAL, "rrl_sample_tokens: logits need at least one vocabulary entry");
   RRL_REQUIRE(choose_fits(B, V), RRL_EINVAL,
-              "rrl_sample_tokens: 2^22 rows or more, rows of over 2^30 entries, or 2^24 parts of them or more");
+              "rrl_sample_tokens: 2^22 rows or more, 2^24 parts of them or more, or rows of over 2^20 entries (the "
+              "sums of 2^30 would be too coarse to draw from)");
   RRL_REQUIRE(logits != nullptr && uniforms != nullptr && params != nullptr && token_out != nullptr &&
                   logp_out != nullptr && workspace != nullptr,
               RRL_EINVAL, "rrl_sample_tokens: null operand");

@@ -3,9 +3,9 @@
 ``sample_next_token_batch`` keeps the reference's rules: one temperature, top-k and
 top-p for the whole batch, and a floor of 1e-9 under every candidate's probability.
 ``sample_tokens`` is for batches of requests that each bring their settings, min-p
-among them, and for rollouts that have to be drawn from exactly the distribution whose
+among them, and for rollouts that have to be drawn from the distribution whose
 log-probs they record: it has no floor, its uniforms are an argument (as
-``verify_draft_tokens``'s are), and its borders are decided in 64 bits
+``verify_draft_tokens``'s are), and its borders are decided in 64-bit sums
 (``rrl_sample_tokens``).
 """
 
@@ -47,9 +47,14 @@ def sample_tokens(
       less; above 1 it counts as 1);
 
     and the token is the first, in vocabulary order, at which the running sum of what is
-    kept exceeds the row's uniform times its whole (a product below 2^-44 of the largest
-    probability counts as 0, and a uniform of 1 takes the last that has any).  A
-    temperature of 0 or less takes the first maximum, whatever the other settings.
+    kept exceeds the row's uniform times its whole (a uniform of 1 takes the last that has
+    any).  A temperature of 0 or less takes the first maximum, whatever the other settings.
+
+    The sums that decide this count a probability in units of 2^-44 of the largest one, to
+    the nearest (of 2^-42 for the longest rows, V is at most 2^20): all of them together are
+    off by at most V 2^-45 of it, 2^-27 for 2^18 entries and 2^-23 for 2^20, where a step
+    of the uniforms is 2^-24; a product below one unit counts as 0.  Log-probs come from
+    float64 sums.
 
     Returns the tokens, their ``log_softmax(logits / temperature)`` (at temperature 1
     where it is greedy) and, unless ``sampling_logprobs=False``, the log-probs of the
