@@ -75,17 +75,19 @@ struct ChooseArgs {
   int parts, part;  // parts of a row, and their entries
   double magic;     // 2^(52 - F): a weight added to it stands in the low bits, in units of 2^-F
   int unit_log2;    // F
+  int bins;         // of a histogram: kBins, or fewer where a row has fewer entries
+  int list_room;    // kListed, or the row's length
   float* peak;      // [B, parts] a part's maximum; +inf: it holds NaN or +inf
   u64* whole;       // [B, parts] sum of all entries, where there is a top-p and no top-k
   u64* left;        // [B, parts, kPW] of those that are left, a wave's run of a part each
   struct Exact* all;   // [B, parts, kPW] the same two sums for log-probs; kept only where
   struct Exact* kept;  // a setting leaves out entries
-  u64* sums;        // [B, parts, kBins], where there may be a top-p
-  uint32_t* counts; // [B, parts, kBins], where there may be a top-k
+  u64* sums;        // [B, parts, bins], where there may be a top-p
+  uint32_t* counts; // [B, parts, bins], where there may be a top-k
   Cut* cut;         // [B], where there may be either
   float* tops;      // [B, parts, kPT] a lane's maximum, where there may be a top-k
   float* reach;     // [B] the least value that the top k can hold
-  float* list_x;    // [B, kListed] entries that the top k can hold, in any order
+  float* list_x;    // [B, list_room] entries that the top k can hold, in any order
   int *list_i, *listed;  // their places, and [B] their number (over kListed: not all are there)
   int64_t* token_out;
   float *logp_out, *logq_out;  // logq_out may be null
@@ -171,19 +173,20 @@ struct Settings {
     return Cut{value_of(k), kNoIndex};
   }
 };
-__device__ __forceinline__ int bin_of(float x, float m, float scale) {
-  return (int)fminf((m - x) * scale, (float)(kBins - 1));
+// The last of `bins` takes all that lies below it.
+__device__ __forceinline__ int bin_of(float x, float m, float scale, int bins) {
+  return (int)fminf((m - x) * scale, (float)(bins - 1));
 }
 
 // The least float (by its key) that falls into a bin up to `bin`.  Whole waves look for the
 // same, 64 places at a time.
-__device__ __forceinline__ float bin_floor(int bin, float m, float scale) {
+__device__ __forceinline__ float bin_floor(int bin, float m, float scale, int bins) {
   const uint32_t lane = threadIdx.x & 63;
   uint32_t lo = key_of(-__FLT_MAX__), hi = key_of(m);  // hi does
   while (lo < hi) {
     const uint32_t step = (hi - lo) / 64 + 1;
     const uint32_t at = hi - lo > lane * step ? lo + lane * step : hi;
-    const uint64_t in = __ballot(bin_of(value_of(at), m, scale) <= bin);
+    const uint64_t in = __ballot(bin_of(value_of(at), m, scale, bins) <= bin);
     if (in) {
       const uint32_t first = (uint32_t)__ffsll((unsigned long long)in) - 1;
       const uint32_t found = hi - lo > first * step ? lo + first * step : hi;
@@ -323,7 +326,7 @@ struct WeighShared {
 // The last bin that the top k reach at most: k lanes' maxima are that large or larger.
 __device__ __forceinline__ int top_bin(const ChooseArgs& a, const Settings& set, float m, int64_t b, WeighShared& sh) {
   const int t = threadIdx.x, lane = t & 63, wv = t >> 6, n = a.parts * kPT;
-  if (set.top_k > n) return kBins - 1;
+  if (set.top_k > n) return a.bins - 1;
   const float scale = set.scale();
   constexpr int kTogether = 8;
   for (int k0 = t; k0 < n; k0 += kTogether * kPT) {
@@ -332,9 +335,9 @@ __device__ __forceinline__ int top_bin(const ChooseArgs& a, const Settings& set,
     for (int k = 0; k < kTogether; ++k) x[k] = a.tops[b * n + min(k0 + k * kPT, n - 1)];
 #pragma unroll
     for (int k = 0; k < kTogether; ++k)
-      if (k0 + k * kPT < n && x[k] != -M<float>::inf()) atomicAdd(&sh.counts[bin_of(x[k], m, scale)], 1u);
+      if (k0 + k * kPT < n && x[k] != -M<float>::inf()) atomicAdd(&sh.counts[bin_of(x[k], m, scale, a.bins)], 1u);
   }
-  if (t == 0) sh.bin = kBins - 1;
+  if (t == 0) sh.bin = a.bins - 1;
   __syncthreads();
   constexpr int kEach = kBins / kPT;
   uint32_t mine[kEach], sum = 0;
@@ -387,7 +390,7 @@ __device__ __forceinline__ void weigh(const ChooseArgs& a, const Settings& set, 
         const double v = mass.w.template unscaled<DIRECT>(x[k]);
         sum += v;
         if (x[k] >= reach) {
-          const int bin = bin_of(x[k], m, scale), at = atomicAdd(&sh.listed, 1);
+          const int bin = bin_of(x[k], m, scale, a.bins), at = atomicAdd(&sh.listed, 1);
           atomicAdd(&sh.counts[bin], 1u);
           if (set.top_p > 0.0) atomicAdd(&sh.sums[bin], mass.of<DIRECT>(v));
           if (at < kPartListed) {
@@ -408,7 +411,7 @@ __device__ __forceinline__ void weigh(const ChooseArgs& a, const Settings& set, 
         const u64 w = mass.of<DIRECT>(v);
         sum += v;
         whole += w;
-        if (w > floor) atomicAdd(&sh.sums[bin_of(x[k], m, scale)], w);
+        if (w > floor) atomicAdd(&sh.sums[bin_of(x[k], m, scale, a.bins)], w);
       }
     }, add);
   } else if (set.min_p > 0.0) {
@@ -460,7 +463,7 @@ __global__ __launch_bounds__(kPT) void choose_weigh_kernel(ChooseArgs a) {
     }
     if (t == 0) sh.listed = 0;
     __syncthreads();
-    if (set.top_k > 0) reach = bin_floor(top_bin(a, set, m, b, sh), m, set.scale());
+    if (set.top_k > 0) reach = bin_floor(top_bin(a, set, m, b, sh), m, set.scale(), a.bins);
   }
   const Mass mass(m, set.c(), a.magic);
   u64 whole = 0, left = 0;
@@ -472,18 +475,18 @@ __global__ __launch_bounds__(kPT) void choose_weigh_kernel(ChooseArgs a) {
   if (set.filtered) {
     whole = block_reduce<kPW>(whole, sh.wave, Add());
     if (t == 0) a.whole[blockIdx.x] = whole;
-    const int64_t to = (int64_t)blockIdx.x * kBins;
+    const int64_t to = (int64_t)blockIdx.x * a.bins;
     if (set.top_p > 0.0)
-      for (int k = t; k < kBins; k += kPT) a.sums[to + k] = sh.sums[k];
+      for (int k = t; k < a.bins; k += kPT) a.sums[to + k] = sh.sums[k];
     if (set.top_k > 0) {
-      for (int k = t; k < kBins; k += kPT) a.counts[to + k] = sh.counts[k];
+      for (int k = t; k < a.bins; k += kPT) a.counts[to + k] = sh.counts[k];
       if (part == 0 && t == 0) a.reach[b] = reach;
       // a run of the row's list; beyond its end, or this part's, nothing is listed
       if (t == 0) sh.base = atomicAdd(&a.listed[b], min(sh.listed, kListed + 1) + (sh.listed > kPartListed ? kListed + 1 : 0));
       __syncthreads();
-      for (int k = t; k < min(sh.listed, kPartListed) && sh.base + k < kListed; k += kPT) {
-        a.list_x[b * kListed + sh.base + k] = sh.list_x[k];
-        a.list_i[b * kListed + sh.base + k] = sh.list_i[k];
+      for (int k = t; k < min(sh.listed, kPartListed) && sh.base + k < a.list_room; k += kPT) {
+        a.list_x[b * a.list_room + sh.base + k] = sh.list_x[k];
+        a.list_i[b * a.list_room + sh.base + k] = sh.list_i[k];
       }
     }
   } else {
@@ -551,8 +554,8 @@ struct BinEntries {
   __device__ __forceinline__ BinEntries(const ChooseArgs& a, int64_t b, float m, float scale, int bin, const Cut& cut_,
                                         bool have_list, CutShared& sh_)
       : row(row_at<Tag>(a, b)), V(a.V), cut(cut_), sh(&sh_), listed(kListed + 1) {
-    lo = bin_floor(bin, m, scale);
-    hi = bin > 0 ? bin_floor(bin - 1, m, scale) : M<float>::inf();  // (its key lies above all others)
+    lo = bin_floor(bin, m, scale, a.bins);
+    hi = bin > 0 ? bin_floor(bin - 1, m, scale, a.bins) : M<float>::inf();  // (its key lies above all others)
     if (have_list) {
       listed = sh->listed;
       return;
@@ -716,13 +719,15 @@ __device__ __forceinline__ Cut select(const BinEntries<Tag>& in, bool by_mass, u
 
 // One bin of every part.
 template <class T>
-__device__ __forceinline__ u64 over_parts(const T* bins, int parts) {
+__device__ __forceinline__ u64 over_parts(const T* all, int64_t b, int bin, int bins, int parts) {
   constexpr int kTogether = 10;
   u64 sum = 0;
+  if (bin >= bins) return sum;
+  const T* const of = all + b * parts * bins + bin;
   for (int k0 = 0; k0 < parts; k0 += kTogether) {
     T v[kTogether];
 #pragma unroll
-    for (int k = 0; k < kTogether; ++k) v[k] = bins[(int64_t)min(k0 + k, parts - 1) * kBins];
+    for (int k = 0; k < kTogether; ++k) v[k] = of[(int64_t)min(k0 + k, parts - 1) * bins];
 #pragma unroll
     for (int k = 0; k < kTogether; ++k) sum += k0 + k < parts ? v[k] : 0;
   }
@@ -742,15 +747,15 @@ __global__ __launch_bounds__(kRT) void choose_cut_kernel(ChooseArgs a) {
   const Mass mass(m, set.c(), a.magic);
   Cut cut{-M<float>::inf(), 0};
   u64 sum = 0;  // of this thread's bin
-  if (set.top_p > 0.0) sum = over_parts(a.sums + (int64_t)b * a.parts * kBins + t, a.parts);
+  if (set.top_p > 0.0) sum = over_parts(a.sums, b, t, a.bins, a.parts);
   bool have_list = false;
   if (set.top_k > 0) {
     const int n = a.listed[b];
     have_list = n <= kListed;
     if (have_list) {
       for (int k = t; k < n; k += kRT) {
-        sh.list_x[k] = a.list_x[b * kListed + k];
-        sh.list_i[k] = a.list_i[b * kListed + k];
+        sh.list_x[k] = a.list_x[b * a.list_room + k];
+        sh.list_i[k] = a.list_i[b * a.list_room + k];
       }
       if (t == 0) sh.listed = n;
     }
@@ -767,7 +772,7 @@ __global__ __launch_bounds__(kRT) void choose_cut_kernel(ChooseArgs a) {
         for (int k = t; k < a.parts; k += kRT) all += a.whole[b * a.parts + k];
       target = (u64)(set.top_p * (double)block_reduce<kRW>(all, sh.wave, Add()));
     } else {
-      mine = over_parts(a.counts + (int64_t)b * a.parts * kBins + t, a.parts);
+      mine = over_parts(a.counts, b, t, a.bins, a.parts);
       cut = Cut{a.reach[b], kNoIndex};  // if these are k
     }
     const int bin = find_bin(sh, mine, above, target);
@@ -1056,7 +1061,7 @@ inline int part_entries(int64_t B, int64_t V) {
 }
 
 struct ChooseLayout {
-  int part;
+  int part, bins, list_room;
   int64_t parts;
   size_t peak, whole, left, all, kept, sums, counts, cut, tops, reach, list_x, list_i, listed, total;
 };
@@ -1064,6 +1069,10 @@ inline ChooseLayout choose_layout(int64_t B, int64_t V, bool top_k, bool top_p) 
   ChooseLayout l;
   l.part = part_entries(B, V);
   l.parts = (V + l.part - 1) / l.part;
+  // no more of either than a row has entries (131,072 rows of 9: 0.3 GB instead of 6)
+  l.bins = 64;
+  while (l.bins < kBins && l.bins < V) l.bins *= 2;
+  l.list_room = (int)min(V, (int64_t)kListed);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -1076,13 +1085,13 @@ inline ChooseLayout choose_layout(int64_t B, int64_t V, bool top_k, bool top_p) 
   l.left = take(8 * n * kPW);
   l.all = take(sizeof(Exact) * n * kPW);
   l.kept = take(sizeof(Exact) * n * kPW);
-  l.sums = take(top_p ? 8 * n * kBins : 0);
-  l.counts = take(top_k ? 4 * n * kBins : 0);
+  l.sums = take(top_p ? 8 * n * l.bins : 0);
+  l.counts = take(top_k ? 4 * n * l.bins : 0);
   l.cut = take(sizeof(Cut) * (size_t)B);
   l.tops = take(top_k ? 4 * n * kPT : 0);
   l.reach = take(top_k ? 4 * (size_t)B : 0);
-  l.list_x = take(top_k ? 4 * (size_t)B * kListed : 0);
-  l.list_i = take(top_k ? 4 * (size_t)B * kListed : 0);
+  l.list_x = take(top_k ? 4 * (size_t)B * l.list_room : 0);
+  l.list_i = take(top_k ? 4 * (size_t)B * l.list_room : 0);
   l.listed = take(top_k ? 4 * (size_t)B : 0);
   l.total = at;
   return l;
@@ -1173,6 +1182,8 @@ extern "C" int rrl_sample_tokens(const void* logits, int32_t dtype, int64_t B, i
   const ChooseLayout l = choose_layout(B, V, top_k, top_p);
   char* w = static_cast<char*>(workspace);
   a.part = l.part;
+  a.bins = l.bins;
+  a.list_room = l.list_room;
   a.parts = (int)l.parts;
   a.peak = reinterpret_cast<float*>(w + l.peak);
   a.whole = reinterpret_cast<u64*>(w + l.whole);

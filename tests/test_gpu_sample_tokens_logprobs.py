@@ -16,6 +16,8 @@ import torch
 
 from rosellm_amd.roseinfer import sample_tokens
 
+from _sample_oracle import choose
+
 pytestmark = pytest.mark.gpu
 
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -109,3 +111,21 @@ def test_log_probs_do_not_depend_on_the_batch(device):
             many = sample_tokens(x.repeat(3, 1), u.repeat(3), **kw)
             for a, b in zip(many, want):
                 assert torch.equal(a[1000:], b)
+
+
+@pytest.mark.parametrize("V", [3, 64, 65, 127, 129, 511, 1023, 1024, 4097])
+def test_short_rows_whose_entries_lie_far_apart(device, V):
+    """Rows with fewer bins than others, the last of which takes most entries."""
+    gen = torch.Generator().manual_seed(V)
+    for dtype in DTYPES:
+        x = (torch.randn(40, V, generator=gen) * torch.linspace(0.1, 60.0, 40)[:, None]).to(dtype)
+        u = torch.rand(40, generator=gen)
+        for kw in (dict(top_k=2), dict(top_k=V - 1, top_p=0.99), dict(top_p=0.9999), dict(top_k=V // 2 + 1, temperature=9.0),
+                   dict(top_p=0.999, temperature=20.0, min_p=1e-5)):
+            out = sample_tokens(x.to(device), u.to(device), **kw)
+            for b in range(40):
+                t, lp, lq = choose(x[b], u[b].item(), kw.get("temperature", 1.0), kw.get("top_k", 0), kw.get("top_p", 1.0),
+                                   kw.get("min_p", 0.0))
+                assert int(out.token_ids[b]) == t, (V, dtype, kw, b)
+                _near(out.logprobs[b:b + 1], torch.tensor([lp], dtype=torch.float64))
+                _near(out.sampling_logprobs[b:b + 1], torch.tensor([lq], dtype=torch.float64))
