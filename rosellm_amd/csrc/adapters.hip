@@ -1029,45 +1029,49 @@ __global__ __launch_bounds__(kAT, RT <= 2 ? 3 : 2) void adapter_outer_kernel(Out
   }
 }
 
-// Joins the runs' sums, in order: a workgroup takes 64 entries, a wave a quarter of the runs.
+// Joins the runs' sums, in order: a workgroup takes 64 entries at a time, a wave a quarter of
+// the runs.
 template <class Tag>
 __global__ __launch_bounds__(kAT) void adapter_join_kernel(OuterArgs a) {
   __shared__ float quarter[kAW][64];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int64_t n0 = a.job[0].wide ? a.job[0].C * a.r : 0, n1 = a.job[1].wide ? a.job[1].C * a.r : 0;
-  const int64_t b0 = (n0 + 63) / 64, b1 = (n1 + 63) / 64;
-  const int64_t ad = blockIdx.x / (b0 + b1);
-  const bool second = blockIdx.x % (b0 + b1) >= b0;
-  const int64_t k = (blockIdx.x % (b0 + b1) - (second ? b0 : 0)) * 64 + lane;
-  const OuterJob& j = a.job[second];
-  const bool in = k < (second ? n1 : n0);
-  // neighbours in the gradient's rows
-  const int64_t c = j.o_sr == 1 ? k / a.r : k % j.C, r = j.o_sr == 1 ? k % a.r : k / j.C;
-  const int64_t size = j.C * a.R, slot0 = ad * a.segments;
-  const float* part = j.part + slot0 * size + (j.o_sr == 1 ? c * a.R + r : r * j.C + c);
+  const int64_t b0 = (n0 + 63) / 64, b1 = (n1 + 63) / 64, blocks = (b0 + b1) * a.ids.A;
   const int begin = a.segments * wv / kAW, end = a.segments * (wv + 1) / kAW;
-  constexpr int kTogether = 8;
-  float sum = 0.0f;
-  for (int s64 = begin; s64 < end; s64 += 64) {
-    const uint64_t seen = __ballot(s64 + lane < end && j.seen[slot0 + min(s64 + lane, end - 1)]);
-    for (int s0 = 0; s0 < 64 && seen >> s0; s0 += kTogether) {
-      float v[kTogether];
+  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const int64_t ad = block / (b0 + b1);
+    const bool second = block % (b0 + b1) >= b0;
+    const int64_t k = (block % (b0 + b1) - (second ? b0 : 0)) * 64 + lane;
+    const OuterJob& j = a.job[second];
+    const bool in = k < (second ? n1 : n0);
+    // neighbours in the gradient's rows
+    const int64_t c = j.o_sr == 1 ? k / a.r : k % j.C, r = j.o_sr == 1 ? k % a.r : k / j.C;
+    const int64_t size = j.C * a.R, slot0 = ad * a.segments;
+    const float* part = j.part + slot0 * size + (j.o_sr == 1 ? c * a.R + r : r * j.C + c);
+    constexpr int kTogether = 8;
+    float sum = 0.0f;
+    for (int s64 = begin; s64 < end; s64 += 64) {
+      const uint64_t seen = __ballot(s64 + lane < end && j.seen[slot0 + min(s64 + lane, end - 1)]);
+      for (int s0 = 0; s0 < 64 && seen >> s0; s0 += kTogether) {
+        float v[kTogether];
 #pragma unroll
-      for (int s = 0; s < kTogether; ++s)
-        v[s] = in && (seen >> (s0 + s) & 1) ? part[(s64 + s0 + s) * size] : 0.0f;
+        for (int s = 0; s < kTogether; ++s)
+          v[s] = in && (seen >> (s0 + s) & 1) ? part[(s64 + s0 + s) * size] : 0.0f;
 #pragma unroll
-      for (int s = 0; s < kTogether; ++s) sum += v[s];
+        for (int s = 0; s < kTogether; ++s) sum += v[s];
+      }
     }
+    __syncthreads();  // the last entries' sums are read
+    quarter[wv][lane] = sum;
+    __syncthreads();
+    if (wv != 0 || !in) continue;
+    sum = ((quarter[0][lane] + quarter[1][lane]) + quarter[2][lane]) + quarter[3][lane];
+    sum *= (a.scales ? a.scales[ad] : 1.0f);
+    if (j.drop) sum *= a.drop.scale;
+    const int64_t o = ad * j.o_sa + c * j.o_sc + r * j.o_sr;
+    if constexpr (std::is_same_v<Tag, TagF32>) reinterpret_cast<float*>(j.out)[o] = sum;
+    else reinterpret_cast<uint16_t*>(j.out)[o] = (uint16_t)Pack16<Tag>::pack_one(sum);
   }
-  quarter[wv][lane] = sum;
-  __syncthreads();
-  if (wv != 0 || !in) return;
-  sum = ((quarter[0][lane] + quarter[1][lane]) + quarter[2][lane]) + quarter[3][lane];
-  sum *= (a.scales ? a.scales[ad] : 1.0f);
-  if (j.drop) sum *= a.drop.scale;
-  const int64_t o = ad * j.o_sa + c * j.o_sc + r * j.o_sr;
-  if constexpr (std::is_same_v<Tag, TagF32>) reinterpret_cast<float*>(j.out)[o] = sum;
-  else reinterpret_cast<uint16_t*>(j.out)[o] = (uint16_t)Pack16<Tag>::pack_one(sum);
 }
 
 // up [A, O, r] as [A, R, P] (P: O rounded up to a multiple of 8) and down [A, r, H] as
@@ -1214,7 +1218,10 @@ int launch_outer(const OuterArgs& a, hipStream_t st) {
 template <class Tag>
 int launch_join(const OuterArgs& a, hipStream_t st) {
   const int64_t each = ((a.job[0].wide ? a.job[0].C * a.r : 0) + 63) / 64 + ((a.job[1].wide ? a.job[1].C * a.r : 0) + 63) / 64;
-  hipLaunchKernelGGL(adapter_join_kernel<Tag>, dim3((uint32_t)(each * a.ids.A)), dim3(kAT), 0, st, a);
+  // four threads an entry: of adapters of 2^30 weights more than a grid counts, so workgroups
+  // take several turns from 2^22 on
+  const int64_t blocks = min(each * a.ids.A, (int64_t)1 << 22);
+  hipLaunchKernelGGL(adapter_join_kernel<Tag>, dim3((uint32_t)blocks), dim3(kAT), 0, st, a);
   return check_launch("adapter_join_kernel");
 }
 
