@@ -1120,7 +1120,7 @@ inline int rank_padded(int r) { return r <= 16 ? 16 : (r <= 32 ? 32 : (r <= 64 ?
 // 2048, rank 64, a direction's two kernels 74 -> 57 us on average; with tiles that are cut,
 // the 37 us above would be 47.
 template <int TM>
-int tile_grid(FusedArgs& a, bool wide, int64_t least, dim3& grid) {
+dim3 tile_grid(FusedArgs& a, bool wide, int64_t least) {
   const int64_t windows = (a.N + kWindow - 1) / kWindow;
   const int rows = (int)min(a.N, (int64_t)kWindow);
   // tiles of a window if it is of one adapter, and at most
@@ -1130,16 +1130,15 @@ int tile_grid(FusedArgs& a, bool wide, int64_t least, dim3& grid) {
   a.slabs = wide ? (int)((a.O + a.slab - 1) / a.slab) : 1;
   a.groups = (int)(windows * most * a.slabs <= 1024 ? most * a.slabs
                                                     : min(most * a.slabs, max(even * a.slabs, 512 / windows)));
+  // a grid's threads are counted in 32 bits (up to 2^30 rows: at least 15 workgroups a window)
+  a.groups = (int)min((int64_t)a.groups, (((int64_t)1 << 32) / kAT - 1) / windows);
   a.in_turn = a.slabs == 1 && a.groups > even ? (int)windows : 0;
-  RRL_REQUIRE(windows * a.groups < ((int64_t)1 << 32) / kAT, RRL_EINVAL, "rrl_adapter: too many rows");
-  grid = dim3((uint32_t)(windows * a.groups));
-  return RRL_OK;
+  return dim3((uint32_t)(windows * a.groups));
 }
 
 template <class Tag, int R16, int TM>
 int launch_expand(FusedArgs a, int64_t least, size_t lds, hipStream_t st) {
-  dim3 grid;
-  if (int rc = tile_grid<TM>(a, true, least, grid)) return rc;
+  const dim3 grid = tile_grid<TM>(a, true, least);
   if (a.r == 16 * R16 && a.O % Stage<Tag, TM, true>::kCols == 0)
     hipLaunchKernelGGL((adapter_expand_kernel<Tag, R16, TM, true>), grid, dim3(kAT), lds, st, a);
   else hipLaunchKernelGGL((adapter_expand_kernel<Tag, R16, TM, false>), grid, dim3(kAT), lds, st, a);
@@ -1169,17 +1168,16 @@ int launch_fused(FusedArgs a, hipStream_t st) {
   a.stream_x = larger_than_cache(a.N, a.K, Frag<Tag>::SZ);
   a.stream_out = larger_than_cache(a.N, a.O, Frag<Tag>::SZ);
   const size_t lds = Window<64>::lds(a.ids.A);
-  dim3 grid;
   const bool few = a.N <= kFewRows<R16>, together = few && a.O <= kFusedColumns;
   if (few) {
     char* const out = a.out;
     if (!together) a.out = nullptr;
-    if (int rc = tile_grid<16>(a, a.out != nullptr, 256, grid)) return rc;
+    const dim3 grid = tile_grid<16>(a, a.out != nullptr, 256);
     hipLaunchKernelGGL((adapter_fused_kernel<Tag, R16>), grid, dim3(kAT), lds, st, a);
     if (int rc = check_launch("adapter_fused_kernel")) return rc;
     a.out = out;
   } else {
-    if (int rc = tile_grid<64>(a, false, 256, grid)) return rc;
+    const dim3 grid = tile_grid<64>(a, false, 256);
     if (a.r == 16 * R16 && a.K % Stage<Tag, 16, true>::kCols == 0)
       hipLaunchKernelGGL((adapter_shrink_kernel<Tag, R16, true>), grid, dim3(kAT), lds, st, a);
     else hipLaunchKernelGGL((adapter_shrink_kernel<Tag, R16, false>), grid, dim3(kAT), lds, st, a);

@@ -38,3 +38,16 @@ def test_gradients_of_over_2_to_the_30_weights(device):
     assert not dd[others].any()
     for a in others.nonzero().flatten().tolist():
         assert not du[a].any(), a
+
+
+@pytest.mark.parametrize("N,r", [(1 << 30, 3), ((1 << 28) + 77, 70)])
+def test_most_rows(device, N, r):
+    """Rows of one entry: t alone takes 69 GB for 2^30 rows of rank 16, and 137 for a quarter of them of rank 128."""
+    x = torch.zeros(N, 1, dtype=torch.bfloat16, device=device)
+    some = torch.cat([torch.arange(0, 3000), torch.arange(N // 2, N // 2 + 3000), torch.arange(N - 3000, N)]).to(device)
+    x[some] = (torch.arange(9000, device=device) % 251 - 125).bfloat16()[:, None]
+    down, up = torch.zeros(1, r, 1, device=device).bfloat16(), torch.zeros(1, 1, r, device=device).bfloat16()
+    down[0, r - 1], up[0, 0, r - 1] = 0.5, 4.0
+    y = adapter_linear(x, down, up)
+    assert y.shape == (N, 1)
+    assert torch.equal(y, x * 2)
