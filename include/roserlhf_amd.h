@@ -554,7 +554,9 @@ RRL_API int rrl_sample_tokens(const void* logits, int32_t dtype, int64_t B, int6
  * counter {i, i >> 32, o, o >> 32} under the key {seed, seed >> 32}; entry j of it the
  * half j % 2 (0: the low one) of word j / 2, a number under 65536, and is kept where
  * that is at least round(65536 p) = 65536 p'.  o = offset + *offset_device (modulo
- * 2^64), so that a captured graph can take another mask at each replay. */
+ * 2^64), so that a captured graph can take another mask at each replay.  Calls with equal
+ * seeds and offsets, of rrl_adapter_* too, drop the same places; rrl_sample_logprobs
+ * takes the words at {row, row >> 32, offset, offset >> 32} under its seed. */
 typedef struct rrl_dropout_params {
   double p;                      /* in [0, 1] */
   uint64_t seed;

@@ -71,12 +71,13 @@ def dropout(x: Tensor, p: float, *, seed: Optional[int] = None, offset: Union[in
     2^-16, by which the kept ones are scaled, so that the expectation is x's.  Its fate
     depends on its place, ``seed`` and ``offset`` alone: equal arguments give equal masks,
     whatever the strides, and the gradient draws the forward's mask again.  Give each
-    call of a step a seed or an offset of its own.  With ``seed=None`` a seed is drawn
-    from ``generator`` (a CPU ``torch.Generator``, default: torch's global one), on the
-    host: a captured graph replays it, and a trace keeps it.  For another mask at each
-    replay, ``offset`` can be an int64 tensor of one element on x's device, which the
-    kernel reads; it must stay as it was until the backward has run (changing it in place
-    before raises there).
+    call of a step a seed or an offset of its own, and a seed that
+    ``sample_next_token_batch``, which draws from the same generator, does not have.
+    With ``seed=None`` a seed is drawn from ``generator`` (a CPU ``torch.Generator``,
+    default: torch's global one), on the host: a captured graph replays it, and a trace
+    keeps it.  For another mask at each replay, ``offset`` can be an int64 tensor of one
+    element on x's device, which the kernel reads; it must stay as it was until the
+    backward has run (changing it in place before raises there).
 
     The mask is drawn in groups of eight entries along the last dimension, which are
     numbered through all rows; ``adapter_linear`` drops its input with the same one.  The
