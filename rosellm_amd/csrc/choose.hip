@@ -370,6 +370,11 @@ __device__ __forceinline__ int top_bin(const ChooseArgs& a, const Settings& set,
   return sh.bin;
 }
 
+// A sum is formed here and not later: where branches follow, the weights of all that a lane
+// holds would wait for it in registers, which leaves two of three waves a SIMD (256 rows with
+// a nucleus 148 us instead of 142, with settings of their own 173 instead of 166).
+__device__ __forceinline__ void here(double& sum) { asm volatile("" : "+v"(sum)); }
+
 // whole and left are this thread's, all and kept the wave's.
 template <class Tag, bool DIRECT>
 __device__ __forceinline__ void weigh(const ChooseArgs& a, const Settings& set, const Mass& mass, float m, int64_t b,
@@ -410,6 +415,7 @@ __device__ __forceinline__ void weigh(const ChooseArgs& a, const Settings& set, 
         const double v = mass.w.template unscaled<DIRECT>(x[k]);
         const u64 w = mass.of<DIRECT>(v);
         sum += v;
+        here(sum);
         whole += w;
         if (w > floor) atomicAdd(&sh.sums[bin_of(x[k], m, scale, a.bins)], w);
       }
