@@ -21,8 +21,9 @@
 // sums of the same weights in float64, which are the same in any order of a row's chunks too.
 //
 // What is left is always the entries above a place (x, v) in descending order.  Rows are
-// cut into parts, a workgroup each, so that a single row fills the chip, and read once a
-// launch (from the caches, but for the first):
+// cut into parts of 8192 entries or more, a workgroup each (a single row of 151,936 is 19
+// of them, on as many of the 256 CUs), and read once a launch (from the caches, but for the
+// first):
 //   1. choose_max: the maximum of each part
 //   2. choose_weigh: each part's sum, and where the row has a top-k or a top-p its
 //      histogram, counts or sums in 1024 bins of 1/16 of a factor of two below m, of the

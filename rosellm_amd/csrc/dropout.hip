@@ -17,7 +17,7 @@ constexpr int kDT = 256;
 struct DropArgs {
   const char *x, *res;  // res may be null
   char* out;            // contiguous [rows, cols]
-  int64_t rows, cols, x_ld, r_ld;
+  int64_t cols, x_ld, r_ld;
   int64_t groups, per_row;
   Drop drop;
 };
@@ -116,7 +116,6 @@ extern "C" int rrl_dropout(const void* x, int32_t dtype, int64_t rows, int64_t c
   a.x = static_cast<const char*>(x);
   a.res = static_cast<const char*>(residual);
   a.out = static_cast<char*>(out);
-  a.rows = rows;
   a.cols = cols;
   a.x_ld = x_ld;
   a.r_ld = r_ld;

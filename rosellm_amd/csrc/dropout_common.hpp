@@ -24,7 +24,7 @@ struct Drop {
   __device__ __forceinline__ uint64_t counter() const {
     return offset + (offset_device ? (uint64_t)*offset_device : 0u);
   }
-  // v[0..8) of group `group`: kept and scaled, or zero (of NaN and infinities too)
+  // a bit for each of the eight entries of a group: set where it is kept
   __device__ __forceinline__ uint32_t keep_bits(uint64_t group, uint64_t at) const {
     uint32_t c[4] = {(uint32_t)group, (uint32_t)(group >> 32), (uint32_t)at, (uint32_t)(at >> 32)};
     philox4x32_10(c, k0, k1);
