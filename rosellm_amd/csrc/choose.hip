@@ -33,12 +33,12 @@
 //   4. choose_left (as 3): the sum of what is left, of each quarter of a part
 //   5. choose_draw: a workgroup a row finds the quarter, then the entry
 //
-// Times, us (bfloat16 rows of 151,936): one row with a nucleus 3 + 7 + 29 + 6 + 7, 64 rows
-// without a filter 5 + 13 + 9, 256 rows with settings of their own 14 + 60 + 40 + 31 + 18.
-// The second launch is bound by issue: 26 instructions an entry, 12 of them float64 (25 us of
-// the 60), and the histograms' atomics; the third by the chain of some fifteen barriers of
-// sixteen waves each (9 us a border) and a read of the row by one CU; the bytes of 256 rows
-// are 16 us at a copy's rate.
+// Times, us (bfloat16 rows of 151,936): one row with a nucleus 3 + 8 + 29 + 6 + 9, 64 rows
+// without a filter 5 + 14 + 9, 256 rows with settings of their own 15 + 65 + 41 + 30 + 18.
+// The second launch is bound by issue: 21 instructions an entry without a filter, 14 of them
+// float64 (32 and 16 with a min-p), and the histograms' atomics; the third by the chain of
+// some fifteen barriers of sixteen waves each (9 us a border) and a read of the row by one CU;
+// the bytes of 256 rows are 16 us at a copy's rate.
 #include "vocab_weights.hpp"
 
 #include <type_traits>
